@@ -57,7 +57,8 @@ typedef enum {
  * gdn_quantized_matmul_f32, its workspace size and
  * gdn_quantized_matmul_rows_workspace_size, 18 gdn_quantized_matmul_rows, which
  * alone uses that workspace, 19 gdn_prefill_chunked_runs and
- * gdn_prefill_fused_runs). */
+ * gdn_prefill_fused_runs, 20 gdn_conv_silu, gdn_selective_scan,
+ * gdn_selective_step, gdn_fp8_matmul and gdn_fp8_dequantize). */
 int gdn_abi_version(void);
 
 /* Message describing the calling thread's last non-zero return. */
@@ -467,6 +468,95 @@ int gdn_quantized_matmul_scheme(const void *x, const void *w, const void *scales
 /* Workspace bytes gdn_quantized_matmul_scheme splits K with for these sizes
  * (0: no split). No reference counterpart: MLX's kernels allocate their own. */
 int64_t gdn_quantized_matmul_scheme_workspace_size(int M, int N, int K);
+
+/*
+ * gdn_conv_silu - the causal depthwise conv of a state-space layer with bias
+ * and SiLU for N packed runs: out[t,c] = silu(bias[c] + sum_j weight[c,j]
+ * x[t-K+1+j,c]), float32 with one rounding.
+ *   x: (T_total, C) act_dtype at x_stride (>= C) elements a row
+ *   conv_state_in: (N, K-1, C) act_dtype, the rows before each run;
+ *   conv_state_out: the same, the last K-1 rows; must not overlap it
+ *   weight: (C, K) float32; bias: (C) float32 or NULL; K 2, 3 or 4
+ *   cu_seqlens: (N+1) int32 or NULL (N runs of T_total / N tokens)
+ *   out: (T_total, C) act_dtype
+ * No reference counterpart (its conv, linear_attention.py:61-79, has no bias
+ * and belongs to the q/k scaling: gdn_frontend).
+ */
+int gdn_conv_silu(const void *x, int64_t x_stride, const void *conv_state_in, void *conv_state_out,
+                  const float *weight, const float *bias, const int32_t *cu_seqlens, int N, int64_t T_total,
+                  void *out, int C, int K, int act_dtype, void *stream);
+
+/*
+ * gdn_selective_scan - the selective state-space scan over N packed runs. Per
+ * head, with d = softplus(dt + dt_bias):
+ *   S_t = exp(-exp(A_log) d_t) S_{t-1} + (d_t x_t) B_t^T,  y_t = S_t C_t + D x_t
+ *   x: (T_total, H, P), B, C: (T_total, G, S) act_dtype, dt: (T_total, H)
+ *      dt_dtype, each at its own row stride in elements (columns of one conv
+ *      output); head h reads group h / (H / G)
+ *   A_log, dt_bias: (H) float32; D: (H) float32 or NULL (no skip)
+ *   state_in: (N, H, P, S) float32 or NULL (zeros); state_out: the same, may be
+ *      state_in
+ *   y: (T_total, H, P) y_dtype
+ *   longest_run: the longest run's tokens (0: not known); it decides only how
+ *      the call is split, and with it the order of the float32 sums
+ *   workspace: gdn_selective_scan_workspace_size(...) bytes of the same
+ *      arguments (0: none); calls sharing one must not overlap
+ * P and S multiples of 8, S at most 256 (else GDN_EUNSUPPORTED); x, B, C (and
+ * their rows), y, states and workspace 16-byte aligned. bfloat16 x with
+ * bfloat16 y runs on the bf16 matrix cores (state and sums float32), all else
+ * on the float32 ones. No reference counterpart.
+ */
+int64_t gdn_selective_scan_workspace_size(int N, int64_t T_total, int64_t longest_run, int G, int H, int P, int S);
+int gdn_selective_scan(const void *x, int64_t x_stride, const void *B, int64_t B_stride, const void *C,
+                       int64_t C_stride, int act_dtype, const void *dt, int64_t dt_stride, int dt_dtype,
+                       const float *A_log, const float *dt_bias, const float *D, const float *state_in,
+                       float *state_out, void *y, int y_dtype, const int32_t *cu_seqlens, int N, int64_t T_total,
+                       int64_t longest_run, int G, int H, int P, int S, void *workspace, int64_t workspace_bytes,
+                       void *stream);
+
+/*
+ * gdn_selective_step - one token of B sequences: gdn_conv_silu's conv over the
+ * channels [x (H*P); B (G*N); C (G*N)] of xbc, then one step of
+ * gdn_selective_scan, in one launch, float32 between them.
+ *   xbc: (B, C) and dt: (B, H) act_dtype at their row strides; conv_state_in:
+ *   (B, K-1, C) act_dtype; state_in: (B, H, P, N) float32, state_out may alias
+ *   it; y: (B, H, P) y_dtype; conv_bias and D may be NULL
+ *   slots, pool, conv_half, conv_arrivals: a pool's, as gdn_decode_step (any H:
+ *   the counter's 2^16 is shared out over the row's workgroups); a row whose
+ *   slot lies outside the pool writes NaN to y and touches no state
+ * N a multiple of 8 up to 256, P up to 256, K 2 to 4 (else GDN_EUNSUPPORTED);
+ * states 16-byte aligned. No reference counterpart.
+ */
+int gdn_selective_step(const void *xbc, int64_t xbc_stride, const void *dt, int64_t dt_stride,
+                       const void *conv_state_in, void *conv_state_out, const float *conv_weight,
+                       const float *conv_bias, const float *A_log, const float *dt_bias, const float *D,
+                       const float *state_in, float *state_out, void *y, int y_dtype, int B, int G, int H, int P,
+                       int N, int K, int act_dtype, const int32_t *slots, int pool, const int32_t *conv_half,
+                       int32_t *conv_arrivals, void *stream);
+
+/*
+ * gdn_fp8_matmul - y = x W^T (+ residual) for W in e4m3 codes with a scale for
+ * each block of 128 x 128, x quantized on the way in: per row and 128 columns
+ * to e4m3 codes q = x / s under s = max(amax |x| / 448, 2^-126) (float32
+ * divisions, nearest even). y[m,n] = sum over blocks of s sw sum(q w): the
+ * inner sums on the 8-bit matrix cores, float32 beyond.
+ *   x: (M, K) x_dtype; w: (N, K) e4m3 (fn) bytes; scales: (ceil(N / 128),
+ *   ceil(K / 128)) float32; y: (M, N) y_dtype; residual: NULL or (M, N) y_dtype
+ *   (may be y), added to the product rounded to y_dtype
+ *   workspace: gdn_fp8_matmul_workspace_size(...) bytes; calls sharing one must
+ *   not overlap
+ * K a multiple of 16; x, w, y and workspace 16-byte aligned. NaN or infinity in
+ * x makes its row NaN. No reference counterpart (a scheme beside
+ * moe_block.py:44-55's).
+ */
+int64_t gdn_fp8_matmul_workspace_size(int M, int N, int K);
+int gdn_fp8_matmul(const void *x, int x_dtype, const void *w, const float *scales, void *y, int y_dtype,
+                   const void *residual, int M, int N, int K, void *workspace, int64_t workspace_bytes,
+                   void *stream);
+
+/* gdn_fp8_dequantize - gdn_fp8_matmul's weights as a dense (N, K) out_dtype
+ * array: code times scale, one rounding. */
+int gdn_fp8_dequantize(const void *w, const float *scales, void *out, int out_dtype, int N, int K, void *stream);
 
 #ifdef __cplusplus
 }

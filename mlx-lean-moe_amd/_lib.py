@@ -16,7 +16,7 @@ import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libgdn.so")
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 GDN_F32, GDN_BF16, GDN_F16 = 0, 1, 2
 GDN_EINVAL, GDN_EUNSUPPORTED = -1, -2
@@ -93,6 +93,19 @@ _SIGNATURES = {
                                              _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int,
                                              _c_int, _c_int, _c_int, _c_void_p, _c_i64, _c_void_p]),
     "gdn_quantized_matmul_scheme_workspace_size": (_c_i64, [_c_int, _c_int, _c_int]),
+    "gdn_conv_silu": (_c_int, [_c_void_p, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int,
+                               _c_i64, _c_void_p, _c_int, _c_int, _c_int, _c_void_p]),
+    "gdn_selective_scan_workspace_size": (_c_i64, [_c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int]),
+    "gdn_selective_scan": (_c_int, [_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_int, _c_void_p,
+                                    _c_i64, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                                    _c_void_p, _c_int, _c_void_p, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int,
+                                    _c_int, _c_void_p, _c_i64, _c_void_p]),
+    "gdn_selective_step": (_c_int, [_c_void_p, _c_i64, _c_void_p, _c_i64] + [_c_void_p] * 10
+                           + [_c_int] * 8 + [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p]),
+    "gdn_fp8_matmul": (_c_int, [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int,
+                                _c_int, _c_int, _c_void_p, _c_i64, _c_void_p]),
+    "gdn_fp8_matmul_workspace_size": (_c_i64, [_c_int, _c_int, _c_int]),
+    "gdn_fp8_dequantize": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p]),
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -176,3 +189,14 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = lib.gdn_last_error().decode(errors="replace")
         raise KernelError(f"{name} returned {rc}: {msg}")
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """:func:`call` with ``device`` as the current one: a launch goes to the
+    current device, whatever device its stream belongs to."""
+
+    if device.index is None or device.index == torch.cuda.current_device():
+        call(name, *args)
+        return
+    with torch.cuda.device(device):
+        call(name, *args)

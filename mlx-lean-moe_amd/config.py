@@ -1,5 +1,6 @@
 """Shape of a gated-delta layer (the reference's ``Qwen3_5LinearAttention``
-dataclass, ``src/mlx_lean_moe/model/qwen3_5/config.py:10-32``)."""
+dataclass, ``src/mlx_lean_moe/model/qwen3_5/config.py:10-32``) and of a
+state-space layer."""
 
 from __future__ import annotations
 
@@ -34,3 +35,24 @@ class LinearAttentionDims:
 
 # The production shape of the path (Hk=16, Hv=32, d=128, K=4).
 QWEN3_5_LINEAR = LinearAttentionDims(16, 32, 128, 128, 4)
+
+
+@dataclass(frozen=True)
+class StateSpaceDims:
+    """A selective state-space layer: ``num_heads // num_groups`` consecutive
+    heads share a group's B and C."""
+
+    num_groups: int
+    num_heads: int
+    state_dim: int
+    head_dim: int
+    conv_kernel_dim: int
+
+    @property
+    def inner_dim(self) -> int:
+        return self.num_heads * self.head_dim
+
+    @property
+    def conv_dim(self) -> int:
+        """Channels of the conv: x, then the groups' B, then their C."""
+        return self.inner_dim + 2 * self.num_groups * self.state_dim

@@ -1,0 +1,742 @@
+// The selective state-space scan over packed runs. Per head, with
+// d_t = softplus(dt_t + dt_bias) and l_t = -exp(A_log) d_t,
+//   S_t = exp(l_t) S_{t-1} + (d_t x_t) B_t^T,   y_t = S_t C_t + D x_t,
+// S head_dim x state_dim, B and C shared by the heads of a group.
+//
+// Within a chunk of Q tokens, with c_t = l_1 + .. + l_t of the chunk and S the
+// state before it, that is
+//   y_t = exp(c_t) S C_t + sum_{s <= t} (C_t . B_s) exp(c_t - c_s) d_s x_s + D x_t
+//   S'  = exp(c_Q) S + sum_s exp(c_Q - c_s) d_s x_s B_s^T,
+// four matrix products: C B^T (Q x Q, one for all heads of a group), the
+// masked and decayed scores times x, S C^T, and x'^T B. They run on the matrix
+// cores; the chain over chunks is only S' in accumulator registers.
+//
+// A long run on few heads leaves most CUs idle, so runs are cut into segments:
+// a first pass forms each segment's own sum of x'^T B (the state after it from
+// an empty one) and its decay, a second one chains these, elementwise, into the
+// state before each segment, and the last one computes y from there. The first
+// pass costs one of the four products again.
+#include <type_traits>
+
+#include "gdn_host.h"
+#include "gdn_ssm.h"
+
+namespace gdn {
+namespace {
+
+constexpr int kScanThreads = 256;
+constexpr double kLog2e = 1.4426950408889634;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+struct ScanArgs {
+    const void *x, *B, *C, *dt;
+    int64_t x_stride, B_stride, C_stride, dt_stride;
+    int dt_dtype;
+    const float *A_log, *dt_bias, *D, *S_in;
+    float* S_out;
+    void* y;
+    int y_dtype;
+    const int32_t* cu;
+    int runs;
+    int64_t T, L, seg;
+    int G, H, P, N;
+    float *part, *decay;  // per (slot, head): a segment's own sum, then the state before it; its decay
+    int segmented;
+};
+
+// The decays of one chunk, per token (all in powers of two): c_t as the sum of
+// two floats, d_t, exp(c_t), and d_t exp(c_Q - c_t). The running sum is in
+// double: what counts are differences of its terms, and a chunk's sum reaches
+// hundreds where single terms are 1e-3.
+template <int Q>
+struct Decays {
+    float hi[Q], lo[Q], d[Q], e[Q], w[Q];
+};
+
+template <int Q>
+GDN_DEV double chunk_decays(Decays<Q>& o, int lane, float d, float rate) {
+    double c = double(d) * double(rate) * kLog2e;
+#pragma unroll
+    for (int off = 1; off < Q; off *= 2) {
+        const double up = __shfl_up(c, off, kWave);
+        if (lane >= off) c += up;
+    }
+    const double end = __shfl(c, Q - 1, kWave);
+    if (lane < Q) {
+        const float hi = float(c);
+        o.hi[lane] = hi;
+        o.lo[lane] = float(c - double(hi));
+        o.d[lane] = d;
+        o.e[lane] = __builtin_amdgcn_exp2f(hi);
+        o.w[lane] = d * __builtin_amdgcn_exp2f(float(end - c));
+    }
+    return end;
+}
+
+GDN_DEV f32x4 mfma_bf16(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+GDN_DEV bf16x8 frag(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
+
+// Column operand of eight rows r0 .. r0 + 3 and r1 .. r1 + 3 at 16 columns of
+// a row-major LDS tile: within each 16-lane group, lane i of a transposing
+// read receives element i % 4 of source lane i / 4 + 4 k, k = 0 .. 3.
+GDN_DEV bf16x8 column_frag(const uint16_t* tile, int stride, int r0, int r1, int col, int sl) {
+    const uint16_t* a = tile + (r0 + (sl >> 2)) * stride + col + 4 * (sl & 3);
+    const uint16_t* b = tile + (r1 + (sl >> 2)) * stride + col + 4 * (sl & 3);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(b));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// bfloat16 inputs and output, 64-token chunks, four waves. A workgroup covers
+// kHeads heads of one group and 64 kTiles / kHeads head_dim rows of each; a
+// wave owns 16 kTiles rows of one head: its S^T (state_dim x rows) in
+// accumulators, which are at once the left operand of S C^T, so the state
+// never passes through LDS. kNP: state_dim rounded up to 32, 64, 128 or 256.
+//
+// Roundings to bfloat16: the decayed scores and, as the operand of S C^T, a
+// copy of the state; both only enter y, which is bfloat16 itself. The state's
+// own update takes x' = d exp(c_Q - c) x in two bfloat16 pieces (2^-18).
+template <int kNP, int kHeads, int kTiles, bool kStateOnly>
+__global__ __launch_bounds__(kScanThreads) void scan_bf16_kernel(ScanArgs a) {
+    constexpr int Q = 64, NS = kNP + 8, PW = 64 * kTiles, PH = PW / kHeads, XS = PW + 8, WS = Q + 8;
+    constexpr int kRowsN = kNP / 8;                     // 16-byte pieces of a B or C row
+    constexpr int kLoadN = Q * kRowsN / kScanThreads, kLoadX = Q * (PW / 8) / kScanThreads;
+    constexpr int NT = kNP / 16, KS = kNP / 32;
+    __shared__ __attribute__((aligned(16))) uint16_t Bs[Q * NS], Cs[kStateOnly ? 8 : Q * NS], Xs[Q * XS],
+        Ws[kStateOnly ? 8 : kHeads * Q * WS];
+    __shared__ __attribute__((aligned(16))) Decays<Q> dec[kHeads];
+    __shared__ float dec_end[kHeads];
+
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, lr = lane & 15;
+    const int P = a.P, N = a.N, H = a.H;
+    const int tiles = (P + PH - 1) / PH, units = H / kHeads * tiles;
+    const int unit = blockIdx.x % units;
+    const int64_t slot = blockIdx.x / units;
+    const int h0 = unit / tiles * kHeads, p0 = unit % tiles * PH;
+    const int grp = h0 / (H / a.G);
+    const Segment sg = segment_of(a.cu, a.runs, a.L, a.seg, slot);
+    if (sg.run < 0) return;
+    const int hb = wave * kHeads / 4, h = h0 + hb;
+    const int pw = wave * 16 * kTiles;   // the wave's first row in the workgroup's, and in its head's
+    const int pl = p0 + pw - hb * PH;
+
+    const uint16_t* xg = static_cast<const uint16_t*>(a.x);
+    const uint16_t* Bg = static_cast<const uint16_t*>(a.B) + grp * N;
+    const uint16_t* Cg = static_cast<const uint16_t*>(a.C) + grp * N;
+
+    uint4 rb[kLoadN], rc[kStateOnly ? 1 : kLoadN], rx[kLoadX];
+    float rdt = 0.f;
+    const auto fetch = [&](int64_t t0) {
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < kLoadN; ++i) {
+            const int at = tid + kScanThreads * i, n = at % kRowsN * 8;
+            const int64_t t = t0 + at / kRowsN;
+            const bool ok = t < sg.t1 && n < N;
+            rb[i] = ok ? *reinterpret_cast<const uint4*>(Bg + t * a.B_stride + n) : zero;
+            if constexpr (!kStateOnly) rc[i] = ok ? *reinterpret_cast<const uint4*>(Cg + t * a.C_stride + n) : zero;
+        }
+#pragma unroll
+        for (int i = 0; i < kLoadX; ++i) {
+            const int at = tid + kScanThreads * i, col = at % (PW / 8) * 8;
+            const int64_t t = t0 + at / (PW / 8);
+            const int p = p0 + col % PH;
+            rx[i] = t < sg.t1 && p < P
+                        ? *reinterpret_cast<const uint4*>(xg + t * a.x_stride + int64_t(h0 + col / PH) * P + p)
+                        : zero;
+        }
+        if (wave < kHeads && t0 + lane < sg.t1)
+            rdt = load_any(a.dt, (t0 + lane) * a.dt_stride + h0 + wave, a.dt_dtype);
+    };
+
+    // the state before the segment: tile j of the wave's S^T holds rows n = 16 j
+    // + 4 g + i, columns p = lr
+    f32x4 S[kTiles][NT];
+    const int64_t slot_state = (slot * H + h) * P, run_state = (int64_t(sg.run) * H + h) * P;
+    const float* from = kStateOnly ? nullptr : a.segmented ? a.part + slot_state * N : a.S_in ? a.S_in + run_state * N : nullptr;
+#pragma unroll
+    for (int pt = 0; pt < kTiles; ++pt)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int p = pl + 16 * pt + lr, n = 16 * j + 4 * g;
+            S[pt][j] = from && p < P && n < N ? *reinterpret_cast<const f32x4*>(from + int64_t(p) * N + n)
+                                              : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    const float rate = wave < kHeads ? -expf(a.A_log[h0 + wave]) : 0.f;
+    const float dtb = wave < kHeads ? a.dt_bias[h0 + wave] : 0.f;
+    const float skip = !kStateOnly && a.D ? a.D[h] : 0.f;
+    double total = 0.0;
+
+    if (sg.t0 < sg.t1) fetch(sg.t0);
+    for (int64_t t0 = sg.t0; t0 < sg.t1; t0 += Q) {
+#pragma unroll
+        for (int i = 0; i < kLoadN; ++i) {
+            const int at = tid + kScanThreads * i, o = at / kRowsN * NS + at % kRowsN * 8;
+            *reinterpret_cast<uint4*>(Bs + o) = rb[i];
+            if constexpr (!kStateOnly) *reinterpret_cast<uint4*>(Cs + o) = rc[i];
+        }
+#pragma unroll
+        for (int i = 0; i < kLoadX; ++i) {
+            const int at = tid + kScanThreads * i;
+            *reinterpret_cast<uint4*>(Xs + at / (PW / 8) * XS + at % (PW / 8) * 8) = rx[i];
+        }
+        if (wave < kHeads) {
+            const float d = t0 + lane < sg.t1 ? softplus(rdt + dtb) : 0.f;
+            const double end = chunk_decays<Q>(dec[wave], lane, d, rate);
+            total += end;
+            if (lane == 0) dec_end[wave] = __builtin_amdgcn_exp2f(float(end));
+        }
+        __syncthreads();
+        if (t0 + Q < sg.t1) fetch(t0 + Q);
+
+        if constexpr (!kStateOnly) {
+            // the wave's 16 tokens' scores against all tokens up to them, as
+            // columns (D: rows s, column t), decayed per head
+            const int t = 16 * wave + lr;
+            bf16x8 cf[KS];
+#pragma unroll
+            for (int k = 0; k < KS; ++k) cf[k] = frag(*reinterpret_cast<const uint4*>(Cs + t * NS + 32 * k + 8 * g));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j > (wave | 1)) break;
+                f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+                if (j <= wave) {
+#pragma unroll
+                    for (int k = 0; k < KS; ++k)
+                        sc = mfma_bf16(frag(*reinterpret_cast<const uint4*>(Bs + (16 * j + lr) * NS + 32 * k + 8 * g)),
+                                       cf[k], sc);
+                }
+                const int s0 = 16 * j + 4 * g;
+#pragma unroll
+                for (int hh = 0; hh < kHeads; ++hh) {
+                    const f32x4 shi = *reinterpret_cast<const f32x4*>(dec[hh].hi + s0);
+                    const f32x4 slo = *reinterpret_cast<const f32x4*>(dec[hh].lo + s0);
+                    const f32x4 sd = *reinterpret_cast<const f32x4*>(dec[hh].d + s0);
+                    const float thi = dec[hh].hi[t], tlo = dec[hh].lo[t];
+                    float v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        v[i] = s0 + i <= t
+                                   ? sc[i] * (sd[i] * __builtin_amdgcn_exp2f((thi - shi[i]) + (tlo - slo[i])))
+                                   : 0.f;
+                    *reinterpret_cast<uint2*>(Ws + (hh * Q + t) * WS + s0) =
+                        make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+                }
+            }
+            __syncthreads();
+        }
+
+        // x^T of the wave's rows: tokens 32 q + 8 g + 0 .. 7 per lane
+        bf16x8 xf[kTiles][2];
+#pragma unroll
+        for (int pt = 0; pt < kTiles; ++pt)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+                xf[pt][q] = column_frag(Xs, XS, 32 * q + 8 * g, 32 * q + 8 * g + 4, pw + 16 * pt, lr);
+
+        if constexpr (!kStateOnly) {
+            f32x4 y[kTiles][4];
+#pragma unroll
+            for (int pt = 0; pt < kTiles; ++pt)
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt) y[pt][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                bf16x8 sf[kTiles];
+#pragma unroll
+                for (int pt = 0; pt < kTiles; ++pt) {
+                    const f32x4 u = S[pt][2 * k], v = S[pt][2 * k + 1];
+                    sf[pt] = frag(make_uint4(pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]),
+                                             pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])));
+                }
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt) {
+                    const uint16_t* cr = Cs + (16 * tt + lr) * NS + 32 * k + 4 * g;
+                    const uint2 c0 = *reinterpret_cast<const uint2*>(cr), c1 = *reinterpret_cast<const uint2*>(cr + 16);
+                    const bf16x8 cf = frag(make_uint4(c0.x, c0.y, c1.x, c1.y));
+#pragma unroll
+                    for (int pt = 0; pt < kTiles; ++pt) y[pt][tt] = mfma_bf16(sf[pt], cf, y[pt][tt]);
+                }
+            }
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt) {
+                const int t = 16 * tt + lr;
+                const float e = dec[hb].e[t];
+#pragma unroll
+                for (int pt = 0; pt < kTiles; ++pt) y[pt][tt] *= e;
+#pragma unroll
+                for (int q = 0; q <= tt / 2; ++q) {
+                    const bf16x8 wf = frag(*reinterpret_cast<const uint4*>(Ws + (hb * Q + t) * WS + 32 * q + 8 * g));
+#pragma unroll
+                    for (int pt = 0; pt < kTiles; ++pt) y[pt][tt] = mfma_bf16(xf[pt][q], wf, y[pt][tt]);
+                }
+#pragma unroll
+                for (int pt = 0; pt < kTiles; ++pt) {
+                    const int p = pl + 16 * pt + 4 * g;
+                    f32x4 o = y[pt][tt];
+                    if (a.D) {
+                        const uint2 xv = *reinterpret_cast<const uint2*>(Xs + t * XS + pw + 16 * pt + 4 * g);
+                        o[0] = __builtin_fmaf(skip, __uint_as_float(xv.x << 16), o[0]);
+                        o[1] = __builtin_fmaf(skip, __uint_as_float(xv.x & 0xFFFF0000u), o[1]);
+                        o[2] = __builtin_fmaf(skip, __uint_as_float(xv.y << 16), o[2]);
+                        o[3] = __builtin_fmaf(skip, __uint_as_float(xv.y & 0xFFFF0000u), o[3]);
+                    }
+                    if (t0 + t < sg.t1 && p < P)
+                        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + ((t0 + t) * H + h) * P + p) =
+                            make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+                }
+            }
+        }
+
+        if (kStateOnly || !a.segmented || t0 + Q < sg.t1) {
+            const float end = dec_end[hb];
+#pragma unroll
+            for (int pt = 0; pt < kTiles; ++pt)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) S[pt][j] *= end;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const f32x4 w0 = *reinterpret_cast<const f32x4*>(dec[hb].w + 32 * q + 8 * g);
+                const f32x4 w1 = *reinterpret_cast<const f32x4*>(dec[hb].w + 32 * q + 8 * g + 4);
+                bf16x8 hi[kTiles], lo[kTiles];
+#pragma unroll
+                for (int pt = 0; pt < kTiles; ++pt) {
+                    float v[8], r[8];
+                    unpack8(__builtin_bit_cast(uint4, xf[pt][q]), v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) r[e] = v[e] *= e < 4 ? w0[e & 3] : w1[e & 3];
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) round_bf16x2(r[e], r[e + 1]);
+                    hi[pt] = frag(pack8(r));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] -= r[e];
+                    lo[pt] = frag(pack8(v));
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const bf16x8 bf = column_frag(Bs, NS, 32 * q + 8 * g, 32 * q + 8 * g + 4, 16 * j, lr);
+#pragma unroll
+                    for (int pt = 0; pt < kTiles; ++pt) {
+                        S[pt][j] = mfma_bf16(bf, lo[pt], S[pt][j]);
+                        S[pt][j] = mfma_bf16(bf, hi[pt], S[pt][j]);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+
+    if (kStateOnly || !a.segmented) {
+        float* to = kStateOnly ? a.part + slot_state * N : a.S_out + run_state * N;
+#pragma unroll
+        for (int pt = 0; pt < kTiles; ++pt)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int p = pl + 16 * pt + lr, n = 16 * j + 4 * g;
+                if (p < P && n < N) *reinterpret_cast<f32x4*>(to + int64_t(p) * N + n) = S[pt][j];
+            }
+        if (kStateOnly && wave < kHeads && lane == 0 && unit % tiles == 0)
+            a.decay[slot * H + h0 + wave] = exp2f(float(total));
+    }
+}
+
+// The same in float32 on the float32 matrix cores, 32-token chunks: inputs of
+// any float type, every operand in full. k of a 16x16x4 product is the lane's
+// quarter g, so step (j, i) takes element 16 j + 4 g + i: a lane's four i are
+// one 16-byte read of a row, and the state's accumulators are again an operand
+// as they lie.
+template <class Act, int kNP, int kHeads, int kTiles, bool kStateOnly>
+__global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
+    constexpr int Q = 32, NS = kNP + 4, PW = 64 * kTiles, PH = PW / kHeads, XS = PW + 4, WS = Q + 4;
+    constexpr int kRowsN = kNP / 8;
+    constexpr int kLoadN = Q * kRowsN / kScanThreads > 0 ? Q * kRowsN / kScanThreads : 1;
+    constexpr int kLoadX = Q * (PW / 8) / kScanThreads;
+    constexpr int NT = kNP / 16;
+    __shared__ __attribute__((aligned(16))) float Bs[Q * NS], Cs[kStateOnly ? 4 : Q * NS], Xs[Q * XS],
+        Ws[kStateOnly ? 4 : kHeads * Q * WS];
+    __shared__ __attribute__((aligned(16))) Decays<Q> dec[kHeads];
+    __shared__ float dec_end[kHeads];
+    using St = typename Act::storage;
+
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, lr = lane & 15;
+    const int P = a.P, N = a.N, H = a.H;
+    const int tiles = (P + PH - 1) / PH, units = H / kHeads * tiles;
+    const int unit = blockIdx.x % units;
+    const int64_t slot = blockIdx.x / units;
+    const int h0 = unit / tiles * kHeads, p0 = unit % tiles * PH;
+    const int grp = h0 / (H / a.G);
+    const Segment sg = segment_of(a.cu, a.runs, a.L, a.seg, slot);
+    if (sg.run < 0) return;
+    const int hb = wave * kHeads / 4, h = h0 + hb;
+    const int pw = wave * 16 * kTiles;
+    const int pl = p0 + pw - hb * PH;
+
+    const St* xg = static_cast<const St*>(a.x);
+    const St* Bg = static_cast<const St*>(a.B) + grp * N;
+    const St* Cg = static_cast<const St*>(a.C) + grp * N;
+
+    float rb[kLoadN][8], rc[kStateOnly ? 1 : kLoadN][8], rx[kLoadX][8];
+    float rdt = 0.f;
+    const auto get = [&](const St* p, bool ok, float (&v)[8]) {
+        if (ok) {
+            load8f<Act>(p, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        }
+    };
+    const auto fetch = [&](int64_t t0) {
+#pragma unroll
+        for (int i = 0; i < kLoadN; ++i) {
+            const int at = tid + kScanThreads * i, n = at % kRowsN * 8;
+            const int64_t t = t0 + at / kRowsN;
+            const bool ok = at < Q * kRowsN && t < sg.t1 && n < N;
+            get(Bg + t * a.B_stride + n, ok, rb[i]);
+            if constexpr (!kStateOnly) get(Cg + t * a.C_stride + n, ok, rc[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kLoadX; ++i) {
+            const int at = tid + kScanThreads * i, col = at % (PW / 8) * 8;
+            const int64_t t = t0 + at / (PW / 8);
+            const int p = p0 + col % PH;
+            get(xg + t * a.x_stride + int64_t(h0 + col / PH) * P + p, t < sg.t1 && p < P, rx[i]);
+        }
+        if (wave < kHeads && lane < Q && t0 + lane < sg.t1)
+            rdt = load_any(a.dt, (t0 + lane) * a.dt_stride + h0 + wave, a.dt_dtype);
+    };
+    const auto put = [](float* p, const float (&v)[8]) {
+        *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    };
+
+    f32x4 S[kTiles][NT];
+    const int64_t slot_state = (slot * H + h) * P, run_state = (int64_t(sg.run) * H + h) * P;
+    const float* from = kStateOnly ? nullptr : a.segmented ? a.part + slot_state * N : a.S_in ? a.S_in + run_state * N : nullptr;
+#pragma unroll
+    for (int pt = 0; pt < kTiles; ++pt)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int p = pl + 16 * pt + lr, n = 16 * j + 4 * g;
+            S[pt][j] = from && p < P && n < N ? *reinterpret_cast<const f32x4*>(from + int64_t(p) * N + n)
+                                              : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    const float rate = wave < kHeads ? -expf(a.A_log[h0 + wave]) : 0.f;
+    const float dtb = wave < kHeads ? a.dt_bias[h0 + wave] : 0.f;
+    const float skip = !kStateOnly && a.D ? a.D[h] : 0.f;
+    double total = 0.0;
+
+    if (sg.t0 < sg.t1) fetch(sg.t0);
+    for (int64_t t0 = sg.t0; t0 < sg.t1; t0 += Q) {
+#pragma unroll
+        for (int i = 0; i < kLoadN; ++i) {
+            const int at = tid + kScanThreads * i, o = at / kRowsN * NS + at % kRowsN * 8;
+            if (at < Q * kRowsN) {
+                put(Bs + o, rb[i]);
+                if constexpr (!kStateOnly) put(Cs + o, rc[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kLoadX; ++i) {
+            const int at = tid + kScanThreads * i;
+            put(Xs + at / (PW / 8) * XS + at % (PW / 8) * 8, rx[i]);
+        }
+        if (wave < kHeads) {
+            const float d = lane < Q && t0 + lane < sg.t1 ? softplus(rdt + dtb) : 0.f;
+            const double end = chunk_decays<Q>(dec[wave], lane, d, rate);
+            total += end;
+            if (lane == 0) dec_end[wave] = __builtin_amdgcn_exp2f(float(end));
+        }
+        __syncthreads();
+        if (t0 + Q < sg.t1) fetch(t0 + Q);
+
+        if constexpr (!kStateOnly) {
+            // tile (tt, j) of the scores per wave: (0, 0), none, (1, 0), (1, 1)
+            const int tt = wave >> 1, j = wave & 1;
+            const int t = 16 * tt + lr, s0 = 16 * j + 4 * g;
+            f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+            if (j <= tt) {
+#pragma unroll
+                for (int k = 0; k < NT; ++k) {
+                    const f32x4 bv = *reinterpret_cast<const f32x4*>(Bs + (16 * j + lr) * NS + 16 * k + 4 * g);
+                    const f32x4 cv = *reinterpret_cast<const f32x4*>(Cs + t * NS + 16 * k + 4 * g);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[i], cv[i], sc, 0, 0, 0);
+                }
+#pragma unroll
+                for (int hh = 0; hh < kHeads; ++hh) {
+                    const float thi = dec[hh].hi[t], tlo = dec[hh].lo[t];
+                    f32x4 v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float diff = (thi - dec[hh].hi[s0 + i]) + (tlo - dec[hh].lo[s0 + i]);
+                        v[i] = s0 + i <= t ? sc[i] * (dec[hh].d[s0 + i] * __builtin_amdgcn_exp2f(diff)) : 0.f;
+                    }
+                    *reinterpret_cast<f32x4*>(Ws + (hh * Q + t) * WS + s0) = v;
+                }
+            }
+            __syncthreads();
+        }
+
+        float xf[kTiles][Q / 16][4];  // x[16 j + 4 g + i] of the lane's row
+#pragma unroll
+        for (int pt = 0; pt < kTiles; ++pt)
+#pragma unroll
+            for (int j = 0; j < Q / 16; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) xf[pt][j][i] = Xs[(16 * j + 4 * g + i) * XS + pw + 16 * pt + lr];
+
+        if constexpr (!kStateOnly) {
+            f32x4 y[kTiles][Q / 16];
+#pragma unroll
+            for (int pt = 0; pt < kTiles; ++pt)
+#pragma unroll
+                for (int tt = 0; tt < Q / 16; ++tt) y[pt][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < NT; ++k)
+#pragma unroll
+                for (int tt = 0; tt < Q / 16; ++tt) {
+                    const f32x4 cv = *reinterpret_cast<const f32x4*>(Cs + (16 * tt + lr) * NS + 16 * k + 4 * g);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int pt = 0; pt < kTiles; ++pt)
+                            y[pt][tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(S[pt][k][i], cv[i], y[pt][tt], 0, 0, 0);
+                }
+#pragma unroll
+            for (int tt = 0; tt < Q / 16; ++tt) {
+                const int t = 16 * tt + lr;
+                const float e = dec[hb].e[t];
+#pragma unroll
+                for (int pt = 0; pt < kTiles; ++pt) y[pt][tt] *= e;
+#pragma unroll
+                for (int j = 0; j <= tt; ++j) {
+                    const f32x4 wv = *reinterpret_cast<const f32x4*>(Ws + (hb * Q + t) * WS + 16 * j + 4 * g);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int pt = 0; pt < kTiles; ++pt)
+                            y[pt][tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(xf[pt][j][i], wv[i], y[pt][tt], 0, 0, 0);
+                }
+#pragma unroll
+                for (int pt = 0; pt < kTiles; ++pt) {
+                    const int p = pl + 16 * pt + 4 * g;
+                    f32x4 o = y[pt][tt];
+                    if (a.D) {
+                        const f32x4 xv = *reinterpret_cast<const f32x4*>(Xs + t * XS + pw + 16 * pt + 4 * g);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(skip, xv[i], o[i]);
+                    }
+                    if (t0 + t < sg.t1 && p < P) {
+                        const int64_t at = ((t0 + t) * H + h) * P + p;
+                        if (a.y_dtype == GDN_F32) {
+                            *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + at) = o;
+                        } else {
+                            uint16_t b[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                b[i] = a.y_dtype == GDN_BF16 ? f32_to_bf16_bits(o[i]) : f32_to_f16_bits(o[i]);
+                            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + at) =
+                                make_uint2(b[0] | uint32_t(b[1]) << 16, b[2] | uint32_t(b[3]) << 16);
+                        }
+                    }
+                }
+            }
+        }
+
+        if (kStateOnly || !a.segmented || t0 + Q < sg.t1) {
+            const float end = dec_end[hb];
+#pragma unroll
+            for (int pt = 0; pt < kTiles; ++pt)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) S[pt][j] *= end;
+#pragma unroll
+            for (int q = 0; q < Q / 16; ++q) {
+                const f32x4 w = *reinterpret_cast<const f32x4*>(dec[hb].w + 16 * q + 4 * g);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float xw[kTiles];
+#pragma unroll
+                    for (int pt = 0; pt < kTiles; ++pt) xw[pt] = xf[pt][q][i] * w[i];
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const float bv = Bs[(16 * q + 4 * g + i) * NS + 16 * j + lr];
+#pragma unroll
+                        for (int pt = 0; pt < kTiles; ++pt)
+                            S[pt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv, xw[pt], S[pt][j], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+
+    if (kStateOnly || !a.segmented) {
+        float* to = kStateOnly ? a.part + slot_state * N : a.S_out + run_state * N;
+#pragma unroll
+        for (int pt = 0; pt < kTiles; ++pt)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int p = pl + 16 * pt + lr, n = 16 * j + 4 * g;
+                if (p < P && n < N) *reinterpret_cast<f32x4*>(to + int64_t(p) * N + n) = S[pt][j];
+            }
+        if (kStateOnly && wave < kHeads && lane == 0 && unit % tiles == 0)
+            a.decay[slot * H + h0 + wave] = exp2f(float(total));
+    }
+}
+
+// Chains the segments' own sums into the state before each of them, in place,
+// and the state after the run: four values of a run's state per thread.
+__global__ __launch_bounds__(kScanThreads) void scan_chain_kernel(ScanArgs a) {
+    const int64_t per = int64_t(a.H) * a.P * a.N / 4;
+    const int64_t i = int64_t(blockIdx.x) * kScanThreads + threadIdx.x;
+    if (i >= per) return;
+    const int r = blockIdx.y + blockIdx.z * 65535;
+    if (r >= a.runs) return;
+    const int h = int(i / (int64_t(a.P) * a.N / 4));
+    const int64_t b = run_start(a.cu, a.L, r), e = run_start(a.cu, a.L, r + 1);
+    const int64_t first = b / a.seg + r, n = (e - b + a.seg - 1) / a.seg;
+    f32x4 S = {0.f, 0.f, 0.f, 0.f};
+    if (a.S_in) S = reinterpret_cast<const f32x4*>(a.S_in)[r * per + i];
+    for (int64_t k = 0; k < n; ++k) {
+        f32x4* at = reinterpret_cast<f32x4*>(a.part) + (first + k) * per + i;
+        const f32x4 own = *at;
+        *at = S;
+        S = S * a.decay[(first + k) * a.H + h] + own;
+    }
+    reinterpret_cast<f32x4*>(a.S_out)[r * per + i] = S;
+}
+
+// How a call is split: tokens a segment, and whether there are several.
+struct ScanPlan {
+    int heads, tiles;  // heads of a workgroup, 16-row tiles of a wave
+    int64_t seg, slots, units;
+    bool segmented;
+    int64_t bytes;
+};
+
+ScanPlan scan_plan(int N, int64_t T, int64_t longest, int G, int H, int P, int S) {
+    ScanPlan p;
+    const int per = H / G;
+    if (P > 64) p.heads = 1, p.tiles = 2;
+    else if (P > 32 && per % 2 == 0) p.heads = 2, p.tiles = 2;
+    else if (P > 32) p.heads = 1, p.tiles = 1;
+    else if (per % 2 == 0) p.heads = 2, p.tiles = 1;
+    else p.heads = 1, p.tiles = 1;
+    const int rows = 64 * p.tiles / p.heads;
+    p.units = int64_t(H / p.heads) * ((P + rows - 1) / rows);
+    if (longest <= 0 || longest > T) longest = T;
+    p.seg = (T * p.units / 512 + 63) / 64 * 64;
+    if (p.seg < 256) p.seg = 256;
+    p.segmented = longest > p.seg;
+    if (!p.segmented) p.seg = T + 1;
+    p.slots = T / p.seg + N;
+    p.bytes = p.segmented ? p.slots * H * (int64_t(P) * S + 4) * 4 : 0;
+    return p;
+}
+
+template <int kNP, int kHeads, int kTiles>
+void launch_scan(const ScanArgs& a, int act_dtype, bool bf16, bool state_only, dim3 grid, hipStream_t s) {
+    const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kScanThreads), 0, s, a); };
+    if (bf16) {
+        if (state_only) go(scan_bf16_kernel<kNP, kHeads, kTiles, true>);
+        else go(scan_bf16_kernel<kNP, kHeads, kTiles, false>);
+        return;
+    }
+    const auto f32 = [&](auto act) {
+        using Act = decltype(act);
+        if (state_only) go(scan_f32_kernel<Act, kNP, kHeads, kTiles, true>);
+        else go(scan_f32_kernel<Act, kNP, kHeads, kTiles, false>);
+    };
+    if (act_dtype == GDN_F32) f32(ActF32{});
+    else if (act_dtype == GDN_F16) f32(ActF16{});
+    else f32(ActBF16{});
+}
+
+template <int kNP>
+void launch_scan_shape(const ScanPlan& p, const ScanArgs& a, int act_dtype, bool bf16, bool state_only, dim3 grid,
+                       hipStream_t s) {
+    if (p.heads == 2 && p.tiles == 2) launch_scan<kNP, 2, 2>(a, act_dtype, bf16, state_only, grid, s);
+    else if (p.heads == 2) launch_scan<kNP, 2, 1>(a, act_dtype, bf16, state_only, grid, s);
+    else if (p.tiles == 2) launch_scan<kNP, 1, 2>(a, act_dtype, bf16, state_only, grid, s);
+    else launch_scan<kNP, 1, 1>(a, act_dtype, bf16, state_only, grid, s);
+}
+
+bool scan_sizes_ok(int N, int64_t T, int G, int H, int P, int S) {
+    return N >= 1 && T >= 0 && T < (int64_t(1) << 31) && G > 0 && H > 0 && H % G == 0 && P > 0 && S > 0;
+}
+
+bool scan_shape_taken(int P, int S) { return P % 8 == 0 && S % 8 == 0 && S <= 256; }
+
+}  // namespace
+}  // namespace gdn
+
+using namespace gdn;
+
+extern "C" int64_t gdn_selective_scan_workspace_size(int N, int64_t T_total, int64_t longest_run, int G, int H,
+                                                     int P, int S) {
+    if (!scan_sizes_ok(N, T_total, G, H, P, S) || !scan_shape_taken(P, S)) return 0;
+    return scan_plan(N, T_total, longest_run, G, H, P, S).bytes;
+}
+
+extern "C" int gdn_selective_scan(const void* x, int64_t x_stride, const void* B, int64_t B_stride, const void* C,
+                                  int64_t C_stride, int act_dtype, const void* dt, int64_t dt_stride, int dt_dtype,
+                                  const float* A_log, const float* dt_bias, const float* D, const float* state_in,
+                                  float* state_out, void* y, int y_dtype, const int32_t* cu_seqlens, int N,
+                                  int64_t T_total, int64_t longest_run, int G, int H, int P, int S, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+    GDN_REQUIRE(scan_sizes_ok(N, T_total, G, H, P, S), "gdn_selective_scan: bad sizes N=%d T=%lld G=%d H=%d P=%d S=%d",
+                N, (long long)T_total, G, H, P, S);
+    GDN_REQUIRE(valid_dtype(act_dtype) && valid_dtype(dt_dtype) && valid_dtype(y_dtype),
+                "gdn_selective_scan: bad dtype");
+    if (!scan_shape_taken(P, S))
+        return fail(GDN_EUNSUPPORTED,
+                    "gdn_selective_scan: head_dim and state_dim are multiples of 8, state_dim at most 256 (got %d, %d)",
+                    P, S);
+    GDN_REQUIRE(cu_seqlens || T_total % N == 0, "gdn_selective_scan: %lld tokens are not divisible into %d runs",
+                (long long)T_total, N);
+    GDN_REQUIRE(state_out && A_log && dt_bias && (T_total == 0 || (x && B && C && dt && y)),
+                "gdn_selective_scan: null pointer");
+    GDN_REQUIRE(x_stride >= int64_t(H) * P && B_stride >= int64_t(G) * S && C_stride >= int64_t(G) * S && dt_stride >= H,
+                "gdn_selective_scan: a row stride is below its row");
+    const int es = dtype_size(act_dtype);
+    const auto at = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(C) |
+                    reinterpret_cast<uintptr_t>(state_in) | reinterpret_cast<uintptr_t>(state_out) |
+                    reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(workspace);
+    GDN_REQUIRE(at % 16 == 0 && (x_stride | B_stride | C_stride) * es % 16 == 0,
+                "gdn_selective_scan: x, B, C (rows too), y, states and workspace must be 16-byte aligned");
+    const int64_t state_bytes = int64_t(N) * H * P * S * 4;
+    GDN_REQUIRE(!state_in || state_in == state_out || !overlaps(state_in, state_bytes, state_out, state_bytes),
+                "gdn_selective_scan: state_out partially overlaps state_in");
+    const ScanPlan p = scan_plan(N, T_total, longest_run, G, H, P, S);
+    GDN_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes),
+                "gdn_selective_scan: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                (long long)p.bytes);
+    GDN_REQUIRE(p.slots * p.units <= INT32_MAX, "gdn_selective_scan: too many workgroups");
+    float* part = static_cast<float*>(workspace);
+    ScanArgs a{x, B, C, dt, x_stride, B_stride, C_stride, dt_stride, dt_dtype, A_log, dt_bias, D, state_in,
+               state_out, y, y_dtype, cu_seqlens, N, T_total, T_total / N, p.seg, G, H, P, S, part,
+               part ? part + p.slots * H * int64_t(P) * S : nullptr, p.segmented};
+    const bool bf16 = act_dtype == GDN_BF16 && y_dtype == GDN_BF16;
+    hipStream_t s = as_stream(stream);
+    const dim3 grid(unsigned(p.slots * p.units));
+    const auto pass = [&](bool state_only) {
+        if (S <= 32) launch_scan_shape<32>(p, a, act_dtype, bf16, state_only, grid, s);
+        else if (S <= 64) launch_scan_shape<64>(p, a, act_dtype, bf16, state_only, grid, s);
+        else if (S <= 128) launch_scan_shape<128>(p, a, act_dtype, bf16, state_only, grid, s);
+        else launch_scan_shape<256>(p, a, act_dtype, bf16, state_only, grid, s);
+    };
+    if (p.segmented) {
+        pass(true);
+        const int64_t per = int64_t(H) * P * S / 4;
+        hipLaunchKernelGGL(scan_chain_kernel,
+                           dim3(unsigned((per + kScanThreads - 1) / kScanThreads), unsigned(N < 65535 ? N : 65535),
+                                unsigned((N + 65534) / 65535)),
+                           dim3(kScanThreads), 0, s, a);
+    }
+    pass(false);
+    return check_launch("gdn_selective_scan");
+}

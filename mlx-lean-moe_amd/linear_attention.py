@@ -32,7 +32,7 @@ from .config import LinearAttentionDims
 from .gated_delta import (PREFILL_MIN_TOKENS, _as, _c, _check_cu_seqlens, _check_out, _longest_run,
                           _require_device, _stream, _with_longest, gated_delta_update)
 from .quant import (LinearWeights, QuantScheme, concat_quantized, quantized_linear,
-                    quantized_linear_split)
+                    quantized_linear_split, stackable)
 from .recurrent_cache import RecurrentCache, RecurrentStatePool
 
 
@@ -440,7 +440,7 @@ class Qwen3_5LinearAttention:
         if len(schemes) != 1 or None in schemes:
             return None
         tensors = [t for t, _ in parts]
-        if len({t["scales"].dtype for t in tensors}) != 1:
+        if len({t["scales"].dtype for t in tensors}) != 1 or not stackable(tensors):
             return None
         return LinearWeights(concat_quantized(tensors), schemes.pop())
 

@@ -9,7 +9,10 @@ matrix or a dict ``{"weight", "scales"[, "biases"]}`` with ``weight`` uint32
 row's little-endian bit stream) and per-group ``scales`` ``(N, K /
 group_size)``. Affine schemes (2-8 bits): ``w = scales * q + biases``;
 mxfp4 / mxfp8 / nvfp4: ``w`` = the e2m1 / e4m3 code's value times a uint8
-scale (e8m0, e4m3 for nvfp4), no biases. Affine 4- and 8-bit projections of
+scale (e8m0, e4m3 for nvfp4), no biases. Beside MLX's schemes, ``fp8_block``
+holds e4m3 codes ``(N, K)`` with one float32 scale per 128 x 128 block, and its
+products take x in e4m3 too, each row's 128 columns under their own scale
+(``gdn_fp8_matmul``). Affine 4- and 8-bit projections of
 bf16 activations run on ``gdn_quantized_matmul``; the other schemes and
 activation dtypes dequantize on the GPU (``gdn_dequantize``) and multiply on
 the vendor BLAS, except that float32 rows times affine 4- and 8-bit codes run
@@ -32,6 +35,7 @@ _SUPPORTED = {
     "mxfp4": ({4}, {32}),
     "mxfp8": ({8}, {32}),
     "nvfp4": ({4}, {16}),
+    "fp8_block": ({8}, {128}),
 }
 # the mode codes of gdn_dequantize
 _MODES = {"affine": 0, "mxfp4": 1, "mxfp8": 2, "nvfp4": 3}
@@ -161,7 +165,9 @@ def _transformed(*operands: torch.Tensor | None) -> bool:
 class QuantScheme:
     """Bit width, group size and packing mode of a quantized projection;
     construction rejects the combinations MLX does not define (the checks
-    of config.py:17-33)."""
+    of config.py:17-33). ``QuantScheme(8, 128, "fp8_block")``, which MLX does
+    not have: e4m3 codes ``weight (N, K)`` (float8_e4m3fn, or uint8 bytes) and
+    ``scales (ceil(N / 128), ceil(K / 128))`` float32, K a multiple of 16."""
 
     bits: int
     group_size: int
@@ -196,9 +202,10 @@ class LinearWeights:
     dense: torch.Tensor | None = None
 
     def with_dense(self) -> "LinearWeights":
-        """These weights with their bf16 dequantization kept alongside."""
+        """These weights with their bf16 dequantization kept alongside (not
+        those of fp8_block, whose products never run on dequantized weights)."""
 
-        if self.quant is None:
+        if self.quant is None or self.quant.mode == "fp8_block":
             return self
         return LinearWeights(self.tensors, self.quant, dequantize(self.tensors, self.quant, torch.bfloat16))
 
@@ -220,7 +227,28 @@ def _scheme_kernel_takes(x: torch.Tensor, rows: int, K: int, quant: QuantScheme)
             and groups <= (128 if quant.mode == "affine" else 256))
 
 
+def _check_fp8_block(tensors: dict, K: int | None):
+    w, scales = tensors["weight"], tensors["scales"]
+    if tensors.get("biases") is not None:
+        raise ValueError("fp8_block weights carry no biases")
+    if w.dtype not in (torch.float8_e4m3fn, torch.uint8) or w.dim() != 2:
+        raise ValueError("fp8_block weight must be a 2-D float8_e4m3fn (or uint8) tensor")
+    N, k = w.shape
+    if K is not None and K != k:
+        raise ValueError(f"input width {K} does not match the weight's {k}")
+    if N == 0 or k == 0 or k % 16:
+        raise ValueError(f"an fp8_block weight has rows of a nonzero multiple of 16 codes, got {(N, k)}")
+    if tuple(scales.shape) != (-(-N // 128), -(-k // 128)) or scales.dtype != torch.float32:
+        raise ValueError(f"fp8_block scales must be float32 of shape {(-(-N // 128), -(-k // 128))}, got "
+                         f"{tuple(scales.shape)} {scales.dtype}")
+    if scales.device != w.device:
+        raise ValueError(f"weight is on {w.device}, its scales on {scales.device}")
+    return w, scales, None, N, k
+
+
 def _check_quantized(tensors: dict, quant: QuantScheme, K: int | None):
+    if quant.mode == "fp8_block":
+        return _check_fp8_block(tensors, K)
     w, scales = tensors["weight"], tensors["scales"]
     biases = tensors.get("biases")
     affine = quant.mode == "affine"
@@ -266,6 +294,10 @@ def dequantize(tensors: dict, quant: QuantScheme, dtype: torch.dtype | None = No
     w, scales = _c(w), _c(scales)
     if w.data_ptr() % 16:
         w = w.clone()
+    if quant.mode == "fp8_block":
+        _lib.call_on(w.device, "gdn_fp8_dequantize", _lib.ptr(w), _lib.ptr(scales), _lib.ptr(out),
+                     _lib.dtype_code(dtype), N, K, _lib.stream_ptr(w.device))
+        return out
     biases = _c(biases) if biases is not None else None
     sb_dtype = _lib.dtype_code(scales.dtype) if quant.mode == "affine" else 0
     _lib.call("gdn_dequantize", _lib.ptr(w), _lib.ptr(scales), _lib.ptr(biases), sb_dtype,
@@ -323,6 +355,8 @@ def quantized_linear(x: torch.Tensor, tensors, quant: QuantScheme | None = None,
     w, scales, biases, N, K = _check_quantized(tensors, quant, x.shape[-1])
     if x.device.type != "cuda":
         raise RuntimeError(f"quantized projections run on ROCm devices only; got {x.device}")
+    if quant.mode == "fp8_block":
+        return _fp8_matmul(x, w, scales, N, K, residual)
     lead = x.shape[:-1]
     rows = x.reshape(-1, K).shape[0]
     if not _on_kernels(quant):
@@ -402,6 +436,33 @@ def _scheme_matmul(x, w, scales, biases, quant: QuantScheme, N: int, K: int, res
     return y.reshape(*lead, N)
 
 
+def _fp8_matmul(x, w, scales, N: int, K: int, residual):
+    """``x @ W.T`` (+ residual) for fp8_block weights (gdn_fp8_matmul): x's
+    rows quantized to e4m3 per 128 columns, float32 sums."""
+
+    if _transformed(x, residual):
+        raise RuntimeError("fp8_block products have no gradient and no function transform; call them under "
+                           "torch.no_grad()")
+    if w.device != x.device:
+        raise ValueError(f"x is on {x.device}, the weights on {w.device}")
+    lead = x.shape[:-1]
+    x2 = _c(x.reshape(-1, K))
+    if x2.data_ptr() % 16:
+        x2 = x2.clone()
+    M = x2.shape[0]
+    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    r = _residual_rows(residual, x, lead, M, N)
+    w, scales = _c(w), _c(scales)
+    if w.data_ptr() % 16:
+        w = w.clone()
+    ws_bytes = fp8_workspace_bytes(M, N, K)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+    code = _lib.dtype_code(x.dtype)
+    _lib.call_on(x.device, "gdn_fp8_matmul", x2.data_ptr(), code, w.data_ptr(), scales.data_ptr(), y.data_ptr(), code,
+                 _lib.ptr(r), M, N, K, ws.data_ptr(), ws_bytes, _lib.stream_ptr(x.device))
+    return y.reshape(*lead, N)
+
+
 def _f32_matmul(x, w, scales, biases, quant: QuantScheme, N: int, K: int, residual):
     """``x @ W.T`` (+ residual) for float32 rows beyond the decode kernel's
     and affine 4- or 8-bit codes (gdn_quantized_matmul_f32): exact weights
@@ -451,7 +512,7 @@ def quantized_linear_split(x: torch.Tensor, weights: LinearWeights, sizes) -> li
     K = x.shape[-1]
     rows = x.reshape(-1, K).shape[0]
     if (x.dtype == torch.bfloat16 and x.device.type == "cuda"
-            and (_on_kernels(quant) and _runs_dense(rows, tensors["weight"].shape[0], K, quant, tensors["scales"].dtype, x,
+            and quant.mode != "fp8_block" and (_on_kernels(quant) and _runs_dense(rows, tensors["weight"].shape[0], K, quant, tensors["scales"].dtype, x,
                                                     kept=weights.dense is not None)
                  or not (_on_kernels(quant) or _scheme_kernel_takes(x, rows, K, quant)))):
         _check_quantized(tensors, quant, K)
@@ -479,6 +540,13 @@ def scheme_workspace_bytes(M: int, N: int, K: int) -> int:
 
 
 @functools.lru_cache(maxsize=256)
+def fp8_workspace_bytes(M: int, N: int, K: int) -> int:
+    """Workspace of gdn_fp8_matmul."""
+
+    return int(_lib.load().gdn_fp8_matmul_workspace_size(M, N, K))
+
+
+@functools.lru_cache(maxsize=256)
 def f32_workspace_bytes(M: int, N: int, K: int, bits: int, group_size: int) -> int:
     """Workspace of gdn_quantized_matmul_f32 (0: sizes it does not take)."""
 
@@ -498,9 +566,22 @@ def workspace_bytes(x_dtype: torch.dtype, sb_dtype: torch.dtype, M: int, N: int,
         _lib.dtype_code(x_dtype), _lib.dtype_code(sb_dtype), M, N, K, bits, group_size))
 
 
+def stackable(parts: list[dict]) -> bool:
+    """Whether the parts' scales stay in place when their rows are stacked:
+    one row of scales per row of codes, or (fp8_block) one per 128 rows of
+    which every part but the last has a multiple."""
+
+    return all(p["weight"].dtype not in (torch.float8_e4m3fn, torch.uint8) or p["weight"].shape[0] % 128 == 0
+               for p in parts[:-1])
+
+
 def concat_quantized(parts: list[dict]) -> dict:
     """Stacks quantized projections that share an input (same K, scheme and
-    scales dtype) along N, so that one launch computes all of them."""
+    scales dtype) along N, so that one launch computes all of them. fp8_block
+    parts stack only where each but the last ends with a block of 128 rows
+    (:func:`stackable`)."""
 
+    if not stackable(parts):
+        raise ValueError("fp8_block projections stack only in whole blocks of 128 rows")
     keys = [k for k in ("weight", "scales", "biases") if k in parts[0]]
     return {key: torch.cat([p[key] for p in parts], dim=0) for key in keys}

@@ -146,6 +146,8 @@ class CheckpointReader:
         raw = os.pread(self._fd(span.shard), span.nbytes, span.begin)
         if len(raw) != span.nbytes:
             raise ValueError(f"{name}: shard {span.shard} is truncated")
+        if span.dtype == "F8_E4M3":  # fp8_block codes, which the reference's decoding does not know
+            return decode_tensor(raw, "U8", span.shape).view(torch.float8_e4m3fn)
         return decode_tensor(raw, span.dtype, span.shape, stored_width=is_quant_metadata(name))
 
     def read_fields(self, name: str, fields) -> dict[str, torch.Tensor]:
@@ -204,10 +206,17 @@ def projection_is_quantized(index: dict[str, TensorSpan], name: str, scheme: Qua
             problems.append(f"the {scheme.mode} scheme has no biases; some are stored")
         elif biases is not None and biases.shape != scales.shape:
             problems.append(f"biases {biases.shape} and scales {scales.shape} differ in shape")
-        if weight.shape[:-1] != scales.shape[:-1]:
+        if scheme.mode == "fp8_block":
+            blocks = tuple(-(-n // 128) for n in weight.shape)
+            if weight.dtype not in ("F8_E4M3", "U8") or scales.dtype != "F32" or scales.shape != blocks:
+                problems.append(f"fp8_block keeps 8-bit codes and F32 scales of shape {blocks}; stored are "
+                                f"{weight.dtype} {weight.shape} and {scales.dtype} {scales.shape}")
+            words = weight.shape[-1]
+        elif weight.shape[:-1] != scales.shape[:-1]:
             problems.append(f"weight {weight.shape} and scales {scales.shape} differ in their "
                             f"leading dimensions")
-        words = scales.shape[-1] * scheme.group_size * scheme.bits // 32
+        if scheme.mode != "fp8_block":
+            words = scales.shape[-1] * scheme.group_size * scheme.bits // 32
         if weight.shape[-1] != words:
             problems.append(f"{scales.shape[-1]} groups of {scheme.group_size} {scheme.bits}-bit "
                             f"codes pack into {words} words a row; weight {weight.shape} has "
