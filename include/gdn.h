@@ -549,7 +549,7 @@ int gdn_selective_step(const void *xbc, int64_t xbc_stride, const void *dt, int6
  * x makes its row NaN. No reference counterpart (a scheme beside
  * moe_block.py:44-55's).
  */
-int64_t gdn_fp8_matmul_workspace_size(int M, int N, int K);
+int64_t gdn_fp8_matmul_workspace_size(int y_dtype, int M, int N, int K);
 int gdn_fp8_matmul(const void *x, int x_dtype, const void *w, const float *scales, void *y, int y_dtype,
                    const void *residual, int M, int N, int K, void *workspace, int64_t workspace_bytes,
                    void *stream);

@@ -104,7 +104,7 @@ _SIGNATURES = {
                            + [_c_int] * 8 + [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p]),
     "gdn_fp8_matmul": (_c_int, [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int,
                                 _c_int, _c_int, _c_void_p, _c_i64, _c_void_p]),
-    "gdn_fp8_matmul_workspace_size": (_c_i64, [_c_int, _c_int, _c_int]),
+    "gdn_fp8_matmul_workspace_size": (_c_i64, [_c_int, _c_int, _c_int, _c_int]),
     "gdn_fp8_dequantize": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p]),
 }
 

@@ -41,12 +41,12 @@ GDN_DEV uint32_t codes4(float a, float b, float c, float d) {
     return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true));
 }
 
-// Rows' codes (M x kb * 128, columns past K zero) and scales (kb x M): 16 lanes
+// Rows' codes (M x kb * 128, columns past K zero) and scales (kb x ldx): 16 lanes
 // a group of 128, 8 values a lane.
 template <class Act>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(const typename Act::storage* __restrict__ x, int M, int K,
                                                            int kb, uint8_t* __restrict__ codes,
-                                                           float* __restrict__ scales) {
+                                                           float* __restrict__ scales, int ldx) {
     const int64_t groups = int64_t(M) * kb;
     const int64_t first = int64_t(blockIdx.x) * 16 + threadIdx.x / 16;
     const int64_t gi = first < groups ? first : groups - 1;
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const typename Act::s
     if (first >= groups) return;
     *reinterpret_cast<uint2*>(codes + int64_t(m) * kb * kB + k) =
         make_uint2(codes4(v[0], v[1], v[2], v[3]), codes4(v[4], v[5], v[6], v[7]));
-    if ((threadIdx.x & 15) == 0) scales[int64_t(b) * M + m] = s;
+    if ((threadIdx.x & 15) == 0) scales[int64_t(b) * ldx + m] = s;
 }
 
 struct Fp8Args {
@@ -71,6 +71,10 @@ struct Fp8Args {
     const void* residual;
     void* y;
     int y_dtype, M, N, K, kb;
+    int ldx;      // columns of sx, a multiple of 256
+    int steps;    // blocks of K a workgroup takes
+    float* part;  // split K: (splits, M, N4) float32, else null
+    int N4;       // N rounded up to 4
 };
 
 GDN_DEV f32x4 mfma_fp8(uint4 a0, uint4 a1, uint4 b0, uint4 b1) {
@@ -135,26 +139,201 @@ GDN_DEV void store4(const Fp8Args& a, int m, int n, f32x4 v) {
         }
 }
 
-// One wave per 16 rows of W and 16 rows of x, operands straight from memory.
-template <bool kExact>
-__global__ __launch_bounds__(64) void fp8_simple_kernel(Fp8Args a) {
-    const int lane = threadIdx.x, g = lane >> 4, lr = lane & 15;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
-    const int n = min(n0 + lr, a.N - 1), m = min(m0 + lr, a.M - 1);
-    const uint8_t* wr = a.w + int64_t(n) * a.K;
-    const uint8_t* qr = a.q + int64_t(m) * a.kb * kB;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int b = 0; b < a.kb; ++b) {
-        const int k = b * kB + 32 * g;
-        const uint4 w0 = k < a.K ? *reinterpret_cast<const uint4*>(wr + k) : zero;
-        const uint4 w1 = k + 16 < a.K ? *reinterpret_cast<const uint4*>(wr + k + 16) : zero;
-        const uint4 q0 = *reinterpret_cast<const uint4*>(qr + k), q1 = *reinterpret_cast<const uint4*>(qr + k + 16);
-        const f32x4 p = kExact ? mfma_widened(w0, w1, q0, q1) : mfma_fp8(w0, w1, q0, q1);
-        const float s = a.sx[int64_t(b) * a.M + m] * a.sw[int64_t(n0 / kB) * a.kb + b];
-        acc += s * p;
+typedef __attribute__((address_space(3))) void lds_void;
+
+// `rows` rows of `width` bytes as a buffer; what lies beyond reads as zero.
+GDN_DEV __amdgpu_buffer_rsrc_t byte_rows(const uint8_t* base, int rows, int width) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, rows * width, 0x00027000);
+}
+
+// A tile of TN rows of W by TM rows of x, kWN x kWM waves, one 128-column block
+// of both a step. The blocks go from memory to LDS without passing registers,
+// into one of two buffers while the other is multiplied. A row's 128 bytes are
+// eight 16-byte pieces, piece c of row r at place c ^ (r % 8): the DMA writes
+// places in order, so a lane fetches the piece that belongs at its place, and
+// the 16 rows of an operand read fall on all banks. Which columns a lane holds
+// does not matter inside a block as long as both operands agree: pieces g and
+// g + 4 of its row.
+//
+// W is the left operand, so a lane's column is one row of x: its scale is one
+// value per 16 rows, times W's scale once a step, and each product of a block
+// costs four multiply-adds to add.
+template <int TN, int TM, int kWN, int kWM, bool kExact>
+__global__ __launch_bounds__(64 * kWN * kWM) void fp8_tile_kernel(Fp8Args a) {
+    constexpr int kWaves = kWN * kWM, RN = TN / (16 * kWN), RM = TM / (16 * kWM);
+    constexpr int kScales = (TN + TM) * kB, kBytes = kScales + 1024, kLoadsW = TN / 8 / kWaves, kLoadsQ = TM / 8 / kWaves;
+    static_assert(TN % (8 * kWaves) == 0 && TM % (8 * kWaves) == 0 && (TN % kB == 0 || kB % TN == 0) && kB % (16 * RN) == 0, "tile");
+    __shared__ __attribute__((aligned(1024))) uint8_t buf0[kBytes], buf1[kBytes];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int g = lane >> 4, lr = lane & 15;
+    const int wn = wave / kWM * (16 * RN), wm = wave % kWM * (16 * RM);
+
+    // consecutive workgroups go to the 8 dies in turn: each die takes a
+    // contiguous share of the tiles, in which neighbours share rows of W
+    const int tiles_m = (a.M + TM - 1) / TM, tiles = tiles_m * ((a.N + TN - 1) / TN);
+    const int share = tiles / 8, rest = tiles % 8, die = blockIdx.x % 8;
+    const int tile = die * share + min(die, rest) + blockIdx.x / 8;
+    const int n0 = tile / tiles_m * TN, m0 = tile % tiles_m * TM;
+    const int b0 = blockIdx.y * a.steps, b1 = min(a.kb, b0 + a.steps);
+
+    const int Kq = a.kb * kB;
+    const auto wr = byte_rows(a.w + int64_t(n0) * a.K, min(TN, a.N - n0), a.K);
+    const auto qr = byte_rows(a.q + int64_t(m0) * Kq, min(TM, a.M - m0), Kq);
+    const auto xr = byte_rows(reinterpret_cast<const uint8_t*>(a.sx + m0), 1, a.kb * a.ldx * 4 - m0 * 4);
+    // The lane's piece of a matrix's first 8 rows of this wave's share; 8 rows
+    // on it is the same piece (r % 8 is the lane's). Rows past the last repeat it.
+    const int r8 = lane >> 3, c16 = ((lane & 7) ^ r8) * 16;
+    const int w_at = (wave * kLoadsW * 8 + r8) * a.K + c16, w_last = (min(TN, a.N - n0) - 1) * a.K + c16;
+    const int q_at = (wave * kLoadsQ * 8 + r8) * Kq + c16, q_last = (min(TM, a.M - m0) - 1) * Kq + c16;
+    const auto fetch = [&](uint8_t* buf, int b) {
+        // W's last block may be short: pieces beyond it are placed past the
+        // buffer's end, which reads as zero (q's rows are padded)
+        const int past = b * kB + c16 >= a.K ? 0x7FFFFF00 : 0;
+        int wa = w_at, qa = q_at;
+        asm volatile("" : "+v"(wa), "+v"(qa));  // (places formed here, not kept in registers across steps)
+#pragma unroll
+        for (int i = 0; i < kLoadsW; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void*)(buf + (wave * kLoadsW + i) * 1024), 16,
+                                                     max(min(wa + i * 8 * a.K, w_last), past), b * kB, 0, 0);
+#pragma unroll
+        for (int i = 0; i < kLoadsQ; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(qr, (lds_void*)(buf + TN * kB + (wave * kLoadsQ + i) * 1024), 16,
+                                                     min(qa + i * 8 * Kq, q_last), b * kB, 0, 0);
+        if (wave == 0)  // the rows' scales of this block
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_void*)(buf + kScales), 16, lane * 16, b * a.ldx * 4, 0, 0);
+    };
+    const float* sw = a.sw + int64_t(min(n0 + wn, a.N - 1) / kB) * a.kb;
+
+    f32x4 acc[RN][RM];
+#pragma unroll
+    for (int i = 0; i < RN; ++i)
+#pragma unroll
+        for (int j = 0; j < RM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // the lane's two pieces of a row r with r % 16 = lr
+    const int at0 = lr * kB + ((g ^ (lr & 7)) << 4), at1 = at0 ^ 64;
+    const auto multiply = [&](const uint8_t* buf, float sn) {
+        const uint8_t* wb = buf + wn * kB;
+        const uint8_t* qb = buf + (TN + wm) * kB;
+        uint4 q[RM][2], w[2][2];
+        float s[RM];
+        w[0][0] = *reinterpret_cast<const uint4*>(wb + at0);
+        w[0][1] = *reinterpret_cast<const uint4*>(wb + at1);
+#pragma unroll
+        for (int j = 0; j < RM; ++j) {
+            q[j][0] = *reinterpret_cast<const uint4*>(qb + 16 * j * kB + at0);
+            q[j][1] = *reinterpret_cast<const uint4*>(qb + 16 * j * kB + at1);
+            s[j] = sn * *reinterpret_cast<const float*>(buf + kScales + (wm + 16 * j + lr) * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < RN; ++i) {
+            if (i + 1 < RN) {  // the next rows of W, while these are multiplied
+                w[(i + 1) & 1][0] = *reinterpret_cast<const uint4*>(wb + 16 * (i + 1) * kB + at0);
+                w[(i + 1) & 1][1] = *reinterpret_cast<const uint4*>(wb + 16 * (i + 1) * kB + at1);
+            }
+            f32x4 p[RM];
+#pragma unroll
+            for (int j = 0; j < RM; ++j)
+                p[j] = kExact ? mfma_widened(w[i & 1][0], w[i & 1][1], q[j][0], q[j][1])
+                              : mfma_fp8(w[i & 1][0], w[i & 1][1], q[j][0], q[j][1]);
+#pragma unroll
+            for (int j = 0; j < RM; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(s[j], p[j][e], acc[i][j][e]);
+            // products and sums stay here and the later rows' reads below: no
+            // more rows of W in registers than two
+#pragma unroll
+            for (int j = 0; j < RM; ++j) asm volatile("" : "+v"(acc[i][j])::"memory");
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    const auto step = [&](uint8_t* cur, uint8_t* next, int b) {
+        const float sn = sw[b];
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's pieces are in LDS
+        __syncthreads();
+        if (b + 1 < b1) fetch(next, b + 1);
+        multiply(cur, sn);
+    };
+    fetch(buf0, b0);
+    for (int b = b0; b < b1; b += 2) {
+        step(buf0, buf1, b);
+        if (b + 1 < b1) step(buf1, buf0, b + 1);
     }
-    store4(a, m0 + lr, n0 + 4 * g, acc);
+    if (kExact || a.part) {
+#pragma unroll
+        for (int i = 0; i < RN; ++i)
+#pragma unroll
+            for (int j = 0; j < RM; ++j) {
+                const int n = n0 + wn + 16 * i + 4 * g, m = m0 + wm + 16 * j + lr;
+                if (!a.part)
+                    store4(a, m, n, acc[i][j]);
+                else if (m < a.M && n < a.N4)
+                    *reinterpret_cast<f32x4*>(a.part + (int64_t(blockIdx.y) * a.M + m) * a.N4 + n) = acc[i][j];
+            }
+        return;
+    }
+    // 16-bit results: a wave's rows of x lie 16 apart in its lanes, four columns
+    // each, and stored like that would write 32 bytes of a line at a time. They
+    // are turned round through the wave's share of LDS (8 values a piece, piece
+    // c of row m at place c ^ m) and leave as whole rows.
+    constexpr int kPieces = 2 * RN, kShare = 512 * RN * RM;
+    static_assert(kShare * kWaves / 2 <= kBytes || kWaves == 1, "a wave's results fit its share of LDS");
+    __syncthreads();
+    uint8_t* own = (wave < kWaves / 2 ? buf0 : buf1) + wave % (kWaves / 2) * kShare;
+#pragma unroll
+    for (int i = 0; i < RN; ++i)
+#pragma unroll
+        for (int j = 0; j < RM; ++j) {
+            const int m = 16 * j + lr, c = (2 * i + (g >> 1)) ^ (m & (kPieces - 1));
+            const f32x4 v = acc[i][j];
+            const uint2 o = a.y_dtype == GDN_BF16
+                                ? make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]))
+                                : make_uint2(f32_to_f16_bits(v[0]) | uint32_t(f32_to_f16_bits(v[1])) << 16,
+                                             f32_to_f16_bits(v[2]) | uint32_t(f32_to_f16_bits(v[3])) << 16);
+            *reinterpret_cast<uint2*>(own + (m * kPieces + c) * 16 + (g & 1) * 8) = o;
+        }
+    // (a wave reads only what it wrote itself: no barrier)
+    for (int p = lane; p < 16 * RM * kPieces; p += 64) {
+        const int row = p / kPieces, c = p % kPieces;
+        const int m = m0 + wm + row, n = n0 + wn + 8 * c;
+        uint4 v = *reinterpret_cast<const uint4*>(own + (row * kPieces + (c ^ (row & (kPieces - 1)))) * 16);
+        if (m >= a.M || n >= a.N) continue;
+        const int64_t at = int64_t(m) * a.N + n;
+        uint16_t* y = static_cast<uint16_t*>(a.y) + at;
+        if (a.N % 8 == 0 && !a.residual) {
+            *reinterpret_cast<uint4*>(y) = v;
+            continue;
+        }
+        uint16_t e[8];
+        __builtin_memcpy(e, &v, 16);
+        const int count = min(8, a.N - n);
+        if (a.residual) {
+            const uint16_t* r = static_cast<const uint16_t*>(a.residual) + at;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < count) {
+                    const float sum = a.y_dtype == GDN_BF16 ? bf16_bits_to_f32(e[k]) + bf16_bits_to_f32(r[k])
+                                                            : f16_bits_to_f32(e[k]) + f16_bits_to_f32(r[k]);
+                    e[k] = a.y_dtype == GDN_BF16 ? f32_to_bf16_bits(sum) : f32_to_f16_bits(sum);
+                }
+        }
+        if (a.N % 8 == 0) {
+            __builtin_memcpy(&v, e, 16);
+            *reinterpret_cast<uint4*>(y) = v;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < count) y[k] = e[k];
+        }
+    }
+}
+
+// Adds the shares of a split product in their order: four columns a thread.
+__global__ __launch_bounds__(256) void fp8_sum_kernel(Fp8Args a, int splits) {
+    const int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4, per = int64_t(a.M) * a.N4;
+    if (i >= per) return;
+    f32x4 v = *reinterpret_cast<const f32x4*>(a.part + i);
+    for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(a.part + s * per + i);
+    store4(a, int(i / a.N4), int(i % a.N4), v);
 }
 
 // The dense weights: code times its block's scale, one rounding. 16 codes a
@@ -177,10 +356,85 @@ __global__ __launch_bounds__(256) void fp8_dequantize_kernel(const uint8_t* __re
     }
 }
 
+template <int TN, int TM, int kWN, int kWM, bool kExact>
+void launch_tiles(const Fp8Args& a, int splits, hipStream_t s) {
+    const dim3 grid(unsigned(((a.N + TN - 1) / TN) * ((a.M + TM - 1) / TM)), unsigned(splits));
+    hipLaunchKernelGGL((fp8_tile_kernel<TN, TM, kWN, kWM, kExact>), grid, dim3(64 * kWN * kWM), 0, s, a);
+}
+
+// The tiles of a product and how many shares of K it is cut into.
+//
+// What a tile costs was measured over 1 to 4096 rows of 64 to 12352 outputs, K
+// 1024 to 8192: a start and an end, and a time per block of K that grows with
+// the workgroups on the CU (memory's latency for the small tiles, the matrix
+// cores and LDS for the large ones). From that the time of each choice: rounds
+// of 256 CUs with so many workgroups each; a split adds a second launch and
+// its partial sums' way through memory. Figures (us, measured; 16-bit results,
+// 2048 -> 12352): 65 rows 12.5 (64 x 64) against 31 (256 x 256), 512 rows 21.8
+// (128 x 256), 28.0, 32.3; 1024 rows 34 (256 x 256), 39, 49; 4096 -> 2048 at
+// 200 rows 17.5 (64 x 64), 14.0 split in two, 36 (128 x 256).
+struct Fp8Tiles {
+    int tn, tm, per_cu;
+    float step1, more, ends;  // us a block of K at one workgroup a CU, for each further one, and apart from the blocks
+};
+constexpr Fp8Tiles kTiles16[] = {{64, 32, 6, .35f, .12f, 2.5f}, {64, 64, 4, .45f, .15f, 3.f}, {128, 256, 1, .87f, 0.f, 7.f},
+                                 {256, 256, 1, 1.65f, 0.f, 8.f}};
+constexpr Fp8Tiles kTilesExact[] = {{64, 32, 6, .43f, .12f, 2.5f}, {64, 64, 4, .53f, .27f, 3.f}, {128, 128, 2, 1.25f, .55f, 5.f}};
+constexpr int kMaxSplits = 8;
+
+struct Fp8Plan {
+    int kind, splits, steps;
+    int64_t part_bytes;
+};
+
+Fp8Plan fp8_plan(bool exact, int M, int N, int kb) {
+    Fp8Plan best{0, 1, kb, 0};
+    float best_us = 1e30f;
+    const int kinds = exact ? 3 : 4;
+    for (int k = 0; k < kinds; ++k) {
+        const Fp8Tiles& t = exact ? kTilesExact[k] : kTiles16[k];
+        const int64_t tiles = ((int64_t(N) + t.tn - 1) / t.tn) * ((int64_t(M) + t.tm - 1) / t.tm);
+        for (int splits = 1; splits <= kMaxSplits && splits * 2 <= kb + 1; splits *= 2) {
+            const int steps = (kb + splits - 1) / splits;
+            const int64_t load = (tiles * splits + 255) / 256, full = load / t.per_cu;
+            const int rest = int(load % t.per_cu);
+            const auto round_us = [&](int n) { return n ? steps * (t.step1 + t.more * (n - 1)) + t.ends : 0.f; };
+            float us = full * round_us(t.per_cu) + round_us(rest);
+            if (splits > 1) us += 2.5f + 8e-6f / 4 * splits * float(M) * float(N);
+            if (us < best_us) {
+                best_us = us;
+                best = {k, splits, steps, splits > 1 ? int64_t(splits) * M * ((int64_t(N) + 3) / 4 * 4) * 4 : 0};
+            }
+        }
+    }
+    best.splits = (kb + best.steps - 1) / best.steps;  // (no share without a block)
+    return best;
+}
+
+void launch_product(const Fp8Plan& p, const Fp8Args& a, hipStream_t s) {
+    if (a.y_dtype == GDN_F32) {
+        if (p.kind == 0) launch_tiles<64, 32, 2, 2, true>(a, p.splits, s);
+        else if (p.kind == 1) launch_tiles<64, 64, 2, 2, true>(a, p.splits, s);
+        else launch_tiles<128, 128, 2, 2, true>(a, p.splits, s);
+    } else {
+        if (p.kind == 0) launch_tiles<64, 32, 2, 2, false>(a, p.splits, s);
+        else if (p.kind == 1) launch_tiles<64, 64, 2, 2, false>(a, p.splits, s);
+        else if (p.kind == 2) launch_tiles<128, 256, 2, 4, false>(a, p.splits, s);
+        else launch_tiles<256, 256, 2, 4, false>(a, p.splits, s);
+    }
+    if (a.part)
+        hipLaunchKernelGGL(fp8_sum_kernel, dim3(unsigned((int64_t(a.M) * a.N4 / 4 + 255) / 256)), dim3(256), 0, s, a,
+                           p.splits);
+}
+
 int64_t codes_bytes(int M, int K) { return (int64_t(M) * ((K + kB - 1) / kB) * kB + 255) / 256 * 256; }
 
+// (a tile's 256 scales are one aligned kilobyte)
+int scale_columns(int M) { return (M + 255) / 256 * 256; }
+
+// (K: a tile's rows are addressed in 31 bits)
 bool fp8_sizes_ok(int M, int N, int K) {
-    return M >= 0 && N > 0 && K > 0 && K % 16 == 0 && K <= INT32_MAX - kB && N <= INT32_MAX - 256 && M <= INT32_MAX - 256;
+    return M >= 0 && N > 0 && K > 0 && K % 16 == 0 && K <= (1 << 22) && N <= INT32_MAX - 256 && M <= INT32_MAX - 256;
 }
 
 }  // namespace
@@ -188,9 +442,10 @@ bool fp8_sizes_ok(int M, int N, int K) {
 
 using namespace gdn;
 
-extern "C" int64_t gdn_fp8_matmul_workspace_size(int M, int N, int K) {
-    if (!fp8_sizes_ok(M, N, K)) return 0;
-    return codes_bytes(M, K) + int64_t(M) * ((K + kB - 1) / kB) * 4;
+extern "C" int64_t gdn_fp8_matmul_workspace_size(int y_dtype, int M, int N, int K) {
+    if (!fp8_sizes_ok(M, N, K) || !valid_dtype(y_dtype)) return 0;
+    const int kb = (K + kB - 1) / kB;
+    return codes_bytes(M, K) + int64_t(scale_columns(M)) * kb * 4 + fp8_plan(y_dtype == GDN_F32, M, N, kb).part_bytes;
 }
 
 extern "C" int gdn_fp8_matmul(const void* x, int x_dtype, const void* w, const float* scales, void* y, int y_dtype,
@@ -203,25 +458,27 @@ extern "C" int gdn_fp8_matmul(const void* x, int x_dtype, const void* w, const f
     GDN_REQUIRE((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(y) |
                  reinterpret_cast<uintptr_t>(workspace)) % 16 == 0,
                 "gdn_fp8_matmul: x, w, y and workspace must be 16-byte aligned");
-    const int64_t need = gdn_fp8_matmul_workspace_size(M, N, K);
+    const int64_t need = gdn_fp8_matmul_workspace_size(y_dtype, M, N, K);
     GDN_REQUIRE(workspace && workspace_bytes >= need, "gdn_fp8_matmul: workspace of %lld bytes, %lld needed",
                 (long long)workspace_bytes, (long long)need);
-    const int kb = (K + kB - 1) / kB;
+    const int kb = (K + kB - 1) / kB, ldx = scale_columns(M);
     const int64_t blocks = (int64_t(M) * kb + 15) / 16;
-    GDN_REQUIRE(blocks <= INT32_MAX && (M + 15) / 16 <= 65535, "gdn_fp8_matmul: too many rows");
+    GDN_REQUIRE(blocks <= INT32_MAX && int64_t(ldx) * kb <= INT32_MAX / 4, "gdn_fp8_matmul: too many rows");
     uint8_t* codes = static_cast<uint8_t*>(workspace);
     float* sx = reinterpret_cast<float*>(codes + codes_bytes(M, K));
     hipStream_t s = as_stream(stream);
     const auto quantize = [&](auto act) {
         using Act = decltype(act);
         hipLaunchKernelGGL(fp8_quantize_kernel<Act>, dim3(unsigned(blocks)), dim3(256), 0, s,
-                           static_cast<const typename Act::storage*>(x), M, K, kb, codes, sx);
+                           static_cast<const typename Act::storage*>(x), M, K, kb, codes, sx, ldx);
     };
     if (x_dtype == GDN_F32) quantize(ActF32{});
     else if (x_dtype == GDN_BF16) quantize(ActBF16{});
     else quantize(ActF16{});
-    const Fp8Args a{codes, static_cast<const uint8_t*>(w), sx, scales, residual, y, y_dtype, M, N, K, kb};
-    hipLaunchKernelGGL(y_dtype == GDN_F32 ? fp8_simple_kernel<true> : fp8_simple_kernel<false>, dim3(unsigned((N + 15) / 16), unsigned((M + 15) / 16)), dim3(64), 0, s, a);
+    const Fp8Plan p = fp8_plan(y_dtype == GDN_F32, M, N, kb);
+    float* part = p.splits > 1 ? sx + int64_t(ldx) * kb : nullptr;
+    launch_product(p, {codes, static_cast<const uint8_t*>(w), sx, scales, residual, y, y_dtype, M, N, K, kb, ldx,
+                       p.steps, part, (N + 3) / 4 * 4}, s);
     return check_launch("gdn_fp8_matmul");
 }
 

@@ -455,9 +455,9 @@ def _fp8_matmul(x, w, scales, N: int, K: int, residual):
     w, scales = _c(w), _c(scales)
     if w.data_ptr() % 16:
         w = w.clone()
-    ws_bytes = fp8_workspace_bytes(M, N, K)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
     code = _lib.dtype_code(x.dtype)
+    ws_bytes = fp8_workspace_bytes(code, M, N, K)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
     _lib.call_on(x.device, "gdn_fp8_matmul", x2.data_ptr(), code, w.data_ptr(), scales.data_ptr(), y.data_ptr(), code,
                  _lib.ptr(r), M, N, K, ws.data_ptr(), ws_bytes, _lib.stream_ptr(x.device))
     return y.reshape(*lead, N)
@@ -540,10 +540,10 @@ def scheme_workspace_bytes(M: int, N: int, K: int) -> int:
 
 
 @functools.lru_cache(maxsize=256)
-def fp8_workspace_bytes(M: int, N: int, K: int) -> int:
+def fp8_workspace_bytes(y_code: int, M: int, N: int, K: int) -> int:
     """Workspace of gdn_fp8_matmul."""
 
-    return int(_lib.load().gdn_fp8_matmul_workspace_size(M, N, K))
+    return int(_lib.load().gdn_fp8_matmul_workspace_size(y_code, M, N, K))
 
 
 @functools.lru_cache(maxsize=256)

@@ -134,7 +134,7 @@ def test_fp8_refusals():
                      (dict(ws=None), "workspace"), (dict(wb=1000), "workspace")):
         _refused(lib.gdn_fp8_matmul(*args(**kw)), E, what)
     assert lib.gdn_fp8_matmul(*args(M=0)) == 0
-    assert lib.gdn_fp8_matmul_workspace_size(4, 64, 250) == 0
+    assert lib.gdn_fp8_matmul_workspace_size(1, 4, 64, 250) == 0
     for a in ((_p(0), _p(1), _p(2), 9, 64, 64), (_p(0), _p(1), _p(2), 0, 64, 60), (_p(0), None, _p(2), 0, 64, 64),
               (ctypes.c_void_p(8), _p(1), _p(2), 0, 64, 64)):
         assert lib.gdn_fp8_dequantize(*a, None) == E
