@@ -76,6 +76,28 @@ GDN_DEV void silu_all(float (&x)[N]) {
     for (int i = 0; i < N; ++i) x[i] = y[i];
 }
 
+// Eight values of 16 bits in 16 bytes, or of float32 in 32, as floats.
+template <class Act, class V, int n>
+GDN_DEV void raw8(const V (&raw)[n], float (&x)[8]) {
+    static_assert(n == int(sizeof(typename Act::storage)) / 2, "eight values");
+    if constexpr (Act::code == GDN_F32) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(raw[e / 4][e % 4]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t d = raw[0][i];
+            if constexpr (Act::code == GDN_BF16) {
+                x[2 * i] = __uint_as_float(d << 16);
+                x[2 * i + 1] = __uint_as_float(d & 0xFFFF0000u);
+            } else {
+                x[2 * i] = f16_bits_to_f32(uint16_t(d & 0xFFFF));
+                x[2 * i + 1] = f16_bits_to_f32(uint16_t(d >> 16));
+            }
+        }
+    }
+}
+
 // Eight consecutive 16-bit or float32 values as floats, from an address
 // aligned to 16 bytes.
 template <class Act>

@@ -45,24 +45,43 @@ struct ScanArgs {
     int segmented;
 };
 
+// The running sum over the wave's lanes (DPP moves: rows of 16, then the rows'
+// ends handed on).
+template <int kCtrl, int kRows>
+GDN_DEV double dpp_add(double c) {
+    const int64_t u = __double_as_longlong(c);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, int(u), kCtrl, kRows, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, int(u >> 32), kCtrl, kRows, 0xF, false);
+    return c + __longlong_as_double(int64_t(lo | uint64_t(hi) << 32));
+}
+
+GDN_DEV double running_sum(double c) {
+    c = dpp_add<0x111, 0xF>(c);  // row_shr 1, 2, 4, 8
+    c = dpp_add<0x112, 0xF>(c);
+    c = dpp_add<0x114, 0xF>(c);
+    c = dpp_add<0x118, 0xF>(c);
+    c = dpp_add<0x142, 0xA>(c);  // row_bcast 15, 31
+    return dpp_add<0x143, 0xC>(c);
+}
+
+GDN_DEV double lane_value(double c, int lane) {
+    const int64_t u = __double_as_longlong(c);
+    const uint32_t lo = __builtin_amdgcn_readlane(int(u), lane), hi = __builtin_amdgcn_readlane(int(u >> 32), lane);
+    return __longlong_as_double(int64_t(lo | uint64_t(hi) << 32));
+}
+
 // The decays of one chunk, per token (all in powers of two): c_t as the sum of
 // two floats, d_t, exp(c_t), and d_t exp(c_Q - c_t). The running sum is in
 // double: what counts are differences of its terms, and a chunk's sum reaches
 // hundreds where single terms are 1e-3.
 template <int Q>
 struct Decays {
-    float hi[Q], lo[Q], d[Q], e[Q], w[Q];
+    float hi[Q], lo[Q], d[Q], e[Q], w[Q], end;
 };
 
 template <int Q>
 GDN_DEV double chunk_decays(Decays<Q>& o, int lane, float d, float rate) {
-    double c = double(d) * double(rate) * kLog2e;
-#pragma unroll
-    for (int off = 1; off < Q; off *= 2) {
-        const double up = __shfl_up(c, off, kWave);
-        if (lane >= off) c += up;
-    }
-    const double end = __shfl(c, Q - 1, kWave);
+    const double c = running_sum(double(d) * double(rate) * kLog2e), end = lane_value(c, Q - 1);
     if (lane < Q) {
         const float hi = float(c);
         o.hi[lane] = hi;
@@ -71,7 +90,49 @@ GDN_DEV double chunk_decays(Decays<Q>& o, int lane, float d, float rate) {
         o.e[lane] = __builtin_amdgcn_exp2f(hi);
         o.w[lane] = d * __builtin_amdgcn_exp2f(float(end - c));
     }
+    if (lane == 0) o.end = __builtin_amdgcn_exp2f(float(end));
     return end;
+}
+
+// For scores rounded to bfloat16, tile by tile of 16 tokens: with r the sum up
+// to the tile t lies in, exp(c_t - c_s) is exp(c_t - r) exp(r - c_s) for every s
+// before the tile, neither above one; only a tile's own pairs take an
+// exponential each. (Near is c - r: 24 bits of it are far more than the score
+// keeps.)
+struct TileDecays {
+    float near[64], d[64], from[64], e[64], w[64], to[3][64], end;
+};
+
+GDN_DEV double tile_decays(TileDecays& o, int lane, float d, float rate) {
+    const double c = running_sum(double(d) * double(rate) * kLog2e), end = lane_value(c, 63);
+    const double r1 = lane_value(c, 15), r2 = lane_value(c, 31), r3 = lane_value(c, 47);
+    const float near = float(c - (lane < 16 ? 0.0 : lane < 32 ? r1 : lane < 48 ? r2 : r3));
+    o.near[lane] = near;
+    o.d[lane] = d;
+    o.from[lane] = __builtin_amdgcn_exp2f(near);
+    o.e[lane] = __builtin_amdgcn_exp2f(float(c));
+    o.w[lane] = d * __builtin_amdgcn_exp2f(float(end - c));
+    o.to[0][lane] = lane < 16 ? d * __builtin_amdgcn_exp2f(float(r1 - c)) : 0.f;
+    o.to[1][lane] = lane < 32 ? d * __builtin_amdgcn_exp2f(float(r2 - c)) : 0.f;
+    o.to[2][lane] = lane < 48 ? d * __builtin_amdgcn_exp2f(float(r3 - c)) : 0.f;
+    if (lane == 0) o.end = __builtin_amdgcn_exp2f(float(end));
+    return end;
+}
+
+// Memory from `p` on as a buffer for 31-bit byte offsets. A lane with nothing
+// to fetch (a token past the segment, a column past the row) asks for kNowhere,
+// beyond the buffer: it reads zero and stores nothing, without a branch.
+constexpr int kNowhere = 0x7FFFFF00;
+
+GDN_DEV __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, p ? kNowhere : 0, 0x00027000);
+}
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+GDN_DEV u32x4 load16(__amdgpu_buffer_rsrc_t r, int at, int more) {
+    return __builtin_amdgcn_raw_buffer_load_b128(r, at, more, 0);
 }
 
 GDN_DEV f32x4 mfma_bf16(bf16x8 a, bf16x8 b, f32x4 c) {
@@ -80,14 +141,15 @@ GDN_DEV f32x4 mfma_bf16(bf16x8 a, bf16x8 b, f32x4 c) {
 
 GDN_DEV bf16x8 frag(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
 
-// Column operand of eight rows r0 .. r0 + 3 and r1 .. r1 + 3 at 16 columns of
-// a row-major LDS tile: within each 16-lane group, lane i of a transposing
-// read receives element i % 4 of source lane i / 4 + 4 k, k = 0 .. 3.
-GDN_DEV bf16x8 column_frag(const uint16_t* tile, int stride, int r0, int r1, int col, int sl) {
-    const uint16_t* a = tile + (r0 + (sl >> 2)) * stride + col + 4 * (sl & 3);
-    const uint16_t* b = tile + (r1 + (sl >> 2)) * stride + col + 4 * (sl & 3);
+// Operand of 16 columns of a row-major LDS tile, rows r0 .. r0 + 7, by
+// transposing reads: within each 16-lane group, lane i receives element i % 4
+// of source lane i / 4 + 4 k, k = 0 .. 3. The 16 columns are four groups of
+// four from col on, kApart apart.
+template <int kApart>
+GDN_DEV bf16x8 column_frag(const uint16_t* tile, int stride, int r0, int col, int sl) {
+    const uint16_t* a = tile + (r0 + (sl >> 2)) * stride + col + kApart * (sl & 3);
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(b));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 4 * stride));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
@@ -101,15 +163,14 @@ GDN_DEV bf16x8 column_frag(const uint16_t* tile, int stride, int r0, int r1, int
 // copy of the state; both only enter y, which is bfloat16 itself. The state's
 // own update takes x' = d exp(c_Q - c) x in two bfloat16 pieces (2^-18).
 template <int kNP, int kHeads, int kTiles, bool kStateOnly>
-__global__ __launch_bounds__(kScanThreads) void scan_bf16_kernel(ScanArgs a) {
+__global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_kernel(ScanArgs a) {
     constexpr int Q = 64, NS = kNP + 8, PW = 64 * kTiles, PH = PW / kHeads, XS = PW + 8, WS = Q + 8;
     constexpr int kRowsN = kNP / 8;                     // 16-byte pieces of a B or C row
     constexpr int kLoadN = Q * kRowsN / kScanThreads, kLoadX = Q * (PW / 8) / kScanThreads;
     constexpr int NT = kNP / 16, KS = kNP / 32;
     __shared__ __attribute__((aligned(16))) uint16_t Bs[Q * NS], Cs[kStateOnly ? 8 : Q * NS], Xs[Q * XS],
         Ws[kStateOnly ? 8 : kHeads * Q * WS];
-    __shared__ __attribute__((aligned(16))) Decays<Q> dec[kHeads];
-    __shared__ float dec_end[kHeads];
+    __shared__ __attribute__((aligned(16))) TileDecays decays[2][kHeads];
 
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, lr = lane & 15;
     const int P = a.P, N = a.N, H = a.H;
@@ -124,72 +185,72 @@ __global__ __launch_bounds__(kScanThreads) void scan_bf16_kernel(ScanArgs a) {
     const int pw = wave * 16 * kTiles;   // the wave's first row in the workgroup's, and in its head's
     const int pl = p0 + pw - hb * PH;
 
-    const uint16_t* xg = static_cast<const uint16_t*>(a.x);
-    const uint16_t* Bg = static_cast<const uint16_t*>(a.B) + grp * N;
-    const uint16_t* Cg = static_cast<const uint16_t*>(a.C) + grp * N;
-
-    uint4 rb[kLoadN], rc[kStateOnly ? 1 : kLoadN], rx[kLoadX];
+    // What a thread fetches of a chunk: the same 16-byte piece of every
+    // 256 / kRowsN-th row of B and C, and of every 2048 / PW-th row of x
+    constexpr int kStepN = kScanThreads / kRowsN, kStepX = kScanThreads * 8 / PW;
+    const int row_n = tid / kRowsN, n_at = tid % kRowsN * 8, row_x = tid / (PW / 8), col_x = tid % (PW / 8) * 8;
+    const int at_b = n_at < N ? int(row_n * a.B_stride + n_at) * 2 : kNowhere;
+    const int at_c = n_at < N ? int(row_n * a.C_stride + n_at) * 2 : kNowhere;
+    const int p_x = p0 + col_x % PH;
+    const int at_x = p_x < P ? int(row_x * a.x_stride + (col_x / PH) * P + p_x) * 2 : kNowhere;
+    u32x4 rb[kLoadN], rc[kStateOnly ? 1 : kLoadN], rx[kLoadX];
     float rdt = 0.f;
     const auto fetch = [&](int64_t t0) {
-        const uint4 zero = make_uint4(0, 0, 0, 0);
+        const int left = int(min(sg.t1 - t0, int64_t(Q)));
+        if (wave < kHeads && lane < left)  // (first: waited for first)
+            rdt = load_any(a.dt, (t0 + lane) * a.dt_stride + h0 + wave, a.dt_dtype);
+        const auto br = buffer_at(static_cast<const uint16_t*>(a.B) + t0 * a.B_stride + grp * N);
+        const auto cr = buffer_at(static_cast<const uint16_t*>(a.C) + t0 * a.C_stride + grp * N);
+        const auto xr = buffer_at(static_cast<const uint16_t*>(a.x) + t0 * a.x_stride + int64_t(h0) * P);
 #pragma unroll
         for (int i = 0; i < kLoadN; ++i) {
-            const int at = tid + kScanThreads * i, n = at % kRowsN * 8;
-            const int64_t t = t0 + at / kRowsN;
-            const bool ok = t < sg.t1 && n < N;
-            rb[i] = ok ? *reinterpret_cast<const uint4*>(Bg + t * a.B_stride + n) : zero;
-            if constexpr (!kStateOnly) rc[i] = ok ? *reinterpret_cast<const uint4*>(Cg + t * a.C_stride + n) : zero;
+            const bool in = row_n + i * kStepN < left;
+            rb[i] = load16(br, in ? at_b : kNowhere, int(i * kStepN * a.B_stride * 2));
+            if constexpr (!kStateOnly) rc[i] = load16(cr, in ? at_c : kNowhere, int(i * kStepN * a.C_stride * 2));
         }
 #pragma unroll
-        for (int i = 0; i < kLoadX; ++i) {
-            const int at = tid + kScanThreads * i, col = at % (PW / 8) * 8;
-            const int64_t t = t0 + at / (PW / 8);
-            const int p = p0 + col % PH;
-            rx[i] = t < sg.t1 && p < P
-                        ? *reinterpret_cast<const uint4*>(xg + t * a.x_stride + int64_t(h0 + col / PH) * P + p)
-                        : zero;
-        }
-        if (wave < kHeads && t0 + lane < sg.t1)
-            rdt = load_any(a.dt, (t0 + lane) * a.dt_stride + h0 + wave, a.dt_dtype);
+        for (int i = 0; i < kLoadX; ++i)
+            rx[i] = load16(xr, row_x + i * kStepX < left ? at_x : kNowhere, int(i * kStepX * a.x_stride * 2));
     };
 
-    // the state before the segment: tile j of the wave's S^T holds rows n = 16 j
-    // + 4 g + i, columns p = lr
+    // the state before the segment: tiles 2 k and 2 k + 1 of the wave's S^T hold
+    // columns p = lr and rows n = 32 k + 8 g + i and + 4 + i, so that the pair is
+    // an operand over n in order
     f32x4 S[kTiles][NT];
     const int64_t slot_state = (slot * H + h) * P, run_state = (int64_t(sg.run) * H + h) * P;
-    const float* from = kStateOnly ? nullptr : a.segmented ? a.part + slot_state * N : a.S_in ? a.S_in + run_state * N : nullptr;
+    const auto from = buffer_at(kStateOnly ? nullptr : a.segmented ? a.part + slot_state * N
+                                             : a.S_in ? a.S_in + run_state * N : nullptr);
+    const auto state_at = [&](int pt, int j) {  // bytes; four values of row n of column p
+        const int p = pl + 16 * pt + lr, n = 32 * (j / 2) + 8 * g + 4 * (j & 1);
+        return p < P && n < N ? (p * N + n) * 4 : kNowhere;
+    };
 #pragma unroll
     for (int pt = 0; pt < kTiles; ++pt)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int p = pl + 16 * pt + lr, n = 16 * j + 4 * g;
-            S[pt][j] = from && p < P && n < N ? *reinterpret_cast<const f32x4*>(from + int64_t(p) * N + n)
-                                              : f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int j = 0; j < NT; ++j) S[pt][j] = __builtin_bit_cast(f32x4, load16(from, state_at(pt, j), 0));
     const float rate = wave < kHeads ? -expf(a.A_log[h0 + wave]) : 0.f;
     const float dtb = wave < kHeads ? a.dt_bias[h0 + wave] : 0.f;
     const float skip = !kStateOnly && a.D ? a.D[h] : 0.f;
     double total = 0.0;
 
-    if (sg.t0 < sg.t1) fetch(sg.t0);
-    for (int64_t t0 = sg.t0; t0 < sg.t1; t0 += Q) {
+    const auto form_decays = [&](TileDecays* dec, int64_t t0) {
+        if (wave < kHeads) total += tile_decays(dec[wave], lane, t0 + lane < sg.t1 ? softplus(rdt + dtb) : 0.f, rate);
+    };
+    if (sg.t0 < sg.t1) {
+        fetch(sg.t0);
+        form_decays(decays[0], sg.t0);
+    }
+    int at_decays = 0;
+    for (int64_t t0 = sg.t0; t0 < sg.t1; t0 += Q, at_decays ^= 1) {
+        const TileDecays* dec = decays[at_decays];
 #pragma unroll
         for (int i = 0; i < kLoadN; ++i) {
-            const int at = tid + kScanThreads * i, o = at / kRowsN * NS + at % kRowsN * 8;
-            *reinterpret_cast<uint4*>(Bs + o) = rb[i];
-            if constexpr (!kStateOnly) *reinterpret_cast<uint4*>(Cs + o) = rc[i];
+            const int o = (row_n + i * kStepN) * NS + n_at;
+            *reinterpret_cast<u32x4*>(Bs + o) = rb[i];
+            if constexpr (!kStateOnly) *reinterpret_cast<u32x4*>(Cs + o) = rc[i];
         }
 #pragma unroll
-        for (int i = 0; i < kLoadX; ++i) {
-            const int at = tid + kScanThreads * i;
-            *reinterpret_cast<uint4*>(Xs + at / (PW / 8) * XS + at % (PW / 8) * 8) = rx[i];
-        }
-        if (wave < kHeads) {
-            const float d = t0 + lane < sg.t1 ? softplus(rdt + dtb) : 0.f;
-            const double end = chunk_decays<Q>(dec[wave], lane, d, rate);
-            total += end;
-            if (lane == 0) dec_end[wave] = __builtin_amdgcn_exp2f(float(end));
-        }
+        for (int i = 0; i < kLoadX; ++i) *reinterpret_cast<u32x4*>(Xs + (row_x + i * kStepX) * XS + col_x) = rx[i];
         __syncthreads();
         if (t0 + Q < sg.t1) fetch(t0 + Q);
 
@@ -213,22 +274,29 @@ __global__ __launch_bounds__(kScanThreads) void scan_bf16_kernel(ScanArgs a) {
                 const int s0 = 16 * j + 4 * g;
 #pragma unroll
                 for (int hh = 0; hh < kHeads; ++hh) {
-                    const f32x4 shi = *reinterpret_cast<const f32x4*>(dec[hh].hi + s0);
-                    const f32x4 slo = *reinterpret_cast<const f32x4*>(dec[hh].lo + s0);
-                    const f32x4 sd = *reinterpret_cast<const f32x4*>(dec[hh].d + s0);
-                    const float thi = dec[hh].hi[t], tlo = dec[hh].lo[t];
-                    float v[4];
+                    float v[4] = {0.f, 0.f, 0.f, 0.f};
+                    if (j < wave) {
+                        const f32x4 to = *reinterpret_cast<const f32x4*>(dec[hh].to[wave - 1] + s0);
+                        const float from = dec[hh].from[t];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        v[i] = s0 + i <= t
-                                   ? sc[i] * (sd[i] * __builtin_amdgcn_exp2f((thi - shi[i]) + (tlo - slo[i])))
-                                   : 0.f;
+                        for (int i = 0; i < 4; ++i) v[i] = sc[i] * (to[i] * from);
+                    } else if (j == wave) {
+                        const f32x4 near = *reinterpret_cast<const f32x4*>(dec[hh].near + s0);
+                        const f32x4 sd = *reinterpret_cast<const f32x4*>(dec[hh].d + s0);
+                        const float tn = dec[hh].near[t];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            v[i] = s0 + i <= t ? sc[i] * (sd[i] * __builtin_amdgcn_exp2f(tn - near[i])) : 0.f;
+                    }
                     *reinterpret_cast<uint2*>(Ws + (hh * Q + t) * WS + s0) =
                         make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
                 }
             }
             __syncthreads();
         }
+        // the next chunk's decays, in the other buffer: the first waves, which
+        // have the fewest scores before their tokens
+        if (t0 + Q < sg.t1) form_decays(decays[at_decays ^ 1], t0 + Q);
 
         // x^T of the wave's rows: tokens 32 q + 8 g + 0 .. 7 per lane
         bf16x8 xf[kTiles][2];
@@ -236,9 +304,11 @@ __global__ __launch_bounds__(kScanThreads) void scan_bf16_kernel(ScanArgs a) {
         for (int pt = 0; pt < kTiles; ++pt)
 #pragma unroll
             for (int q = 0; q < 2; ++q)
-                xf[pt][q] = column_frag(Xs, XS, 32 * q + 8 * g, 32 * q + 8 * g + 4, pw + 16 * pt, lr);
+                xf[pt][q] = column_frag<4>(Xs, XS, 32 * q + 8 * g, pw + 16 * pt, lr);
 
         if constexpr (!kStateOnly) {
+            const int left = int(min(sg.t1 - t0, int64_t(Q)));
+            const auto yr = buffer_at(static_cast<uint16_t*>(a.y) + (t0 * H + h) * P);
             f32x4 y[kTiles][4];
 #pragma unroll
             for (int pt = 0; pt < kTiles; ++pt)
@@ -255,9 +325,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_bf16_kernel(ScanArgs a) {
                 }
 #pragma unroll
                 for (int tt = 0; tt < 4; ++tt) {
-                    const uint16_t* cr = Cs + (16 * tt + lr) * NS + 32 * k + 4 * g;
-                    const uint2 c0 = *reinterpret_cast<const uint2*>(cr), c1 = *reinterpret_cast<const uint2*>(cr + 16);
-                    const bf16x8 cf = frag(make_uint4(c0.x, c0.y, c1.x, c1.y));
+                    const bf16x8 cf = frag(*reinterpret_cast<const uint4*>(Cs + (16 * tt + lr) * NS + 32 * k + 8 * g));
 #pragma unroll
                     for (int pt = 0; pt < kTiles; ++pt) y[pt][tt] = mfma_bf16(sf[pt], cf, y[pt][tt]);
                 }
@@ -285,15 +353,14 @@ __global__ __launch_bounds__(kScanThreads) void scan_bf16_kernel(ScanArgs a) {
                         o[2] = __builtin_fmaf(skip, __uint_as_float(xv.y << 16), o[2]);
                         o[3] = __builtin_fmaf(skip, __uint_as_float(xv.y & 0xFFFF0000u), o[3]);
                     }
-                    if (t0 + t < sg.t1 && p < P)
-                        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + ((t0 + t) * H + h) * P + p) =
-                            make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+                    __builtin_amdgcn_raw_buffer_store_b64(u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])}, yr,
+                                                          t < left && p < P ? (t * H * P + p) * 2 : kNowhere, 0, 0);
                 }
             }
         }
 
         if (kStateOnly || !a.segmented || t0 + Q < sg.t1) {
-            const float end = dec_end[hb];
+            const float end = dec[hb].end;
 #pragma unroll
             for (int pt = 0; pt < kTiles; ++pt)
 #pragma unroll
@@ -318,7 +385,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_bf16_kernel(ScanArgs a) {
                 }
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const bf16x8 bf = column_frag(Bs, NS, 32 * q + 8 * g, 32 * q + 8 * g + 4, 16 * j, lr);
+                    const bf16x8 bf = column_frag<8>(Bs, NS, 32 * q + 8 * g, 32 * (j / 2) + 4 * (j & 1), lr);
 #pragma unroll
                     for (int pt = 0; pt < kTiles; ++pt) {
                         S[pt][j] = mfma_bf16(bf, lo[pt], S[pt][j]);
@@ -331,14 +398,12 @@ __global__ __launch_bounds__(kScanThreads) void scan_bf16_kernel(ScanArgs a) {
     }
 
     if (kStateOnly || !a.segmented) {
-        float* to = kStateOnly ? a.part + slot_state * N : a.S_out + run_state * N;
+        const auto to = buffer_at(kStateOnly ? a.part + slot_state * N : a.S_out + run_state * N);
 #pragma unroll
         for (int pt = 0; pt < kTiles; ++pt)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int p = pl + 16 * pt + lr, n = 16 * j + 4 * g;
-                if (p < P && n < N) *reinterpret_cast<f32x4*>(to + int64_t(p) * N + n) = S[pt][j];
-            }
+            for (int j = 0; j < NT; ++j)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, S[pt][j]), to, state_at(pt, j), 0, 0);
         if (kStateOnly && wave < kHeads && lane == 0 && unit % tiles == 0)
             a.decay[slot * H + h0 + wave] = exp2f(float(total));
     }
@@ -359,7 +424,6 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
     __shared__ __attribute__((aligned(16))) float Bs[Q * NS], Cs[kStateOnly ? 4 : Q * NS], Xs[Q * XS],
         Ws[kStateOnly ? 4 : kHeads * Q * WS];
     __shared__ __attribute__((aligned(16))) Decays<Q> dec[kHeads];
-    __shared__ float dec_end[kHeads];
     using St = typename Act::storage;
 
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, lr = lane & 15;
@@ -375,55 +439,55 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
     const int pw = wave * 16 * kTiles;
     const int pl = p0 + pw - hb * PH;
 
-    const St* xg = static_cast<const St*>(a.x);
-    const St* Bg = static_cast<const St*>(a.B) + grp * N;
-    const St* Cg = static_cast<const St*>(a.C) + grp * N;
-
-    float rb[kLoadN][8], rc[kStateOnly ? 1 : kLoadN][8], rx[kLoadX][8];
+    constexpr int es = sizeof(St), kStepN = kScanThreads / kRowsN, kStepX = kScanThreads * 8 / PW;
+    const int row_n = tid / kRowsN, n_at = tid % kRowsN * 8, row_x = tid / (PW / 8), col_x = tid % (PW / 8) * 8;
+    const int at_b = n_at < N && row_n < Q ? int(row_n * a.B_stride + n_at) * es : kNowhere;
+    const int at_c = n_at < N && row_n < Q ? int(row_n * a.C_stride + n_at) * es : kNowhere;
+    const int p_x = p0 + col_x % PH;
+    const int at_x = p_x < P ? int(row_x * a.x_stride + (col_x / PH) * P + p_x) * es : kNowhere;
+    constexpr int kRaw = es / 2;  // 16-byte loads of eight values
+    u32x4 rb[kLoadN][kRaw], rc[kStateOnly ? 1 : kLoadN][kRaw], rx[kLoadX][kRaw];
     float rdt = 0.f;
-    const auto get = [&](const St* p, bool ok, float (&v)[8]) {
-        if (ok) {
-            load8f<Act>(p, v);
-        } else {
+    const auto get = [&](__amdgpu_buffer_rsrc_t r, int at, int more, u32x4 (&v)[kRaw]) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = 0.f;
-        }
+        for (int e = 0; e < kRaw; ++e) v[e] = load16(r, at, more + 16 * e);
     };
     const auto fetch = [&](int64_t t0) {
+        const int left = int(min(sg.t1 - t0, int64_t(Q)));
+        const auto br = buffer_at(static_cast<const St*>(a.B) + t0 * a.B_stride + grp * N);
+        const auto cr = buffer_at(static_cast<const St*>(a.C) + t0 * a.C_stride + grp * N);
+        const auto xr = buffer_at(static_cast<const St*>(a.x) + t0 * a.x_stride + int64_t(h0) * P);
 #pragma unroll
         for (int i = 0; i < kLoadN; ++i) {
-            const int at = tid + kScanThreads * i, n = at % kRowsN * 8;
-            const int64_t t = t0 + at / kRowsN;
-            const bool ok = at < Q * kRowsN && t < sg.t1 && n < N;
-            get(Bg + t * a.B_stride + n, ok, rb[i]);
-            if constexpr (!kStateOnly) get(Cg + t * a.C_stride + n, ok, rc[i]);
+            const bool in = row_n + i * kStepN < left;
+            get(br, in ? at_b : kNowhere, int(i * kStepN * a.B_stride * es), rb[i]);
+            if constexpr (!kStateOnly) get(cr, in ? at_c : kNowhere, int(i * kStepN * a.C_stride * es), rc[i]);
         }
 #pragma unroll
-        for (int i = 0; i < kLoadX; ++i) {
-            const int at = tid + kScanThreads * i, col = at % (PW / 8) * 8;
-            const int64_t t = t0 + at / (PW / 8);
-            const int p = p0 + col % PH;
-            get(xg + t * a.x_stride + int64_t(h0 + col / PH) * P + p, t < sg.t1 && p < P, rx[i]);
-        }
-        if (wave < kHeads && lane < Q && t0 + lane < sg.t1)
+        for (int i = 0; i < kLoadX; ++i)
+            get(xr, row_x + i * kStepX < left ? at_x : kNowhere, int(i * kStepX * a.x_stride * es), rx[i]);
+        if (wave < kHeads && lane < left)
             rdt = load_any(a.dt, (t0 + lane) * a.dt_stride + h0 + wave, a.dt_dtype);
     };
-    const auto put = [](float* p, const float (&v)[8]) {
+    const auto put = [](float* p, const u32x4 (&raw)[kRaw]) {
+        float v[8];
+        raw8<Act>(raw, v);
         *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
         *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
     };
 
     f32x4 S[kTiles][NT];
     const int64_t slot_state = (slot * H + h) * P, run_state = (int64_t(sg.run) * H + h) * P;
-    const float* from = kStateOnly ? nullptr : a.segmented ? a.part + slot_state * N : a.S_in ? a.S_in + run_state * N : nullptr;
+    const auto from = buffer_at(kStateOnly ? nullptr : a.segmented ? a.part + slot_state * N
+                                             : a.S_in ? a.S_in + run_state * N : nullptr);
+    const auto state_at = [&](int pt, int j) {
+        const int p = pl + 16 * pt + lr, n = 16 * j + 4 * g;
+        return p < P && n < N ? (p * N + n) * 4 : kNowhere;
+    };
 #pragma unroll
     for (int pt = 0; pt < kTiles; ++pt)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int p = pl + 16 * pt + lr, n = 16 * j + 4 * g;
-            S[pt][j] = from && p < P && n < N ? *reinterpret_cast<const f32x4*>(from + int64_t(p) * N + n)
-                                              : f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int j = 0; j < NT; ++j) S[pt][j] = __builtin_bit_cast(f32x4, load16(from, state_at(pt, j), 0));
     const float rate = wave < kHeads ? -expf(a.A_log[h0 + wave]) : 0.f;
     const float dtb = wave < kHeads ? a.dt_bias[h0 + wave] : 0.f;
     const float skip = !kStateOnly && a.D ? a.D[h] : 0.f;
@@ -433,22 +497,17 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
     for (int64_t t0 = sg.t0; t0 < sg.t1; t0 += Q) {
 #pragma unroll
         for (int i = 0; i < kLoadN; ++i) {
-            const int at = tid + kScanThreads * i, o = at / kRowsN * NS + at % kRowsN * 8;
-            if (at < Q * kRowsN) {
+            const int o = (row_n + i * kStepN) * NS + n_at;
+            if (kLoadN * kStepN <= Q || row_n < Q) {
                 put(Bs + o, rb[i]);
                 if constexpr (!kStateOnly) put(Cs + o, rc[i]);
             }
         }
 #pragma unroll
-        for (int i = 0; i < kLoadX; ++i) {
-            const int at = tid + kScanThreads * i;
-            put(Xs + at / (PW / 8) * XS + at % (PW / 8) * 8, rx[i]);
-        }
+        for (int i = 0; i < kLoadX; ++i) put(Xs + (row_x + i * kStepX) * XS + col_x, rx[i]);
         if (wave < kHeads) {
             const float d = lane < Q && t0 + lane < sg.t1 ? softplus(rdt + dtb) : 0.f;
-            const double end = chunk_decays<Q>(dec[wave], lane, d, rate);
-            total += end;
-            if (lane == 0) dec_end[wave] = __builtin_amdgcn_exp2f(float(end));
+            total += chunk_decays<Q>(dec[wave], lane, d, rate);
         }
         __syncthreads();
         if (t0 + Q < sg.t1) fetch(t0 + Q);
@@ -490,6 +549,8 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
                 for (int i = 0; i < 4; ++i) xf[pt][j][i] = Xs[(16 * j + 4 * g + i) * XS + pw + 16 * pt + lr];
 
         if constexpr (!kStateOnly) {
+            const int left = int(min(sg.t1 - t0, int64_t(Q)));
+            const auto yr = buffer_at(static_cast<char*>(a.y) + ((t0 * H + h) * P) * (a.y_dtype == GDN_F32 ? 4 : 2));
             f32x4 y[kTiles][Q / 16];
 #pragma unroll
             for (int pt = 0; pt < kTiles; ++pt)
@@ -530,25 +591,24 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(skip, xv[i], o[i]);
                     }
-                    if (t0 + t < sg.t1 && p < P) {
-                        const int64_t at = ((t0 + t) * H + h) * P + p;
-                        if (a.y_dtype == GDN_F32) {
-                            *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + at) = o;
-                        } else {
-                            uint16_t b[4];
+                    const bool in = t < left && p < P;
+                    const int at = (t * H * P + p) * (a.y_dtype == GDN_F32 ? 4 : 2);
+                    if (a.y_dtype == GDN_F32) {
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), yr, in ? at : kNowhere, 0, 0);
+                    } else {
+                        uint16_t b[4];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                b[i] = a.y_dtype == GDN_BF16 ? f32_to_bf16_bits(o[i]) : f32_to_f16_bits(o[i]);
-                            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + at) =
-                                make_uint2(b[0] | uint32_t(b[1]) << 16, b[2] | uint32_t(b[3]) << 16);
-                        }
+                        for (int i = 0; i < 4; ++i)
+                            b[i] = a.y_dtype == GDN_BF16 ? f32_to_bf16_bits(o[i]) : f32_to_f16_bits(o[i]);
+                        __builtin_amdgcn_raw_buffer_store_b64(u32x2{b[0] | uint32_t(b[1]) << 16, b[2] | uint32_t(b[3]) << 16},
+                                                              yr, in ? at : kNowhere, 0, 0);
                     }
                 }
             }
         }
 
         if (kStateOnly || !a.segmented || t0 + Q < sg.t1) {
-            const float end = dec_end[hb];
+            const float end = dec[hb].end;
 #pragma unroll
             for (int pt = 0; pt < kTiles; ++pt)
 #pragma unroll
@@ -575,14 +635,12 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
     }
 
     if (kStateOnly || !a.segmented) {
-        float* to = kStateOnly ? a.part + slot_state * N : a.S_out + run_state * N;
+        const auto to = buffer_at(kStateOnly ? a.part + slot_state * N : a.S_out + run_state * N);
 #pragma unroll
         for (int pt = 0; pt < kTiles; ++pt)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int p = pl + 16 * pt + lr, n = 16 * j + 4 * g;
-                if (p < P && n < N) *reinterpret_cast<f32x4*>(to + int64_t(p) * N + n) = S[pt][j];
-            }
+            for (int j = 0; j < NT; ++j)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, S[pt][j]), to, state_at(pt, j), 0, 0);
         if (kStateOnly && wave < kHeads && lane == 0 && unit % tiles == 0)
             a.decay[slot * H + h0 + wave] = exp2f(float(total));
     }
@@ -702,6 +760,9 @@ extern "C" int gdn_selective_scan(const void* x, int64_t x_stride, const void* B
                 "gdn_selective_scan: null pointer");
     GDN_REQUIRE(x_stride >= int64_t(H) * P && B_stride >= int64_t(G) * S && C_stride >= int64_t(G) * S && dt_stride >= H,
                 "gdn_selective_scan: a row stride is below its row");
+    // (a chunk's rows are addressed in 31 bits)
+    GDN_REQUIRE(x_stride <= (1 << 22) && B_stride <= (1 << 22) && C_stride <= (1 << 22) && int64_t(P) * S <= (1 << 28),
+                "gdn_selective_scan: rows or states too wide");
     const int es = dtype_size(act_dtype);
     const auto at = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(C) |
                     reinterpret_cast<uintptr_t>(state_in) | reinterpret_cast<uintptr_t>(state_out) |
