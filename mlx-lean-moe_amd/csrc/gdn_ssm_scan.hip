@@ -172,7 +172,7 @@ __global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_ke
         Ws[kStateOnly ? 8 : kHeads * Q * WS];
     __shared__ __attribute__((aligned(16))) TileDecays decays[2][kHeads];
 
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, lr = lane & 15;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, lr = lane & 15;
     const int P = a.P, N = a.N, H = a.H;
     const int tiles = (P + PH - 1) / PH, units = H / kHeads * tiles;
     const int unit = blockIdx.x % units;
@@ -372,15 +372,19 @@ __global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_ke
                 bf16x8 hi[kTiles], lo[kTiles];
 #pragma unroll
                 for (int pt = 0; pt < kTiles; ++pt) {
-                    float v[8], r[8];
+                    // hi: the upper 16 bits as they are; lo: what is left
+                    float v[8];
                     unpack8(__builtin_bit_cast(uint4, xf[pt][q]), v);
+                    uint32_t up[4];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) r[e] = v[e] *= e < 4 ? w0[e & 3] : w1[e & 3];
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2) round_bf16x2(r[e], r[e + 1]);
-                    hi[pt] = frag(pack8(r));
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] -= r[e];
+                    for (int e = 0; e < 8; e += 2) {
+                        v[e] *= e < 4 ? w0[e & 3] : w1[e & 3];
+                        v[e + 1] *= e < 4 ? w0[(e & 3) + 1] : w1[(e & 3) + 1];
+                        up[e / 2] = __builtin_amdgcn_perm(__float_as_uint(v[e + 1]), __float_as_uint(v[e]), 0x07060302u);
+                        v[e] -= __uint_as_float(__float_as_uint(v[e]) & 0xFFFF0000u);
+                        v[e + 1] -= __uint_as_float(__float_as_uint(v[e + 1]) & 0xFFFF0000u);
+                    }
+                    hi[pt] = frag(make_uint4(up[0], up[1], up[2], up[3]));
                     lo[pt] = frag(pack8(v));
                 }
 #pragma unroll
@@ -426,7 +430,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
     __shared__ __attribute__((aligned(16))) Decays<Q> dec[kHeads];
     using St = typename Act::storage;
 
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, lr = lane & 15;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, lr = lane & 15;
     const int P = a.P, N = a.N, H = a.H;
     const int tiles = (P + PH - 1) / PH, units = H / kHeads * tiles;
     const int unit = blockIdx.x % units;

@@ -238,10 +238,10 @@ def _check_fp8_block(tensors: dict, K: int | None):
         raise ValueError(f"input width {K} does not match the weight's {k}")
     if N == 0 or k == 0 or k % 16:
         raise ValueError(f"an fp8_block weight has rows of a nonzero multiple of 16 codes, got {(N, k)}")
-    if tuple(scales.shape) != (-(-N // 128), -(-k // 128)) or scales.dtype != torch.float32:
+    if scales.shape != (-(-N // 128), -(-k // 128)) or scales.dtype != torch.float32:
         raise ValueError(f"fp8_block scales must be float32 of shape {(-(-N // 128), -(-k // 128))}, got "
                          f"{tuple(scales.shape)} {scales.dtype}")
-    if scales.device != w.device:
+    if scales.get_device() != w.get_device():
         raise ValueError(f"weight is on {w.device}, its scales on {scales.device}")
     return w, scales, None, N, k
 
@@ -440,27 +440,35 @@ def _fp8_matmul(x, w, scales, N: int, K: int, residual):
     """``x @ W.T`` (+ residual) for fp8_block weights (gdn_fp8_matmul): x's
     rows quantized to e4m3 per 128 columns, float32 sums."""
 
-    if _transformed(x, residual):
+    if _followed(x, residual):
         raise RuntimeError("fp8_block products have no gradient and no function transform; call them under "
                            "torch.no_grad()")
-    if w.device != x.device:
+    if w.get_device() != x.get_device():
         raise ValueError(f"x is on {x.device}, the weights on {w.device}")
-    lead = x.shape[:-1]
-    x2 = _c(x.reshape(-1, K))
+    shape = x.shape
+    x2 = x if x.is_contiguous() else x.contiguous()
     if x2.data_ptr() % 16:
         x2 = x2.clone()
-    M = x2.shape[0]
-    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    r = _residual_rows(residual, x, lead, M, N)
+    M = x2.numel() // K
+    y = torch.empty((*shape[:-1], N), dtype=x.dtype, device=x.device)
+    r = None if residual is None else _residual_rows(residual, x, shape[:-1], M, N)
     w, scales = _c(w), _c(scales)
     if w.data_ptr() % 16:
         w = w.clone()
     code = _lib.dtype_code(x.dtype)
     ws_bytes = fp8_workspace_bytes(code, M, N, K)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
     _lib.call_on(x.device, "gdn_fp8_matmul", x2.data_ptr(), code, w.data_ptr(), scales.data_ptr(), y.data_ptr(), code,
-                 _lib.ptr(r), M, N, K, ws.data_ptr(), ws_bytes, _lib.stream_ptr(x.device))
-    return y.reshape(*lead, N)
+                 _lib.ptr(r), M, N, K, _lib.ptr(ws), ws_bytes, _lib.stream_ptr(x.device))
+    return y
+
+
+def _followed(*operands: torch.Tensor | None) -> bool:
+    """_transformed of calls that may cost little: a tensor outside forward
+    mode's levels has no tangent, and one that a transform wraps has no data_ptr
+    (which raises by itself)."""
+
+    return (torch.is_grad_enabled() or getattr(forward_ad, "_current_level", 0) >= 0) and _transformed(*operands)
 
 
 def _f32_matmul(x, w, scales, biases, quant: QuantScheme, N: int, K: int, residual):

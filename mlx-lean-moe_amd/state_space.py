@@ -20,11 +20,14 @@ tensors; none has a gradient.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
 from .config import StateSpaceDims
-from .gated_delta import _as, _c, _check_cu_seqlens, _check_out, _promote, _require_device, _stream
+from .gated_delta import (_FLOATS, _as, _c, _check_cu_seqlens, _check_out, _promote, _require_device,
+                          _stream)
 from .linear_attention import _index_array, _rows, check_half_bits, check_slots
 
 _MAX_STATE = 256   # state_dim, both kernels
@@ -65,28 +68,61 @@ def _runs(cu_seqlens, T: int, device) -> PackedRuns:
     return cu_seqlens
 
 
+def _operands(*tensors) -> torch.device:
+    """The one GPU that holds these tensors (None skipped), floats without a
+    gradient all of them. A step or a short prompt is host-bound, hence the
+    integer comparisons (a device object each costs more)."""
+
+    index, device = -1, None
+    for t in tensors:
+        if t is None:
+            continue
+        i = t.get_device()
+        if device is None:
+            index, device = i, t.device
+        if i != index or i < 0 or t.dtype not in _FLOATS:
+            return _require_device(*tensors)  # raises what is wrong
+    _no_gradient(*tensors)
+    return device
+
+
 def _no_gradient(*tensors) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError("the state-space operators have no gradient; call them under torch.no_grad()")
+    if not torch.is_grad_enabled():
+        return
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise RuntimeError("the state-space operators have no gradient; call them under torch.no_grad()")
 
 
 def _f32_vector(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
-    if t.shape != (n,):
+    if t.ndim != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must have shape ({n},), got {tuple(t.shape)}")
-    return _c(_as(t, _F32))
+    return t if t.dtype is _F32 and t.is_contiguous() else t.float().contiguous()
 
 
-def _token_rows(t: torch.Tensor, T: int, width: int) -> torch.Tensor:
-    """``t`` as ``(T, width)`` rows that the kernels read in 16-byte pieces:
-    a view where the rows are packed, aligned and no closer than their width
-    (column slices of one projection or conv output), else a copy."""
+def _token_rows(t: torch.Tensor, T: int, heads: int, dim: int) -> tuple[torch.Tensor, int]:
+    """``t (tokens, heads, dim)``, batch-first or packed, as rows that the
+    kernels read in 16-byte pieces, and their stride: in place where the rows
+    are packed, aligned and no closer than their width (column slices of one
+    projection or conv output), else a copy."""
 
-    t = t.reshape(T, width)
-    if T <= 1 or t.stride(0) < width or t.stride(0) * t.element_size() % 16 or t.stride(1) != 1:
-        t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    st, width = t.stride(), heads * dim
+    step, packed = st[-3], st[-1] == 1 and (st[-2] == dim or heads == 1)
+    if t.ndim == 4 and t.shape[0] > 1:
+        if t.shape[1] == 1:
+            step = st[0]
+        else:
+            packed = packed and st[0] == t.shape[1] * step
+    if T <= 1:
+        step = width
+    if packed and step >= width and step * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
+        return t, step
+    return t.clone(memory_format=torch.contiguous_format), width
+
+
+@functools.lru_cache(maxsize=1024)
+def _scan_workspace(*sizes: int) -> int:
+    return int(_lib.load().gdn_selective_scan_workspace_size(*sizes))
 
 
 def conv_silu(x: torch.Tensor, conv_state: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
@@ -114,8 +150,7 @@ def conv_silu(x: torch.Tensor, conv_state: torch.Tensor, weight: torch.Tensor, b
         raise ValueError(f"bias must have shape ({C},), got {tuple(bias.shape)}")
     if T >= 2 ** 31:
         raise ValueError("the token count must fit int32")
-    device = _require_device(x, conv_state, weight, bias)
-    _no_gradient(x, conv_state, weight, bias)
+    device = _operands(x, conv_state, weight, bias)
     cu = None
     if cu_seqlens is not None:
         runs = _runs(cu_seqlens, T, device)
@@ -174,8 +209,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, B: torch.Tensor, C: torch.
     if P % 8 or N % 8 or N > _MAX_STATE:
         raise ValueError(f"head_dim and state_dim must be multiples of 8, state_dim at most {_MAX_STATE}; "
                          f"got {P} and {N}")
-    device = _require_device(x, dt, B, C, A_log, dt_bias, D, state)
-    _no_gradient(x, dt, B, C, A_log, dt_bias, D, state)
+    device = _operands(x, dt, B, C, A_log, dt_bias, D, state)
     if packed:
         T = x.shape[0]
         runs = _runs(cu_seqlens, T, device)
@@ -199,11 +233,15 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, B: torch.Tensor, C: torch.
     D = None if D is None else _f32_vector(D, H, "D")
     act = _promote(x, B, C)
     shape = x.shape
-    x = _token_rows(_as(x, act), T, H * P)
-    B, C = _token_rows(_as(B, act), T, G * N), _token_rows(_as(C, act), T, G * N)
-    dt = dt.reshape(T, H)
-    if T > 1 and (dt.stride(0) < H or dt.stride(1) != 1):
-        dt = dt.contiguous()
+    x, x_step = _token_rows(_as(x, act), T, H, P)
+    B, B_step = _token_rows(_as(B, act), T, G, N)
+    C, C_step = _token_rows(_as(C, act), T, G, N)
+    dt_step = H
+    if not dt.is_contiguous():
+        if packed and dt.stride(1) == 1 and dt.stride(0) >= H:
+            dt_step = dt.stride(0)
+        else:
+            dt = dt.contiguous()
     in_place = state is not None and state_out is state
     if state is not None and not in_place:
         state = _c(_as(state, _F32))
@@ -216,13 +254,12 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, B: torch.Tensor, C: torch.
         _check_out(state_out, (R, H, P, N), _F32, device, src, "state_out")
         if state_out.data_ptr() % 16:
             raise ValueError("state_out must be 16-byte aligned")
-    nbytes = int(_lib.load().gdn_selective_scan_workspace_size(R, T, longest, G, H, P, N))
+    nbytes = _scan_workspace(R, T, longest, G, H, P, N)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    strides = [t.stride(0) if T > 1 else t.shape[1] for t in (x, B, C, dt)]
-    _lib.call_on(device, "gdn_selective_scan", _lib.ptr(x), strides[0], _lib.ptr(B), strides[1], _lib.ptr(C),
-                 strides[2], _lib.dtype_code(act), _lib.ptr(dt), strides[3], _lib.dtype_code(dt.dtype),
-                 _lib.ptr(A_log), _lib.ptr(dt_bias), _lib.ptr(D), _lib.ptr(state), _lib.ptr(state_out), _lib.ptr(y),
-                 y_code, _lib.ptr(cu), R, T, longest, G, H, P, N, _lib.ptr(ws), nbytes, _stream(device))
+    _lib.call_on(device, "gdn_selective_scan", x.data_ptr(), x_step, B.data_ptr(), B_step, C.data_ptr(), C_step,
+                 _lib.dtype_code(act), dt.data_ptr(), dt_step, _lib.dtype_code(dt.dtype), A_log.data_ptr(),
+                 dt_bias.data_ptr(), _lib.ptr(D), _lib.ptr(state), state_out.data_ptr(), y.data_ptr(), y_code,
+                 _lib.ptr(cu), R, T, longest, G, H, P, N, _lib.ptr(ws), nbytes, _stream(device))
     return y, state_out
 
 
@@ -256,8 +293,7 @@ def selective_step(xbc: torch.Tensor, dt: torch.Tensor, conv_state: torch.Tensor
                          f"{_MAX_HEAD} and 2 to 4 taps; got {N}, {P} and {K}")
     if xbc.shape[1] != C or dt.shape != (rows, H) or conv_weight.shape[:2] != (C, K) or conv_weight.numel() != C * K:
         raise ValueError("selective_step: xbc, dt or conv_weight do not match the dims")
-    device = _require_device(xbc, dt, conv_state, ssm_state, conv_weight, conv_bias, A_log, dt_bias, D)
-    _no_gradient(xbc, dt, conv_state, ssm_state, conv_weight, conv_bias, A_log, dt_bias, D)
+    device = _operands(xbc, dt, conv_state, ssm_state, conv_weight, conv_bias, A_log, dt_bias, D)
     pool = rows
     slot_t = half_t = None
     if slots is not None:
