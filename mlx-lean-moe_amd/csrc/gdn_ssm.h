@@ -6,33 +6,36 @@
 
 namespace gdn {
 
-// A packed batch is cut into segments of `seg` tokens, counted from each
-// run's first token. Run r's segments take the slots floor(cu[r] / seg) + r
-// and on: distinct for all runs whatever their lengths (a run of len tokens
-// has at most floor(cu[r + 1] / seg) - floor(cu[r] / seg) + 1 of them), one
-// slot at least for an empty run, and T / seg + N in all, which the host
-// knows without the offsets. With seg > T run r has slot r alone.
+// A packed batch is cut into segments of 2^shift tokens, counted from each run's
+// first token. Run r's segments take the slots (cu[r] >> shift) + r and on:
+// distinct for all runs whatever their lengths (a run of len tokens has at most
+// (cu[r + 1] >> shift) - (cu[r] >> shift) + 1 of them), one slot at least for an
+// empty run, and (T >> shift) + N in all, which the host knows without the
+// offsets. With shift 31 run r has slot r alone.
 struct Segment {
     int run;          // -1: no run has this slot
     int64_t t0, t1;   // its tokens
-    bool first, last; // of its run
 };
 
 GDN_DEV int64_t run_start(const int32_t* cu, int64_t L, int r) { return cu ? int64_t(cu[r]) : r * L; }
 
-GDN_DEV Segment segment_of(const int32_t* cu, int N, int64_t L, int64_t seg, int64_t slot) {
-    int lo = 0, hi = N;  // the last run whose first slot is not past `slot`
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (run_start(cu, L, mid) / seg + mid <= slot) lo = mid; else hi = mid;
+// The slot's run is the last whose first slot is not past it: found 64 runs at
+// a time, one load each step (a binary search waits for six).
+GDN_DEV Segment segment_of(const int32_t* cu, int N, int64_t L, int shift, int slot) {
+    const int lane = threadIdx.x % kWave;
+    int lo = 0, count = N;
+    while (count > 1) {
+        const int step = (count + kWave - 1) / kWave, at = lane * step;
+        const bool before = at < count && int(run_start(cu, L, lo + at) >> shift) + lo + at <= slot;
+        const int last = __popcll(__ballot(before)) - 1;  // (lane 0's always is)
+        lo += last * step;
+        count = min(step, count - last * step);
     }
     const int64_t b = run_start(cu, L, lo), e = run_start(cu, L, lo + 1);
-    const int64_t k = slot - (b / seg + lo);
+    const int k = slot - int(b >> shift) - lo;
     Segment s;
-    s.t0 = b + k * seg;
-    s.t1 = e - s.t0 < seg ? e : s.t0 + seg;
-    s.first = k == 0;
-    s.last = s.t1 >= e;
+    s.t0 = b + (int64_t(k) << shift);
+    s.t1 = min(e, s.t0 + (int64_t(1) << shift));
     s.run = k == 0 || s.t0 < e ? lo : -1;
     return s;
 }

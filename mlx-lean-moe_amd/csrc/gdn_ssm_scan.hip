@@ -25,6 +25,7 @@ namespace gdn {
 namespace {
 
 constexpr int kScanThreads = 256;
+constexpr int kMaxGridY = 65535;
 constexpr double kLog2e = 1.4426950408889634;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -39,10 +40,11 @@ struct ScanArgs {
     int y_dtype;
     const int32_t* cu;
     int runs;
-    int64_t T, L, seg;
+    int64_t L;
+    int shift;  // segments of 2^shift tokens
     int G, H, P, N;
     float *part, *decay;  // per (slot, head): a segment's own sum, then the state before it; its decay
-    int segmented;
+    int segmented, slots;
 };
 
 // The running sum over the wave's lanes (DPP moves: rows of 16, then the rows'
@@ -161,7 +163,7 @@ GDN_DEV bf16x8 column_frag(const uint16_t* tile, int stride, int r0, int col, in
 //
 // Roundings to bfloat16: the decayed scores and, as the operand of S C^T, a
 // copy of the state; both only enter y, which is bfloat16 itself. The state's
-// own update takes x' = d exp(c_Q - c) x in two bfloat16 pieces (2^-18).
+// own update takes x' = d exp(c_Q - c) x in three bfloat16 pieces, all 24 bits.
 template <int kNP, int kHeads, int kTiles, bool kStateOnly>
 __global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_kernel(ScanArgs a) {
     constexpr int Q = 64, NS = kNP + 8, PW = 64 * kTiles, PH = PW / kHeads, XS = PW + 8, WS = Q + 8;
@@ -174,12 +176,13 @@ __global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_ke
 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, lr = lane & 15;
     const int P = a.P, N = a.N, H = a.H;
-    const int tiles = (P + PH - 1) / PH, units = H / kHeads * tiles;
-    const int unit = blockIdx.x % units;
-    const int64_t slot = blockIdx.x / units;
-    const int h0 = unit / tiles * kHeads, p0 = unit % tiles * PH;
-    const int grp = h0 / (H / a.G);
-    const Segment sg = segment_of(a.cu, a.runs, a.L, a.seg, slot);
+    const int tiles = (P + PH - 1) / PH;
+    const int unit = blockIdx.x, slot = blockIdx.y + blockIdx.z * kMaxGridY;
+    if (slot >= a.slots) return;
+    const int pair = tiles == 1 ? unit : unit / tiles;
+    const int h0 = pair * kHeads, p0 = tiles == 1 ? 0 : (unit - pair * tiles) * PH;
+    const int grp = a.G == 1 ? 0 : h0 / (H / a.G);
+    const Segment sg = segment_of(a.cu, a.runs, a.L, a.shift, slot);
     if (sg.run < 0) return;
     const int hb = wave * kHeads / 4, h = h0 + hb;
     const int pw = wave * 16 * kTiles;   // the wave's first row in the workgroup's, and in its head's
@@ -213,21 +216,6 @@ __global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_ke
             rx[i] = load16(xr, row_x + i * kStepX < left ? at_x : kNowhere, int(i * kStepX * a.x_stride * 2));
     };
 
-    // the state before the segment: tiles 2 k and 2 k + 1 of the wave's S^T hold
-    // columns p = lr and rows n = 32 k + 8 g + i and + 4 + i, so that the pair is
-    // an operand over n in order
-    f32x4 S[kTiles][NT];
-    const int64_t slot_state = (slot * H + h) * P, run_state = (int64_t(sg.run) * H + h) * P;
-    const auto from = buffer_at(kStateOnly ? nullptr : a.segmented ? a.part + slot_state * N
-                                             : a.S_in ? a.S_in + run_state * N : nullptr);
-    const auto state_at = [&](int pt, int j) {  // bytes; four values of row n of column p
-        const int p = pl + 16 * pt + lr, n = 32 * (j / 2) + 8 * g + 4 * (j & 1);
-        return p < P && n < N ? (p * N + n) * 4 : kNowhere;
-    };
-#pragma unroll
-    for (int pt = 0; pt < kTiles; ++pt)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) S[pt][j] = __builtin_bit_cast(f32x4, load16(from, state_at(pt, j), 0));
     const float rate = wave < kHeads ? -expf(a.A_log[h0 + wave]) : 0.f;
     const float dtb = wave < kHeads ? a.dt_bias[h0 + wave] : 0.f;
     const float skip = !kStateOnly && a.D ? a.D[h] : 0.f;
@@ -236,10 +224,26 @@ __global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_ke
     const auto form_decays = [&](TileDecays* dec, int64_t t0) {
         if (wave < kHeads) total += tile_decays(dec[wave], lane, t0 + lane < sg.t1 ? softplus(rdt + dtb) : 0.f, rate);
     };
-    if (sg.t0 < sg.t1) {
-        fetch(sg.t0);
-        form_decays(decays[0], sg.t0);
-    }
+    // the state before the segment: tiles 2 k and 2 k + 1 of the wave's S^T hold
+    // columns p = lr and rows n = 32 k + 8 g + i and + 4 + i, so that the pair is
+    // an operand over n in order
+    f32x4 S[kTiles][NT];
+    const int64_t slot_state = (int64_t(slot) * H + h) * P, run_state = (int64_t(sg.run) * H + h) * P;
+    const auto from = buffer_at(kStateOnly ? nullptr : a.segmented ? a.part + slot_state * N
+                                             : a.S_in ? a.S_in + run_state * N : nullptr);
+    const auto state_at = [&](int pt, int j) {  // bytes; four values of row n of column p
+        const int p = pl + 16 * pt + lr, n = 32 * (j / 2) + 8 * g + 4 * (j & 1);
+        return p < P && n < N ? (p * N + n) * 4 : kNowhere;
+    };
+    // (the first chunk's loads go out before the state's, which it needs last)
+    if (sg.t0 < sg.t1) fetch(sg.t0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int pt = 0; pt < kTiles; ++pt)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) S[pt][j] = __builtin_bit_cast(f32x4, load16(from, state_at(pt, j), 0));
+    __builtin_amdgcn_sched_barrier(0);
+    if (sg.t0 < sg.t1) form_decays(decays[0], sg.t0);
     int at_decays = 0;
     for (int64_t t0 = sg.t0; t0 < sg.t1; t0 += Q, at_decays ^= 1) {
         const TileDecays* dec = decays[at_decays];
@@ -369,32 +373,33 @@ __global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_ke
             for (int q = 0; q < 2; ++q) {
                 const f32x4 w0 = *reinterpret_cast<const f32x4*>(dec[hb].w + 32 * q + 8 * g);
                 const f32x4 w1 = *reinterpret_cast<const f32x4*>(dec[hb].w + 32 * q + 8 * g + 4);
-                bf16x8 hi[kTiles], lo[kTiles];
+                // three pieces: the upper 16 bits as they are, twice, and the rest
+                bf16x8 xw[3][kTiles];
 #pragma unroll
                 for (int pt = 0; pt < kTiles; ++pt) {
-                    // hi: the upper 16 bits as they are; lo: what is left
                     float v[8];
                     unpack8(__builtin_bit_cast(uint4, xf[pt][q]), v);
-                    uint32_t up[4];
 #pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        v[e] *= e < 4 ? w0[e & 3] : w1[e & 3];
-                        v[e + 1] *= e < 4 ? w0[(e & 3) + 1] : w1[(e & 3) + 1];
-                        up[e / 2] = __builtin_amdgcn_perm(__float_as_uint(v[e + 1]), __float_as_uint(v[e]), 0x07060302u);
-                        v[e] -= __uint_as_float(__float_as_uint(v[e]) & 0xFFFF0000u);
-                        v[e + 1] -= __uint_as_float(__float_as_uint(v[e + 1]) & 0xFFFF0000u);
+                    for (int e = 0; e < 8; ++e) v[e] *= e < 4 ? w0[e & 3] : w1[e & 3];
+#pragma unroll
+                    for (int c = 0; c < 3; ++c) {
+                        uint32_t up[4];
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) {
+                            up[e / 2] = __builtin_amdgcn_perm(__float_as_uint(v[e + 1]), __float_as_uint(v[e]), 0x07060302u);
+                            v[e] -= __uint_as_float(__float_as_uint(v[e]) & 0xFFFF0000u);
+                            v[e + 1] -= __uint_as_float(__float_as_uint(v[e + 1]) & 0xFFFF0000u);
+                        }
+                        xw[c][pt] = frag(make_uint4(up[0], up[1], up[2], up[3]));
                     }
-                    hi[pt] = frag(make_uint4(up[0], up[1], up[2], up[3]));
-                    lo[pt] = frag(pack8(v));
                 }
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     const bf16x8 bf = column_frag<8>(Bs, NS, 32 * q + 8 * g, 32 * (j / 2) + 4 * (j & 1), lr);
 #pragma unroll
-                    for (int pt = 0; pt < kTiles; ++pt) {
-                        S[pt][j] = mfma_bf16(bf, lo[pt], S[pt][j]);
-                        S[pt][j] = mfma_bf16(bf, hi[pt], S[pt][j]);
-                    }
+                    for (int c = 2; c >= 0; --c)
+#pragma unroll
+                        for (int pt = 0; pt < kTiles; ++pt) S[pt][j] = mfma_bf16(bf, xw[c][pt], S[pt][j]);
                 }
             }
         }
@@ -408,8 +413,8 @@ __global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_ke
 #pragma unroll
             for (int j = 0; j < NT; ++j)
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, S[pt][j]), to, state_at(pt, j), 0, 0);
-        if (kStateOnly && wave < kHeads && lane == 0 && unit % tiles == 0)
-            a.decay[slot * H + h0 + wave] = exp2f(float(total));
+        if (kStateOnly && wave < kHeads && lane == 0 && p0 == 0)
+            a.decay[int64_t(slot) * H + h0 + wave] = exp2f(float(total));
     }
 }
 
@@ -418,12 +423,12 @@ __global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_ke
 // quarter g, so step (j, i) takes element 16 j + 4 g + i: a lane's four i are
 // one 16-byte read of a row, and the state's accumulators are again an operand
 // as they lie.
-template <class Act, int kNP, int kHeads, int kTiles, bool kStateOnly>
-__global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
-    constexpr int Q = 32, NS = kNP + 4, PW = 64 * kTiles, PH = PW / kHeads, XS = PW + 4, WS = Q + 4;
+template <class Act, int kNP, int kHeads, int kWaves, bool kStateOnly>
+__global__ __launch_bounds__(64 * kWaves, kNP <= 128 ? kWaves / 2 : kWaves / 4) void scan_f32_kernel(ScanArgs a) {
+    constexpr int Q = 32, kThreads = 64 * kWaves, NS = kNP + 4, PW = 16 * kWaves, PH = PW / kHeads, XS = PW + 4, WS = Q + 4;
     constexpr int kRowsN = kNP / 8;
-    constexpr int kLoadN = Q * kRowsN / kScanThreads > 0 ? Q * kRowsN / kScanThreads : 1;
-    constexpr int kLoadX = Q * (PW / 8) / kScanThreads;
+    constexpr int kLoadN = Q * kRowsN / kThreads > 0 ? Q * kRowsN / kThreads : 1;
+    constexpr int kLoadX = Q * (PW / 8) / kThreads;
     constexpr int NT = kNP / 16;
     __shared__ __attribute__((aligned(16))) float Bs[Q * NS], Cs[kStateOnly ? 4 : Q * NS], Xs[Q * XS],
         Ws[kStateOnly ? 4 : kHeads * Q * WS];
@@ -432,18 +437,19 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, lr = lane & 15;
     const int P = a.P, N = a.N, H = a.H;
-    const int tiles = (P + PH - 1) / PH, units = H / kHeads * tiles;
-    const int unit = blockIdx.x % units;
-    const int64_t slot = blockIdx.x / units;
-    const int h0 = unit / tiles * kHeads, p0 = unit % tiles * PH;
-    const int grp = h0 / (H / a.G);
-    const Segment sg = segment_of(a.cu, a.runs, a.L, a.seg, slot);
+    const int tiles = (P + PH - 1) / PH;
+    const int unit = blockIdx.x, slot = blockIdx.y + blockIdx.z * kMaxGridY;
+    if (slot >= a.slots) return;
+    const int pair = tiles == 1 ? unit : unit / tiles;
+    const int h0 = pair * kHeads, p0 = tiles == 1 ? 0 : (unit - pair * tiles) * PH;
+    const int grp = a.G == 1 ? 0 : h0 / (H / a.G);
+    const Segment sg = segment_of(a.cu, a.runs, a.L, a.shift, slot);
     if (sg.run < 0) return;
-    const int hb = wave * kHeads / 4, h = h0 + hb;
-    const int pw = wave * 16 * kTiles;
+    const int hb = wave * kHeads / kWaves, h = h0 + hb;
+    const int pw = wave * 16;
     const int pl = p0 + pw - hb * PH;
 
-    constexpr int es = sizeof(St), kStepN = kScanThreads / kRowsN, kStepX = kScanThreads * 8 / PW;
+    constexpr int es = sizeof(St), kStepN = kThreads / kRowsN, kStepX = kThreads * 8 / PW;
     const int row_n = tid / kRowsN, n_at = tid % kRowsN * 8, row_x = tid / (PW / 8), col_x = tid % (PW / 8) * 8;
     const int at_b = n_at < N && row_n < Q ? int(row_n * a.B_stride + n_at) * es : kNowhere;
     const int at_c = n_at < N && row_n < Q ? int(row_n * a.C_stride + n_at) * es : kNowhere;
@@ -480,24 +486,24 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
         *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
     };
 
-    f32x4 S[kTiles][NT];
-    const int64_t slot_state = (slot * H + h) * P, run_state = (int64_t(sg.run) * H + h) * P;
-    const auto from = buffer_at(kStateOnly ? nullptr : a.segmented ? a.part + slot_state * N
-                                             : a.S_in ? a.S_in + run_state * N : nullptr);
-    const auto state_at = [&](int pt, int j) {
-        const int p = pl + 16 * pt + lr, n = 16 * j + 4 * g;
-        return p < P && n < N ? (p * N + n) * 4 : kNowhere;
-    };
-#pragma unroll
-    for (int pt = 0; pt < kTiles; ++pt)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) S[pt][j] = __builtin_bit_cast(f32x4, load16(from, state_at(pt, j), 0));
     const float rate = wave < kHeads ? -expf(a.A_log[h0 + wave]) : 0.f;
     const float dtb = wave < kHeads ? a.dt_bias[h0 + wave] : 0.f;
     const float skip = !kStateOnly && a.D ? a.D[h] : 0.f;
     double total = 0.0;
 
+    f32x4 S[NT];
+    const int64_t slot_state = (int64_t(slot) * H + h) * P, run_state = (int64_t(sg.run) * H + h) * P;
+    const auto from = buffer_at(kStateOnly ? nullptr : a.segmented ? a.part + slot_state * N
+                                             : a.S_in ? a.S_in + run_state * N : nullptr);
+    const auto state_at = [&](int j) {
+        const int p = pl + lr, n = 16 * j + 4 * g;
+        return p < P && n < N ? (p * N + n) * 4 : kNowhere;
+    };
     if (sg.t0 < sg.t1) fetch(sg.t0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) S[j] = __builtin_bit_cast(f32x4, load16(from, state_at(j), 0));
+    __builtin_amdgcn_sched_barrier(0);
     for (int64_t t0 = sg.t0; t0 < sg.t1; t0 += Q) {
 #pragma unroll
         for (int i = 0; i < kLoadN; ++i) {
@@ -517,11 +523,12 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
         if (t0 + Q < sg.t1) fetch(t0 + Q);
 
         if constexpr (!kStateOnly) {
-            // tile (tt, j) of the scores per wave: (0, 0), none, (1, 0), (1, 1)
-            const int tt = wave >> 1, j = wave & 1;
+            // tile (tt, j) of the scores per wave: (0, 0), none, (1, 0), (1, 1);
+            // of eight waves the upper four take the second head's, if any
+            const int tt = (wave >> 1) & 1, j = wave & 1, part = wave >> 2;
             const int t = 16 * tt + lr, s0 = 16 * j + 4 * g;
             f32x4 sc = {0.f, 0.f, 0.f, 0.f};
-            if (j <= tt) {
+            if (j <= tt && part < kHeads) {
 #pragma unroll
                 for (int k = 0; k < NT; ++k) {
                     const f32x4 bv = *reinterpret_cast<const f32x4*>(Bs + (16 * j + lr) * NS + 16 * k + 4 * g);
@@ -530,7 +537,8 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
                     for (int i = 0; i < 4; ++i) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[i], cv[i], sc, 0, 0, 0);
                 }
 #pragma unroll
-                for (int hh = 0; hh < kHeads; ++hh) {
+                for (int hi = 0; hi < (kWaves == 8 ? 1 : kHeads); ++hi) {
+                    const int hh = kWaves == 8 ? part : hi;
                     const float thi = dec[hh].hi[t], tlo = dec[hh].lo[t];
                     f32x4 v;
 #pragma unroll
@@ -544,22 +552,18 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
             __syncthreads();
         }
 
-        float xf[kTiles][Q / 16][4];  // x[16 j + 4 g + i] of the lane's row
+        float xf[Q / 16][4];  // x[16 j + 4 g + i] of the lane's row
 #pragma unroll
-        for (int pt = 0; pt < kTiles; ++pt)
+        for (int j = 0; j < Q / 16; ++j)
 #pragma unroll
-            for (int j = 0; j < Q / 16; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) xf[pt][j][i] = Xs[(16 * j + 4 * g + i) * XS + pw + 16 * pt + lr];
+            for (int i = 0; i < 4; ++i) xf[j][i] = Xs[(16 * j + 4 * g + i) * XS + pw + lr];
 
         if constexpr (!kStateOnly) {
             const int left = int(min(sg.t1 - t0, int64_t(Q)));
             const auto yr = buffer_at(static_cast<char*>(a.y) + ((t0 * H + h) * P) * (a.y_dtype == GDN_F32 ? 4 : 2));
-            f32x4 y[kTiles][Q / 16];
+            f32x4 y[Q / 16];
 #pragma unroll
-            for (int pt = 0; pt < kTiles; ++pt)
-#pragma unroll
-                for (int tt = 0; tt < Q / 16; ++tt) y[pt][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int tt = 0; tt < Q / 16; ++tt) y[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < NT; ++k)
 #pragma unroll
@@ -567,46 +571,36 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
                     const f32x4 cv = *reinterpret_cast<const f32x4*>(Cs + (16 * tt + lr) * NS + 16 * k + 4 * g);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int pt = 0; pt < kTiles; ++pt)
-                            y[pt][tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(S[pt][k][i], cv[i], y[pt][tt], 0, 0, 0);
+                        y[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(S[k][i], cv[i], y[tt], 0, 0, 0);
                 }
 #pragma unroll
             for (int tt = 0; tt < Q / 16; ++tt) {
-                const int t = 16 * tt + lr;
-                const float e = dec[hb].e[t];
-#pragma unroll
-                for (int pt = 0; pt < kTiles; ++pt) y[pt][tt] *= e;
+                const int t = 16 * tt + lr, p = pl + 4 * g;
+                y[tt] *= dec[hb].e[t];
 #pragma unroll
                 for (int j = 0; j <= tt; ++j) {
                     const f32x4 wv = *reinterpret_cast<const f32x4*>(Ws + (hb * Q + t) * WS + 16 * j + 4 * g);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int pt = 0; pt < kTiles; ++pt)
-                            y[pt][tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(xf[pt][j][i], wv[i], y[pt][tt], 0, 0, 0);
+                        y[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(xf[j][i], wv[i], y[tt], 0, 0, 0);
                 }
+                f32x4 o = y[tt];
+                if (a.D) {
+                    const f32x4 xv = *reinterpret_cast<const f32x4*>(Xs + t * XS + pw + 4 * g);
 #pragma unroll
-                for (int pt = 0; pt < kTiles; ++pt) {
-                    const int p = pl + 16 * pt + 4 * g;
-                    f32x4 o = y[pt][tt];
-                    if (a.D) {
-                        const f32x4 xv = *reinterpret_cast<const f32x4*>(Xs + t * XS + pw + 16 * pt + 4 * g);
+                    for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(skip, xv[i], o[i]);
+                }
+                const bool in = t < left && p < P;
+                const int at = (t * H * P + p) * (a.y_dtype == GDN_F32 ? 4 : 2);
+                if (a.y_dtype == GDN_F32) {
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), yr, in ? at : kNowhere, 0, 0);
+                } else {
+                    uint16_t b[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(skip, xv[i], o[i]);
-                    }
-                    const bool in = t < left && p < P;
-                    const int at = (t * H * P + p) * (a.y_dtype == GDN_F32 ? 4 : 2);
-                    if (a.y_dtype == GDN_F32) {
-                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), yr, in ? at : kNowhere, 0, 0);
-                    } else {
-                        uint16_t b[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            b[i] = a.y_dtype == GDN_BF16 ? f32_to_bf16_bits(o[i]) : f32_to_f16_bits(o[i]);
-                        __builtin_amdgcn_raw_buffer_store_b64(u32x2{b[0] | uint32_t(b[1]) << 16, b[2] | uint32_t(b[3]) << 16},
-                                                              yr, in ? at : kNowhere, 0, 0);
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        b[i] = a.y_dtype == GDN_BF16 ? f32_to_bf16_bits(o[i]) : f32_to_f16_bits(o[i]);
+                    __builtin_amdgcn_raw_buffer_store_b64(u32x2{b[0] | uint32_t(b[1]) << 16, b[2] | uint32_t(b[3]) << 16},
+                                                          yr, in ? at : kNowhere, 0, 0);
                 }
             }
         }
@@ -614,24 +608,17 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
         if (kStateOnly || !a.segmented || t0 + Q < sg.t1) {
             const float end = dec[hb].end;
 #pragma unroll
-            for (int pt = 0; pt < kTiles; ++pt)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) S[pt][j] *= end;
+            for (int j = 0; j < NT; ++j) S[j] *= end;
 #pragma unroll
             for (int q = 0; q < Q / 16; ++q) {
                 const f32x4 w = *reinterpret_cast<const f32x4*>(dec[hb].w + 16 * q + 4 * g);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float xw[kTiles];
+                    const float xw = xf[q][i] * w[i];
 #pragma unroll
-                    for (int pt = 0; pt < kTiles; ++pt) xw[pt] = xf[pt][q][i] * w[i];
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const float bv = Bs[(16 * q + 4 * g + i) * NS + 16 * j + lr];
-#pragma unroll
-                        for (int pt = 0; pt < kTiles; ++pt)
-                            S[pt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv, xw[pt], S[pt][j], 0, 0, 0);
-                    }
+                    for (int j = 0; j < NT; ++j)
+                        S[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(Bs[(16 * q + 4 * g + i) * NS + 16 * j + lr], xw, S[j],
+                                                                    0, 0, 0);
                 }
             }
         }
@@ -641,41 +628,54 @@ __global__ __launch_bounds__(kScanThreads) void scan_f32_kernel(ScanArgs a) {
     if (kStateOnly || !a.segmented) {
         const auto to = buffer_at(kStateOnly ? a.part + slot_state * N : a.S_out + run_state * N);
 #pragma unroll
-        for (int pt = 0; pt < kTiles; ++pt)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, S[pt][j]), to, state_at(pt, j), 0, 0);
-        if (kStateOnly && wave < kHeads && lane == 0 && unit % tiles == 0)
-            a.decay[slot * H + h0 + wave] = exp2f(float(total));
+        for (int j = 0; j < NT; ++j)
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, S[j]), to, state_at(j), 0, 0);
+        if (kStateOnly && wave < kHeads && lane == 0 && p0 == 0)
+            a.decay[int64_t(slot) * H + h0 + wave] = exp2f(float(total));
     }
 }
 
 // Chains the segments' own sums into the state before each of them, in place,
-// and the state after the run: four values of a run's state per thread.
+// and the state after the run: four values of a run's state per thread, the
+// next kAhead segments' sums in flight.
 __global__ __launch_bounds__(kScanThreads) void scan_chain_kernel(ScanArgs a) {
+    constexpr int kAhead = 8;
     const int64_t per = int64_t(a.H) * a.P * a.N / 4;
     const int64_t i = int64_t(blockIdx.x) * kScanThreads + threadIdx.x;
-    if (i >= per) return;
-    const int r = blockIdx.y + blockIdx.z * 65535;
-    if (r >= a.runs) return;
-    const int h = int(i / (int64_t(a.P) * a.N / 4));
+    const int r = blockIdx.y + blockIdx.z * kMaxGridY;
+    if (i >= per || r >= a.runs) return;
+    const int h = int(uint32_t(i) / uint32_t(a.P * a.N / 4));
     const int64_t b = run_start(a.cu, a.L, r), e = run_start(a.cu, a.L, r + 1);
-    const int64_t first = b / a.seg + r, n = (e - b + a.seg - 1) / a.seg;
+    const int64_t first = (b >> a.shift) + r;
+    const int n = int((e - b + (int64_t(1) << a.shift) - 1) >> a.shift);
     f32x4 S = {0.f, 0.f, 0.f, 0.f};
     if (a.S_in) S = reinterpret_cast<const f32x4*>(a.S_in)[r * per + i];
-    for (int64_t k = 0; k < n; ++k) {
-        f32x4* at = reinterpret_cast<f32x4*>(a.part) + (first + k) * per + i;
-        const f32x4 own = *at;
-        *at = S;
-        S = S * a.decay[(first + k) * a.H + h] + own;
+    f32x4* part = reinterpret_cast<f32x4*>(a.part) + first * per + i;
+    const float* decay = a.decay + first * a.H + h;
+    for (int k0 = 0; k0 < n; k0 += kAhead) {
+        f32x4 own[kAhead];
+        float d[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (k0 + k < n) {
+                own[k] = part[(k0 + k) * per];
+                d[k] = decay[int64_t(k0 + k) * a.H];
+            }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (k0 + k < n) {
+                part[(k0 + k) * per] = S;
+                S = S * d[k] + own[k];
+            }
     }
     reinterpret_cast<f32x4*>(a.S_out)[r * per + i] = S;
 }
 
 // How a call is split: tokens a segment, and whether there are several.
 struct ScanPlan {
-    int heads, tiles;  // heads of a workgroup, 16-row tiles of a wave
-    int64_t seg, slots, units;
+    int heads, waves;  // of a workgroup (waves of 16 head_dim rows)
+    int shift;
+    int64_t slots, units;
     bool segmented;
     int64_t bytes;
 };
@@ -683,35 +683,33 @@ struct ScanPlan {
 ScanPlan scan_plan(int N, int64_t T, int64_t longest, int G, int H, int P, int S) {
     ScanPlan p;
     const int per = H / G;
-    if (P > 64) p.heads = 1, p.tiles = 2;
-    else if (P > 32 && per % 2 == 0) p.heads = 2, p.tiles = 2;
-    else if (P > 32) p.heads = 1, p.tiles = 1;
-    else if (per % 2 == 0) p.heads = 2, p.tiles = 1;
-    else p.heads = 1, p.tiles = 1;
-    const int rows = 64 * p.tiles / p.heads;
+    p.heads = P <= 64 && per % 2 == 0 ? 2 : 1;
+    p.waves = P > 64 || (P > 32 && p.heads == 2) ? 8 : 4;
+    const int rows = 16 * p.waves / p.heads;
     p.units = int64_t(H / p.heads) * ((P + rows - 1) / rows);
     if (longest <= 0 || longest > T) longest = T;
-    p.seg = (T * p.units / 512 + 63) / 64 * 64;
-    if (p.seg < 256) p.seg = 256;
-    p.segmented = longest > p.seg;
-    if (!p.segmented) p.seg = T + 1;
-    p.slots = T / p.seg + N;
+    p.shift = 8;
+    while (p.shift < 31 && (T >> p.shift) * p.units > 640) ++p.shift;
+    p.segmented = longest > (int64_t(1) << p.shift);
+    if (!p.segmented) p.shift = 31;
+    p.slots = (T >> p.shift) + N;
     p.bytes = p.segmented ? p.slots * H * (int64_t(P) * S + 4) * 4 : 0;
     return p;
 }
 
-template <int kNP, int kHeads, int kTiles>
+template <int kNP, int kHeads, int kWaves>
 void launch_scan(const ScanArgs& a, int act_dtype, bool bf16, bool state_only, dim3 grid, hipStream_t s) {
-    const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kScanThreads), 0, s, a); };
+    // (kWaves of 16 head_dim rows, or in bfloat16 four of up to 32)
+    const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(bf16 ? kScanThreads : 64 * kWaves), 0, s, a); };
     if (bf16) {
-        if (state_only) go(scan_bf16_kernel<kNP, kHeads, kTiles, true>);
-        else go(scan_bf16_kernel<kNP, kHeads, kTiles, false>);
+        if (state_only) go(scan_bf16_kernel<kNP, kHeads, kWaves / 4, true>);
+        else go(scan_bf16_kernel<kNP, kHeads, kWaves / 4, false>);
         return;
     }
     const auto f32 = [&](auto act) {
         using Act = decltype(act);
-        if (state_only) go(scan_f32_kernel<Act, kNP, kHeads, kTiles, true>);
-        else go(scan_f32_kernel<Act, kNP, kHeads, kTiles, false>);
+        if (state_only) go(scan_f32_kernel<Act, kNP, kHeads, kWaves, true>);
+        else go(scan_f32_kernel<Act, kNP, kHeads, kWaves, false>);
     };
     if (act_dtype == GDN_F32) f32(ActF32{});
     else if (act_dtype == GDN_F16) f32(ActF16{});
@@ -721,10 +719,10 @@ void launch_scan(const ScanArgs& a, int act_dtype, bool bf16, bool state_only, d
 template <int kNP>
 void launch_scan_shape(const ScanPlan& p, const ScanArgs& a, int act_dtype, bool bf16, bool state_only, dim3 grid,
                        hipStream_t s) {
-    if (p.heads == 2 && p.tiles == 2) launch_scan<kNP, 2, 2>(a, act_dtype, bf16, state_only, grid, s);
-    else if (p.heads == 2) launch_scan<kNP, 2, 1>(a, act_dtype, bf16, state_only, grid, s);
-    else if (p.tiles == 2) launch_scan<kNP, 1, 2>(a, act_dtype, bf16, state_only, grid, s);
-    else launch_scan<kNP, 1, 1>(a, act_dtype, bf16, state_only, grid, s);
+    if (p.heads == 2 && p.waves == 8) launch_scan<kNP, 2, 8>(a, act_dtype, bf16, state_only, grid, s);
+    else if (p.heads == 2) launch_scan<kNP, 2, 4>(a, act_dtype, bf16, state_only, grid, s);
+    else if (p.waves == 8) launch_scan<kNP, 1, 8>(a, act_dtype, bf16, state_only, grid, s);
+    else launch_scan<kNP, 1, 4>(a, act_dtype, bf16, state_only, grid, s);
 }
 
 bool scan_sizes_ok(int N, int64_t T, int G, int H, int P, int S) {
@@ -780,14 +778,18 @@ extern "C" int gdn_selective_scan(const void* x, int64_t x_stride, const void* B
     GDN_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes),
                 "gdn_selective_scan: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                 (long long)p.bytes);
-    GDN_REQUIRE(p.slots * p.units <= INT32_MAX, "gdn_selective_scan: too many workgroups");
+    GDN_REQUIRE(p.slots <= INT32_MAX && p.units <= INT32_MAX && int64_t(H) * P * S / 4 <= INT32_MAX,
+                "gdn_selective_scan: too many runs or heads");
     float* part = static_cast<float*>(workspace);
     ScanArgs a{x, B, C, dt, x_stride, B_stride, C_stride, dt_stride, dt_dtype, A_log, dt_bias, D, state_in,
-               state_out, y, y_dtype, cu_seqlens, N, T_total, T_total / N, p.seg, G, H, P, S, part,
-               part ? part + p.slots * H * int64_t(P) * S : nullptr, p.segmented};
+               state_out, y, y_dtype, cu_seqlens, N, T_total / N, p.shift, G, H, P, S, part,
+               part ? part + p.slots * H * int64_t(P) * S : nullptr, p.segmented, int(p.slots)};
     const bool bf16 = act_dtype == GDN_BF16 && y_dtype == GDN_BF16;
     hipStream_t s = as_stream(stream);
-    const dim3 grid(unsigned(p.slots * p.units));
+    const auto tall = [](int64_t x, int64_t n) {
+        return dim3(unsigned(x), unsigned(n < kMaxGridY ? n : kMaxGridY), unsigned((n + kMaxGridY - 1) / kMaxGridY));
+    };
+    const dim3 grid = tall(p.units, p.slots);
     const auto pass = [&](bool state_only) {
         if (S <= 32) launch_scan_shape<32>(p, a, act_dtype, bf16, state_only, grid, s);
         else if (S <= 64) launch_scan_shape<64>(p, a, act_dtype, bf16, state_only, grid, s);
@@ -797,10 +799,7 @@ extern "C" int gdn_selective_scan(const void* x, int64_t x_stride, const void* B
     if (p.segmented) {
         pass(true);
         const int64_t per = int64_t(H) * P * S / 4;
-        hipLaunchKernelGGL(scan_chain_kernel,
-                           dim3(unsigned((per + kScanThreads - 1) / kScanThreads), unsigned(N < 65535 ? N : 65535),
-                                unsigned((N + 65534) / 65535)),
-                           dim3(kScanThreads), 0, s, a);
+        hipLaunchKernelGGL(scan_chain_kernel, tall((per + kScanThreads - 1) / kScanThreads, N), dim3(kScanThreads), 0, s, a);
     }
     pass(false);
     return check_launch("gdn_selective_scan");
