@@ -543,8 +543,8 @@ int gdn_selective_step(const void *xbc, int64_t xbc_stride, const void *dt, int6
  *   x: (M, K) x_dtype; w: (N, K) e4m3 (fn) bytes; scales: (ceil(N / 128),
  *   ceil(K / 128)) float32; y: (M, N) y_dtype; residual: NULL or (M, N) y_dtype
  *   (may be y), added to the product rounded to y_dtype
- *   workspace: gdn_fp8_matmul_workspace_size(...) bytes; calls sharing one must
- *   not overlap
+ *   workspace: gdn_fp8_matmul_workspace_size(...) bytes (0: none needed, for
+ *   few rows); calls sharing one must not overlap
  * K a multiple of 16; x, w, y and workspace 16-byte aligned. NaN or infinity in
  * x makes its row NaN. No reference counterpart (a scheme beside
  * moe_block.py:44-55's).

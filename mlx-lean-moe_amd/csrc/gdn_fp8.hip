@@ -5,8 +5,10 @@
 //   y[m, n] = sum_b s[m, b] sw[n / 128, b] sum_{k in b} q[m, k] w[n, k],
 // the inner sums on the 8-bit matrix cores (one 16x16x128 product per block, so
 // scales meet float32 sums only), the outer one in float32.
-#include "gdn_host.h"
+#include <type_traits>
+
 #include "gdn_common.h"
+#include "gdn_host.h"
 #include "gdn_ssm.h"
 
 namespace gdn {
@@ -34,6 +36,26 @@ GDN_DEV float scale_of(uint32_t amax_bits) {
     return s < 0x1p-126f ? 0x1p-126f : s;
 }
 
+// x / s to the last bit for the lane's values, s one group's scale: two
+// Newton corrections of x times the rounded reciprocal, each remainder exact
+// (the second starts within one ulp and so ends correctly rounded). Remainders
+// of the smallest scales would leave float32: divisions there.
+template <int N>
+GDN_DEV void divide_all(float (&x)[N], float s) {
+    if (s < 0x1p-80f) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = x[e] / s;
+        return;
+    }
+    const float inv = 1.f / s;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        float r = x[e] * inv;
+        r = __builtin_fmaf(__builtin_fmaf(-r, s, x[e]), inv, r);
+        x[e] = __builtin_fmaf(__builtin_fmaf(-r, s, x[e]), inv, r);
+    }
+}
+
 // Codes of four values.
 GDN_DEV uint32_t codes4(float a, float b, float c, float d) {
     int r = 0;
@@ -57,8 +79,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const typename Act::s
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
     const float s = scale_of(row16_max(top));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = v[e] / s;
+    divide_all(v, s);
     if (first >= groups) return;
     *reinterpret_cast<uint2*>(codes + int64_t(m) * kb * kB + k) =
         make_uint2(codes4(v[0], v[1], v[2], v[3]), codes4(v[4], v[5], v[6], v[7]));
@@ -327,6 +348,100 @@ __global__ __launch_bounds__(64 * kWN * kWM) void fp8_tile_kernel(Fp8Args a) {
     }
 }
 
+// Up to 16 rows of x, in one launch: each workgroup quantizes them itself into
+// LDS (codes and scales, K whole), while its first blocks of W are on their
+// way, then its 16 waves take kNs x 16 rows of W and every (16 / kNs)-th block
+// of K each, straight from memory into the left operand, and add their sums in
+// LDS. No wave waits for another until then. W is read once, and that is what
+// bounds it; the launches that the tiles need (rows' codes, product, sum of the
+// split) cost more than the product at these sizes. Every workgroup quantizes the
+// same rows, so there is an end to it: kSkinnyGroups groups of 128 values.
+// Measured, us, this against the launches of the tiles: 2048 -> 12352 1 row 7.8
+// (3.3 TB/s), 12.7; 16 rows 11.7, 16.2; 4096 -> 2048 1 row 5.3, 11.1; 12 rows (384
+// groups) 10.6, 11.7; 16 rows (512) 12.7, 11.9; 8192 -> 8192 4 rows (256) 18.3,
+// 21.0; 8 rows (512) 23.8, 21.7.
+constexpr int kSkinnyRows = 16, kSkinnyWaves = 16, kSkinnyGroups = 384;
+constexpr int kAhead = 4;  // blocks of W in flight a wave
+
+template <class Act, int kNs, bool kExact>
+__global__ __launch_bounds__(64 * kSkinnyWaves) void fp8_skinny_kernel(Fp8Args a, const typename Act::storage* x) {
+    constexpr int kGroups = kSkinnyWaves / kNs;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int g = lane >> 4, lr = lane & 15;
+    const int Kq = a.kb * kB, stride = Kq + 16;  // (rows 16 bytes apart in the banks)
+    uint8_t* codes = lds;
+    float* sx = reinterpret_cast<float*>(lds + a.M * stride);
+
+    const int sub = wave % kNs, group = wave / kNs;
+    const int n0 = (blockIdx.x * kNs + sub) * 16;
+    const uint8_t* wr = a.w + int64_t(min(n0 + lr, a.N - 1)) * a.K + 32 * g;
+    const float* sw = a.sw + int64_t(min(n0, a.N - 1) / kB) * a.kb;
+    uint4 w[kAhead][2];
+    float sn[kAhead];
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    const auto fetch = [&](int b, uint4 (&v)[2], float& s) {
+        const int k = b * kB + 32 * g;
+        v[0] = v[1] = zero;
+        s = 0.f;
+        if (b < a.kb) {
+            s = sw[b];
+            if (k < a.K) v[0] = *reinterpret_cast<const uint4*>(wr + b * kB);
+            if (k + 16 < a.K) v[1] = *reinterpret_cast<const uint4*>(wr + b * kB + 16);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) fetch(group + i * kGroups, w[i], sn[i]);
+
+    for (int at = tid / 16; at < a.M * a.kb; at += 4 * kSkinnyWaves) {
+        const int m = at / a.kb, b = at % a.kb, k = b * kB + (tid & 15) * 8;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (k < a.K) load8f<Act>(x + int64_t(m) * a.K + k, v);
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+        const float s = scale_of(row16_max(top));
+        divide_all(v, s);
+        *reinterpret_cast<uint2*>(codes + m * stride + k) =
+            make_uint2(codes4(v[0], v[1], v[2], v[3]), codes4(v[4], v[5], v[6], v[7]));
+        if ((tid & 15) == 0) sx[m * a.kb + b] = s;
+    }
+    __syncthreads();
+
+    const int m = min(lr, a.M - 1);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int b0 = group; b0 < a.kb; b0 += kAhead * kGroups)
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int b = b0 + i * kGroups;
+            if (b >= a.kb) break;
+            const uint8_t* q = codes + m * stride + b * kB + 32 * g;
+            const uint4 q0 = *reinterpret_cast<const uint4*>(q), q1 = *reinterpret_cast<const uint4*>(q + 16);
+            const f32x4 p = kExact ? mfma_widened(w[i][0], w[i][1], q0, q1) : mfma_fp8(w[i][0], w[i][1], q0, q1);
+            const float s = sx[m * a.kb + b] * sn[i];
+            fetch(b + kAhead * kGroups, w[i], sn[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(s, p[e], acc[e]);
+        }
+    __syncthreads();
+    f32x4* sums = reinterpret_cast<f32x4*>(lds);  // over the codes
+    sums[wave * 64 + lane] = acc;
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+        for (int i = 1; i < kGroups; ++i) acc += sums[(i * kNs + sub) * 64 + lane];
+        store4(a, lr, n0 + 4 * g, acc);
+    }
+}
+
+// LDS of a skinny product: codes and scales, and at least the 16 waves' sums.
+int64_t skinny_bytes(int M, int kb) {
+    const int64_t need = int64_t(M) * (kb * kB + 16 + kb * 4);
+    return need > kSkinnyWaves * 1024 ? need : kSkinnyWaves * 1024;
+}
+
+bool skinny(int M, int kb) { return M <= kSkinnyRows && int64_t(M) * kb <= kSkinnyGroups; }
+
 // Adds the shares of a split product in their order: four columns a thread.
 __global__ __launch_bounds__(256) void fp8_sum_kernel(Fp8Args a, int splits) {
     const int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4, per = int64_t(a.M) * a.N4;
@@ -445,6 +560,7 @@ using namespace gdn;
 extern "C" int64_t gdn_fp8_matmul_workspace_size(int y_dtype, int M, int N, int K) {
     if (!fp8_sizes_ok(M, N, K) || !valid_dtype(y_dtype)) return 0;
     const int kb = (K + kB - 1) / kB;
+    if (skinny(M, kb)) return 0;
     return codes_bytes(M, K) + int64_t(scale_columns(M)) * kb * 4 + fp8_plan(y_dtype == GDN_F32, M, N, kb).part_bytes;
 }
 
@@ -458,15 +574,43 @@ extern "C" int gdn_fp8_matmul(const void* x, int x_dtype, const void* w, const f
     GDN_REQUIRE((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(y) |
                  reinterpret_cast<uintptr_t>(workspace)) % 16 == 0,
                 "gdn_fp8_matmul: x, w, y and workspace must be 16-byte aligned");
+    const int kb = (K + kB - 1) / kB, ldx = scale_columns(M);
+    hipStream_t s = as_stream(stream);
+    if (skinny(M, kb)) {
+        const Fp8Args a{nullptr, static_cast<const uint8_t*>(w), nullptr, scales, residual, y, y_dtype, M, N, K, kb, 0, kb,
+                        nullptr, 0};
+        const unsigned bytes = unsigned(skinny_bytes(M, kb));
+        // 64 rows of W a workgroup, 32 or 16: as many as still give most CUs one
+        // (1 row, us, 16, 32 and 64: 12352 outputs 9.8, 8.0, 7.8; 8192 5.2, 4.9, 5.1;
+        // 2048 5.3, 7.0, 10.5)
+        const auto go = [&](auto act, auto exact) {
+            using Act = decltype(act);
+            constexpr bool E = decltype(exact)::value;
+            const auto* xs = static_cast<const typename Act::storage*>(x);
+            const dim3 threads(64 * kSkinnyWaves);
+            const auto launch = [&](auto kernel, int rows) {
+                hipLaunchKernelGGL(kernel, dim3(unsigned((N + rows - 1) / rows)), threads, bytes, s, a, xs);
+            };
+            if (N > 64 * 190) launch(fp8_skinny_kernel<Act, 4, E>, 64);
+            else if (N > 32 * 190) launch(fp8_skinny_kernel<Act, 2, E>, 32);
+            else launch(fp8_skinny_kernel<Act, 1, E>, 16);
+        };
+        const auto typed = [&](auto act) {
+            if (y_dtype == GDN_F32) go(act, std::true_type{});
+            else go(act, std::false_type{});
+        };
+        if (x_dtype == GDN_F32) typed(ActF32{});
+        else if (x_dtype == GDN_BF16) typed(ActBF16{});
+        else typed(ActF16{});
+        return check_launch("gdn_fp8_matmul");
+    }
     const int64_t need = gdn_fp8_matmul_workspace_size(y_dtype, M, N, K);
     GDN_REQUIRE(workspace && workspace_bytes >= need, "gdn_fp8_matmul: workspace of %lld bytes, %lld needed",
                 (long long)workspace_bytes, (long long)need);
-    const int kb = (K + kB - 1) / kB, ldx = scale_columns(M);
     const int64_t blocks = (int64_t(M) * kb + 15) / 16;
     GDN_REQUIRE(blocks <= INT32_MAX && int64_t(ldx) * kb <= INT32_MAX / 4, "gdn_fp8_matmul: too many rows");
     uint8_t* codes = static_cast<uint8_t*>(workspace);
     float* sx = reinterpret_cast<float*>(codes + codes_bytes(M, K));
-    hipStream_t s = as_stream(stream);
     const auto quantize = [&](auto act) {
         using Act = decltype(act);
         hipLaunchKernelGGL(fp8_quantize_kernel<Act>, dim3(unsigned(blocks)), dim3(256), 0, s,

@@ -131,7 +131,7 @@ def test_fp8_refusals():
                                  wb=1 << 20), **kw}[k] for k in "x xd w s y yd r M N K ws wb".split()] + [None]
     for kw, what in ((dict(K=250), "bad sizes"), (dict(N=0), "bad sizes"), (dict(M=-1), "bad sizes"),
                      (dict(xd=7), "dtype"), (dict(w=None), "null"), (dict(x=ctypes.c_void_p(8)), "aligned"),
-                     (dict(ws=None), "workspace"), (dict(wb=1000), "workspace")):
+                     (dict(M=40, ws=None), "workspace"), (dict(M=40, wb=1000), "workspace")):
         _refused(lib.gdn_fp8_matmul(*args(**kw)), E, what)
     assert lib.gdn_fp8_matmul(*args(M=0)) == 0
     assert lib.gdn_fp8_matmul_workspace_size(1, 4, 64, 250) == 0
