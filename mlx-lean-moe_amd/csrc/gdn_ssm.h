@@ -49,9 +49,9 @@ template <int kDt, int N>
 GDN_DEV void silu_all(float (&x)[N]) {
 #pragma clang fp contract(off)
     constexpr float kL = 1.44269504088896341f, kLLow = 1.92596299112661746e-8f, kLn2 = 0.693147180559945309f;
-    bool low = false;
+    float least = x[0];
 #pragma unroll
-    for (int i = 0; i < N; ++i) low = low || x[i] < -80.f;
+    for (int i = 1; i < N; ++i) least = fminf(least, x[i]);
     float y[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -67,7 +67,7 @@ GDN_DEV void silu_all(float (&x)[N]) {
             y[i] = x[i] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-x[i] * kL));
         }
     }
-    if (__builtin_amdgcn_ballot_w64(low) != 0) {
+    if (__builtin_amdgcn_ballot_w64(least < -80.f) != 0) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (x[i] < -80.f) {

@@ -3,39 +3,61 @@
 // the rows before a run taken from its conv state; the new state is the last
 // K - 1 rows of state and run together. float32 throughout, one rounding.
 //
-// It reads and writes each element once: memory-bound. A thread owns kVec
-// neighbouring channels (16 bytes where the layout allows) over a tile of
-// kTile tokens and slides the K - 1 previous rows through registers, so that
-// a row is read once plus K - 1 halo rows a tile.
+// It reads and writes each element once: memory-bound, with the vector units
+// close behind (about 70 cycles of a SIMD per 64 elements, exp2 and reciprocal
+// half of them). A lane owns V neighbouring channels (16 bytes where the layout
+// allows) over a tile of tokens and slides the K - 1 previous rows through
+// registers; the rows of a tile come kConvAhead at a time, the next while these
+// are used. A workgroup's four waves hold the same channels of four tiles that
+// follow each other, so the taps (4 V K bytes a lane, as much as a tile of 16-bit
+// values) and the K - 1 rows before a tile come from the CU's own cache.
+//
+// Measured, 6144 channels: 4096 bf16 tokens 26.4 us (3.8 TB/s; a copy of the same
+// bytes 20.9), 16384 82.8 (4.9 TB/s; 75), 41 5.5; 4096 float32 tokens 39.7 (5.1
+// TB/s; 39.0).
 #include "gdn_host.h"
 #include "gdn_ssm.h"
 
 namespace gdn {
 namespace {
 
-constexpr int kConvThreads = 256;
-constexpr int kConvTile = 16;
+constexpr int kConvWaves = 4, kConvThreads = kConvWaves * kWave;
+constexpr int kConvAhead = 4;
 
 template <class Act, int V>
-GDN_DEV void conv_load(const typename Act::storage* p, float (&x)[V]) {
+GDN_DEV void conv_raw(const typename Act::storage* p, typename Act::storage (&x)[V]) {
     if constexpr (V == 1) {
-        x[0] = Act::load(p, 0);
+        x[0] = p[0];
     } else {
         typedef typename Act::storage vec __attribute__((ext_vector_type(V)));
         const vec v = *reinterpret_cast<const vec*>(p);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const typename Act::storage s = v[e];
-            x[e] = Act::load(&s, 0);
-        }
+        for (int e = 0; e < V; ++e) x[e] = v[e];
     }
+}
+
+template <class Act, int V>
+GDN_DEV void conv_load(const typename Act::storage* p, float (&x)[V]) {
+    typename Act::storage raw[V];
+    conv_raw<Act, V>(p, raw);
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = Act::load(raw, e);
 }
 
 template <class Act, int V>
 GDN_DEV void conv_store(typename Act::storage* p, const float (&x)[V]) {
     typename Act::storage s[V];
+    if constexpr (Act::code == GDN_BF16 && V % 2 == 0) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) Act::store(s, e, x[e]);
+        for (int e = 0; e < V; e += 2) {
+            const uint32_t two = pack_bf16x2(x[e], x[e + 1]);
+            s[e] = uint16_t(two);
+            s[e + 1] = uint16_t(two >> 16);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) Act::store(s, e, x[e]);
+    }
     if constexpr (V == 1) {
         p[0] = s[0];
     } else {
@@ -47,16 +69,18 @@ GDN_DEV void conv_store(typename Act::storage* p, const float (&x)[V]) {
     }
 }
 
-// Blocks y < token_tiles take tokens; the others each write one run's state.
-template <class Act, int V, int K>
+// Waves y < token_tiles take tokens; the others each write one run's state.
+template <class Act, int V, int K, int kConvTile>
 __global__ __launch_bounds__(kConvThreads) void conv_silu_kernel(
     const typename Act::storage* __restrict__ x, int64_t x_stride,
     const typename Act::storage* __restrict__ cs_in, typename Act::storage* __restrict__ cs_out,
     const float* __restrict__ w, const float* __restrict__ bias, const int32_t* __restrict__ cu, int N, int64_t L,
     int64_t T, int64_t token_tiles, typename Act::storage* __restrict__ out, int C) {
-    const int c = (blockIdx.x * kConvThreads + threadIdx.x) * V;
+    const int c = (blockIdx.x * kWave + threadIdx.x % kWave) * V;
     if (c >= C) return;
-    for (int64_t by = blockIdx.y; by < token_tiles + N; by += gridDim.y) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t rows = token_tiles + N, step = int64_t(gridDim.y) * kConvWaves;
+    for (int64_t by = int64_t(blockIdx.y) * kConvWaves + wave; by < rows; by += step) {
         if (by >= token_tiles) {
             const int r = int(by - token_tiles);
             const int64_t b = run_start(cu, L, r), e = run_start(cu, L, r + 1);
@@ -89,18 +113,8 @@ __global__ __launch_bounds__(kConvThreads) void conv_silu_kernel(
                 else conv_load<Act, V>(cs_in + (int64_t(r) * (K - 1) + (s - b) + (K - 1)) * C + c, win[j]);
             }
         };
-        fill(t0);
-        for (int64_t t = t0; t < t1; ++t) {
-            if (t >= e1) {
-                do {
-                    ++r;
-                    b = e1;
-                    e1 = run_start(cu, L, r + 1);
-                } while (t >= e1);
-                fill(t);
-            }
-            float xv[V], o[V];
-            conv_load<Act, V>(x + t * x_stride + c, xv);
+        const auto token = [&](int64_t t, const float (&xv)[V]) {
+            float o[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 float a = bv[e];
@@ -113,6 +127,41 @@ __global__ __launch_bounds__(kConvThreads) void conv_silu_kernel(
             }
             silu_all<Act::code>(o);
             conv_store<Act, V>(out + t * C + c, o);
+        };
+        if (t1 - t0 == kConvTile && e1 >= t1) {
+            typename Act::storage raw[2][kConvAhead][V];
+            const auto fetch = [&](int64_t t, typename Act::storage (&v)[kConvAhead][V]) {
+#pragma unroll
+                for (int i = 0; i < kConvAhead; ++i) conv_raw<Act, V>(x + (t + i) * x_stride + c, v[i]);
+            };
+            fetch(t0, raw[0]);
+            fill(t0);
+#pragma unroll
+            for (int i = 0; i < kConvTile / kConvAhead; ++i) {
+                if ((i + 1) * kConvAhead < kConvTile) fetch(t0 + (i + 1) * kConvAhead, raw[(i + 1) & 1]);
+#pragma unroll
+                for (int k = 0; k < kConvAhead; ++k) {
+                    float xv[V];
+#pragma unroll
+                    for (int e = 0; e < V; ++e) xv[e] = Act::load(raw[i & 1][k], e);
+                    token(t0 + i * kConvAhead + k, xv);
+                }
+            }
+            continue;
+        }
+        fill(t0);
+        for (int64_t t = t0; t < t1; ++t) {
+            if (t >= e1) {
+                do {
+                    ++r;
+                    b = e1;
+                    e1 = run_start(cu, L, r + 1);
+                } while (t >= e1);
+                fill(t);
+            }
+            float xv[V];
+            conv_load<Act, V>(x + t * x_stride + c, xv);
+            token(t, xv);
         }
     }
 }
@@ -139,30 +188,41 @@ extern "C" int gdn_conv_silu(const void* x, int64_t x_stride, const void* conv_s
     const int64_t state_bytes = int64_t(N) * (K - 1) * C * es;
     GDN_REQUIRE(!overlaps(conv_state_in, state_bytes, conv_state_out, state_bytes),
                 "gdn_conv_silu: conv_state_out overlaps conv_state_in");
-    const int64_t L = T_total / N, token_tiles = (T_total + kConvTile - 1) / kConvTile;
+    const int64_t L = T_total / N;
     const auto fits = [&](int v) {  // v channels in one aligned access everywhere
         const auto at = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(conv_state_in) |
                         reinterpret_cast<uintptr_t>(conv_state_out) | reinterpret_cast<uintptr_t>(out);
         return C % v == 0 && x_stride % v == 0 && at % (uintptr_t(v) * es) == 0;
     };
-    const int64_t rows = token_tiles + N;
-    const auto launch = [&](auto act, auto vec) {
+    const auto launch = [&](auto act, auto vec, auto tile) {
         using Act = decltype(act);
-        constexpr int V = decltype(vec)::value;
-        const dim3 grid(unsigned((C + kConvThreads * V - 1) / (kConvThreads * V)),
-                        unsigned(rows < 65535 ? rows : 65535));
-        const auto kern = K == 4 ? conv_silu_kernel<Act, V, 4> : K == 3 ? conv_silu_kernel<Act, V, 3>
-                                                                       : conv_silu_kernel<Act, V, 2>;
+        constexpr int V = decltype(vec)::value, kTile = decltype(tile)::value;
+        const int64_t token_tiles = (T_total + kTile - 1) / kTile, rows = (token_tiles + N + kConvWaves - 1) / kConvWaves;
+        const dim3 grid(unsigned((C + kWave * V - 1) / (kWave * V)), unsigned(rows < 65535 ? rows : 65535));
+        const auto kern = K == 4   ? conv_silu_kernel<Act, V, 4, kTile>
+                          : K == 3 ? conv_silu_kernel<Act, V, 3, kTile>
+                                   : conv_silu_kernel<Act, V, 2, kTile>;
         hipLaunchKernelGGL(kern, grid, dim3(kConvThreads), 0, as_stream(stream),
                            static_cast<const typename Act::storage*>(x), x_stride,
                            static_cast<const typename Act::storage*>(conv_state_in),
                            static_cast<typename Act::storage*>(conv_state_out), weight, bias, cu_seqlens, N, L,
                            T_total, token_tiles, static_cast<typename Act::storage*>(out), C);
     };
+    // Tiles of 8 tokens; of 16 where lanes hold 8 channels, there are 8 waves of
+    // them a CU and runs have 64 tokens on average. us with 8 and 16, bf16, 6144
+    // channels: 41 tokens 5.5, 6.8; 512 6.8, 8.5; 4096 28.5, 26.4; 16384 91, 83;
+    // 256 runs of 8 17.4, 24.8 (a tile that runs share goes row by row). 4096
+    // float32 tokens 39.7, 42.1.
+    const auto tiled = [&](auto act, auto vec) {
+        if constexpr (decltype(vec)::value == 8)
+            if (T_total / 16 * (C / (kWave * 8)) >= 2048 && L >= 64)
+                return launch(act, vec, std::integral_constant<int, 16>{});
+        launch(act, vec, std::integral_constant<int, 8>{});
+    };
     const auto pick = [&](auto act, auto wide, auto narrow) {
-        if (fits(decltype(wide)::value)) launch(act, wide);
-        else if (fits(decltype(narrow)::value)) launch(act, narrow);
-        else launch(act, std::integral_constant<int, 1>{});
+        if (fits(decltype(wide)::value)) tiled(act, wide);
+        else if (fits(decltype(narrow)::value)) tiled(act, narrow);
+        else tiled(act, std::integral_constant<int, 1>{});
     };
     using I2 = std::integral_constant<int, 2>;
     using I4 = std::integral_constant<int, 4>;
