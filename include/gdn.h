@@ -477,7 +477,8 @@ int64_t gdn_quantized_matmul_scheme_workspace_size(int M, int N, int K);
  *   conv_state_in: (N, K-1, C) act_dtype, the rows before each run;
  *   conv_state_out: the same, the last K-1 rows; must not overlap it
  *   weight: (C, K) float32; bias: (C) float32 or NULL; K 2, 3 or 4
- *   cu_seqlens: (N+1) int32 or NULL (N runs of T_total / N tokens)
+ *   cu_seqlens: (N+1) int32 from 0, not descending, at most T_total (rows of out
+ *   behind the last are left as they are), or NULL (N runs of T_total / N tokens)
  *   out: (T_total, C) act_dtype
  * No reference counterpart (its conv, linear_attention.py:61-79, has no bias
  * and belongs to the q/k scaling: gdn_frontend).

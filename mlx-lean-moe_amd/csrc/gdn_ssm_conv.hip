@@ -79,6 +79,7 @@ __global__ __launch_bounds__(kConvThreads) void conv_silu_kernel(
     const int c = (blockIdx.x * kWave + threadIdx.x % kWave) * V;
     if (c >= C) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t end = cu ? min(T, int64_t(cu[N])) : T;  // rows behind the last run are left as they are
     const int64_t rows = token_tiles + N, step = int64_t(gridDim.y) * kConvWaves;
     for (int64_t by = int64_t(blockIdx.y) * kConvWaves + wave; by < rows; by += step) {
         if (by >= token_tiles) {
@@ -101,7 +102,8 @@ __global__ __launch_bounds__(kConvThreads) void conv_silu_kernel(
             for (int j = 0; j < K; ++j) wr[e][j] = w[int64_t(c + e) * K + j];
             bv[e] = bias ? bias[c + e] : 0.f;
         }
-        const int64_t t0 = by * kConvTile, t1 = t0 + kConvTile < T ? t0 + kConvTile : T;
+        const int64_t t0 = by * kConvTile, t1 = min(t0 + kConvTile, end);
+        if (t0 >= end) continue;
         int r = cu ? find_run(cu, N, t0) : int(t0 / L);
         int64_t b = run_start(cu, L, r), e1 = run_start(cu, L, r + 1);
         float win[K - 1][V];

@@ -21,6 +21,7 @@ import pytest
 import torch
 
 import mlx_lean_moe_amd as gdn
+from mlx_lean_moe_amd import _lib
 from oracle import state_space_ref as R
 
 pytestmark = pytest.mark.gpu
@@ -77,6 +78,30 @@ def test_conv_silu(gpu, act, lens, C, K):
     out, new = gdn.conv_silu(x, st, w, b, cu)
     assert out.dtype == new.dtype == DT[act]
     _check_conv(out, new, x, st, w, b, lens, act)
+
+
+@pytest.mark.parametrize("act", ["bf16", "f16"])
+def test_conv_silu_of_many_tokens(gpu, act):
+    lens = [2100, 1, 0, 90, 2205]
+    x, st, w, b, cu = _conv_case(gpu, act, lens, 4104, 4, True, pad=8, seed=3)
+    out, new = gdn.conv_silu(x, st, w, b, cu)
+    _check_conv(out, new, x, st, w, b, lens, act)
+
+
+@pytest.mark.parametrize("T,C", [(60, 24), (4600, 4096)])
+def test_rows_behind_the_last_run_stay(gpu, T, C):
+    """At the C boundary the offsets may end before the arrays: what lies behind
+    the last run is neither read nor written."""
+    lens = [T // 2, T // 4 + 3]
+    end = sum(lens)
+    x, st, w, b, cu = _conv_case(gpu, "bf16", lens, C, 4, True, seed=4)
+    x = torch.cat([x, torch.full((T - end, C), float("nan"), device=gpu, dtype=x.dtype)])
+    out, new = torch.full_like(x, 7.0), torch.empty_like(st)
+    cu = torch.tensor(cu, dtype=torch.int32, device=gpu)
+    _lib.call_on(x.device, "gdn_conv_silu", x.data_ptr(), C, st.data_ptr(), new.data_ptr(), w.data_ptr(), b.data_ptr(),
+                 cu.data_ptr(), 2, T, out.data_ptr(), C, 4, _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
+    assert (out[end:] == 7).all()
+    _check_conv(out[:end], new, x[:end], st, w, b, lens, "bf16")
 
 
 @pytest.mark.parametrize("pad", [16, 6, 1])
