@@ -32,6 +32,7 @@ from .linear_attention import _index_array, _rows, check_half_bits, check_slots
 
 _MAX_STATE = 256   # state_dim, both kernels
 _MAX_HEAD = 256    # head_dim, the step kernel
+_MAX_STEP = 1 << 22  # elements between the rows that the scan reads in place
 _F32 = torch.float32
 
 
@@ -103,8 +104,9 @@ def _f32_vector(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
 def _token_rows(t: torch.Tensor, T: int, heads: int, dim: int) -> tuple[torch.Tensor, int]:
     """``t (tokens, heads, dim)``, batch-first or packed, as rows that the
     kernels read in 16-byte pieces, and their stride: in place where the rows
-    are packed, aligned and no closer than their width (column slices of one
-    projection or conv output), else a copy."""
+    are packed, aligned, no closer than their width and no further apart than
+    the kernels address (column slices of one projection or conv output), else a
+    copy."""
 
     st, width = t.stride(), heads * dim
     step, packed = st[-3], st[-1] == 1 and (st[-2] == dim or heads == 1)
@@ -115,7 +117,7 @@ def _token_rows(t: torch.Tensor, T: int, heads: int, dim: int) -> tuple[torch.Te
             packed = packed and st[0] == t.shape[1] * step
     if T <= 1:
         step = width
-    if packed and step >= width and step * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
+    if packed and width <= step <= _MAX_STEP and step * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
         return t, step
     return t.clone(memory_format=torch.contiguous_format), width
 

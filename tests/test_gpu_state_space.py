@@ -262,6 +262,16 @@ def test_scan_inputs_that_no_kernel_reads_in_place(gpu):
     _check_scan(gdn.selective_scan(**case, cu_seqlens=[0, 50, 87]), case, lens, "bf16", "bf16")
 
 
+def test_scan_of_rows_far_apart(gpu):
+    """Rows further apart than the kernels address in place."""
+    case = _scan_case(gpu, "bf16", [3], (2, 8, 1, 16), seed=9)
+    far = torch.empty(3, (1 << 22) + 8, dtype=torch.bfloat16, device=gpu)
+    far[:, :16] = case["x"].reshape(3, 16)
+    want = gdn.selective_scan(**case, cu_seqlens=[0, 3])
+    got = gdn.selective_scan(**dict(case, x=far[:, :16].unflatten(1, (2, 8))), cu_seqlens=[0, 3])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_scan_of_no_tokens(gpu):
     case = _scan_case(gpu, "bf16", [0, 0], (2, 64, 1, 128), seed=9)
     y, S = gdn.selective_scan(**case, cu_seqlens=[0, 0, 0])
