@@ -79,6 +79,17 @@ def test_larger_products_with_residual(gpu, act, M, N, K):
         assert torch.equal(y, plain + res)
 
 
+@pytest.mark.parametrize("act", ["bf16", "f32"])
+@pytest.mark.parametrize("M,N,K", [(1, 6100, 256), (16, 6100, 144), (1, 12170, 128), (16, 12170, 272), (12, 130, 4096),
+                                   (13, 130, 4096), (1, 20, 49168)])
+def test_few_rows_of_many_outputs_and_of_long_rows(gpu, act, M, N, K):
+    """Each width of the workgroups that quantize the rows themselves, and both
+    sides of where they leave that to a launch of its own."""
+    W, x = _weights(gpu, N, K, 4), _x(gpu, M, K, act, 4)
+    res = _x(gpu, M, N, act, 5)
+    _check(gdn.quantized_linear(x, W, FP8, residual=res), x, W, act, res)
+
+
 @pytest.mark.parametrize("act", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("M", [1, 16, 40, 200, 700])
 def test_codes_and_scales_are_the_definitions(gpu, act, M):
