@@ -90,6 +90,17 @@ def test_few_rows_of_many_outputs_and_of_long_rows(gpu, act, M, N, K):
     _check(gdn.quantized_linear(x, W, FP8, residual=res), x, W, act, res)
 
 
+@pytest.mark.parametrize("act", ["bf16", "f32"])
+@pytest.mark.parametrize("M,N,K", [(2100, 8261, 256), (2100, 8256, 256), (4100, 4160, 144)])
+def test_columns_in_two_launches(gpu, act, M, N, K):
+    """Products whose last round of tiles is cut off, with odd and even rows."""
+    W, x = _weights(gpu, N, K, 6), _x(gpu, M, K, act, 6)
+    res = _x(gpu, M, N, act, 7)
+    _check(gdn.quantized_linear(x, W, FP8, residual=res), x, W, act, res)
+    if N % 8 == 0:
+        _check(gdn.quantized_linear(x, W, FP8), x, W, act)
+
+
 @pytest.mark.parametrize("act", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("M", [1, 16, 40, 200, 700])
 def test_codes_and_scales_are_the_definitions(gpu, act, M):
