@@ -450,7 +450,7 @@ def _fp8_matmul(x, w, scales, N: int, K: int, residual):
     if x2.data_ptr() % 16:
         x2 = x2.clone()
     M = x2.numel() // K
-    y = torch.empty((*shape[:-1], N), dtype=x.dtype, device=x.device)
+    y = x2.new_empty((*shape[:-1], N))
     r = None if residual is None else _residual_rows(residual, x, shape[:-1], M, N)
     w, scales = _c(w), _c(scales)
     if w.data_ptr() % 16:

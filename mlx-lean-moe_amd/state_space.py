@@ -167,9 +167,9 @@ def conv_silu(x: torch.Tensor, conv_state: torch.Tensor, weight: torch.Tensor, b
     conv_state = _c(_as(conv_state, x.dtype))
     weight = _c(_as(weight, _F32))
     bias = None if bias is None else _c(_as(bias, _F32))
-    out = torch.empty((T, C), dtype=x.dtype, device=device)
+    out = x.new_empty((T, C))
     if conv_out is None:
-        conv_out = torch.empty((N, K - 1, C), dtype=x.dtype, device=device)
+        conv_out = x.new_empty((N, K - 1, C))
     else:
         _check_out(conv_out, (N, K - 1, C), x.dtype, device, conv_state, "conv_out")
     _lib.call_on(device, "gdn_conv_silu", _lib.ptr(x), stride, _lib.ptr(conv_state), _lib.ptr(conv_out),
@@ -248,9 +248,9 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, B: torch.Tensor, C: torch.
     if state is not None and not in_place:
         state = _c(_as(state, _F32))
         state = state if state.data_ptr() % 16 == 0 else state.clone()
-    y = torch.empty(shape, dtype=y_dtype, device=device)
+    y = x.new_empty(shape) if y_dtype is act else torch.empty(shape, dtype=y_dtype, device=device)
     if state_out is None:
-        state_out = torch.empty((R, H, P, N), dtype=_F32, device=device)
+        state_out = A_log.new_empty((R, H, P, N))
     else:
         src = torch.empty(0, device=device) if state is None or in_place else state
         _check_out(state_out, (R, H, P, N), _F32, device, src, "state_out")
@@ -345,7 +345,7 @@ def selective_step(xbc: torch.Tensor, dt: torch.Tensor, conv_state: torch.Tensor
         if state_out.data_ptr() % 16:
             raise ValueError("state_out must be 16-byte aligned")
     y_dtype = y_dtype or act
-    y = torch.empty((rows, H, P), dtype=y_dtype, device=device)
+    y = xbc.new_empty((rows, H, P)) if y_dtype is act else torch.empty((rows, H, P), dtype=y_dtype, device=device)
     _lib.call_on(device, "gdn_selective_step", _lib.ptr(xbc), s_x, _lib.ptr(dt), s_dt, _lib.ptr(conv_state),
                  _lib.ptr(conv_out), _lib.ptr(conv_weight), _lib.ptr(conv_bias), _lib.ptr(A_log), _lib.ptr(dt_bias),
                  _lib.ptr(D), _lib.ptr(ssm_state), _lib.ptr(state_out), _lib.ptr(y), _lib.dtype_code(y_dtype), rows,
