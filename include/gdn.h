@@ -507,7 +507,8 @@ int gdn_conv_silu(const void *x, int64_t x_stride, const void *conv_state_in, vo
  * bfloat16 y runs on the bf16 matrix cores (state and sums float32), all else
  * on the float32 ones. No reference counterpart.
  */
-int64_t gdn_selective_scan_workspace_size(int N, int64_t T_total, int64_t longest_run, int G, int H, int P, int S);
+int64_t gdn_selective_scan_workspace_size(int act_dtype, int y_dtype, int N, int64_t T_total, int64_t longest_run,
+                                          int G, int H, int P, int S);
 int gdn_selective_scan(const void *x, int64_t x_stride, const void *B, int64_t B_stride, const void *C,
                        int64_t C_stride, int act_dtype, const void *dt, int64_t dt_stride, int dt_dtype,
                        const float *A_log, const float *dt_bias, const float *D, const float *state_in,

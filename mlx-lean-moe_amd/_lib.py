@@ -95,7 +95,7 @@ _SIGNATURES = {
     "gdn_quantized_matmul_scheme_workspace_size": (_c_i64, [_c_int, _c_int, _c_int]),
     "gdn_conv_silu": (_c_int, [_c_void_p, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int,
                                _c_i64, _c_void_p, _c_int, _c_int, _c_int, _c_void_p]),
-    "gdn_selective_scan_workspace_size": (_c_i64, [_c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int]),
+    "gdn_selective_scan_workspace_size": (_c_i64, [_c_int, _c_int, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int]),
     "gdn_selective_scan": (_c_int, [_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_int, _c_void_p,
                                     _c_i64, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                                     _c_void_p, _c_int, _c_void_p, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int,

@@ -695,13 +695,17 @@ __global__ __launch_bounds__(kScanThreads) void scan_chain_kernel(ScanArgs a) {
 // the pass that sums each of them (0.6 of the main one), the chain's way
 // through memory (both ways, 5.3 TB/s) and each workgroup's start and end, and
 // shorten the longest walk. The estimate below is the time of each choice from
-// a chunk's time with one and two workgroups on a CU (64 tokens, 64 rows of 128
-// states, bfloat16) and that start; it ranks them as measured (us, 64 heads):
+// 64 tokens' time with one and two workgroups on a CU (64 rows of 128 states,
+// bfloat16 and float32 kernels) and that start; it ranks them as measured (us, 64 heads):
 //   41 tokens narrow 8.6, wide 11.8; 300 whole and narrow 25.5, wide 35.5, in
 //   segments of 64 28.6; 1000 in 128s 39.6, whole 100; 4096 in 256s 82, 512s
 //   95, 128s 107, whole 380; 8192 in 512s 129, 256s 151; 8 runs of 2000 whole
-//   and narrow 169, wide 200, in 1024s 212; 16 runs of 0 to 4096 (20 k tokens)
+//   and narrow 169, wide 200, in 1024s 212; 16 runs of 0 to 4096 (11 k tokens)
 //   in 512s 202, 1024s 220, whole 407.
+// float32, 32 heads of 128: 256 tokens narrow in 64s 32.1, whole 43.9, wide in 64s
+//   36.5; 1000 wide in 64s 66.6, 128s 67.1, narrow 73; 2500 wide in 128s 145, 256s
+//   162; 8192 in 512s 314, 256s 326; 8 runs of 1000 to 2000, 64 heads
+//   of 64: whole and narrow 422, wide 501, in 256s 513.
 struct ScanPlan {
     int heads, waves;  // of a workgroup (waves of 16 head_dim rows)
     int shift;
@@ -710,7 +714,7 @@ struct ScanPlan {
     int64_t bytes;
 };
 
-ScanPlan scan_plan(int N, int64_t T, int64_t longest, int G, int H, int P, int S) {
+ScanPlan scan_plan(bool bf16, int N, int64_t T, int64_t longest, int G, int H, int P, int S) {
     const int per = H / G;
     if (longest <= 0 || longest > T) longest = T;
     ScanPlan best{};
@@ -722,7 +726,8 @@ ScanPlan scan_plan(int N, int64_t T, int64_t longest, int G, int H, int P, int S
         if (narrow && P <= 32 && per % 2 == 0) continue;  // (half of its rows would be empty)
         const int rows = 16 * p.waves / p.heads;
         p.units = int64_t(H / p.heads) * ((P + rows - 1) / rows);
-        const double alone = narrow ? 4.1 : 5.9, paired = narrow ? 5.1 : 6.2, ends = 9.0;
+        const double alone = bf16 ? (narrow ? 4.1 : 5.9) : (narrow ? 10.4 : 14.6);
+        const double paired = bf16 ? (narrow ? 5.1 : 6.2) : (narrow ? 13.0 : 22.0), ends = 9.0;
         for (int shift = 6; shift <= 12; ++shift) {
             p.segmented = shift < 12 && longest > (int64_t(1) << shift);
             if (shift < 12 && !p.segmented) continue;  // the same as whole runs
@@ -774,6 +779,8 @@ bool scan_sizes_ok(int N, int64_t T, int G, int H, int P, int S) {
     return N >= 1 && T >= 0 && T < (int64_t(1) << 31) && G > 0 && H > 0 && H % G == 0 && P > 0 && S > 0;
 }
 
+bool on_bf16(int act_dtype, int y_dtype) { return act_dtype == GDN_BF16 && y_dtype == GDN_BF16; }
+
 bool scan_shape_taken(int P, int S) { return P % 8 == 0 && S % 8 == 0 && S <= 256; }
 
 }  // namespace
@@ -781,10 +788,12 @@ bool scan_shape_taken(int P, int S) { return P % 8 == 0 && S % 8 == 0 && S <= 25
 
 using namespace gdn;
 
-extern "C" int64_t gdn_selective_scan_workspace_size(int N, int64_t T_total, int64_t longest_run, int G, int H,
-                                                     int P, int S) {
-    if (!scan_sizes_ok(N, T_total, G, H, P, S) || !scan_shape_taken(P, S)) return 0;
-    return scan_plan(N, T_total, longest_run, G, H, P, S).bytes;
+extern "C" int64_t gdn_selective_scan_workspace_size(int act_dtype, int y_dtype, int N, int64_t T_total,
+                                                     int64_t longest_run, int G, int H, int P, int S) {
+    if (!scan_sizes_ok(N, T_total, G, H, P, S) || !scan_shape_taken(P, S) || !valid_dtype(act_dtype) ||
+        !valid_dtype(y_dtype))
+        return 0;
+    return scan_plan(on_bf16(act_dtype, y_dtype), N, T_total, longest_run, G, H, P, S).bytes;
 }
 
 extern "C" int gdn_selective_scan(const void* x, int64_t x_stride, const void* B, int64_t B_stride, const void* C,
@@ -819,7 +828,8 @@ extern "C" int gdn_selective_scan(const void* x, int64_t x_stride, const void* B
     const int64_t state_bytes = int64_t(N) * H * P * S * 4;
     GDN_REQUIRE(!state_in || state_in == state_out || !overlaps(state_in, state_bytes, state_out, state_bytes),
                 "gdn_selective_scan: state_out partially overlaps state_in");
-    const ScanPlan p = scan_plan(N, T_total, longest_run, G, H, P, S);
+    const bool bf16 = on_bf16(act_dtype, y_dtype);
+    const ScanPlan p = scan_plan(bf16, N, T_total, longest_run, G, H, P, S);
     GDN_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes),
                 "gdn_selective_scan: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                 (long long)p.bytes);
@@ -829,7 +839,6 @@ extern "C" int gdn_selective_scan(const void* x, int64_t x_stride, const void* B
     ScanArgs a{x, B, C, dt, x_stride, B_stride, C_stride, dt_stride, dt_dtype, A_log, dt_bias, D, state_in,
                state_out, y, y_dtype, cu_seqlens, N, T_total / N, p.shift, G, H, P, S, part,
                part ? part + p.slots * H * int64_t(P) * S : nullptr, p.segmented, int(p.slots)};
-    const bool bf16 = act_dtype == GDN_BF16 && y_dtype == GDN_BF16;
     hipStream_t s = as_stream(stream);
     const auto tall = [](int64_t x, int64_t n) {
         return dim3(unsigned(x), unsigned(n < kMaxGridY ? n : kMaxGridY), unsigned((n + kMaxGridY - 1) / kMaxGridY));

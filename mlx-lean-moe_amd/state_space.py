@@ -256,10 +256,11 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, B: torch.Tensor, C: torch.
         _check_out(state_out, (R, H, P, N), _F32, device, src, "state_out")
         if state_out.data_ptr() % 16:
             raise ValueError("state_out must be 16-byte aligned")
-    nbytes = _scan_workspace(R, T, longest, G, H, P, N)
+    act_code = _lib.dtype_code(act)
+    nbytes = _scan_workspace(act_code, y_code, R, T, longest, G, H, P, N)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _lib.call_on(device, "gdn_selective_scan", x.data_ptr(), x_step, B.data_ptr(), B_step, C.data_ptr(), C_step,
-                 _lib.dtype_code(act), dt.data_ptr(), dt_step, _lib.dtype_code(dt.dtype), A_log.data_ptr(),
+                 act_code, dt.data_ptr(), dt_step, _lib.dtype_code(dt.dtype), A_log.data_ptr(),
                  dt_bias.data_ptr(), _lib.ptr(D), _lib.ptr(state), state_out.data_ptr(), y.data_ptr(), y_code,
                  _lib.ptr(cu), R, T, longest, G, H, P, N, _lib.ptr(ws), nbytes, _stream(device))
     return y, state_out

@@ -90,7 +90,9 @@ def test_selective_scan_refusals():
     _refused(_scan(xs=132), E, "aligned")
     _refused(_scan(x=ctypes.c_void_p(8)), E, "aligned")
     _refused(_scan(si=ctypes.c_void_p((1 << 26) + 16)), E, "overlaps")
-    size = _lib.load().gdn_selective_scan_workspace_size
+    of_dtypes = _lib.load().gdn_selective_scan_workspace_size
+    size = lambda *sizes: of_dtypes(1, 1, *sizes)  # bfloat16
+    assert of_dtypes(0, 0, 1, 4096, 4096, 1, 2, 64, 64) > 0 and of_dtypes(0, 9, 1, 4096, 4096, 1, 2, 64, 64) == 0
     need = size(1, 4096, 4096, 1, 2, 64, 64)
     assert need > 0 and size(1, 64, 64, 1, 2, 64, 64) == 0 and size(1, 4096, 4096, 1, 2, 60, 64) == 0
     # runs that are all short need no workspace, whatever their number
