@@ -125,6 +125,10 @@ def decode_tensor(raw: bytes, dtype: str, shape: tuple[int, ...], *,
     return torch.frombuffer(buf, dtype=torch_dtype).reshape(shape)
 
 
+# how safetensors files tag e4m3 codes
+_E4M3_TAGS = ("F8_E4M3", "U8")
+
+
 class CheckpointReader:
     """Whole-tensor reads out of a checkpoint's shards by name
     (expert_loader.py:164-180): one ``os.pread`` per tensor, one descriptor
@@ -141,12 +145,18 @@ class CheckpointReader:
             fd = self._fds[shard] = os.open(str(self.model_dir / shard), os.O_RDONLY)
         return fd
 
-    def read_tensor(self, name: str) -> torch.Tensor:
+    def read_tensor(self, name: str, *, codes: bool = False) -> torch.Tensor:
+        """One tensor. ``codes``: an ``F8_E4M3`` tensor (or the same bytes as
+        ``U8``) as float8_e4m3fn, for callers that hold its scales; without it
+        such a tensor is refused, its values being none without them."""
+
         span = self.index[name]
         raw = os.pread(self._fd(span.shard), span.nbytes, span.begin)
         if len(raw) != span.nbytes:
             raise ValueError(f"{name}: shard {span.shard} is truncated")
-        if span.dtype == "F8_E4M3":  # fp8_block codes, which the reference's decoding does not know
+        if codes:
+            if span.dtype not in _E4M3_TAGS:
+                raise ValueError(f"{name}: {span.dtype} holds no e4m3 codes")
             return decode_tensor(raw, "U8", span.shape).view(torch.float8_e4m3fn)
         return decode_tensor(raw, span.dtype, span.shape, stored_width=is_quant_metadata(name))
 
@@ -183,7 +193,10 @@ def projection_is_quantized(index: dict[str, TensorSpan], name: str, scheme: Qua
     the codes of a float scheme (mxfp4, mxfp8, nvfp4), which has none; biases
     not shaped like the scales; weight and scales disagreeing in their leading
     (row) dimensions; a packed row width other than the scale groups'
-    ``groups * group_size * bits / 32`` words. These are the conditions the
+    ``groups * group_size * bits / 32`` words; fp8_block codes or scales of
+    other types or shapes. 8-bit codes with neither scales nor biases (a
+    checkpoint that names its scales otherwise) are a :class:`LayoutError` too,
+    no plain matrix. The packed schemes' are the conditions the
     reference's loader enforces (expert_loader.py:95-141) with one more:
     that loader only shape-checks biases stored beside float-scheme codes
     and hands them to the matmul, whose float modes have no bias term; here
@@ -195,6 +208,10 @@ def projection_is_quantized(index: dict[str, TensorSpan], name: str, scheme: Qua
     if weight is None:
         raise KeyError(f"{name}.weight is not in the checkpoint")
     if scales is None and biases is None:
+        if weight.dtype == "F8_E4M3" or (scheme.mode == "fp8_block" and weight.dtype == "U8"):
+            beside = sorted(k for k in index if k.startswith(f"{name}.") and k != f"{name}.weight")
+            raise LayoutError(f"{name}: 8-bit codes are stored without {name}.scales; beside them "
+                              f"{'are ' + ', '.join(beside) if beside else 'is nothing'}")
         return False
     problems = []
     if scales is None:
@@ -208,7 +225,7 @@ def projection_is_quantized(index: dict[str, TensorSpan], name: str, scheme: Qua
             problems.append(f"biases {biases.shape} and scales {scales.shape} differ in shape")
         if scheme.mode == "fp8_block":
             blocks = tuple(-(-n // 128) for n in weight.shape)
-            if weight.dtype not in ("F8_E4M3", "U8") or scales.dtype != "F32" or scales.shape != blocks:
+            if weight.dtype not in _E4M3_TAGS or scales.dtype != "F32" or scales.shape != blocks:
                 problems.append(f"fp8_block keeps 8-bit codes and F32 scales of shape {blocks}; stored are "
                                 f"{weight.dtype} {weight.shape} and {scales.dtype} {scales.shape}")
             words = weight.shape[-1]
@@ -231,6 +248,9 @@ def read_projection(reader: CheckpointReader, name: str, scheme: QuantScheme) ->
     quantized fields under ``scheme`` (expert_loader.py:144-161)."""
 
     if projection_is_quantized(reader.index, name, scheme):
+        if scheme.mode == "fp8_block":
+            return LinearWeights({"weight": reader.read_tensor(f"{name}.weight", codes=True),
+                                  "scales": reader.read_tensor(f"{name}.scales")}, scheme)
         return LinearWeights(reader.read_fields(name, ("weight", "scales", "biases")), scheme)
     return LinearWeights(reader.read_tensor(f"{name}.weight"), None)
 
