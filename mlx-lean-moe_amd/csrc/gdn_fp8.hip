@@ -131,12 +131,17 @@ GDN_DEV f32x4 mfma_widened(uint4 a0, uint4 a1, uint4 b0, uint4 b1) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(a1.z, a1.w), widen8(b1.z, b1.w), c, 0, 0, 0);
 }
 
+// Whether rows of y start on multiples of `count` elements, and this launch's
+// columns end on one: both, since rows lie ldy apart whatever part of their
+// columns the launch takes.
+GDN_DEV bool whole_pieces(const Fp8Args& a, int count) { return ((a.N | a.ldy) & (count - 1)) == 0; }
+
 // Four results of row m, columns n .. n + 3: the product rounded to y's type,
 // then the residual added and rounded again.
 GDN_DEV void store4(const Fp8Args& a, int m, int n, f32x4 v) {
     if (m >= a.M) return;
     const int64_t at = int64_t(m) * a.ldy + n;
-    if (a.N % 4 == 0 && n + 3 < a.N) {
+    if (whole_pieces(a, 4) && n + 3 < a.N) {
         if (a.residual) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = round_to(v[i], a.y_dtype) + load_any(a.residual, at + i, a.y_dtype);
@@ -320,6 +325,7 @@ __global__ __launch_bounds__(64 * kWN * kWM) void fp8_tile_kernel(Fp8Args a) {
                                              f32_to_f16_bits(v[2]) | uint32_t(f32_to_f16_bits(v[3])) << 16);
             *reinterpret_cast<uint2*>(own + (m * kPieces + c) * 16 + (g & 1) * 8) = o;
         }
+    const bool whole = whole_pieces(a, 8);
     // (a wave reads only what it wrote itself: no barrier)
     for (int p = lane; p < 16 * RM * kPieces; p += 64) {
         const int row = p / kPieces, c = p % kPieces;
@@ -328,7 +334,7 @@ __global__ __launch_bounds__(64 * kWN * kWM) void fp8_tile_kernel(Fp8Args a) {
         if (m >= a.M || n >= a.N) continue;
         const int64_t at = int64_t(m) * a.ldy + n;
         uint16_t* y = static_cast<uint16_t*>(a.y) + at;
-        if (a.N % 8 == 0 && !a.residual) {
+        if (whole && !a.residual) {
             *reinterpret_cast<uint4*>(y) = v;
             continue;
         }
@@ -345,7 +351,7 @@ __global__ __launch_bounds__(64 * kWN * kWM) void fp8_tile_kernel(Fp8Args a) {
                     e[k] = a.y_dtype == GDN_BF16 ? f32_to_bf16_bits(sum) : f32_to_f16_bits(sum);
                 }
         }
-        if (a.N % 8 == 0) {
+        if (whole) {
             __builtin_memcpy(&v, e, 16);
             *reinterpret_cast<uint4*>(y) = v;
         } else {
