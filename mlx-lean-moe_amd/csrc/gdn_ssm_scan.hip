@@ -75,9 +75,10 @@ GDN_DEV double lane_value(double c, int lane) {
 // The decays of one chunk, per token (all in powers of two): c_t as the sum of
 // two floats, d_t, exp(c_t), and d_t exp(c_Q - c_t). The running sum is in
 // double: what counts are differences of its terms, and a chunk's sum reaches
-// hundreds where single terms are 1e-3.
+// hundreds where single terms are 1e-3. (These are read 16 bytes at a time, and
+// stand in arrays.)
 template <int Q>
-struct Decays {
+struct alignas(16) Decays {
     float hi[Q], lo[Q], d[Q], e[Q], w[Q], end;
 };
 
@@ -101,7 +102,7 @@ GDN_DEV double chunk_decays(Decays<Q>& o, int lane, float d, float rate) {
 // before the tile, neither above one; only a tile's own pairs take an
 // exponential each. (Near is c - r: 24 bits of it are far more than the score
 // keeps.)
-struct TileDecays {
+struct alignas(16) TileDecays {
     float near[64], d[64], from[64], e[64], w[64], to[3][64], end;
 };
 
