@@ -72,10 +72,21 @@ GDN_DEV double lane_value(double c, int lane) {
     return __longlong_as_double(int64_t(lo | uint64_t(hi) << 32));
 }
 
+// The exponent of a token's decay, a power of two. At -256 and below the decay is
+// zero in float32, and so is every product with it: the exponent stays at -256
+// there, so that one such token does not take the bits of the sum that the decays
+// between later tokens are differences of (a step of 1000 at a rate of 8000 is an
+// exponent of 1e7, which leaves 24 bits of a tile's sum no digit behind the
+// point). NaN stays NaN.
+GDN_DEV double exponent(float d, float rate) {
+    const double l = double(d) * double(rate) * kLog2e;
+    return l < -256.0 ? -256.0 : l;
+}
+
 // The decays of one chunk, per token (all in powers of two): c_t as the sum of
 // two floats, d_t, exp(c_t), and d_t exp(c_Q - c_t). The running sum is in
 // double: what counts are differences of its terms, and a chunk's sum reaches
-// hundreds where single terms are 1e-3. (These are read 16 bytes at a time, and
+// thousands where single terms are 1e-3. (These are read 16 bytes at a time, and
 // stand in arrays.)
 template <int Q>
 struct alignas(16) Decays {
@@ -84,7 +95,7 @@ struct alignas(16) Decays {
 
 template <int Q>
 GDN_DEV double chunk_decays(Decays<Q>& o, int lane, float d, float rate) {
-    const double c = running_sum(double(d) * double(rate) * kLog2e), end = lane_value(c, Q - 1);
+    const double c = running_sum(exponent(d, rate)), end = lane_value(c, Q - 1);
     if (lane < Q) {
         const float hi = float(c);
         o.hi[lane] = hi;
@@ -100,14 +111,14 @@ GDN_DEV double chunk_decays(Decays<Q>& o, int lane, float d, float rate) {
 // For scores rounded to bfloat16, tile by tile of 16 tokens: with r the sum up
 // to the tile t lies in, exp(c_t - c_s) is exp(c_t - r) exp(r - c_s) for every s
 // before the tile, neither above one; only a tile's own pairs take an
-// exponential each. (Near is c - r: 24 bits of it are far more than the score
-// keeps.)
+// exponential each. (Near is c - r, at most 16 x 256: its 24 bits leave a decay
+// 2^-12, the score keeps 2^-8.)
 struct alignas(16) TileDecays {
     float near[64], d[64], from[64], e[64], w[64], to[3][64], end;
 };
 
 GDN_DEV double tile_decays(TileDecays& o, int lane, float d, float rate) {
-    const double c = running_sum(double(d) * double(rate) * kLog2e), end = lane_value(c, 63);
+    const double c = running_sum(exponent(d, rate)), end = lane_value(c, 63);
     const double r1 = lane_value(c, 15), r2 = lane_value(c, 31), r3 = lane_value(c, 47);
     const float near = float(c - (lane < 16 ? 0.0 : lane < 32 ? r1 : lane < 48 ? r2 : r3));
     o.near[lane] = near;
