@@ -29,6 +29,7 @@ constexpr int kMaxGridY = 65535;
 constexpr double kLog2e = 1.4426950408889634;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
 struct ScanArgs {
     const void *x, *B, *C, *dt;
@@ -331,6 +332,34 @@ __global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_ke
             for (int q = 0; q < 2; ++q)
                 xf[pt][q] = column_frag<4>(Xs, XS, 32 * q + 8 * g, pw + 16 * pt, lr);
 
+        // Scores of pairs that are none are zero, and zero times a value that is
+        // not finite is NaN at tokens before it: such values of x leave the
+        // product (for zeros) and are added to their own and later tokens alone.
+        bool apart = false;
+        if constexpr (!kStateOnly) {
+            u16x8 top = {};
+#pragma unroll
+            for (int pt = 0; pt < kTiles; ++pt)
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x8, xf[pt][q]) & uint16_t(0x7FFF));
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) any |= top[e] >= 0x7F80;
+            apart = __builtin_amdgcn_ballot_w64(any) != 0;
+            if (apart) {
+#pragma unroll
+                for (int pt = 0; pt < kTiles; ++pt)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        u16x8 v = __builtin_bit_cast(u16x8, xf[pt][q]);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = (v[e] & 0x7F80) == 0x7F80 ? 0 : v[e];
+                        xf[pt][q] = __builtin_bit_cast(bf16x8, v);
+                    }
+            }
+        }
+
         if constexpr (!kStateOnly) {
             const int left = int(min(sg.t1 - t0, int64_t(Q)));
             const auto yr = buffer_at(static_cast<uint16_t*>(a.y) + (t0 * H + h) * P);
@@ -371,6 +400,16 @@ __global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_ke
                 for (int pt = 0; pt < kTiles; ++pt) {
                     const int p = pl + 16 * pt + 4 * g;
                     f32x4 o = y[pt][tt];
+                    if (apart)
+#pragma clang loop unroll(disable)
+                        for (int r = 0; r <= t; ++r) {
+                            const float w = bf16_bits_to_f32(Ws[(hb * Q + t) * WS + r]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint16_t v = Xs[r * XS + pw + 16 * pt + 4 * g + i];
+                                if ((v & 0x7F80) == 0x7F80) o[i] = __builtin_fmaf(w, bf16_bits_to_f32(v), o[i]);
+                            }
+                        }
                     if (a.D) {
                         const uint2 xv = *reinterpret_cast<const uint2*>(Xs + t * XS + pw + 16 * pt + 4 * g);
                         o[0] = __builtin_fmaf(skip, __uint_as_float(xv.x << 16), o[0]);
@@ -385,6 +424,13 @@ __global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_ke
         }
 
         if (kStateOnly || !a.segmented || t0 + Q < sg.t1) {
+            if (apart) {
+#pragma unroll
+                for (int pt = 0; pt < kTiles; ++pt)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q)
+                        xf[pt][q] = column_frag<4>(Xs, XS, 32 * q + 8 * g, pw + 16 * pt, lr);
+            }
             const float end = dec[hb].end;
 #pragma unroll
             for (int pt = 0; pt < kTiles; ++pt)
@@ -584,6 +630,21 @@ __global__ __launch_bounds__(64 * kWaves, kNP <= 128 ? kWaves / 2 : kWaves / 4) 
         for (int j = 0; j < Q / 16; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) xf[j][i] = Xs[(16 * j + 4 * g + i) * XS + pw + lr];
+        bool apart = false;  // (as in the bfloat16 kernel)
+        if constexpr (!kStateOnly) {
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < Q / 16; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) any |= !__builtin_isfinite(xf[j][i]);
+            apart = __builtin_amdgcn_ballot_w64(any) != 0;
+            if (apart) {
+#pragma unroll
+                for (int j = 0; j < Q / 16; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) xf[j][i] = __builtin_isfinite(xf[j][i]) ? xf[j][i] : 0.f;
+            }
+        }
 
         if constexpr (!kStateOnly) {
             const int left = int(min(sg.t1 - t0, int64_t(Q)));
@@ -612,6 +673,16 @@ __global__ __launch_bounds__(64 * kWaves, kNP <= 128 ? kWaves / 2 : kWaves / 4) 
                         y[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(xf[j][i], wv[i], y[tt], 0, 0, 0);
                 }
                 f32x4 o = y[tt];
+                if (apart)
+#pragma clang loop unroll(disable)
+                    for (int r = 0; r <= t; ++r) {
+                        const float w = Ws[(hb * Q + t) * WS + r];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float v = Xs[r * XS + pw + 4 * g + i];
+                            if (!__builtin_isfinite(v)) o[i] = __builtin_fmaf(w, v, o[i]);
+                        }
+                    }
                 if (a.D) {
                     const f32x4 xv = *reinterpret_cast<const f32x4*>(Xs + t * XS + pw + 4 * g);
 #pragma unroll
@@ -633,6 +704,12 @@ __global__ __launch_bounds__(64 * kWaves, kNP <= 128 ? kWaves / 2 : kWaves / 4) 
         }
 
         if (kStateOnly || !a.segmented || t0 + Q < sg.t1) {
+            if (apart) {
+#pragma unroll
+                for (int j = 0; j < Q / 16; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) xf[j][i] = Xs[(16 * j + 4 * g + i) * XS + pw + lr];
+            }
             const float end = dec[hb].end;
 #pragma unroll
             for (int j = 0; j < NT; ++j) S[j] *= end;

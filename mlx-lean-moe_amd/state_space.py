@@ -195,8 +195,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, B: torch.Tensor, C: torch.
     default), the state float32, in ``state_out`` when given (which may be
     ``state`` itself, and must not overlap it otherwise). bfloat16 inputs with
     bfloat16 y run on the bf16 matrix cores with float32 sums, every other mix
-    on the float32 ones. NaN or infinity in a token reaches, besides every
-    later token of its run, the tokens up to 63 before it."""
+    on the float32 ones. NaN or infinity in a token reaches that and the later
+    tokens of its run, none before it."""
 
     packed = cu_seqlens is not None
     lead = 1 if packed else 2

@@ -68,3 +68,72 @@ def test_steps_that_forget_everything_among_small_ones(gpu, act, lens):
     else:
         _within(y, ref, U[act] * ref.abs() + e * ya + 2.0 ** -48, "y")
     _within(S, state, e * sa + 1e-30, "state")
+
+
+@pytest.mark.parametrize("act,y_act", [("bf16", "bf16"), ("f32", "f32"), ("f16", "f16"), ("bf16", "f32")])
+@pytest.mark.parametrize("lens,dims", [([100, 0, 41], (4, 64, 2, 128)), ([300], (3, 40, 1, 64)), ([130, 64], (2, 128, 2, 256)),
+                                       ([20, 90], (32, 96, 1, 16))])
+def test_values_that_are_not_finite_reach_no_earlier_token(gpu, act, y_act, lens, dims):
+    """One bad value of x at a time: the tokens before it, the other heads and the
+    other rows of its head hold the bits that they hold without it; its own row of
+    y and of the state, from its token to the end of its run, holds what the
+    recurrence gives, no number."""
+    H, P, G, N = dims
+    case = _case(gpu, act, lens, dims, 50)
+    cu = _offsets(lens)
+    call = lambda **k: gdn.selective_scan(**dict(case, **k), cu_seqlens=cu, y_dtype=DT[y_act])
+    y0, S0 = call()
+    assert torch.isfinite(y0).all() and torch.isfinite(S0).all()
+    for n, t in enumerate((0, 7, 15, 16, 31, 32, 33, 47, 62, 63, 64, 77, 95, 99)):
+        run = max(r for r in range(len(lens)) if cu[r] <= t)
+        end = cu[run + 1]
+        h, p = (5 * n + 1) % H, (13 * n + 2) % P
+        x = case["x"].clone()
+        x[t, h, p] = (float("nan"), float("inf"), float("-inf"))[n % 3]
+        y, S = call(x=x)
+        assert not torch.isfinite(y[t:end, h, p]).any() and not torch.isfinite(S[run, h, p]).any(), (t, h, p)
+        y[t:end, h, p], S[run, h, p] = y0[t:end, h, p], S0[run, h, p]
+        assert torch.equal(y, y0) and torch.equal(S, S0), (t, h, p)
+
+
+@pytest.mark.parametrize("act", ["bf16", "f32"])
+def test_gates_and_states_that_are_not_finite_reach_no_earlier_token(gpu, act):
+    """The same of dt, B and C: a step spoils its head, a row of B its group's
+    heads, both from their token on, a row of C its group's heads at its token."""
+    lens, (H, P, G, N) = [150, 30], (4, 64, 2, 128)
+    case = _case(gpu, act, lens, (H, P, G, N), 51)
+    call = lambda **k: gdn.selective_scan(**dict(case, **k), cu_seqlens=[0, 150, 180])
+    y0, S0 = call()
+    for t in (0, 9, 16, 40, 63, 64, 100, 149):
+        for name in ("dt", "B", "C"):
+            v = case[name].clone()
+            v[(t, 2) if name == "dt" else (t, 1, t % N)] = float("nan")
+            heads = slice(2, 3) if name == "dt" else slice(2, 4)
+            y, S = call(**{name: v})
+            at = slice(t, t + 1) if name == "C" else slice(t, 150)
+            assert torch.isnan(y[at, heads]).all(), (name, t)
+            y[at, heads] = y0[at, heads]
+            if name != "C":
+                assert torch.isnan(S[0, heads]).any()
+                S[0, heads] = S0[0, heads]
+            assert torch.equal(y, y0) and torch.equal(S, S0), (name, t)
+
+
+@pytest.mark.parametrize("act", ["bf16", "f32"])
+def test_whole_tokens_that_are_not_finite(gpu, act):
+    """Every value of a token bad, and later tokens bad again (padding that was
+    never written): what stands before them is as without them."""
+    lens, dims = [170], (4, 64, 2, 128)
+    case = _case(gpu, act, lens, dims, 52)
+    for end in (1, 20, 64, 101):
+        alone = {k: v[:end] if k in ("x", "dt", "B", "C") else v for k, v in case.items()}
+        bad = dict(case)
+        for k in ("x", "B", "C"):
+            bad[k] = case[k].clone()
+            bad[k][end:] = float("nan")
+        y, _ = gdn.selective_scan(**bad, cu_seqlens=[0, 170])
+        ref, _, ya, _ = scan64(**alone, lens=[end])
+        u = U[act]
+        e = (170 + 128 + 128) * 2.0 ** -24 + 2.0 ** -18
+        _within(y[:end], ref, u * ref.abs() + ((u * 1.01 if act == "bf16" else 0) + e) * ya + 2.0 ** -48, "y")
+        assert torch.isnan(y[end:]).all()
