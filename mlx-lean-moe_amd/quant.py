@@ -440,9 +440,8 @@ def _fp8_matmul(x, w, scales, N: int, K: int, residual):
     """``x @ W.T`` (+ residual) for fp8_block weights (gdn_fp8_matmul): x's
     rows quantized to e4m3 per 128 columns, float32 sums."""
 
-    if _followed(x, residual):
-        raise RuntimeError("fp8_block products have no gradient and no function transform; call them under "
-                           "torch.no_grad()")
+    if _followed(x, residual, w, scales):
+        raise RuntimeError("fp8_block products have no gradient and no forward mode; call them under torch.no_grad()")
     if w.get_device() != x.get_device():
         raise ValueError(f"x is on {x.device}, the weights on {w.device}")
     shape = x.shape
@@ -464,11 +463,16 @@ def _fp8_matmul(x, w, scales, N: int, K: int, residual):
 
 
 def _followed(*operands: torch.Tensor | None) -> bool:
-    """_transformed of calls that may cost little: a tensor outside forward
-    mode's levels has no tangent, and one that a transform wraps has no data_ptr
-    (which raises by itself)."""
+    """Whether autograd or forward mode follows these operands, for calls that
+    may cost little: tangents are looked for only inside a level of forward mode,
+    and a tensor that a function transform wraps has no data_ptr (which raises
+    by itself)."""
 
-    return (torch.is_grad_enabled() or getattr(forward_ad, "_current_level", 0) >= 0) and _transformed(*operands)
+    if torch.is_grad_enabled():
+        for t in operands:
+            if t is not None and t.requires_grad:
+                return True
+    return getattr(forward_ad, "_current_level", 0) >= 0 and _transformed(*operands)
 
 
 def _f32_matmul(x, w, scales, biases, quant: QuantScheme, N: int, K: int, residual):

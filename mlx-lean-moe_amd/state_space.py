@@ -15,7 +15,8 @@ layer, and :func:`gated_rms_norm` follows it as it follows that.
   a slot pool if asked
 
 The reference has no such layer. Every call runs on the GPU that holds its
-tensors; none has a gradient.
+tensors; none has a gradient (a tensor that needs one, or that forward mode
+follows, raises ``RuntimeError``).
 """
 
 from __future__ import annotations
@@ -29,6 +30,7 @@ from .config import StateSpaceDims
 from .gated_delta import (_FLOATS, _as, _c, _check_cu_seqlens, _check_out, _promote, _require_device,
                           _stream)
 from .linear_attention import _index_array, _rows, check_half_bits, check_slots
+from .quant import _followed
 
 _MAX_STATE = 256   # state_dim, both kernels
 _MAX_HEAD = 256    # head_dim, the step kernel
@@ -88,11 +90,9 @@ def _operands(*tensors) -> torch.device:
 
 
 def _no_gradient(*tensors) -> None:
-    if not torch.is_grad_enabled():
-        return
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            raise RuntimeError("the state-space operators have no gradient; call them under torch.no_grad()")
+    if _followed(*tensors):
+        raise RuntimeError("the state-space operators have no gradient and no forward mode; call them under "
+                           "torch.no_grad()")
 
 
 def _f32_vector(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
