@@ -72,8 +72,10 @@ template <class Act>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(const typename Act::storage* __restrict__ x, int M, int K,
                                                            int kb, uint8_t* __restrict__ codes,
                                                            float* __restrict__ scales, int ldx) {
-    const int b = int(blockIdx.x % unsigned(kb)), row = int(blockIdx.x / unsigned(kb)) * 16 + threadIdx.x / 16;
-    const int m = min(row, M - 1), k = b * kB + (threadIdx.x & 15) * 8;
+    const unsigned id = blockIdx.y * gridDim.x + blockIdx.x;
+    const int b = int(id % unsigned(kb));
+    const int64_t row = int64_t(id / unsigned(kb)) * 16 + threadIdx.x / 16;
+    const int m = int(min(row, int64_t(M - 1))), k = b * kB + (threadIdx.x & 15) * 8;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (k < K) load8f<Act>(x + int64_t(m) * K + k, v);
     uint32_t top = 0;
@@ -388,7 +390,9 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void fp8_skinny_kernel(Fp8Args a
     float* sx = reinterpret_cast<float*>(lds + a.M * stride);
 
     const int sub = wave % kNs, group = wave / kNs;
-    const int n0 = (blockIdx.x * kNs + sub) * 16;
+    const unsigned id = blockIdx.y * gridDim.x + blockIdx.x;
+    if (int64_t(id) * (16 * kNs) >= a.N) return;  // (the last row of the grid may be short)
+    const int n0 = (int(id) * kNs + sub) * 16;
     const uint8_t* wr = a.w + int64_t(min(n0 + lr, a.N - 1)) * a.K + 32 * g;
     const float* sw = a.sw + int64_t(min(n0, a.N - 1) / kB) * a.kb;
     uint4 w[kAhead][2];
@@ -470,7 +474,7 @@ __global__ __launch_bounds__(256) void fp8_sum_kernel(Fp8Args a, int splits) {
 __global__ __launch_bounds__(256) void fp8_dequantize_kernel(const uint8_t* __restrict__ w,
                                                              const float* __restrict__ sw, void* __restrict__ out,
                                                              int out_dtype, int N, int K, int kb) {
-    const int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 16;
+    const int64_t i = ((int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * 256 + threadIdx.x) * 16;
     if (i >= int64_t(N) * K) return;
     const int n = int(i / K), k = int(i % K);
     const uint4 c = *reinterpret_cast<const uint4*>(w + i);
@@ -523,6 +527,7 @@ Fp8Plan fp8_plan(bool exact, int M, int N, int kb) {
     for (int k = 0; k < kinds; ++k) {
         const Fp8Tiles& t = exact ? kTilesExact[k] : kTiles16[k];
         const int64_t tiles = ((int64_t(N) + t.tn - 1) / t.tn) * ((int64_t(M) + t.tm - 1) / t.tm);
+        if (k + 1 < kinds && tiles * 512 >= int64_t(1) << 32) continue;  // more threads than a grid dimension holds
         for (int splits = 1; splits <= kMaxSplits && splits * 2 <= kb + 1; splits *= 2) {
             const int steps = (kb + splits - 1) / splits;
             const int64_t load = (tiles * splits + 255) / 256, full = load / t.per_cu;
@@ -630,7 +635,7 @@ extern "C" int gdn_fp8_matmul(const void* x, int x_dtype, const void* w, const f
             const auto* xs = static_cast<const typename Act::storage*>(x);
             const dim3 threads(64 * kSkinnyWaves);
             const auto launch = [&](auto kernel, int rows) {
-                hipLaunchKernelGGL(kernel, dim3(unsigned((N + rows - 1) / rows)), threads, bytes, s, a, xs);
+                hipLaunchKernelGGL(kernel, rows_of_blocks((int64_t(N) + rows - 1) / rows), threads, bytes, s, a, xs);
             };
             if (N > 64 * 190) launch(fp8_skinny_kernel<Act, 4, E>, 64);
             else if (N > 32 * 190) launch(fp8_skinny_kernel<Act, 2, E>, 32);
@@ -655,7 +660,7 @@ extern "C" int gdn_fp8_matmul(const void* x, int x_dtype, const void* w, const f
     float* sx = reinterpret_cast<float*>(codes + codes_bytes(M, K));
     const auto quantize = [&](auto act) {
         using Act = decltype(act);
-        hipLaunchKernelGGL(fp8_quantize_kernel<Act>, dim3(unsigned(blocks)), dim3(256), 0, s,
+        hipLaunchKernelGGL(fp8_quantize_kernel<Act>, rows_of_blocks(blocks), dim3(256), 0, s,
                            static_cast<const typename Act::storage*>(x), M, K, kb, codes, sx, ldx);
     };
     if (x_dtype == GDN_F32) quantize(ActF32{});
@@ -682,7 +687,7 @@ extern "C" int gdn_fp8_dequantize(const void* w, const float* scales, void* out,
     GDN_REQUIRE(reinterpret_cast<uintptr_t>(w) % 16 == 0, "gdn_fp8_dequantize: w must be 16-byte aligned");
     const int64_t blocks = (int64_t(N) * K / 16 + 255) / 256;
     GDN_REQUIRE(blocks <= INT32_MAX, "gdn_fp8_dequantize: too many weights");
-    hipLaunchKernelGGL(fp8_dequantize_kernel, dim3(unsigned(blocks)), dim3(256), 0, as_stream(stream),
+    hipLaunchKernelGGL(fp8_dequantize_kernel, rows_of_blocks(blocks), dim3(256), 0, as_stream(stream),
                        static_cast<const uint8_t*>(w), scales, out, out_dtype, N, K, (K + kB - 1) / kB);
     return check_launch("gdn_fp8_dequantize");
 }

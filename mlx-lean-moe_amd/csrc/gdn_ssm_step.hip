@@ -43,6 +43,7 @@ struct StepArgs {
     void* y;
     int y_dtype, G, H, P, N, K;
     int split;  // workgroups of a head
+    int B;
     const int32_t* slots;
     int pool;
     const int32_t* half;
@@ -59,7 +60,9 @@ __global__ __launch_bounds__(kStepThreads) void step_kernel(StepArgs a) {
     using S = typename Act::storage;
     const int P = a.P, N = a.N, H = a.H, K1 = a.K - 1, tid = threadIdx.x;
     const int per = H / a.G, blocks = H * a.split;  // of a row
-    const int b = blockIdx.x / blocks, block = blockIdx.x % blocks;
+    const unsigned id = blockIdx.y * gridDim.x + blockIdx.x;
+    const int b = int(id / unsigned(blocks)), block = int(id % unsigned(blocks));
+    if (b >= a.B) return;  // (the last row of the grid may be short)
     const int h = block / a.split, part = block % a.split, grp = h / per;
     const int share = (P + a.split - 1) / a.split;
     const int p_lo = min(P, part * share), rows = min(P, p_lo + share) - p_lo;
@@ -246,7 +249,7 @@ extern "C" int gdn_selective_step(const void* xbc, int64_t xbc_stride, const voi
     while (heads * split < 64 && P / (split * 2) >= 16) split *= 2;
     GDN_REQUIRE(heads * split <= INT32_MAX && int64_t(H) * split < kStepCounter, "gdn_selective_step: B * H too large");
     const StepArgs args{xbc, xbc_stride, dt, dt_stride, conv_state_in, conv_state_out, conv_weight, conv_bias,
-                        A_log, dt_bias, D, state_in, state_out, y, y_dtype, G, H, P, N, K, split, slots, pool,
+                        A_log, dt_bias, D, state_in, state_out, y, y_dtype, G, H, P, N, K, split, B, slots, pool,
                         conv_half, conv_arrivals};
     const auto launch = [&](auto act, auto threads, auto pass) {
         using Act = decltype(act);
@@ -254,7 +257,7 @@ extern "C" int gdn_selective_step(const void* xbc, int64_t xbc_stride, const voi
         const auto kern = lanes == 2 ? step_kernel<Act, 2, T, R> : lanes == 4 ? step_kernel<Act, 4, T, R>
                           : lanes == 8 ? step_kernel<Act, 8, T, R> : lanes == 16 ? step_kernel<Act, 16, T, R>
                           : lanes == 32 ? step_kernel<Act, 32, T, R> : step_kernel<Act, 64, T, R>;
-        hipLaunchKernelGGL(kern, dim3(unsigned(heads * split)), dim3(T), 0, as_stream(stream), args);
+        hipLaunchKernelGGL(kern, rows_of_blocks(heads * split), dim3(T), 0, as_stream(stream), args);
     };
     const auto sized = [&](auto act) {
         using std::integral_constant;
