@@ -30,7 +30,7 @@ int check_launch(const char* what) {
 __global__ void gates_kernel(const void* a, const void* b, int ab_dtype, const float* A_log,
                              const float* dt_bias, float* g, void* beta, int beta_dtype,
                              int64_t n, int Hv) {
-    const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+    const int64_t i = (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= n) return;
     const int h = int(i % Hv);
     if (g) g[i] = expf(log_forget_gate(load_any(a, i, ab_dtype), A_log[h], dt_bias[h]));
@@ -44,7 +44,7 @@ __global__ void gates_kernel(const void* a, const void* b, int ab_dtype, const f
 __global__ void gated_rmsnorm_kernel(const void* x, int x_dtype, const void* z, int z_dtype,
                                      int64_t z_stride, int heads, const float* w, float eps,
                                      void* out, int out_dtype, int64_t rows, int D) {
-    const int64_t row = int64_t(blockIdx.x) * (blockDim.x / kWave) + threadIdx.x / kWave;
+    const int64_t row = (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * (blockDim.x / kWave) + threadIdx.x / kWave;
     const int lane = threadIdx.x % kWave;
     if (row >= rows) return;  // uniform per wave
     const int64_t base = row * D;
@@ -90,8 +90,8 @@ __global__ __launch_bounds__(256) void gated_rmsnorm_vec_kernel(const void* __re
                                                                 void* __restrict__ out, int64_t rows) {
     constexpr int D = 8 * kLanes, kRows = kWave / kLanes;
     const int lane = threadIdx.x % kWave;
-    const int64_t row = (int64_t(blockIdx.x) * (blockDim.x / kWave) + threadIdx.x / kWave) * kRows +
-                        lane / kLanes;
+    const int64_t block = int64_t(blockIdx.y) * gridDim.x + blockIdx.x;
+    const int64_t row = (block * (blockDim.x / kWave) + threadIdx.x / kWave) * kRows + lane / kLanes;
     const bool live = row < rows;
     const int64_t rr = live ? row : rows - 1;
     const int64_t at = rr * D + (lane % kLanes) * 8;
@@ -141,7 +141,7 @@ extern "C" int gdn_gates(const void* a, const void* b, int ab_dtype, const float
     const int64_t n = rows * Hv;
     const int threads = 256;
     const int64_t blocks = (n + threads - 1) / threads;
-    hipLaunchKernelGGL(gates_kernel, dim3(unsigned(blocks)), dim3(threads), 0, as_stream(stream),
+    hipLaunchKernelGGL(gates_kernel, rows_of_blocks(blocks), dim3(threads), 0, as_stream(stream),
                        a, b, ab_dtype, A_log, dt_bias, g, beta, beta_dtype, n, Hv);
     return check_launch("gdn_gates");
 }
@@ -162,7 +162,7 @@ extern "C" int gdn_gated_rmsnorm(const void* x, int x_dtype, const void* z, int 
         (x_dtype == GDN_F32 || x_dtype == z_dtype) && (D == 64 || D == 128 || D == 256) && aligned(x) &&
         aligned(z) && aligned(w) && aligned(out) && z_stride * dtype_size(z_dtype) % 16 == 0) {
         const int64_t per_block = 4 * (kWave / (D / 8));  // rows: four waves
-        const dim3 grid(static_cast<unsigned>((rows + per_block - 1) / per_block));
+        const dim3 grid = rows_of_blocks((rows + per_block - 1) / per_block);
         const auto launch = [&](auto act, auto xt) {
             using Act = decltype(act);
             using X = decltype(xt);
@@ -179,7 +179,7 @@ extern "C" int gdn_gated_rmsnorm(const void* x, int x_dtype, const void* z, int 
     }
     const int waves = 4;
     const int64_t blocks = (rows + waves - 1) / waves;
-    hipLaunchKernelGGL(gated_rmsnorm_kernel, dim3(unsigned(blocks)), dim3(waves * kWave), 0,
+    hipLaunchKernelGGL(gated_rmsnorm_kernel, rows_of_blocks(blocks), dim3(waves * kWave), 0,
                        as_stream(stream), x, x_dtype, z, z_dtype, z_stride, heads, w, eps, out, out_dtype,
                        rows, D);
     return check_launch("gdn_gated_rmsnorm");

@@ -409,6 +409,7 @@ extern "C" int gdn_frontend(const void* qkv, int64_t qkv_stride, const void* con
     }
     const int64_t blocks = T_total + (S > 0 ? N : 0);
     if (blocks == 0) return 0;
+    GDN_REQUIRE(one_grid_row(blocks, kFrontThreads), "gdn_frontend: %lld tokens exceed the grid", (long long)T_total);
     const size_t lds = size_t(C) * sizeof(float);
     if (act_dtype == GDN_F32) {
         hipLaunchKernelGGL(frontend_kernel<ActF32>, dim3(unsigned(blocks)), dim3(kFrontThreads),

@@ -25,8 +25,12 @@ inline bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
     return pa < pb + nb && pb < pa + na;
 }
 
-// A grid of at least `n` workgroups, in rows: a grid dimension holds less than
-// 2^32 threads, which workgroups of 1024 reach at 2^22.
+// A grid dimension holds less than 2^32 threads; a launch of more runs on what is
+// left of the count and reports nothing.
+inline bool one_grid_row(int64_t blocks, int threads) { return blocks < (int64_t(1) << 32) / threads; }
+
+// A grid of at least `n` workgroups of up to 1024 threads, in rows that a grid
+// dimension holds.
 inline dim3 rows_of_blocks(int64_t n) {
     constexpr int64_t row = int64_t(1) << 21;
     return dim3(unsigned(n < row ? n : row), unsigned((n + row - 1) / row));

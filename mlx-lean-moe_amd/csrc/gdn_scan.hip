@@ -264,6 +264,7 @@ extern "C" int gdn_scan_reference(const void* q, const void* k, int qk_dtype, co
     const int64_t rows = int64_t(N) * Hv * Dv;
     const int threads = 64;
     const int64_t blocks = (rows + threads - 1) / threads;
+    GDN_REQUIRE(one_grid_row(blocks, threads), "gdn_scan_reference: N * Hv * Dv exceeds the grid");
     const int64_t L_uniform = cu_seqlens ? 0 : T_total / N;
     hipLaunchKernelGGL(scan_reference_kernel, dim3(unsigned(blocks)), dim3(threads), 0,
                        as_stream(stream), q, k, qk_dtype, v, v_dtype, g, g_dtype, beta,
@@ -283,6 +284,7 @@ extern "C" int gdn_scan(const void* q, const void* k, int qk_dtype, const void* 
         return rc;
     const int64_t tiles = (Dv + kScanRows - 1) / kScanRows;
     const int64_t blocks = int64_t(N) * Hv * tiles;
+    GDN_REQUIRE(one_grid_row(blocks, kScanThreads), "gdn_scan: N * Hv * Dv exceeds the grid");
     const int64_t L_uniform = cu_seqlens ? 0 : T_total / N;
     hipStream_t s = as_stream(stream);
     const uintptr_t addr = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k);

@@ -91,3 +91,27 @@ def test_dequantize_of_2_to_the_36_codes(gpu):
             codes = w[n:n + 8].view(torch.float8_e4m3fn).float()
             s = scales[n // 128:n // 128 + 1].repeat_interleave(128, 1)
             assert torch.equal(out[n:n + 8], (codes * s).bfloat16()), n
+
+
+def test_gates_of_2_to_the_32_elements(gpu):
+    _needs(gpu, 40)
+    rows, H = (1 << 26) + 3, 64
+    a = (torch.arange(rows, device=gpu, dtype=torch.int32) % 61 - 30).bfloat16()[:, None].expand(rows, H).contiguous()
+    A_log, dt_bias = torch.linspace(-3, 2, H, device=gpu), torch.linspace(-1, 1, H, device=gpu)
+    g = gdn.forget_gate(a, A_log, dt_bias)
+    want = gdn.forget_gate(a[:61], A_log, dt_bias)
+    for r0 in (0, rows // 61 // 2 * 61, (rows // 61 - 1) * 61):
+        assert torch.equal(g[r0:r0 + 61], want), r0
+    assert torch.equal(g[-3:], gdn.forget_gate(a[-3:], A_log, dt_bias))
+
+
+def test_gated_norm_of_2_to_the_26_rows(gpu):
+    """A wave a row: 2^32 threads and some more."""
+    _needs(gpu, 16)
+    rows, D = (1 << 26) + 5, 8
+    x = (torch.arange(rows, device=gpu, dtype=torch.int32) % 97 - 48).bfloat16()[:, None].expand(rows, D).contiguous()
+    z = x.flip(0).contiguous()
+    w = torch.linspace(0.5, 1.5, D, device=gpu)
+    y = gdn.gated_rms_norm(x, z, w, 1e-6)
+    for r0 in (0, rows // 2 - 50, rows - 100):
+        assert torch.equal(y[r0:r0 + 100], gdn.gated_rms_norm(x[r0:r0 + 100], z[r0:r0 + 100], w, 1e-6)), r0
