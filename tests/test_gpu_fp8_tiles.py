@@ -10,11 +10,14 @@ import pytest
 import torch
 
 import mlx_lean_moe_amd as gdn
+from . import plans
 
 pytestmark = pytest.mark.gpu
 
 DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 U = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11, "f32": 2.0 ** -24}
+# float16 values below 2^-14 lie 2^-24 apart: half of that is what rounding takes
+LEAST = {"bf16": 1e-30, "f16": 2.0 ** -25, "f32": 1e-30}
 FP8 = gdn.QuantScheme(8, 128, "fp8_block")
 
 
@@ -47,7 +50,7 @@ def _check(y, x, W, act, residual=None):
     K = x.shape[1]
     ref, mag = _reference(x, W)
     tol = mag * ((128 + K / 128 + 8) * 2.0 ** -24 if act == "f32" else 2.0 ** -11)
-    tol = tol + U[act] * (ref.abs() + tol) + 2.0 ** -24 * U[act]
+    tol = tol + U[act] * (ref.abs() + tol) + LEAST[act]
     if residual is not None:
         ref = ref + residual.double()
         tol = tol + U[act] * (ref.abs() + tol)
@@ -64,3 +67,28 @@ def test_columns_in_two_launches_of_rows_that_start_anywhere(gpu, act, M, N, K):
     x, W, res = _case(gpu, M, N, K, act, M + N)
     _check(gdn.quantized_linear(x, W, FP8), x, W, act)
     _check(gdn.quantized_linear(x, W, FP8, residual=res), x, W, act, res)
+
+
+@pytest.mark.parametrize("exact,M,N,K,launches", plans.FP8_LAYOUTS, ids=lambda v: "+".join(v) if isinstance(v, list) else None)
+def test_each_tile(gpu, exact, M, N, K, launches):
+    """Which sizes take which tiles is held by test_plans_host.py."""
+    for act in ("f32",) if exact else ("bf16", "f16"):
+        x, W, res = _case(gpu, M, N, K, act, M + K)
+        _check(gdn.quantized_linear(x, W, FP8), x, W, act)
+        _check(gdn.quantized_linear(x, W, FP8, residual=res), x, W, act, res)
+
+
+@pytest.mark.parametrize("exact,M,N,K,launches", [c for c in plans.FP8_LAYOUTS if c[1] > 1000][::2],
+                         ids=lambda v: "+".join(v) if isinstance(v, list) else None)
+def test_rows_that_are_not_finite_stay_their_own_in_large_tiles(gpu, exact, M, N, K, launches):
+    act = "f32" if exact else "bf16"
+    x, W, _ = _case(gpu, M, N, K, act, 3)
+    clean = gdn.quantized_linear(x, W, FP8)
+    rows = [0, 255, 700, M - 1]
+    for i, m in enumerate(rows):
+        x[m, (131 * i + K - 1) % K] = float("nan") if i % 2 else float("-inf")
+    y = gdn.quantized_linear(x, W, FP8)
+    assert torch.isnan(y[rows]).all()
+    keep = torch.ones(M, dtype=torch.bool, device=gpu)
+    keep[rows] = False
+    assert torch.equal(y[keep], clean[keep])
