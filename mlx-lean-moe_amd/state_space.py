@@ -46,7 +46,10 @@ class PackedRuns:
     of a model (and to capture the calls into a graph)."""
 
     def __init__(self, offsets, device: torch.device | str = "cuda") -> None:
-        host = torch.as_tensor(offsets).to("cpu", torch.int64)
+        host = torch.as_tensor(offsets)
+        if host.numel() and (host.is_floating_point() or host.is_complex() or host.dtype == torch.bool):
+            raise ValueError(f"offsets must be whole numbers, got {host.dtype}")
+        host = host.to("cpu", torch.int64)
         if host.ndim != 1 or host.numel() < 2:
             raise ValueError("offsets must be 1-D with at least two entries")
         self.offsets = tuple(_check_cu_seqlens(host, int(host[-1])))
@@ -63,7 +66,7 @@ class PackedRuns:
 
 def _runs(cu_seqlens, T: int, device) -> PackedRuns:
     if not isinstance(cu_seqlens, PackedRuns):
-        return PackedRuns(_check_cu_seqlens(cu_seqlens, T), device)
+        cu_seqlens = PackedRuns(cu_seqlens, device)
     if cu_seqlens.tokens != T:
         raise ValueError(f"cu_seqlens must run from 0 to the token count {T}")
     if cu_seqlens.on_device.device != device:
