@@ -11,6 +11,7 @@ import pytest
 import torch
 
 import mlx_lean_moe_amd as gdn
+from mlx_lean_moe_amd import _lib
 from .scan64 import scan64
 
 pytestmark = pytest.mark.gpu
@@ -137,3 +138,32 @@ def test_whole_tokens_that_are_not_finite(gpu, act):
         e = (170 + 128 + 128) * 2.0 ** -24 + 2.0 ** -18
         _within(y[:end], ref, u * ref.abs() + ((u * 1.01 if act == "bf16" else 0) + e) * ya + 2.0 ** -48, "y")
         assert torch.isnan(y[end:]).all()
+
+
+@pytest.mark.parametrize("act", ["bf16", "f32"])
+@pytest.mark.parametrize("lens,tail", [([40, 0, 9], 30), ([700, 64, 1], 200), ([3, 1500], 1)])
+def test_rows_behind_the_last_run_stay_at_the_c_boundary(gpu, act, lens, tail):
+    """The offsets may end before the arrays, and the longest run may be given,
+    left out or given too short: rows behind the last run are neither read nor
+    written, and how the call is cut changes the sums' order only."""
+    H, P, G, N = dims = (4, 64, 2, 128)
+    case = _case(gpu, act, lens, dims, 70)
+    ref, state, ya, sa = scan64(**case, lens=lens)
+    end, T, R = sum(lens), sum(lens) + tail, len(lens)
+    bad = lambda t: torch.cat([t, torch.full((tail, *t.shape[1:]), float("nan"), device=gpu, dtype=t.dtype)])
+    x, dt, B, C = (bad(case[k]) for k in ("x", "dt", "B", "C"))
+    cu = torch.tensor(_offsets(lens), dtype=torch.int32, device=gpu)
+    code, lib = _lib.dtype_code(DT[act]), _lib.load()
+    e, u = (T + 128 + 128) * 2.0 ** -24 + 2.0 ** -18, U[act]
+    for longest in (max(lens), 0, 1, 65):
+        y = torch.full((T, H, P), 7.0, device=gpu, dtype=DT[act])
+        S = torch.empty(R, H, P, N, device=gpu)
+        size = lib.gdn_selective_scan_workspace_size(code, code, R, T, longest, G, H, P, N)
+        ws = torch.empty(max(size, 1), dtype=torch.uint8, device=gpu)
+        _lib.call_on(gpu, "gdn_selective_scan", x.data_ptr(), H * P, B.data_ptr(), G * N, C.data_ptr(), G * N, code,
+                     dt.data_ptr(), H, code, case["A_log"].data_ptr(), case["dt_bias"].data_ptr(), case["D"].data_ptr(),
+                     case["state"].data_ptr(), S.data_ptr(), y.data_ptr(), code, cu.data_ptr(), R, T, longest, G, H, P, N,
+                     ws.data_ptr(), size, _lib.stream_ptr(gpu))
+        assert (y[end:] == 7).all()
+        _within(y[:end], ref, u * ref.abs() + ((u * 1.01 if act == "bf16" else 0) + e) * ya + 1e-30, "y")
+        _within(S, state, e * sa + 1e-30, "state")
