@@ -504,8 +504,11 @@ int gdn_conv_silu(const void *x, int64_t x_stride, const void *conv_state_in, vo
  *      arguments (0: none); calls sharing one must not overlap
  * P and S multiples of 8, S at most 256 (else GDN_EUNSUPPORTED); x, B, C (and
  * their rows), y, states and workspace 16-byte aligned. bfloat16 x with
- * bfloat16 y runs on the bf16 matrix cores (state and sums float32), all else
- * on the float32 ones. No reference counterpart.
+ * bfloat16 y runs on the bf16 matrix cores (state and sums float32; the decayed
+ * scores and a copy of the state are rounded to bfloat16 on their way to y), all
+ * else on the float32 ones, in full: float32 y avoids those roundings. Rows of y
+ * behind the last run are left as they are; NaN and infinity reach no token before
+ * their own. No reference counterpart.
  */
 int64_t gdn_selective_scan_workspace_size(int act_dtype, int y_dtype, int N, int64_t T_total, int64_t longest_run,
                                           int G, int H, int P, int S);
@@ -540,8 +543,10 @@ int gdn_selective_step(const void *xbc, int64_t xbc_stride, const void *dt, int6
  * gdn_fp8_matmul - y = x W^T (+ residual) for W in e4m3 codes with a scale for
  * each block of 128 x 128, x quantized on the way in: per row and 128 columns
  * to e4m3 codes q = x / s under s = max(amax |x| / 448, 2^-126) (float32
- * divisions, nearest even). y[m,n] = sum over blocks of s sw sum(q w): the
- * inner sums on the 8-bit matrix cores, float32 beyond.
+ * divisions, nearest even). y[m,n] = sum over blocks of s sw sum(q w), float32
+ * beyond the inner sums. Those run on the 8-bit matrix cores for 16-bit y, which
+ * keep some 13 bits below the largest product of a block, and on the bf16 ones with
+ * the codes widened exactly, float32 sums, for float32 y.
  *   x: (M, K) x_dtype; w: (N, K) e4m3 (fn) bytes; scales: (ceil(N / 128),
  *   ceil(K / 128)) float32; y: (M, N) y_dtype; residual: NULL or (M, N) y_dtype
  *   (may be y), added to the product rounded to y_dtype

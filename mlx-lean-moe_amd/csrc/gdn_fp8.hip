@@ -4,7 +4,8 @@
 // divisions, then one rounding to nearest even). Then
 //   y[m, n] = sum_b s[m, b] sw[n / 128, b] sum_{k in b} q[m, k] w[n, k],
 // the inner sums on the 8-bit matrix cores (one 16x16x128 product per block, so
-// scales meet float32 sums only), the outer one in float32.
+// scales meet float32 sums only), the outer one in float32. float32 results take
+// the codes widened to bfloat16 instead (at mfma_widened).
 #include <type_traits>
 
 #include "gdn_common.h"
@@ -68,7 +69,7 @@ GDN_DEV uint32_t codes4(float a, float b, float c, float d) {
 // a group of 128, 8 values a lane. A workgroup takes one block of 16 rows, whose
 // scales are one 64-byte line (the groups of one row, whose scales lie far apart:
 // the same within 5 %). Measured, bf16: 200 rows of 4096 3.5 us, 4096 of 2048
-// 9.5 (2.6 TB/s); four groups a lane 10.6.
+// 10.9 (2.3 TB/s; the fastest of 23 calls 9.5, with four groups a lane 10.6).
 template <class Act>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(const typename Act::storage* __restrict__ x, int M, int K,
                                                            int kb, uint8_t* __restrict__ codes,
@@ -194,7 +195,9 @@ GDN_DEV __amdgpu_buffer_rsrc_t byte_rows(const uint8_t* base, int rows, int widt
 // slots: 256 x 256 tiles of 4096 x 12288 x 2048 117 us (1.76 PFLOP/s; the vendor's
 // product with one scale for each operand reached 2.7 at 8192^3). Small tiles are
 // bound by the latency of a block's loads; rows and outputs too few for a tile a
-// CU split K.
+// CU split K. float32 results, 4096 x 12352 x 2048: 252 us in all, 200 rows 27. A
+// residual is read two bytes at a time: 4096 rows 4096 -> 2048 62 us with, 52
+// without.
 template <int TN, int TM, int kWN, int kWM, bool kExact>
 __global__ __launch_bounds__(64 * kWN * kWM) void fp8_tile_kernel(Fp8Args a) {
     constexpr int kWaves = kWN * kWM, RN = TN / (16 * kWN), RM = TM / (16 * kWM);
@@ -469,7 +472,8 @@ __global__ __launch_bounds__(256) void fp8_sum_kernel(Fp8Args a, int splits) {
 }
 
 // The dense weights: code times its block's scale, one rounding. 16 codes a
-// thread.
+// thread, stored one by one, 32 bytes from lane to lane, which bounds it: 12352 x
+// 2048 to bfloat16 64 us (1.2 TB/s), to float32 115.
 __global__ __launch_bounds__(256) void fp8_dequantize_kernel(const uint8_t* __restrict__ w,
                                                              const float* __restrict__ sw, void* __restrict__ out,
                                                              int out_dtype, int N, int K, int kb) {

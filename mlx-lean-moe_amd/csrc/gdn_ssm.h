@@ -1,5 +1,5 @@
 // Shared pieces of the state-space operators: the run and segment layout of
-// packed prompts and the per-token step and decay.
+// packed prompts, SiLU, and eight values as floats.
 #pragma once
 
 #include "gdn_common.h"

@@ -12,9 +12,11 @@
 // follow each other, so the taps (4 V K bytes a lane, as much as a tile of 16-bit
 // values) and the K - 1 rows before a tile come from the CU's own cache.
 //
-// Measured, 6144 channels: 4096 bf16 tokens 26.4 us (3.8 TB/s; a copy of the same
-// bytes 20.9), 16384 82.8 (4.9 TB/s; 75), 41 5.5; 4096 float32 tokens 39.7 (5.1
-// TB/s; 39.0).
+// Measured, 6144 channels, over 1.6 GB of different inputs in turn, so that none
+// are in a cache: 4096 bf16 tokens 27.2 us (3.7 TB/s; a copy of the same bytes
+// 21.5), 16384 88 (4.6 TB/s; 78), 512 8.1 (4.3), 41 6.2 (2.0); 4096 float32 tokens
+// 41.1 (4.9 TB/s; 39.6). On one input over and over, which the last-level cache
+// holds in part: 21.9, 85, 6.4, 5.5 and 33.0.
 #include "gdn_host.h"
 #include "gdn_ssm.h"
 
@@ -212,7 +214,7 @@ extern "C" int gdn_conv_silu(const void* x, int64_t x_stride, const void* conv_s
     };
     // Tiles of 8 tokens; of 16 where lanes hold 8 channels, there are 8 waves of
     // them a CU and runs have 64 tokens on average. us with 8 and 16, bf16, 6144
-    // channels: 41 tokens 5.5, 6.8; 512 6.8, 8.5; 4096 28.5, 26.4; 16384 91, 83;
+    // channels, inputs from memory: 41 tokens 5.5, 6.8; 512 6.8, 8.5; 4096 28.5, 26.4; 16384 91, 83;
     // 256 runs of 8 17.4, 24.8 (a tile that runs share goes row by row). 4096
     // float32 tokens 39.7, 42.1.
     const auto tiled = [&](auto act, auto vec) {

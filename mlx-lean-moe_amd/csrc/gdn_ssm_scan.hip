@@ -176,17 +176,19 @@ GDN_DEV bf16x8 column_frag(const uint16_t* tile, int stride, int r0, int col, in
 // never passes through LDS. kNP: state_dim rounded up to 32, 64, 128 or 256.
 //
 // Roundings to bfloat16: the decayed scores and, as the operand of S C^T, a
-// copy of the state; both only enter y, which is bfloat16 itself. The state's
-// own update takes x' = d exp(c_Q - c) x in three bfloat16 pieces, all 24 bits
+// copy of the state; both only enter y, which is bfloat16 itself (error against
+// 64 bits 1.9e-3, of y's own rounding alone 1.7e-3, nearly all of the difference
+// the scores': the state in two pieces gave 1.9e-3 too and cost 4 %; scores in two
+// pieces would leave LDS room for one workgroup a CU). The state's own update takes x' = d exp(c_Q - c) x in three bfloat16 pieces, all 24 bits
 // (two left 2.7e-6 of the state behind, and took 0.85 of the time).
 //
-// Bound by the chain of chunks: two workgroups a CU leave the matrix cores 18 %,
-// the vector units 32 % and LDS 44 % busy, 6.2 us a chunk. Eight waves a
-// workgroup, 128 registers each, spilled and took twice as long; LDS rows with
-// their pieces permuted or spaced apart were no faster. Measured, state_dim 128:
-// 41 tokens of 32 heads of 64 9.5 us; 4096 of 64 heads in segments of 256 26.7
-// for their sums, 12.7 for the chain, 43.5 for y (87 MB without the segments'
-// states: 1.0 TB/s).
+// Bound by the chain of chunks: two workgroups a CU leave the matrix cores 19 %,
+// the vector units 36 % and LDS 40 % busy (12 of them bank conflicts), 6.2 us a
+// chunk. Eight waves a workgroup, 128 registers each, spilled and took twice as
+// long; LDS rows with their pieces permuted or spaced apart were no faster.
+// Measured, state_dim 128: 41 tokens of 32 heads of 64 9.5 us; 4096 of 64 heads in
+// segments of 256 26.7 for their sums, 12.5 for the chain, 44.2 for y (87 MB
+// without the segments' states: 1.0 TB/s).
 template <int kNP, int kHeads, int kTiles, bool kStateOnly>
 __global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_kernel(ScanArgs a) {
     constexpr int Q = 64, NS = kNP + 8, PW = 64 * kTiles, PH = PW / kHeads, XS = PW + 8, WS = Q + 8;
@@ -494,9 +496,10 @@ __global__ __launch_bounds__(kScanThreads, kNP <= 128 ? 2 : 1) void scan_bf16_ke
 //
 // Bound by the float32 matrix cores' rate and the LDS reads of their operands
 // (each 16-byte read feeds four steps). Measured, float32, 1531 tokens of 32
-// heads of 128, state_dim 128: 34.2 us for the segments' sums, 10.0 for the
-// chain, 54.1 for y (with four waves a workgroup the three took 115, with eight
-// 93).
+// heads of 128, state_dim 128: 34.6 us for the segments' sums, 10.2 for the
+// chain, 54.7 for y (with four waves a workgroup the three took 115, with eight
+// 93). float16 and bfloat16 with float32 y run here too, 4096 tokens of 64 heads of
+// 64 170 us (bfloat16 y on the kernel above 84).
 template <class Act, int kNP, int kHeads, int kWaves, bool kStateOnly>
 __global__ __launch_bounds__(64 * kWaves, kNP <= 128 ? kWaves / 2 : kWaves / 4) void scan_f32_kernel(ScanArgs a) {
     constexpr int Q = 32, kThreads = 64 * kWaves, NS = kNP + 4, PW = 16 * kWaves, PH = PW / kHeads, XS = PW + 4, WS = Q + 4;

@@ -7,7 +7,9 @@ float32 state, B and C shared by the consecutive heads of a group, and the
 short causal conv with SiLU in front of it. The decay is
 :func:`gated_delta.forget_gate` of ``dt``; the state layout, the conv taps and
 the slot pool (:class:`RecurrentStatePool`) are those of the gated-delta
-layer, and :func:`gated_rms_norm` follows it as it follows that.
+layer. :func:`gated_rms_norm` behind it is ``silu(z) * rms_norm(y)`` per head, for
+layers that normalise first and gate then; those that gate first and normalise
+the product, over a head or a group's channels, bring their own norm.
 
 * :func:`conv_silu`       -- conv + SiLU + conv-state roll over packed prompts
 * :func:`selective_scan`  -- the recurrence over prompts (batch-first or packed)
@@ -197,8 +199,11 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, B: torch.Tensor, C: torch.
     Returns ``(y, new_state)``: y shaped as x in ``y_dtype`` (x's dtype by
     default), the state float32, in ``state_out`` when given (which may be
     ``state`` itself, and must not overlap it otherwise). bfloat16 inputs with
-    bfloat16 y run on the bf16 matrix cores with float32 sums, every other mix
-    on the float32 ones. NaN or infinity in a token reaches that and the later
+    bfloat16 y run on the bf16 matrix cores with float32 sums and state; the
+    decayed scores and a copy of the state are rounded to bfloat16 on their way to
+    y (error 1.9e-3 of its norm, 1.7e-3 of it y's own rounding). Every other mix
+    runs on the float32 ones, in full: so do bfloat16 inputs under
+    ``y_dtype=torch.float32``, at about twice the time. NaN or infinity in a token reaches that and the later
     tokens of its run, none before it."""
 
     packed = cu_seqlens is not None

@@ -1,7 +1,8 @@
 """NumPy float64 restatement of the state-space operators and of the
 block-scaled 8-bit product, straight from their definitions (test
-infrastructure only). ``scan`` and ``step`` also return what the same sums give
-with every operand's absolute value: the yardstick of rounding errors."""
+infrastructure only). ``conv_silu``, ``scan`` and ``fp8_block_matmul`` also return
+what the same sums give with every term's absolute value: the yardstick of
+rounding errors."""
 
 from __future__ import annotations
 
