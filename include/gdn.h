@@ -118,7 +118,8 @@ int gdn_scan_reference(const void *q, const void *k, int qk_dtype, const void *v
 /*
  * gdn_scan - sequential recurrence with the state held in registers across
  * the token loop: 32 lanes per state row, 8 rows per workgroup. Same
- * arguments and layout as gdn_scan_reference; Dk in {32, 64, 128, 256}.
+ * arguments and layout as gdn_scan_reference; Dk in {32, 64, 128, 256}; N * Hv *
+ * ceil(Dv / 8) below 2^24 workgroups, a grid's (GDN_EINVAL from there on).
  * Replaces the Metal kernel lean_moe_gated_delta_scan_f32
  * (_gated_delta_metal.py:35-114), generalised to a batch of runs and to
  * bf16/f16 inputs.

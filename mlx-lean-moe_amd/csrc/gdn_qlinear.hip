@@ -1105,7 +1105,7 @@ template <int kBits, class SB, class O>
 __global__ void dequantize_kernel(const uint32_t* __restrict__ w, const typename SB::storage* __restrict__ scales,
                                   const typename SB::storage* __restrict__ biases,
                                   typename O::storage* __restrict__ out, int N, int K, int group_size) {
-    const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;  // one word
+    const int64_t i = (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x;  // one word
     const int64_t wpr = K / Packing<kBits>::per_word;
     if (i >= int64_t(N) * wpr) return;
     const int64_t n = i / wpr, k0 = (i % wpr) * Packing<kBits>::per_word;
@@ -1161,7 +1161,7 @@ template <int kBits, class SB>
 int launch_dequant_out(const uint32_t* w, const void* scales, const void* biases, void* out,
                        int out_dtype, int N, int K, int group_size, hipStream_t s) {
     const int64_t words = int64_t(N) * (K / Packing<kBits>::per_word);
-    const dim3 grid(unsigned((words + 255) / 256));
+    const dim3 grid = rows_of_blocks((words + 255) / 256);
     const auto* sc = static_cast<const typename SB::storage*>(scales);
     const auto* bi = static_cast<const typename SB::storage*>(biases);
     if (out_dtype == GDN_F32)
@@ -1927,9 +1927,7 @@ extern "C" int gdn_dequantize(const void* w, const void* scales, const void* bia
     GDN_REQUIRE(mode != GDN_QUANT_AFFINE || valid_dtype(sb_dtype), "gdn_dequantize: bad scales/biases dtype");
     GDN_REQUIRE(int64_t(N) * ((K + 31) / 32) < (int64_t(1) << 31), "gdn_dequantize: %lld elements exceed the grid",
                 (long long)N * K);
-    // rows of at most 2^23 blocks: a grid dimension holds less than 2^32 threads
-    const int64_t blocks = (int64_t(N) * (K / 8) + 255) / 256, row = int64_t(1) << 23;
-    const dim3 grid(unsigned(blocks < row ? blocks : row), unsigned((blocks + row - 1) / row));
+    const dim3 grid = rows_of_blocks((int64_t(N) * (K / 8) + 255) / 256);
     auto kernel = dequantize_scheme_kernel<GDN_QUANT_AFFINE, 2>;
     switch (mode) {
         case GDN_QUANT_MXFP4: kernel = dequantize_scheme_kernel<GDN_QUANT_MXFP4, 4>; break;

@@ -115,3 +115,17 @@ def test_gated_norm_of_2_to_the_26_rows(gpu):
     y = gdn.gated_rms_norm(x, z, w, 1e-6)
     for r0 in (0, rows // 2 - 50, rows - 100):
         assert torch.equal(y[r0:r0 + 100], gdn.gated_rms_norm(x[r0:r0 + 100], z[r0:r0 + 100], w, 1e-6)), r0
+
+
+def test_dequantize_of_2_to_the_32_words(gpu):
+    """8-bit affine codes, a word of four a thread: 2^32 threads and some more."""
+    _needs(gpu, 80)
+    N, K, gs = (1 << 20) + 16, 1 << 14, 128
+    w = torch.randint(-2 ** 31, 2 ** 31 - 1, (N, K // 4), dtype=torch.int32, device=gpu)
+    s = torch.rand(N, K // gs, device=gpu).bfloat16()
+    out = gdn.dequantize({"weight": w, "scales": s, "biases": s}, gdn.QuantScheme(8, gs), torch.bfloat16)
+    shifts = torch.arange(0, 32, 8, device=gpu, dtype=torch.int32)
+    for n in (0, 5, N // 2, N - (1 << 16), N - 8):
+        q = ((w[n:n + 8, :, None] >> shifts) & 255).reshape(8, K).float()
+        sc = s[n:n + 8].float().repeat_interleave(gs, 1)
+        assert torch.equal(out[n:n + 8], torch.addcmul(sc, sc, q).bfloat16()), n
