@@ -177,10 +177,11 @@ GDN_DEV bf16x8 column_frag(const uint16_t* tile, int stride, int r0, int col, in
 //
 // Roundings to bfloat16: the decayed scores and, as the operand of S C^T, a
 // copy of the state; both only enter y, which is bfloat16 itself (error against
-// 64 bits 1.9e-3, of y's own rounding alone 1.7e-3, nearly all of the difference
-// the scores': the state in two pieces gave 1.9e-3 too and cost 4 %; scores in two
-// pieces would leave LDS room for one workgroup a CU). The state's own update takes x' = d exp(c_Q - c) x in three bfloat16 pieces, all 24 bits
-// (two left 2.7e-6 of the state behind, and took 0.85 of the time).
+// 64 bits 1.9e-3, 1.7e-3 of it y's own rounding; nearly all of the difference is
+// the scores': the state in two pieces gave 1.9e-3 too and cost 4 %, and scores in
+// two pieces would leave LDS room for one workgroup a CU). The state's own update
+// takes x' = d exp(c_Q - c) x in three bfloat16 pieces, all 24 bits (two left 2.7e-6
+// of the state behind, and took 0.85 of the time).
 //
 // Bound by the chain of chunks: two workgroups a CU leave the matrix cores 19 %,
 // the vector units 36 % and LDS 40 % busy (12 of them bank conflicts), 6.2 us a

@@ -14,6 +14,12 @@ pytestmark = pytest.mark.gpu
 FP8 = gdn.QuantScheme(8, 128, "fp8_block")
 
 
+@pytest.fixture(autouse=True)
+def _return_memory():
+    yield
+    torch.cuda.empty_cache()
+
+
 def _needs(gpu, gib):
     torch.cuda.empty_cache()
     if torch.cuda.mem_get_info(gpu)[0] < gib << 30:
