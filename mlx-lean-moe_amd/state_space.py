@@ -203,8 +203,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, B: torch.Tensor, C: torch.
     decayed scores and a copy of the state are rounded to bfloat16 on their way to
     y (error 1.9e-3 of its norm, 1.7e-3 of it y's own rounding). Every other mix
     runs on the float32 ones, in full: so do bfloat16 inputs under
-    ``y_dtype=torch.float32``, at about twice the time. NaN or infinity in a token reaches that and the later
-    tokens of its run, none before it."""
+    ``y_dtype=torch.float32``, at about twice the time. NaN or infinity in a token
+    reaches that and the later tokens of its run, none before it."""
 
     packed = cu_seqlens is not None
     lead = 1 if packed else 2
