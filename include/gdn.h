@@ -58,7 +58,8 @@ typedef enum {
  * gdn_quantized_matmul_rows_workspace_size, 18 gdn_quantized_matmul_rows, which
  * alone uses that workspace, 19 gdn_prefill_chunked_runs and
  * gdn_prefill_fused_runs, 20 gdn_conv_silu, gdn_selective_scan,
- * gdn_selective_step, gdn_fp8_matmul and gdn_fp8_dequantize). */
+ * gdn_selective_step, gdn_fp8_matmul and gdn_fp8_dequantize, 21 gdn_rms_norm
+ * and gdn_fp8_matmul_codes). */
 int gdn_abi_version(void);
 
 /* Message describing the calling thread's last non-zero return. */
@@ -295,6 +296,26 @@ int gdn_prefill_fused_runs(const void *qkv, int64_t qkv_stride, const void *conv
 int gdn_gated_rmsnorm(const void *x, int x_dtype, const void *z, int z_dtype, int64_t z_stride,
                       int heads, const float *w, float eps, void *out, int out_dtype, int64_t rows,
                       int D, void *stream);
+
+/*
+ * gdn_rms_norm - y = s w / sqrt(mean(s^2) + eps) over rows of K, s = x, or x +
+ * residual rounded to dtype, which is written to sum. y is the exact value rounded
+ * to float32, then to dtype; sums are held in 64 bits.
+ *   x, residual (or NULL), sum (NULL without a residual): (rows, K) dtype at their
+ *      own row strides in elements; sum may be x or residual (the same pointer and
+ *      stride) and must not overlap them otherwise
+ *   w: (K) float32 or NULL (ones)
+ *   out: (rows, K) dtype packed, or NULL
+ *   codes, scales: NULL, or y in e4m3 as gdn_fp8_matmul_codes takes it (K a
+ *      multiple of 16): per 128 columns scale = max(amax |y| / 448, 2^-126), code =
+ *      e4m3(y / scale), what gdn_fp8_matmul makes of out; scale_stride at least
+ *      rows. NaN or infinity in y makes its group's codes NaN.
+ * At least one of out and codes. Rows may start at any element. Replaces the
+ * decoder layer's norm (transformer.py:110-112).
+ */
+int gdn_rms_norm(const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, void *sum,
+                 int64_t sum_stride, const float *w, float eps, int dtype, void *out, void *codes,
+                 float *scales, int scale_stride, int64_t rows, int K, void *stream);
 
 /*
  * gdn_quantized_matmul - y = x W^T for an affine-quantized W in MLX's packing,
@@ -561,6 +582,20 @@ int64_t gdn_fp8_matmul_workspace_size(int y_dtype, int M, int N, int K);
 int gdn_fp8_matmul(const void *x, int x_dtype, const void *w, const float *scales, void *y, int y_dtype,
                    const void *residual, int M, int N, int K, void *workspace, int64_t workspace_bytes,
                    void *stream);
+
+/*
+ * gdn_fp8_matmul_codes - gdn_fp8_matmul of rows that are in codes already, as
+ * gdn_rms_norm writes them: the same y from the same codes and scales, to the bit.
+ *   codes: (M, ceil(K / 128) * 128) e4m3 bytes, the columns past K zero;
+ *   row_scales: (ceil(K / 128), scale_stride) float32, row m's at column m;
+ *   scale_stride a multiple of 256, at least M; the rest as gdn_fp8_matmul
+ *   workspace: gdn_fp8_matmul_codes_workspace_size(...) bytes (0: none needed);
+ *   calls sharing one must not overlap
+ */
+int64_t gdn_fp8_matmul_codes_workspace_size(int y_dtype, int M, int N, int K);
+int gdn_fp8_matmul_codes(const void *codes, const float *row_scales, int scale_stride, const void *w,
+                         const float *scales, void *y, int y_dtype, const void *residual, int M, int N, int K,
+                         void *workspace, int64_t workspace_bytes, void *stream);
 
 /* gdn_fp8_dequantize - gdn_fp8_matmul's weights as a dense (N, K) out_dtype
  * array: code times scale, one rounding. */

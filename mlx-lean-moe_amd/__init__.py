@@ -12,7 +12,8 @@ from .gated_delta import (beta_gate, forget_gate, gated_delta_scan, gated_delta_
                           gated_delta_update)
 from .linear_attention import (DecodeGraph, PrefillGraph, Qwen3_5LinearAttention, conv_frontend,
                                fused_decode_step, fused_prefill_ok, gated_rms_norm, prefill_fused)
-from .quant import LinearWeights, QuantScheme, dequantize, quantized_linear
+from .norm import rms_norm
+from .quant import LinearWeights, QuantizedRows, QuantScheme, dequantize, quantized_linear
 from .recurrent_cache import RecurrentCache, RecurrentStatePool
 from .state_space import PackedRuns, conv_silu, selective_scan, selective_step
 
@@ -23,6 +24,7 @@ __all__ = [
     "LinearWeights",
     "PackedRuns",
     "QuantScheme",
+    "QuantizedRows",
     "QWEN3_5_LINEAR",
     "Qwen3_5LinearAttention",
     "RecurrentCache",
@@ -41,6 +43,7 @@ __all__ = [
     "gated_rms_norm",
     "prefill_fused",
     "quantized_linear",
+    "rms_norm",
     "selective_scan",
     "selective_step",
 ]

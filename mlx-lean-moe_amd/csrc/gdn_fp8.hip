@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "gdn_common.h"
+#include "gdn_fp8.h"
 #include "gdn_fp8_plan.h"
 #include "gdn_host.h"
 #include "gdn_ssm.h"
@@ -16,54 +17,7 @@
 namespace gdn {
 namespace {
 
-constexpr int kB = 128;  // block of the scales, both ways
-constexpr float kE4m3Max = 448.f;
-
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-// The largest |x| of 16 lanes as float bits, NaN above all.
-GDN_DEV uint32_t row16_max(uint32_t v) {
-#define GDN_DPP_MAX(CTRL) \
-    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, 0xF, 0xF, false)))
-    GDN_DPP_MAX(0xB1);
-    GDN_DPP_MAX(0x4E);
-    GDN_DPP_MAX(0x141);
-    GDN_DPP_MAX(0x140);
-#undef GDN_DPP_MAX
-    return v;
-}
-
-GDN_DEV float scale_of(uint32_t amax_bits) {
-    const float s = __uint_as_float(amax_bits) / kE4m3Max;
-    return s < 0x1p-126f ? 0x1p-126f : s;
-}
-
-// x / s to the last bit for the lane's values, s one group's scale: two
-// Newton corrections of x times the rounded reciprocal, each remainder exact
-// (the second starts within one ulp and so ends correctly rounded). Remainders
-// of the smallest scales would leave float32: divisions there.
-template <int N>
-GDN_DEV void divide_all(float (&x)[N], float s) {
-    if (s < 0x1p-80f) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) x[e] = x[e] / s;
-        return;
-    }
-    const float inv = 1.f / s;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-        float r = x[e] * inv;
-        r = __builtin_fmaf(__builtin_fmaf(-r, s, x[e]), inv, r);
-        x[e] = __builtin_fmaf(__builtin_fmaf(-r, s, x[e]), inv, r);
-    }
-}
-
-// Codes of four values.
-GDN_DEV uint32_t codes4(float a, float b, float c, float d) {
-    int r = 0;
-    r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, r, false);
-    return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true));
-}
 
 // Rows' codes (M x kb * 128, columns past K zero) and scales (kb x ldx): 16 lanes
 // a group of 128, 8 values a lane. A workgroup takes one block of 16 rows, whose
@@ -383,6 +337,12 @@ __global__ __launch_bounds__(64 * kWN * kWM) void fp8_tile_kernel(Fp8Args a) {
 constexpr int kSkinnyWaves = 16;
 constexpr int kAhead = 4;  // blocks of W in flight a wave
 
+// Rows that are in codes already (Fp8Args' q and sx) instead of an activation type.
+struct InCodes {
+    using storage = uint8_t;
+    static constexpr int code = -1;
+};
+
 template <class Act, int kNs, bool kExact>
 __global__ __launch_bounds__(64 * kSkinnyWaves) void fp8_skinny_kernel(Fp8Args a, const typename Act::storage* x) {
     constexpr int kGroups = kSkinnyWaves / kNs;
@@ -417,16 +377,21 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void fp8_skinny_kernel(Fp8Args a
 
     for (int at = tid / 16; at < a.M * a.kb; at += 4 * kSkinnyWaves) {
         const int m = at / a.kb, b = at % a.kb, k = b * kB + (tid & 15) * 8;
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (k < a.K) load8f<Act>(x + int64_t(m) * a.K + k, v);
-        uint32_t top = 0;
+        if constexpr (Act::code == InCodes::code) {
+            *reinterpret_cast<uint2*>(codes + m * stride + k) = *reinterpret_cast<const uint2*>(a.q + m * Kq + k);
+            if ((tid & 15) == 0) sx[m * a.kb + b] = a.sx[int64_t(b) * a.ldx + m];
+        } else {
+            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (k < a.K) load8f<Act>(x + int64_t(m) * a.K + k, v);
+            uint32_t top = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
-        const float s = scale_of(row16_max(top));
-        divide_all(v, s);
-        *reinterpret_cast<uint2*>(codes + m * stride + k) =
-            make_uint2(codes4(v[0], v[1], v[2], v[3]), codes4(v[4], v[5], v[6], v[7]));
-        if ((tid & 15) == 0) sx[m * a.kb + b] = s;
+            for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+            const float s = scale_of(row16_max(top));
+            divide_all(v, s);
+            *reinterpret_cast<uint2*>(codes + m * stride + k) =
+                make_uint2(codes4(v[0], v[1], v[2], v[3]), codes4(v[4], v[5], v[6], v[7]));
+            if ((tid & 15) == 0) sx[m * a.kb + b] = s;
+        }
     }
     __syncthreads();
 
@@ -514,10 +479,48 @@ void launch_product(const Fp8Plan& p, const Fp8Args& a, hipStream_t s) {
                            p.splits);
 }
 
-int64_t codes_bytes(int M, int K) { return (int64_t(M) * ((K + kB - 1) / kB) * kB + 255) / 256 * 256; }
+// Few rows: one launch of whichever x the rows come as.
+template <class Act>
+void launch_skinny(const Fp8Args& a, const void* x, hipStream_t s) {
+    const unsigned bytes = unsigned(skinny_bytes(a.M, a.kb));
+    // 64 rows of W a workgroup, 32 or 16: as many as still give most CUs one
+    // (1 row, us, 16, 32 and 64: 12352 outputs 9.8, 8.0, 7.8; 8192 5.2, 4.9, 5.1;
+    // 2048 5.3, 7.0, 10.5)
+    const auto go = [&](auto exact) {
+        constexpr bool E = decltype(exact)::value;
+        const auto launch = [&](auto kernel, int rows) {
+            hipLaunchKernelGGL(kernel, rows_of_blocks((int64_t(a.N) + rows - 1) / rows), dim3(64 * kSkinnyWaves), bytes, s,
+                               a, static_cast<const typename Act::storage*>(x));
+        };
+        if (a.N > 64 * 190) launch(fp8_skinny_kernel<Act, 4, E>, 64);
+        else if (a.N > 32 * 190) launch(fp8_skinny_kernel<Act, 2, E>, 32);
+        else launch(fp8_skinny_kernel<Act, 1, E>, 16);
+    };
+    if (a.y_dtype == GDN_F32) go(std::true_type{});
+    else go(std::false_type{});
+}
 
-// (a tile's 256 scales are one aligned kilobyte)
-int scale_columns(int M) { return (M + 255) / 256 * 256; }
+// The product of rows in codes: `a` as for all columns, cut as planned, the
+// shares of a split K in `part`.
+void launch_cut(const Fp8Cut& cut, const Fp8Args& a, float* part, hipStream_t s) {
+    const int ys = dtype_size(a.y_dtype);
+    const auto product = [&](const Fp8Plan& p, int n0, int cols) {
+        Fp8Args b = a;
+        b.w += int64_t(n0) * a.K;
+        b.sw += int64_t(n0 / kB) * a.kb;
+        if (a.residual) b.residual = static_cast<const char*>(a.residual) + int64_t(n0) * ys;
+        b.y = static_cast<char*>(a.y) + int64_t(n0) * ys;
+        b.N = cols;
+        b.steps = p.steps;
+        b.part = p.splits > 1 ? part : nullptr;
+        b.N4 = (cols + 3) / 4 * 4;
+        launch_product(p, b, s);
+    };
+    product(cut.first, 0, cut.n0);
+    if (cut.n0 < a.N) product(cut.rest, cut.n0, a.N - cut.n0);
+}
+
+int64_t codes_bytes(int M, int K) { return (int64_t(M) * ((K + kB - 1) / kB) * kB + 255) / 256 * 256; }
 
 // (K: a tile's rows are addressed in 31 bits)
 bool fp8_sizes_ok(int M, int N, int K) {
@@ -551,29 +554,9 @@ extern "C" int gdn_fp8_matmul(const void* x, int x_dtype, const void* w, const f
     if (skinny(M, kb)) {
         const Fp8Args a{nullptr, static_cast<const uint8_t*>(w), nullptr, scales, residual, y, y_dtype, M, N, K, kb, 0, kb,
                         nullptr, 0, N};
-        const unsigned bytes = unsigned(skinny_bytes(M, kb));
-        // 64 rows of W a workgroup, 32 or 16: as many as still give most CUs one
-        // (1 row, us, 16, 32 and 64: 12352 outputs 9.8, 8.0, 7.8; 8192 5.2, 4.9, 5.1;
-        // 2048 5.3, 7.0, 10.5)
-        const auto go = [&](auto act, auto exact) {
-            using Act = decltype(act);
-            constexpr bool E = decltype(exact)::value;
-            const auto* xs = static_cast<const typename Act::storage*>(x);
-            const dim3 threads(64 * kSkinnyWaves);
-            const auto launch = [&](auto kernel, int rows) {
-                hipLaunchKernelGGL(kernel, rows_of_blocks((int64_t(N) + rows - 1) / rows), threads, bytes, s, a, xs);
-            };
-            if (N > 64 * 190) launch(fp8_skinny_kernel<Act, 4, E>, 64);
-            else if (N > 32 * 190) launch(fp8_skinny_kernel<Act, 2, E>, 32);
-            else launch(fp8_skinny_kernel<Act, 1, E>, 16);
-        };
-        const auto typed = [&](auto act) {
-            if (y_dtype == GDN_F32) go(act, std::true_type{});
-            else go(act, std::false_type{});
-        };
-        if (x_dtype == GDN_F32) typed(ActF32{});
-        else if (x_dtype == GDN_BF16) typed(ActBF16{});
-        else typed(ActF16{});
+        if (x_dtype == GDN_F32) launch_skinny<ActF32>(a, x, s);
+        else if (x_dtype == GDN_BF16) launch_skinny<ActBF16>(a, x, s);
+        else launch_skinny<ActF16>(a, x, s);
         return check_launch("gdn_fp8_matmul");
     }
     const Fp8Cut cut = fp8_cut(y_dtype == GDN_F32, M, N, kb);
@@ -592,17 +575,45 @@ extern "C" int gdn_fp8_matmul(const void* x, int x_dtype, const void* w, const f
     if (x_dtype == GDN_F32) quantize(ActF32{});
     else if (x_dtype == GDN_BF16) quantize(ActBF16{});
     else quantize(ActF16{});
-    const int ys = dtype_size(y_dtype);
-    const auto product = [&](const Fp8Plan& p, int n0, int cols) {
-        float* part = p.splits > 1 ? sx + int64_t(ldx) * kb : nullptr;
-        launch_product(p, {codes, static_cast<const uint8_t*>(w) + int64_t(n0) * K, sx, scales + int64_t(n0 / kB) * kb,
-                           residual ? static_cast<const char*>(residual) + int64_t(n0) * ys : nullptr,
-                           static_cast<char*>(y) + int64_t(n0) * ys, y_dtype, M, cols, K, kb, ldx, p.steps, part,
-                           (cols + 3) / 4 * 4, N}, s);
-    };
-    product(cut.first, 0, cut.n0);
-    if (cut.n0 < N) product(cut.rest, cut.n0, N - cut.n0);
+    launch_cut(cut, {codes, static_cast<const uint8_t*>(w), sx, scales, residual, y, y_dtype, M, N, K, kb, ldx, 0, nullptr,
+                     0, N}, sx + int64_t(ldx) * kb, s);
     return check_launch("gdn_fp8_matmul");
+}
+
+extern "C" int64_t gdn_fp8_matmul_codes_workspace_size(int y_dtype, int M, int N, int K) {
+    if (!fp8_sizes_ok(M, N, K) || !valid_dtype(y_dtype)) return 0;
+    const int kb = (K + kB - 1) / kB;
+    return skinny(M, kb) ? 0 : fp8_cut(y_dtype == GDN_F32, M, N, kb).part_bytes();
+}
+
+extern "C" int gdn_fp8_matmul_codes(const void* codes, const float* row_scales, int scale_stride, const void* w,
+                                    const float* scales, void* y, int y_dtype, const void* residual, int M, int N, int K,
+                                    void* workspace, int64_t workspace_bytes, void* stream) {
+    GDN_REQUIRE(fp8_sizes_ok(M, N, K), "gdn_fp8_matmul_codes: bad sizes M=%d N=%d K=%d (K a multiple of 16)", M, N, K);
+    GDN_REQUIRE(valid_dtype(y_dtype), "gdn_fp8_matmul_codes: bad dtype");
+    if (M == 0) return 0;
+    GDN_REQUIRE(codes && row_scales && w && scales && y, "gdn_fp8_matmul_codes: null pointer");
+    GDN_REQUIRE((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(row_scales) |
+                 reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(y) |
+                 reinterpret_cast<uintptr_t>(workspace)) % 16 == 0,
+                "gdn_fp8_matmul_codes: codes, their scales, w, y and workspace must be 16-byte aligned");
+    GDN_REQUIRE(scale_stride >= M && scale_stride % 256 == 0,
+                "gdn_fp8_matmul_codes: scales %d apart for %d rows (a multiple of 256)", scale_stride, M);
+    const int kb = (K + kB - 1) / kB;
+    hipStream_t s = as_stream(stream);
+    const Fp8Args a{static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(w), row_scales, scales, residual, y,
+                    y_dtype, M, N, K, kb, scale_stride, kb, nullptr, 0, N};
+    if (skinny(M, kb)) {
+        launch_skinny<InCodes>(a, codes, s);
+        return check_launch("gdn_fp8_matmul_codes");
+    }
+    const Fp8Cut cut = fp8_cut(y_dtype == GDN_F32, M, N, kb);
+    GDN_REQUIRE(cut.part_bytes() == 0 || (workspace && workspace_bytes >= cut.part_bytes()),
+                "gdn_fp8_matmul_codes: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                (long long)cut.part_bytes());
+    GDN_REQUIRE(int64_t(scale_stride) * kb <= INT32_MAX / 4, "gdn_fp8_matmul_codes: too many rows");
+    launch_cut(cut, a, static_cast<float*>(workspace), s);
+    return check_launch("gdn_fp8_matmul_codes");
 }
 
 extern "C" int gdn_fp8_dequantize(const void* w, const float* scales, void* out, int out_dtype, int N, int K,

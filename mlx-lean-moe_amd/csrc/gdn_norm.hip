@@ -1,0 +1,272 @@
+// RMS norm over rows, with the residual's addition in front of it and, if asked,
+// the result in e4m3 codes:
+//   s = T(x + r),   y = T(s w / sqrt(mean(s^2) + eps)),
+//   per 128 columns: scale = max(amax |y| / 448, 2^-126), code = e4m3(y / scale),
+// T the rounding to the rows' type. y is the exact value rounded to float32 and
+// then to T: sums are held in 64 bits (a square of two float32 values is exact
+// there), and so is each product that falls near a border of T. So neither y nor
+// the codes depend on the order of a sum, and the codes are those that
+// gdn_fp8_matmul makes of y.
+#include <type_traits>
+
+#include "gdn_common.h"
+#include "gdn_fp8.h"
+#include "gdn_host.h"
+
+namespace gdn {
+namespace {
+
+struct NormArgs {
+    const void *x, *residual;
+    void *sum, *out;
+    const float* w;
+    uint8_t* codes;
+    float* scales;
+    int64_t x_stride, r_stride, s_stride, rows;
+    int K, kb, ldx;
+    float eps;
+};
+
+// Eight consecutive values at any alignment of their own type (global memory
+// takes 16-byte accesses at any address); beyond `count` of them zeros.
+template <class Act>
+GDN_DEV void load_up_to8(const typename Act::storage* p, int count, float (&v)[8]) {
+    if (count >= 8) {
+        typename Act::storage raw[8];
+        __builtin_memcpy(raw, p, sizeof(raw));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = Act::load(raw, e);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < count ? Act::load(p, e) : 0.f;
+}
+
+template <class Act>
+GDN_DEV void store_up_to8(typename Act::storage* p, int count, const float (&v)[8]) {
+    if (count >= 8) {
+        typename Act::storage raw[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) Act::store(raw, e, v[e]);
+        __builtin_memcpy(p, raw, sizeof(raw));
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < count) Act::store(p, e, v[e]);
+}
+
+// y of eight values, rounded to the rows' type. In 16 bits the float32 product
+// of three factors, each rounding at most half a last place, lies within 3 last
+// places of the exact value: further than 4 from a border of the type (a tie of
+// the dropped bits) both round alike, else the eight go through 64 bits, as do
+// values near the type's or float32's smallest, and rows (`wild`) whose factor
+// float32 does not hold well.
+template <class Act>
+GDN_DEV void scaled8(const float (&v)[8], double r, float r32, bool wild, const float (&w)[8], float (&y)[8]) {
+    if constexpr (Act::code != GDN_F32) {
+        constexpr uint32_t kMask = Act::code == GDN_BF16 ? 0xFFFFu : 0x1FFFu, kTie = (kMask + 1) / 2;
+        constexpr float kSmall = Act::code == GDN_BF16 ? 0x1p-100f : 0x1p-14f;
+        bool close = wild;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float t = v[e] * r32, f = t * w[e];
+            const uint32_t low = __float_as_uint(f) & kMask;
+            close |= low - (kTie - 4) <= 8u || (fminf(fabsf(t), fabsf(f)) < kSmall && v[e] != 0.f);
+            y[e] = f;
+        }
+        if (close) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = float(double(v[e]) * r * double(w[e]));
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = Act::round(y[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = float(double(v[e]) * r * double(w[e]));
+    }
+}
+
+// The eight columns from k of a row: the stream's values (kept or read again).
+template <class Act>
+GDN_DEV void stream8(const NormArgs& a, int64_t row, int k, bool live, float (&v)[8]) {
+    using S = typename Act::storage;
+    load_up_to8<Act>(static_cast<const S*>(a.x) + row * a.x_stride + k, a.K - k, v);
+    if (!a.residual) return;
+    float r[8];
+    load_up_to8<Act>(static_cast<const S*>(a.residual) + row * a.r_stride + k, a.K - k, r);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = Act::round(v[e] + r[e]);
+    if (live) store_up_to8<Act>(static_cast<S*>(a.sum) + row * a.s_stride + k, a.K - k, v);
+}
+
+GDN_DEV double squares8(const float (&v)[8], double acc) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc = __builtin_fma(double(v[e]), double(v[e]), acc);
+    return acc;
+}
+
+struct Factor {
+    double r;
+    float r32;
+    bool wild;
+};
+
+GDN_DEV Factor factor_of(double sum, int K, float eps) {
+    Factor f;
+    f.r = 1.0 / sqrt(sum / double(K) + double(eps));
+    f.r32 = float(f.r);
+    f.wild = !(f.r32 > 0x1p-60f && f.r32 < 0x1p60f);
+    return f;
+}
+
+// y of the eight columns from k, stored as they are asked for. With codes,
+// sixteen consecutive lanes hold the columns of one scale.
+template <class Act, bool kCodes>
+GDN_DEV void finish8(const NormArgs& a, int64_t row, int k, bool live, const float (&v)[8], const Factor& f) {
+    float w[8], y[8];
+    if (a.w) {
+        load_up_to8<ActF32>(a.w + k, a.K - k, w);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = 1.f;
+    }
+    scaled8<Act>(v, f.r, f.r32, f.wild, w, y);
+    if (a.out && live) store_up_to8<Act>(static_cast<typename Act::storage*>(a.out) + row * a.K + k, a.K - k, y);
+    if constexpr (kCodes) {
+        if (k >= a.K)  // (w of one where there is none: a row of NaN has them here too)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = 0.f;
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(y[e]) & 0x7FFFFFFFu);
+        const float s = scale_of(row16_max(top));
+        divide_all(y, s);
+        if (live && k < a.kb * kB) {
+            *reinterpret_cast<uint2*>(a.codes + row * (int64_t(a.kb) * kB) + k) =
+                make_uint2(codes4(y[0], y[1], y[2], y[3]), codes4(y[4], y[5], y[6], y[7]));
+            if ((threadIdx.x & 15) == 0) a.scales[int64_t(k / kB) * a.ldx + row] = s;
+        }
+    }
+}
+
+// The sum over a row's kLanes threads, in all of them.
+template <int kLanes>
+GDN_DEV double row_sum(double v) {
+    if constexpr (kLanes <= kWave) {
+        return group_sum<kLanes>(v);
+    } else {
+        __shared__ double part[kLanes / kWave];
+        v = group_sum<kWave>(v);
+        if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = v;
+        __syncthreads();
+        v = part[0];
+#pragma unroll
+        for (int i = 1; i < kLanes / kWave; ++i) v += part[i];
+        return v;
+    }
+}
+
+// A row's columns stay in the registers of its kLanes threads, kVec times eight
+// in each: memory is read once and written once, and that is what bounds it.
+template <class Act, int kLanes, int kVec, bool kCodes>
+__global__ __launch_bounds__(kLanes <= kWave ? 256 : kLanes) void rms_norm_kernel(NormArgs a) {
+    constexpr int kRows = kLanes <= kWave ? 256 / kLanes : 1;
+    const int64_t id = int64_t(blockIdx.y) * gridDim.x + blockIdx.x;
+    const int64_t mine = id * kRows + (kRows > 1 ? int(threadIdx.x) / kLanes : 0);
+    if (id * kRows >= a.rows) return;  // (the last row of the grid may be short)
+    const bool live = mine < a.rows;
+    const int64_t row = live ? mine : a.rows - 1;
+    const int lane = threadIdx.x % kLanes;
+    float v[kVec][8];
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+        stream8<Act>(a, row, (j * kLanes + lane) * 8, live, v[j]);
+        sum = squares8(v[j], sum);
+    }
+    const Factor f = factor_of(row_sum<kLanes>(sum), a.K, a.eps);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) finish8<Act, kCodes>(a, row, (j * kLanes + lane) * 8, live, v[j], f);
+}
+
+// Rows longer than registers hold: the stream is read again for the second pass
+// (from `sum` where there is a residual: each thread reads what it wrote).
+template <class Act, bool kCodes>
+__global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs a) {
+    const int64_t row = int64_t(blockIdx.y) * gridDim.x + blockIdx.x;
+    if (row >= a.rows) return;
+    const int end = (a.K + 8191) / 8192 * 8192;
+    float v[8];
+    double sum = 0.0;
+    for (int k = threadIdx.x * 8; k < end; k += 8192) {
+        stream8<Act>(a, row, k, true, v);
+        sum = squares8(v, sum);
+    }
+    const Factor f = factor_of(row_sum<1024>(sum), a.K, a.eps);
+    NormArgs again = a;
+    if (a.residual) again.x = a.sum, again.x_stride = a.s_stride, again.residual = nullptr;
+    for (int k = threadIdx.x * 8; k < end; k += 8192) {
+        stream8<Act>(again, row, k, true, v);
+        finish8<Act, kCodes>(a, row, k, true, v, f);
+    }
+}
+
+template <class Act, bool kCodes>
+void launch_norm(const NormArgs& a, hipStream_t s) {
+    const auto rows = [&](auto kernel, int lanes) {
+        const int per = lanes <= kWave ? 256 / lanes : 1;
+        hipLaunchKernelGGL(kernel, rows_of_blocks((a.rows + per - 1) / per), dim3(lanes <= kWave ? 256 : lanes), 0, s, a);
+    };
+    if (a.K <= 128) rows(rms_norm_kernel<Act, 16, 1, kCodes>, 16);
+    else if (a.K <= 512) rows(rms_norm_kernel<Act, 64, 1, kCodes>, 64);
+    else if (a.K <= 2048) rows(rms_norm_kernel<Act, 256, 1, kCodes>, 256);
+    else if (a.K <= 4096) rows(rms_norm_kernel<Act, 256, 2, kCodes>, 256);
+    else if (a.K <= 8192) rows(rms_norm_kernel<Act, 256, 4, kCodes>, 256);
+    else if (a.K <= 16384) rows(rms_norm_kernel<Act, 1024, 2, kCodes>, 1024);
+    else rows(rms_norm_long_kernel<Act, kCodes>, 1024);
+}
+
+}  // namespace
+}  // namespace gdn
+
+using namespace gdn;
+
+extern "C" int gdn_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, void* sum,
+                            int64_t sum_stride, const float* w, float eps, int dtype, void* out, void* codes,
+                            float* scales, int scale_stride, int64_t rows, int K, void* stream) {
+    GDN_REQUIRE(rows >= 0 && K > 0 && K <= INT32_MAX - 8192, "gdn_rms_norm: bad sizes rows=%lld K=%d", (long long)rows, K);
+    GDN_REQUIRE(valid_dtype(dtype), "gdn_rms_norm: bad dtype");
+    if (rows == 0) return 0;
+    GDN_REQUIRE(x && (out || codes), "gdn_rms_norm: null pointer");
+    GDN_REQUIRE(!residual == !sum, "gdn_rms_norm: a residual goes with a sum");
+    GDN_REQUIRE(x_stride >= K && (!residual || (residual_stride >= K && sum_stride >= K)),
+                "gdn_rms_norm: rows closer than their width of %d", K);
+    if (residual) {  // in place in either input, or apart from both
+        const int es = dtype_size(dtype);
+        const auto span = [&](int64_t stride) { return ((rows - 1) * stride + K) * es; };
+        GDN_REQUIRE((sum == x && sum_stride == x_stride) || !overlaps(sum, span(sum_stride), x, span(x_stride)),
+                    "gdn_rms_norm: sum overlaps x");
+        GDN_REQUIRE((sum == residual && sum_stride == residual_stride) ||
+                        !overlaps(sum, span(sum_stride), residual, span(residual_stride)),
+                    "gdn_rms_norm: sum overlaps residual");
+    }
+    const int kb = (K + kB - 1) / kB;
+    if (codes) {
+        GDN_REQUIRE(scales && K % 16 == 0, "gdn_rms_norm: codes need scales and K a multiple of 16, got %d", K);
+        GDN_REQUIRE(rows <= INT32_MAX - 256 && scale_stride >= rows, "gdn_rms_norm: scales %d apart for %lld rows",
+                    scale_stride, (long long)rows);
+        GDN_REQUIRE(reinterpret_cast<uintptr_t>(codes) % 16 == 0, "gdn_rms_norm: codes must be 16-byte aligned");
+    }
+    const NormArgs a{x, residual, sum, out, w, static_cast<uint8_t*>(codes), scales, x_stride, residual_stride,
+                     sum_stride, rows, K, kb, scale_stride, eps};
+    const auto go = [&](auto act) {
+        using Act = decltype(act);
+        if (codes) launch_norm<Act, true>(a, as_stream(stream));
+        else launch_norm<Act, false>(a, as_stream(stream));
+    };
+    if (dtype == GDN_F32) go(ActF32{});
+    else if (dtype == GDN_BF16) go(ActBF16{});
+    else go(ActF16{});
+    return check_launch("gdn_rms_norm");
+}

@@ -182,6 +182,59 @@ class QuantScheme:
                              f"group_size={self.group_size}")
 
 
+class QuantizedRows:
+    """Rows ``(..., K)`` in e4m3 codes, each row's 128 columns under a float32
+    scale of their own: what :func:`rms_norm` gives with ``quantize=True`` and
+    :func:`quantized_linear` multiplies by fp8_block weights without quantizing
+    them again. K is a multiple of 16.
+
+    ``dtype`` is the activation dtype that products of them come in; ``rows`` the
+    values in that dtype where they were kept (``keep_rows=True``), which every
+    other kind of weights, and low-rank adapters, take instead of the codes."""
+
+    __slots__ = ("shape", "dtype", "rows", "_codes", "_scales")
+
+    def __init__(self, shape, dtype: torch.dtype, codes: torch.Tensor, scales: torch.Tensor,
+                 rows: torch.Tensor | None = None) -> None:
+        """``codes (M, ceil(K / 128) * 128)`` uint8, ``scales (ceil(K / 128), S)``
+        float32 with row m's in column m (S a multiple of 256): the layout that the
+        products read."""
+
+        self.shape, self.dtype, self.rows = torch.Size(shape), dtype, rows
+        self._codes, self._scales = codes, scales
+
+    @property
+    def device(self) -> torch.device:
+        return self._codes.device
+
+    @property
+    def ndim(self) -> int:
+        return len(self.shape)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """The codes ``(..., K)`` as float8_e4m3fn values."""
+        return self._codes[:, :self.shape[-1]].view(torch.float8_e4m3fn).view(self.shape)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """The scales ``(..., ceil(K / 128))``."""
+        return self._scales[:, :self._codes.shape[0]].T.reshape(*self.shape[:-1], -1)
+
+    def dequantize(self) -> torch.Tensor:
+        """The float32 values ``(..., K)`` that codes and scales stand for."""
+        wide = self.scales.repeat_interleave(128, dim=-1)[..., :self.shape[-1]]
+        return self.codes.float() * wide
+
+    def reshape(self, *lead_and_width) -> "QuantizedRows":
+        """The same rows under other leading axes."""
+        shape = torch.empty(self.shape, device="meta").reshape(*lead_and_width).shape
+        if shape[-1:] != self.shape[-1:]:
+            raise ValueError(f"the width {self.shape[-1]} of quantized rows stays")
+        return QuantizedRows(shape, self.dtype, self._codes, self._scales,
+                             None if self.rows is None else self.rows.reshape(shape))
+
+
 @dataclass(frozen=True)
 class LinearWeights:
     """One projection's weights as read: a dense matrix (``quant`` None) or
@@ -334,12 +387,20 @@ def quantized_linear(x: torch.Tensor, tensors, quant: QuantScheme | None = None,
     ``residual`` (the result's shape and dtype) is added to the product
     rounded to that dtype, as the decoder layer's ``h = x + attention(...)``
     (transformer.py:110-112) adds two arrays of it; on the quantized
-    kernels the add is part of the store."""
+    kernels the add is part of the store.
+
+    ``x`` may be :class:`QuantizedRows`: fp8_block weights multiply its codes,
+    with the result that its values in their dtype would give; weights of any
+    other kind multiply the rows kept beside them."""
 
     dense = None
     if isinstance(tensors, LinearWeights):
         quant, dense = tensors.quant, tensors.dense
         tensors = tensors.tensors
+    if isinstance(x, QuantizedRows):
+        if quant is not None and quant.mode == "fp8_block" and not isinstance(tensors, torch.Tensor):
+            return _fp8_matmul_codes(x, tensors, quant, residual)
+        x = _kept_rows(x)
 
     def with_residual(out: torch.Tensor) -> torch.Tensor:
         if residual is None:
@@ -462,6 +523,39 @@ def _fp8_matmul(x, w, scales, N: int, K: int, residual):
     return y
 
 
+def _kept_rows(x):
+    if not isinstance(x, QuantizedRows):
+        return x
+    if x.rows is None:
+        raise ValueError("only fp8_block weights multiply codes; keep the rows beside them (keep_rows=True)")
+    return x.rows
+
+
+def _fp8_matmul_codes(x: QuantizedRows, tensors, quant: QuantScheme, residual):
+    """``x @ W.T`` (+ residual) for rows in codes and fp8_block weights
+    (gdn_fp8_matmul_codes)."""
+
+    w, scales, _, N, K = _check_quantized(tensors, quant, x.shape[-1])
+    if _followed(residual, w, scales):
+        raise RuntimeError("fp8_block products have no gradient and no forward mode; call them under torch.no_grad()")
+    codes, lead = x._codes, x.shape[:-1]
+    if w.get_device() != codes.get_device() or codes.get_device() < 0:
+        raise ValueError(f"x is on {x.device}, the weights on {w.device}")
+    M = codes.shape[0]
+    y = torch.empty((*lead, N), dtype=x.dtype, device=codes.device)
+    r = None if residual is None else _residual_rows(residual, y, lead, M, N)
+    w, scales = _c(w), _c(scales)
+    if w.data_ptr() % 16:
+        w = w.clone()
+    code = _lib.dtype_code(x.dtype)
+    ws_bytes = fp8_codes_workspace_bytes(code, M, N, K)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=codes.device) if ws_bytes else None
+    _lib.call_on(codes.device, "gdn_fp8_matmul_codes", codes.data_ptr(), x._scales.data_ptr(), x._scales.shape[1],
+                 w.data_ptr(), scales.data_ptr(), y.data_ptr(), code, _lib.ptr(r), M, N, K, _lib.ptr(ws), ws_bytes,
+                 _lib.stream_ptr(codes.device))
+    return y
+
+
 def _followed(*operands: torch.Tensor | None) -> bool:
     """Whether autograd or forward mode follows these operands, for calls that
     may cost little: tangents are looked for only inside a level of forward mode,
@@ -517,12 +611,14 @@ def quantized_linear_split(x: torch.Tensor, weights: LinearWeights, sizes) -> li
     of the one quantized launch at decode sizes."""
 
     tensors, quant = weights.tensors, weights.quant
+    if quant.mode != "fp8_block":
+        x = _kept_rows(x)
     sizes = [int(n) for n in sizes]
     if sum(sizes) != tensors["weight"].shape[0]:
         raise ValueError(f"block sizes {sizes} do not add up to the {tensors['weight'].shape[0]} "
                          f"stacked rows")
     K = x.shape[-1]
-    rows = x.reshape(-1, K).shape[0]
+    rows = 0 if isinstance(x, QuantizedRows) else x.reshape(-1, K).shape[0]
     if (x.dtype == torch.bfloat16 and x.device.type == "cuda"
             and quant.mode != "fp8_block" and (_on_kernels(quant) and _runs_dense(rows, tensors["weight"].shape[0], K, quant, tensors["scales"].dtype, x,
                                                     kept=weights.dense is not None)
@@ -556,6 +652,13 @@ def fp8_workspace_bytes(y_code: int, M: int, N: int, K: int) -> int:
     """Workspace of gdn_fp8_matmul."""
 
     return int(_lib.load().gdn_fp8_matmul_workspace_size(y_code, M, N, K))
+
+
+@functools.lru_cache(maxsize=256)
+def fp8_codes_workspace_bytes(y_code: int, M: int, N: int, K: int) -> int:
+    """Workspace of gdn_fp8_matmul_codes (0: none)."""
+
+    return int(_lib.load().gdn_fp8_matmul_codes_workspace_size(y_code, M, N, K))
 
 
 @functools.lru_cache(maxsize=256)
