@@ -59,7 +59,7 @@ typedef enum {
  * alone uses that workspace, 19 gdn_prefill_chunked_runs and
  * gdn_prefill_fused_runs, 20 gdn_conv_silu, gdn_selective_scan,
  * gdn_selective_step, gdn_fp8_matmul and gdn_fp8_dequantize, 21 gdn_rms_norm
- * and gdn_fp8_matmul_codes). */
+ * and gdn_fp8_matmul_codes, 22 gdn_add_low_rank). */
 int gdn_abi_version(void);
 
 /* Message describing the calling thread's last non-zero return. */
@@ -600,6 +600,38 @@ int gdn_fp8_matmul_codes(const void *codes, const float *row_scales, int scale_s
 /* gdn_fp8_dequantize - gdn_fp8_matmul's weights as a dense (N, K) out_dtype
  * array: code times scale, one rounding. */
 int gdn_fp8_dequantize(const void *w, const float *scales, void *out, int out_dtype, int N, int K, void *stream);
+
+/*
+ * gdn_add_low_rank - low-rank adapters of many requests, added to a projection's
+ * output in place: for row i with adapter a and each block j of its columns,
+ *   outs[j][i] = dtype(outs[j][i] + c sum_r (sum_k x[i,k] A[r,k]) B[n,r]),
+ * sums in float32; the inner one is kept to 16 bits at least where dtype has 16.
+ *   x: (M, K) dtype at its row stride; outs[j]: (M, widths[j]) dtype at
+ *      out_strides[j] (host arrays of `blocks` entries, 1 to 8), not overlapping x
+ *      or each other; a block of width 0 is left out
+ *   A: (rows, Kp) dtype, Kp = K rounded up to 128 bytes, zeros past K; an adapter's
+ *      rows are those of its blocks in turn, each block's ranks rounded up to 16
+ *   B: dtype elements; block j of adapter a is (widths[j], its ranks rounded up to
+ *      16) at element table[a][j].b, zeros past its ranks
+ *   table: (adapters, blocks) of {int64 b; int32 a_row; int32 rank; float c; int32
+ *      t_col}: B's first element, A's first row, the ranks (0: none), the scale, and
+ *      the ranks rounded up of the blocks before it; rank_total: the most padded
+ *      ranks that an adapter has in all
+ *   order: (M) int32, the rows that have an adapter, sorted by it; tiles:
+ *      (tile_count, 3) int32 {adapter, first place in order, rows}, at most
+ *      tile_rows (16 or 64) rows each; no row in two. A tile of no rows, or with an
+ *      adapter or places that do not exist, is skipped. Rows in no tile are left as
+ *      they are.
+ *   workspace: gdn_add_low_rank_workspace_size(...) bytes; calls sharing one must
+ *      not overlap
+ * A, B, table and workspace 16-byte aligned; x and outs at any element. No
+ * reference counterpart.
+ */
+int64_t gdn_add_low_rank_workspace_size(int dtype, int tiles, int tile_rows, int rank_total, int M, int K);
+int gdn_add_low_rank(const void *x, int64_t x_stride, int dtype, const void *A, const void *B, const void *table,
+                     int adapters, int blocks, int rank_total, void *const *outs, const int64_t *out_strides,
+                     const int *widths, const int32_t *order, const int32_t *tiles, int tile_count, int tile_rows,
+                     int M, int K, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -12,16 +12,19 @@ from .gated_delta import (beta_gate, forget_gate, gated_delta_scan, gated_delta_
                           gated_delta_update)
 from .linear_attention import (DecodeGraph, PrefillGraph, Qwen3_5LinearAttention, conv_frontend,
                                fused_decode_step, fused_prefill_ok, gated_rms_norm, prefill_fused)
+from .low_rank import AdapterRows, LowRankAdapters, add_low_rank
 from .norm import rms_norm
 from .quant import LinearWeights, QuantizedRows, QuantScheme, dequantize, quantized_linear
 from .recurrent_cache import RecurrentCache, RecurrentStatePool
 from .state_space import PackedRuns, conv_silu, selective_scan, selective_step
 
 __all__ = [
+    "AdapterRows",
     "DecodeGraph",
     "PrefillGraph",
     "LinearAttentionDims",
     "LinearWeights",
+    "LowRankAdapters",
     "PackedRuns",
     "QuantScheme",
     "QuantizedRows",
@@ -30,6 +33,7 @@ __all__ = [
     "RecurrentCache",
     "RecurrentStatePool",
     "StateSpaceDims",
+    "add_low_rank",
     "beta_gate",
     "conv_frontend",
     "conv_silu",

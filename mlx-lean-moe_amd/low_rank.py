@@ -1,0 +1,274 @@
+"""Low-rank adapters of many requests at once beside a shared projection, on
+MI355X: row i of a batch, with adapter a of S (or none), gets
+
+    y_i + scale_a * (x_i A_a^T) B_a^T
+
+on top of the projection's y_i, whatever the projection's scheme.
+
+* :class:`LowRankAdapters` -- the adapters of one projection, or of several that
+  share their input (a stacked one's column blocks), laid out once
+* :class:`AdapterRows`     -- which adapter each row of a batch has: made once a
+  step and passed to every projection of every layer
+* :func:`add_low_rank`     -- the addition, in place
+
+The reference serves one model without adapters; none of this has a counterpart
+there. No gradient: tensors that need one raise ``RuntimeError``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+
+import numpy as np
+import torch
+
+from . import _lib
+from .gated_delta import _FLOATS, _require_device, _stream
+from .quant import QuantizedRows, _followed, _kept_rows
+
+_MAX_BLOCKS = 8
+_MAX_RANKS = 1 << 16
+# Rows a tile: 64 where an adapter has that many on average. (A tile's rows share one
+# reading of the adapter; small ones have shorter products.)
+_TILE_ROWS, _LARGE_TILE_ROWS = 16, 64
+_LARGE_FROM = 32
+_TABLE = np.dtype([("b", "<i8"), ("a_row", "<i4"), ("rank", "<i4"), ("scale", "<f4"), ("t_col", "<i4")])
+
+
+def _pad16(n: int) -> int:
+    return -(-n // 16) * 16
+
+
+class LowRankAdapters:
+    """The adapters of the projections that share one input, in the layout that
+    :func:`add_low_rank` reads.
+
+    ``projections`` holds, for each projection (column block of a stacked one), its
+    S adapters in order: ``(A (r, K), B (N, r), scale)``, or None where that adapter
+    leaves the projection alone. Ranks may differ. A whole projection without
+    adapters is None. All tensors are of one float dtype, which is that of the rows,
+    on one device. The adapters' values are copied: changing the tensors later
+    changes nothing here."""
+
+    def __init__(self, projections) -> None:
+        projections = list(projections)
+        if not 1 <= len(projections) <= _MAX_BLOCKS:
+            raise ValueError(f"1 to {_MAX_BLOCKS} projections share their adapters' input, got {len(projections)}")
+        given = [t for block in projections if block is not None for pair in block if pair is not None for t in pair[:2]]
+        if not given:
+            raise ValueError("no projection has an adapter")
+        counts = {len(block) for block in projections if block is not None}
+        if len(counts) != 1:
+            raise ValueError(f"every projection lists the same adapters, got {sorted(counts)} of them")
+        if _followed(*given):
+            raise RuntimeError("adapters have no gradient; detach them")
+        self.count = counts.pop()
+        self.device = _require_device(*given)
+        self.dtype = given[0].dtype
+        self.hidden = given[0].shape[-1]
+        widths: list[int] = []
+        for j, block in enumerate(projections):
+            width = 0
+            for pair in block or ():
+                if pair is None:
+                    continue
+                A, B, _ = pair
+                if A.dtype != self.dtype or B.dtype != self.dtype:
+                    raise ValueError(f"adapters share one dtype, got {A.dtype} and {B.dtype} beside {self.dtype}")
+                if A.ndim != 2 or B.ndim != 2 or A.shape[1] != self.hidden or B.shape[1] != A.shape[0] or 0 in B.shape:
+                    raise ValueError(f"an adapter is A (r, {self.hidden}) and B (N, r), got {tuple(A.shape)} and "
+                                     f"{tuple(B.shape)}")
+                if width not in (0, B.shape[0]):
+                    raise ValueError(f"projection {j} has {width} outputs, an adapter {B.shape[0]}")
+                width = B.shape[0]
+            widths.append(width)
+        if self.hidden == 0:
+            raise ValueError("adapters need rows of at least one value")
+        self.widths = tuple(widths)
+        step = 128 // self.dtype.itemsize
+        table = np.zeros((self.count, len(projections)), dtype=_TABLE)
+        a_rows = b_size = 0
+        for a in range(self.count):
+            t_col = 0
+            for j, block in enumerate(projections):
+                pair = None if block is None else block[a]
+                rank = 0 if pair is None else pair[0].shape[0]
+                table[a, j] = (b_size, a_rows, rank, 0.0 if pair is None else float(pair[2]), t_col)
+                t_col += _pad16(rank)
+                a_rows += _pad16(rank)
+                b_size += widths[j] * _pad16(rank)
+        self.rank_total = max(int(table[a, -1]["t_col"]) + _pad16(int(table[a, -1]["rank"])) for a in range(self.count))
+        if self.rank_total > _MAX_RANKS:
+            raise ValueError(f"an adapter's ranks add up to at most {_MAX_RANKS}, got {self.rank_total}")
+        self._A = torch.zeros((a_rows, -(-self.hidden // step) * step), dtype=self.dtype, device=self.device)
+        self._B = torch.zeros(b_size, dtype=self.dtype, device=self.device)
+        for j, block in enumerate(projections):
+            for a, pair in enumerate(block or ()):
+                if pair is None:
+                    continue
+                at, padded = table[a, j], _pad16(int(table[a, j]["rank"]))
+                rank = pair[0].shape[0]
+                self._A[int(at["a_row"]):int(at["a_row"]) + rank, :self.hidden] = pair[0]
+                rows = self._B[int(at["b"]):int(at["b"]) + widths[j] * padded].view(widths[j], padded)
+                rows[:, :rank] = pair[1]
+        self._table = torch.from_numpy(table.reshape(-1).view(np.uint8)).to(self.device)
+
+
+class AdapterRows:
+    """Which of ``count`` adapters each row of a batch has, -1 for none: checked,
+    sorted and copied to ``device`` once, for every projection of every layer.
+    ``index`` is a host sequence or a tensor of whole numbers (read back to the host
+    if it is on the GPU)."""
+
+    def __init__(self, index, count: int, device: torch.device | str = "cuda") -> None:
+        if count < 1:
+            raise ValueError(f"AdapterRows needs at least one adapter, got {count}")
+        self.count = int(count)
+        index = self._checked(index)
+        self.rows = len(index)
+        used = len(np.unique(index[index >= 0]))
+        with_one = int((index >= 0).sum())
+        self.tile_rows = _LARGE_TILE_ROWS if used and with_one >= _LARGE_FROM * used else _TILE_ROWS
+        # as many tiles as any such batch takes: one that is not full an adapter
+        self.tiles = min(self.rows, -(-self.rows // self.tile_rows) + min(self.count, self.rows))
+        self._plan = torch.from_numpy(self._planned(index)).to(device)
+        self.device = self._plan.device
+
+    @classmethod
+    def of_runs(cls, runs, index, count: int) -> "AdapterRows":
+        """The rows of packed prompts (:class:`PackedRuns`), run r's all with
+        ``index[r]``."""
+
+        index = cls._host(index)
+        if len(index) != len(runs):
+            raise ValueError(f"{len(runs)} runs, {len(index)} adapters")
+        return cls(np.repeat(index, np.diff(runs.offsets)), count, runs.on_device.device)
+
+    def assign(self, index) -> None:
+        """Other adapters for the same number of rows, in the same device memory: what
+        a captured graph's next replay uses. The copy goes to the current stream."""
+
+        index = self._checked(index)
+        if len(index) != self.rows:
+            raise ValueError(f"{self.rows} rows, {len(index)} adapters")
+        self._plan.copy_(torch.from_numpy(self._planned(index)))
+
+    @staticmethod
+    def _host(index) -> np.ndarray:
+        index = torch.as_tensor(index)
+        if index.numel() and (index.is_floating_point() or index.is_complex() or index.dtype == torch.bool):
+            raise ValueError(f"adapters are numbered by whole numbers, got {index.dtype}")
+        if index.ndim != 1:
+            raise ValueError("adapters are listed one a row")
+        return index.to("cpu", torch.int64).numpy()
+
+    def _checked(self, index) -> np.ndarray:
+        index = self._host(index)
+        if len(index) and (index.min() < -1 or index.max() >= self.count):
+            raise ValueError(f"adapters must lie in [0, {self.count}), or be -1")
+        if len(index) >= 2 ** 31 - 256:
+            raise ValueError("the row count must fit int32")
+        return index
+
+    def _planned(self, index: np.ndarray) -> np.ndarray:
+        """The rows that have an adapter, sorted by it (the rest of the array unused),
+        then {adapter, first place, rows} for each tile."""
+
+        plan = np.zeros(self.rows + 3 * self.tiles, dtype=np.int32)
+        order = np.argsort(index, kind="stable")
+        order = order[np.searchsorted(index[order], 0):]
+        plan[:len(order)] = order
+        adapters, first, rows = np.unique(index[order], return_index=True, return_counts=True)
+        pieces = -(-rows // self.tile_rows)
+        which = np.repeat(np.arange(len(adapters)), pieces)
+        piece = np.arange(len(which)) - np.repeat(np.cumsum(pieces) - pieces, pieces)
+        tiles = plan[self.rows:].reshape(-1, 3)
+        tiles[:len(which), 0] = adapters[which]
+        tiles[:len(which), 1] = first[which] + piece * self.tile_rows
+        tiles[:len(which), 2] = np.minimum(rows[which] - piece * self.tile_rows, self.tile_rows)
+        return plan
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(*sizes: int) -> int:
+    return int(_lib.load().gdn_add_low_rank_workspace_size(*sizes))
+
+
+def add_low_rank(outs, x: torch.Tensor, adapters: LowRankAdapters, rows: AdapterRows):
+    """Adds to each row of ``outs`` what its adapter makes of the row of ``x``, in
+    place, and returns ``outs``.
+
+    ``x (M, hidden)`` is the projections' input (any row stride; of
+    :class:`QuantizedRows` the kept rows), ``outs`` their outputs: for one projection
+    a tensor ``(M, N)``, else a list with one for each projection of ``adapters``
+    (None where it has no adapters), in x's dtype at any row stride, e.g. column
+    slices of a stacked output. Sums are float32; a result is rounded once more to
+    its dtype. ``x A^T`` is kept to 16 bits at least for 16-bit dtypes, in full for
+    float32. Rows without an adapter are left as they are."""
+
+    single = isinstance(outs, torch.Tensor)
+    blocks = [outs] if single else outs
+    x = _kept_rows(x)
+    if x.ndim != 2 or x.shape[1] != adapters.hidden:
+        raise ValueError(f"x must be (rows, {adapters.hidden}), got {tuple(x.shape)}")
+    M, dtype = x.shape[0], x.dtype
+    if dtype is not adapters.dtype:
+        raise ValueError(f"the adapters are {adapters.dtype}, x {dtype}")
+    if rows.rows != M or rows.count != adapters.count:
+        raise ValueError(f"rows of {rows.rows} with {rows.count} adapters, x has {M} and there are {adapters.count}")
+    if len(blocks) != len(adapters.widths):
+        raise ValueError(f"{len(adapters.widths)} projections, {len(blocks)} outputs")
+    device = adapters.device
+    if x.device != device or rows.device != device:
+        raise ValueError(f"the adapters are on {device}, x on {x.device}, its adapters' numbers on {rows.device}")
+    if x.stride(1) != 1 or (M > 1 and x.stride(0) < adapters.hidden):
+        x = x.contiguous()
+    x_stride = x.stride(0)
+    pointers, strides = [], []
+    written = [x]
+    for j, (out, width) in enumerate(zip(blocks, adapters.widths)):
+        if not width:
+            pointers.append(None)
+            strides.append(0)
+            continue
+        if out is None or out.shape != (M, width) or out.dtype is not dtype or out.device != device:
+            raise ValueError(f"output {j} must be {(M, width)} {dtype} on {device}")
+        if (out.stride(1) != 1 and width > 1) or (M > 1 and out.stride(0) < width):
+            raise ValueError(f"output {j} must consist of packed rows")
+        for other in written:
+            if _overlap(out, other):
+                raise ValueError(f"output {j} overlaps {'x' if other is x else 'another output'}")
+        written.append(out)
+        pointers.append(out.data_ptr())
+        strides.append(out.stride(0))
+    if _followed(*written):
+        raise RuntimeError("adapters have no gradient and no forward mode; call add_low_rank under torch.no_grad()")
+    n = len(pointers)
+    code = _lib.dtype_code(dtype)
+    nbytes = _workspace(code, rows.tiles, rows.tile_rows, adapters.rank_total, M, adapters.hidden)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    plan = rows._plan.data_ptr()
+    _lib.call_on(device, "gdn_add_low_rank", x.data_ptr(), x_stride, code, adapters._A.data_ptr(), adapters._B.data_ptr(),
+                 adapters._table.data_ptr(), adapters.count, n, adapters.rank_total, (ctypes.c_void_p * n)(*pointers),
+                 (ctypes.c_int64 * n)(*strides), (ctypes.c_int * n)(*adapters.widths), plan, plan + 4 * M, rows.tiles,
+                 rows.tile_rows, M, adapters.hidden, ws.data_ptr(), nbytes, _stream(device))
+    return outs
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two arrays of packed rows share an element: column slices of one
+    buffer lie between each other without doing so."""
+
+    size, rows = a.element_size(), a.shape[0]
+    if not rows:
+        return False
+    pa, pb = a.data_ptr(), b.data_ptr()
+    wa, wb = a.shape[1] * size, b.shape[1] * size
+    sa, sb = a.stride(0) * size, b.stride(0) * size
+    if pa + (rows - 1) * sa + wa <= pb or pb + (rows - 1) * sb + wb <= pa:
+        return False
+    if sa != sb or rows == 1:
+        return True
+    off = (pb - pa) % sa
+    return off < wa or off > sa - wb
