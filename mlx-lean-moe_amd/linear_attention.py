@@ -31,7 +31,9 @@ from . import _lib
 from .config import LinearAttentionDims
 from .gated_delta import (PREFILL_MIN_TOKENS, _as, _c, _check_cu_seqlens, _check_out, _longest_run,
                           _require_device, _stream, _with_longest, gated_delta_update)
-from .quant import (LinearWeights, QuantScheme, concat_quantized, quantized_linear,
+from .low_rank import AdapterRows, LowRankAdapters, add_low_rank
+from .norm import rms_norm
+from .quant import (LinearWeights, QuantizedRows, QuantScheme, concat_quantized, quantized_linear,
                     quantized_linear_split, stackable)
 from .recurrent_cache import RecurrentCache, RecurrentStatePool
 
@@ -397,11 +399,19 @@ class Qwen3_5LinearAttention:
 
     def __init__(self, dims: LinearAttentionDims, in_proj_qkv, in_proj_z, in_proj_a, in_proj_b,
                  conv1d_weight, A_log, dt_bias, norm_weight, out_proj,
-                 rms_norm_eps: float = 1e-6, quant: QuantScheme | None = None) -> None:
+                 rms_norm_eps: float = 1e-6, quant: QuantScheme | None = None,
+                 input_norm_weight: torch.Tensor | None = None) -> None:
         """Projections are dense ``(N, K)`` tensors, quantized dicts
         ``{"weight", "scales", "biases"}`` (scheme ``quant``, the reference's
         ``config.other_quant``) or :class:`LinearWeights` carrying their own
-        scheme (linear_attention.py:95-101)."""
+        scheme (linear_attention.py:95-101).
+
+        With ``input_norm_weight (hidden,)`` the layer takes the decoder layer's
+        stream and norms it itself (:func:`rms_norm` with ``rms_norm_eps``, in
+        e4m3 codes where fp8_block projections follow): ``layer(x, cache,
+        residual=x)`` is then ``x + attention(rms_norm(x))``
+        (transformer.py:110-112). Without, x is normed already, and may be
+        :class:`QuantizedRows`."""
 
         self.linear = dims
         self.rms_norm_eps = rms_norm_eps
@@ -417,6 +427,36 @@ class Qwen3_5LinearAttention:
         self.A_log = A_log.float().contiguous()
         self.dt_bias = dt_bias.float().contiguous()
         self.norm_weight = norm_weight.float().contiguous()
+        self.input_norm_weight = None if input_norm_weight is None else input_norm_weight.float().contiguous()
+        in_codes = [self._scheme_of(w)[1] for w in (in_proj_qkv, in_proj_z, in_proj_a, in_proj_b)]
+        in_codes = [q is not None and q.mode == "fp8_block" for q in in_codes]
+        self._any_codes, self._all_codes = any(in_codes), all(in_codes)
+        self._in_adapters: LowRankAdapters | None = None
+        self._out_adapters: LowRankAdapters | None = None
+
+    def set_adapters(self, *, in_proj_qkv=None, in_proj_z=None, in_proj_a=None, in_proj_b=None,
+                     out_proj=None) -> None:
+        """Low-rank adapters beside the layer's projections, in place of any set
+        before: for each projection the list of its S adapters as
+        :class:`LowRankAdapters` takes one, or None. A call uses them where it is
+        given ``adapter_rows``; graphs captured before keep the adapters that they
+        were captured with."""
+
+        ins = [in_proj_qkv, in_proj_z, in_proj_a, in_proj_b]
+        counts = {len(p) for p in (*ins, out_proj) if p is not None}
+        if len(counts) > 1:
+            raise ValueError(f"every projection lists the same adapters, got {sorted(counts)} of them")
+        d = self.linear
+        with_in = LowRankAdapters(ins) if any(p is not None for p in ins) else None
+        with_out = LowRankAdapters([out_proj]) if out_proj is not None else None
+        for made, widths in ((with_in, (d.conv_dim, d.value_dim, d.num_value_heads, d.num_value_heads)), (with_out, None)):
+            if made is None or widths is None:
+                continue
+            if any(n not in (0, w) for n, w in zip(made.widths, widths)):
+                raise ValueError(f"in_proj adapters have {made.widths} outputs, the projections {widths}")
+        if with_out is not None and with_out.hidden != d.value_dim:
+            raise ValueError(f"out_proj adapters take {with_out.hidden} values, the projection {d.value_dim}")
+        self._in_adapters, self._out_adapters = with_in, with_out
 
     def new_cache(self, dtype: torch.dtype = torch.float32) -> RecurrentCache:
         d = self.linear
@@ -468,7 +508,30 @@ class Qwen3_5LinearAttention:
             tensors = tensors.to(rows.dtype)
         return quantized_linear(rows, tensors, quant, residual=residual)
 
-    def _project(self, rows: torch.Tensor):
+    def _out(self, rows: torch.Tensor, residual, adapter_rows: AdapterRows | None) -> torch.Tensor:
+        y = self._proj(rows, self.out_proj, residual)
+        if adapter_rows is not None and self._out_adapters is not None:
+            add_low_rank(y, rows, self._out_adapters, adapter_rows)
+        return y
+
+    def _project(self, rows: torch.Tensor, adapter_rows: AdapterRows | None = None):
+        """The input projections of ``rows``, normed first if the layer does that,
+        with what the rows' adapters add."""
+
+        if adapter_rows is not None and self._in_adapters is None and self._out_adapters is None:
+            raise ValueError("adapter_rows given, but the layer has no adapters (set_adapters)")
+        adapt = adapter_rows is not None and self._in_adapters is not None
+        if self.input_norm_weight is not None:
+            if isinstance(rows, QuantizedRows):
+                raise ValueError("the layer norms its input itself (input_norm_weight) and takes plain rows")
+            rows = rms_norm(rows, self.input_norm_weight, self.rms_norm_eps, quantize=self._any_codes,
+                            keep_rows=self._any_codes and (adapt or not self._all_codes))
+        qkv, z, a, b = self._projected(rows)
+        if adapt:
+            add_low_rank([qkv, z.view(z.shape[0], self.linear.value_dim), a, b], rows, self._in_adapters, adapter_rows)
+        return qkv, z, a, b
+
+    def _projected(self, rows: torch.Tensor):
         d = self.linear
         L = rows.shape[0]
         if self._in_stacked is not None:
@@ -524,32 +587,34 @@ class Qwen3_5LinearAttention:
         return out.reshape(T, d.value_dim), new_conv, new_ssm
 
     def __call__(self, x: torch.Tensor, cache: RecurrentCache,
-                 residual: torch.Tensor | None = None) -> torch.Tensor:
+                 residual: torch.Tensor | None = None, adapter_rows: AdapterRows | None = None) -> torch.Tensor:
         """``x``: ``(hidden,)`` for one decode step or ``(L, hidden)`` for a
         prompt; returns the same rank (linear_attention.py:81-127). With
         ``residual`` (x's shape and dtype) the result is ``residual +
         layer(x)``, the decoder layer's ``h = rows + attention(rms_norm(rows))``
-        (transformer.py:110-112), added in out_proj's store."""
+        (transformer.py:110-112), added in out_proj's store. ``adapter_rows``:
+        the adapters (:meth:`set_adapters`) of x's rows."""
 
         if x.ndim not in (1, 2):
             raise ValueError(f"Qwen3_5LinearAttention expects 1-D or 2-D x, got shape {tuple(x.shape)}")
         squeeze = x.ndim == 1
-        rows = x[None, :] if squeeze else x
+        rows = x.reshape(1, -1) if squeeze else x
         if residual is not None and squeeze:
             residual = residual[None, :]
         conv_state, ssm_state = cache.state()
-        out, new_conv, new_ssm = self._rows_step(rows, conv_state, ssm_state, residual)
+        out, new_conv, new_ssm = self._rows_step(rows, conv_state, ssm_state, residual, adapter_rows=adapter_rows)
         cache.update(new_conv, new_ssm, advance=rows.shape[0])
         return out[0] if squeeze else out
 
-    def _rows_step(self, rows, conv_state, ssm_state, residual=None, conv_out=None, ssm_out=None):
+    def _rows_step(self, rows, conv_state, ssm_state, residual=None, conv_out=None, ssm_out=None,
+                   adapter_rows=None):
         """The layer over ``rows (L, hidden)`` of one sequence from
         ``conv_state (K-1, C)`` and ``ssm_state (Hv, Dv, Dk)``: returns
         ``(out (L, hidden), new_conv, new_ssm)``, the new states in fresh
         tensors, or in ``conv_out`` and ``ssm_out`` when given."""
 
         d = self.linear
-        qkv, z, a, b = self._project(rows)
+        qkv, z, a, b = self._project(rows, adapter_rows)
         act = qkv.dtype
         outs = conv_out is not None or ssm_out is not None
         if rows.shape[0] == 1 and _fused_decode_ok(d, act) and not outs:
@@ -561,7 +626,7 @@ class Qwen3_5LinearAttention:
                 qkv, z, a, b, conv_state[None], ssm_state[None],
                 conv_out=None if conv_out is None else conv_out[None],
                 ssm_out=None if ssm_out is None else ssm_out[None])
-        return self._proj(out, self.out_proj, residual), new_conv[0], new_ssm[0]
+        return self._out(out, residual, adapter_rows), new_conv[0], new_ssm[0]
 
     def _decode_fused(self, qkv, z, a, b, conv_state, ssm_state, in_place: bool,
                       conv_out: torch.Tensor | None = None):
@@ -571,21 +636,22 @@ class Qwen3_5LinearAttention:
                                  state_out=ssm_state if in_place else None)
 
     def decode_batch(self, x: torch.Tensor, pool: RecurrentStatePool, slots=None,
-                     residual: torch.Tensor | None = None) -> torch.Tensor:
+                     residual: torch.Tensor | None = None,
+                     adapter_rows: AdapterRows | None = None) -> torch.Tensor:
         """One decode token for each of the pool's sequences: ``x (pool.batch,
         hidden)`` -> ``(pool.batch, hidden)``; or, with ``slots`` (distinct
         pool indices, e.g. the sequences a scheduler has active this step),
         ``x (len(slots), hidden)`` for those slots only. One kernel launch
         updates the slots' ssm tiles in place and rolls their conv state into
-        the other half of the pool's conv buffer. ``residual`` as in
-        ``__call__``."""
+        the other half of the pool's conv buffer. ``residual`` and
+        ``adapter_rows`` as in ``__call__``."""
 
         d = self.linear
         rows = pool.batch if slots is None else len(slots)
         if x.ndim != 2 or x.shape[0] != rows:
             raise ValueError("decode_batch expects x of shape (pool.batch, hidden), or "
                              "(len(slots), hidden) with slots")
-        qkv, z, a, b = self._project(x)
+        qkv, z, a, b = self._project(x, adapter_rows)
         if not _fused_decode_ok(d, qkv.dtype) or pool.conv_buf.dtype != qkv.dtype:
             raise ValueError("decode_batch needs Dk = Dv = 128, K = 4 and a pool in the "
                              "activation dtype (float32 or bfloat16)")
@@ -598,7 +664,12 @@ class Qwen3_5LinearAttention:
             self.dt_bias, self.norm_weight, self.rms_norm_eps, d, slots=slot_t,
             conv_half=pool.conv_half_dev, conv_arrivals=pool.conv_arrivals if counted else None)
         pool.advance(slot_list, slot_t, device_flipped=counted)
-        return self._proj(out.reshape(rows, d.value_dim), self.out_proj, residual)
+        return self._out(out.reshape(rows, d.value_dim), residual, adapter_rows)
+
+
+def _plain_rows(x_example) -> None:
+    if isinstance(x_example, QuantizedRows):
+        raise ValueError("a graph copies plain rows in; give the layer its input_norm_weight for codes inside")
 
 
 class DecodeGraph:
@@ -614,11 +685,16 @@ class DecodeGraph:
     With ``residual_example`` the step adds a residual as ``decode_batch``
     does, read from ``self.residual`` (``step(x, residual)`` copies it in).
     Shapes, slots and every buffer are fixed at capture; the pool's contents
-    may change between steps (e.g. ``pool.load``)."""
+    may change between steps (e.g. ``pool.load``). With ``adapter_rows`` the step
+    adds the layer's adapters; ``adapter_rows.assign`` gives the next steps'
+    rows other ones."""
 
     def __init__(self, layer: "Qwen3_5LinearAttention", pool: RecurrentStatePool, slots,
-                 x_example: torch.Tensor, residual_example: torch.Tensor | None = None) -> None:
-        self.layer, self.pool = layer, pool
+                 x_example: torch.Tensor, residual_example: torch.Tensor | None = None,
+                 adapter_rows: AdapterRows | None = None) -> None:
+        _plain_rows(x_example)
+        self.layer, self.pool, self.adapter_rows = layer, pool, adapter_rows
+        self._adapters = (layer._in_adapters, layer._out_adapters)  # what the graph reads, whatever the layer gets later
         self.slots = check_slots(slots, len(slots), pool.batch)
         if x_example.ndim != 2 or x_example.shape[0] != len(self.slots):
             raise ValueError("x_example must be (len(slots), hidden)")
@@ -636,7 +712,7 @@ class DecodeGraph:
                                   pool.ssm_state.shape[1], pool.ssm_state.shape[2],
                                   pool.ssm_state.shape[3], dtype=pool.conv_buf.dtype,
                                   device=self.x.device)
-        layer.decode_batch(self.x, warm, slots=list(range(n)), residual=self.residual)
+        layer.decode_batch(self.x, warm, slots=list(range(n)), residual=self.residual, adapter_rows=adapter_rows)
         torch.cuda.synchronize(self.x.device)
         del warm
         # the slot array must exist before capture (no host copy in the
@@ -650,7 +726,8 @@ class DecodeGraph:
         torch.cuda.synchronize(self.x.device)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
-            self.out = layer.decode_batch(self.x, pool, slots=self.slots, residual=self.residual)
+            self.out = layer.decode_batch(self.x, pool, slots=self.slots, residual=self.residual,
+                                          adapter_rows=adapter_rows)
         # capture ran decode_batch's host bookkeeping once and none of its
         # device work: undo the former
         pool.flip_host(self._idx, tokens=-1)
@@ -690,10 +767,11 @@ class PrefillGraph:
     returned output holds until the next step. Writing the chunk straight
     into ``self.x`` (and calling ``step(cache)``) skips its copy. Shapes and
     buffers are fixed at capture; a prompt's last, shorter chunk runs through
-    ``layer`` as usual."""
+    ``layer`` as usual. ``adapter_rows`` as in :class:`DecodeGraph`."""
 
     def __init__(self, layer: "Qwen3_5LinearAttention", x_example: torch.Tensor,
-                 residual_example: torch.Tensor | None = None) -> None:
+                 residual_example: torch.Tensor | None = None, adapter_rows: AdapterRows | None = None) -> None:
+        _plain_rows(x_example)
         if x_example.ndim != 2 or x_example.shape[0] < 2:
             raise ValueError("x_example must be (chunk, hidden) with at least two tokens")
         d = layer.linear
@@ -708,7 +786,9 @@ class PrefillGraph:
                                  dtype=torch.float32, device=dev) for _ in range(2)]
         # one eager call first: lazily built operands (workspace sizes, BLAS
         # handles) exist before capture
-        layer._rows_step(self.x, self._conv[0], self._ssm[0], self.residual)
+        self.adapter_rows = adapter_rows
+        self._adapters = (layer._in_adapters, layer._out_adapters)  # what the graphs read, whatever the layer gets later
+        layer._rows_step(self.x, self._conv[0], self._ssm[0], self.residual, adapter_rows=adapter_rows)
         torch.cuda.synchronize(dev)
         self._graphs, self._outs = [], []
         for i in (0, 1):
@@ -716,7 +796,8 @@ class PrefillGraph:
             pool = self._graphs[0].pool() if self._graphs else None
             with torch.cuda.graph(graph, pool=pool):
                 out, _, _ = layer._rows_step(self.x, self._conv[i], self._ssm[i], self.residual,
-                                             conv_out=self._conv[1 - i], ssm_out=self._ssm[1 - i])
+                                             conv_out=self._conv[1 - i], ssm_out=self._ssm[1 - i],
+                                             adapter_rows=adapter_rows)
             self._graphs.append(graph)
             self._outs.append(out)
         self.out = self._outs[0]

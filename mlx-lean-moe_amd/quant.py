@@ -377,7 +377,7 @@ def decode_kernel_takes(M: int, K: int, bits: int, group_size: int, sb_dtype: to
 
 
 def quantized_linear(x: torch.Tensor, tensors, quant: QuantScheme | None = None, *,
-                     residual: torch.Tensor | None = None) -> torch.Tensor:
+                     residual: torch.Tensor | None = None, adapters=None, adapter_rows=None) -> torch.Tensor:
     """Linear projection for self-describing, legacy quantized, or dense
     weights (moe_block.py:27-55): ``x @ W.T`` over the last axis of ``x``.
     Quantized weights give ``x``'s dtype; dense ones the promotion of ``x``'s
@@ -391,8 +391,21 @@ def quantized_linear(x: torch.Tensor, tensors, quant: QuantScheme | None = None,
 
     ``x`` may be :class:`QuantizedRows`: fp8_block weights multiply its codes,
     with the result that its values in their dtype would give; weights of any
-    other kind multiply the rows kept beside them."""
+    other kind multiply the rows kept beside them.
 
+    ``adapters`` (:class:`LowRankAdapters` of this projection) with
+    ``adapter_rows`` (:class:`AdapterRows` of x's rows): what each row's adapter
+    makes of it is added to the result (:func:`add_low_rank`), which is rounded once
+    more."""
+
+    if (adapters is None) != (adapter_rows is None):
+        raise ValueError("adapters and adapter_rows go together")
+    if adapters is not None:
+        from .low_rank import add_low_rank
+
+        y = quantized_linear(x, tensors, quant, residual=residual)
+        add_low_rank(y.view(-1, y.shape[-1]), _kept_rows(x).reshape(-1, x.shape[-1]), adapters, adapter_rows)
+        return y
     dense = None
     if isinstance(tensors, LinearWeights):
         quant, dense = tensors.quant, tensors.dense

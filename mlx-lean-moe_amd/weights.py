@@ -309,11 +309,13 @@ def _to_device(w: LinearWeights, device) -> LinearWeights:
 
 def load_linear_attention(model_dir: str | Path, layer_index: int, *, device="cuda",
                           hf_config: dict | None = None,
-                          tensor_prefix: str = "language_model.model"):
+                          tensor_prefix: str = "language_model.model", input_norm: bool = False):
     """The gated-delta layer ``layer_index`` of a checkpoint
     (transformer.py:52-65): projections with their own schemes (stored-width
     scales and biases), ``conv1d.weight (C, K, 1)``, ``A_log``, ``dt_bias``
-    and ``norm.weight`` widened to float32, on ``device``."""
+    and ``norm.weight`` widened to float32, on ``device``. ``input_norm`` reads
+    the decoder layer's ``input_layernorm.weight`` as well and gives it to the
+    layer, which then takes the stream (``input_norm_weight``)."""
 
     from .linear_attention import Qwen3_5LinearAttention
 
@@ -331,10 +333,13 @@ def load_linear_attention(model_dir: str | Path, layer_index: int, *, device="cu
         A_log = reader.read_tensor(f"{prefix}.A_log")
         dt_bias = reader.read_tensor(f"{prefix}.dt_bias")
         norm = reader.read_tensor(f"{prefix}.norm.weight")
+        input_weight = (reader.read_tensor(f"{tensor_prefix}.layers.{layer_index}.input_layernorm.weight")
+                        if input_norm else None)
     if tuple(conv.shape) != (dims.conv_dim, dims.conv_kernel_dim, 1):
         raise ValueError(f"{prefix}.conv1d.weight has shape {tuple(conv.shape)}, expected "
                          f"{(dims.conv_dim, dims.conv_kernel_dim, 1)}")
     f32 = lambda t: t.to(device=device, dtype=torch.float32)
     return Qwen3_5LinearAttention(dims, proj["in_proj_qkv"], proj["in_proj_z"], proj["in_proj_a"],
                                   proj["in_proj_b"], f32(conv), f32(A_log), f32(dt_bias), f32(norm),
-                                  proj["out_proj"], rms_norm_eps=eps)
+                                  proj["out_proj"], rms_norm_eps=eps,
+                                  input_norm_weight=None if input_weight is None else f32(input_weight))
