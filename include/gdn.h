@@ -605,33 +605,37 @@ int gdn_fp8_dequantize(const void *w, const float *scales, void *out, int out_dt
  * gdn_add_low_rank - low-rank adapters of many requests, added to a projection's
  * output in place: for row i with adapter a and each block j of its columns,
  *   outs[j][i] = dtype(outs[j][i] + c sum_r (sum_k x[i,k] A[r,k]) B[n,r]),
- * sums in float32; the inner one is kept to 16 bits at least where dtype has 16.
+ * sums in float32; c times the inner one is kept to 16 bits where dtype has 16.
  *   x: (M, K) dtype at its row stride; outs[j]: (M, widths[j]) dtype at
  *      out_strides[j] (host arrays of `blocks` entries, 1 to 8), not overlapping x
  *      or each other; a block of width 0 is left out
- *   A: (rows, Kp) dtype, Kp = K rounded up to 128 bytes, zeros past K; an adapter's
- *      rows are those of its blocks in turn, each block's ranks rounded up to 16
- *   B: dtype elements; block j of adapter a is (widths[j], its ranks rounded up to
- *      16) at element table[a][j].b, zeros past its ranks
+ *   A: an adapter's ranks are those of its blocks in turn, each block's rounded up to
+ *      16, K rounded up to 128 bytes, zeros in both; with P elements in 16 bytes,
+ *      element (16 c + l, 8 P s + 4 P h + P g + e) at [c][s][h][g][l][e]
+ *   B: block j of adapter a, its columns rounded up to 64 and its ranks to 16, zeros in
+ *      both, from element table[a][j].b: in 16 bits element (64 n + 32 p + 8 q + 4 u +
+ *      v, 16 c + 8 g + e) at [n][c][p][u][g][q][v][e], in float32 (64 n + 16 p + 4 q +
+ *      v, 16 c + 4 g + e) at [n][c][p][g][q][v][e]
  *   table: (adapters, blocks) of {int64 b; int32 a_row; int32 rank; float c; int32
- *      t_col}: B's first element, A's first row, the ranks (0: none), the scale, and
+ *      t_col}: B's first element, A's first rank, the ranks (0: none), the scale, and
  *      the ranks rounded up of the blocks before it; rank_total: the most padded
- *      ranks that an adapter has in all
+ *      ranks that an adapter has in all, rank_block: in one block
  *   order: (M) int32, the rows that have an adapter, sorted by it; tiles:
  *      (tile_count, 3) int32 {adapter, first place in order, rows}, at most
- *      tile_rows (16 or 64) rows each; no row in two. A tile of no rows, or with an
+ *      tile_rows (16 or 256) rows each; no row in two. A tile of no rows, or with an
  *      adapter or places that do not exist, is skipped. Rows in no tile are left as
  *      they are.
- *   workspace: gdn_add_low_rank_workspace_size(...) bytes; calls sharing one must
- *      not overlap
+ *   workspace: gdn_add_low_rank_workspace_size(...) bytes, 4 for each rank of each
+ *      place for a row in the tiles; calls sharing one must not overlap
  * A, B, table and workspace 16-byte aligned; x and outs at any element. No
  * reference counterpart.
  */
-int64_t gdn_add_low_rank_workspace_size(int dtype, int tiles, int tile_rows, int rank_total, int M, int K);
+int64_t gdn_add_low_rank_workspace_size(int rank_total, int tile_count, int tile_rows);
 int gdn_add_low_rank(const void *x, int64_t x_stride, int dtype, const void *A, const void *B, const void *table,
-                     int adapters, int blocks, int rank_total, void *const *outs, const int64_t *out_strides,
-                     const int *widths, const int32_t *order, const int32_t *tiles, int tile_count, int tile_rows,
-                     int M, int K, void *workspace, int64_t workspace_bytes, void *stream);
+                     int adapters, int blocks, int rank_total, int rank_block, void *const *outs,
+                     const int64_t *out_strides, const int *widths, const int32_t *order, const int32_t *tiles,
+                     int tile_count, int tile_rows, int M, int K, void *workspace, int64_t workspace_bytes,
+                     void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,11 +1,16 @@
 // Low-rank adapters of many requests at once, added to a projection's output:
 // for row i with adapter a, and each block j of the output's columns,
-//   t = x_i A_a^T (all blocks' ranks side by side),   out_j[i] += c t_j B_aj^T.
+//   t = c x_i A_a^T (all blocks' ranks side by side),   out_j[i] += t_j B_aj^T.
 // The rows come sorted by adapter and cut into tiles of one adapter (a plan that
 // the caller keeps for all projections of a step), so each product is a plain
-// one: the first gives t in float32, K split over waves and workgroups, the second
-// reads B once a tile and the output once. Both run on the matrix cores; 16-bit
-// adapters take t as two pieces of their type, which keeps 16 bits of it.
+// one on the matrix cores, with float32 sums. The first leaves t as the second's
+// operand: float32, or (16-bit adapters) two bfloat16 pieces, the upper 8 bits of
+// the float32 value and what they leave, which is 16 bits of it. float16 B is taken
+// in two such pieces as well (8 + 3 bits: all of it), since t need not fit float16.
+//
+// A, B and t lie in memory in the order in which a wave's lanes take them: a load of
+// 16 bytes a lane is 1 KB in one piece (rows of them instead, 32 to 128 bytes a row
+// and load, cost the second product a third of its time at 64 ranks).
 #include <type_traits>
 
 #include "gdn_common.h"
@@ -18,8 +23,8 @@ namespace {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 struct AdapterBlock {
-    int64_t b;      // first element of B (width, padded rank)
-    int32_t a_row;  // first row of A
+    int64_t b;      // first element of B (width rounded up to 64, padded rank)
+    int32_t a_row;  // first rank in A
     int32_t rank;   // without padding to 16; 0: no adapter here
     float scale;
     int32_t t_col;  // first column of t
@@ -27,37 +32,45 @@ struct AdapterBlock {
 
 struct LowRankArgs {
     const void *x, *A, *B;
-    const AdapterBlock* table;    // (S, blocks)
-    const int32_t *order, *tiles; // rows by adapter; {adapter, first place in order, rows} a tile
-    float* t;                     // (splits, M, rank_total)
+    const AdapterBlock* table;     // (S, blocks)
+    const int32_t *order, *tiles;  // rows by adapter; {adapter, first place in order, rows} a tile
+    uint8_t* t;                    // (16 rows of a tile, 16 ranks) after each other: 1 KB each
     void* out[kLowRankBlocks];
     int64_t out_stride[kLowRankBlocks];
     int width[kLowRankBlocks], group_end[kLowRankBlocks];
     int64_t x_stride;
-    int S, blocks, rank_total, M, K, Kp, tile_count, splits, per_wave, steps;
+    int S, blocks, rank_total, M, K, steps;
+    int tile_count, parts, rows;   // parts of `rows` rows a tile
 };
 
 GDN_DEV int pad16(int r) { return (r + 15) & ~15; }
 
 struct Tile {
     int adapter, start, count;
+    int64_t block;  // of t: its first 16 rows
 };
 
-// A tile of the plan; count 0 where it holds none, or what no plan holds.
-template <int kRows>
-GDN_DEV Tile tile_of(const LowRankArgs& p, int i) {
-    Tile t{p.tiles[3 * i], p.tiles[3 * i + 1], min(p.tiles[3 * i + 2], kRows)};
-    if (uint32_t(t.adapter) >= uint32_t(p.S) || t.start < 0 || t.start > p.M - t.count) t.count = 0;
+// Part i of the plan's tiles; count 0 or less where it holds none, or what no plan
+// holds.
+GDN_DEV Tile part_of(const LowRankArgs& p, int i) {
+    const int at = i / p.parts, from = i % p.parts * p.rows;
+    Tile t{p.tiles[3 * at], p.tiles[3 * at + 1], p.tiles[3 * at + 2], (int64_t(at) * p.parts * p.rows + from) / 16};
+    if (uint32_t(t.adapter) >= uint32_t(p.S) || t.start < 0 || t.count < 0 || t.start > p.M - t.count) t.count = 0;
+    t.start += from;
+    t.count = min(t.count - from, p.rows);
     return t;
 }
 
-// One wave's product of a 16 x 16 tile over 128 bytes of both operands' rows, two
-// 16-byte pieces a lane (which of the k they are does not matter as long as
-// both sides agree).
+GDN_DEV f32x4 mfma_bf16(const uint4& a, const uint4& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// A product of 16 x 16 results over a 16-byte piece of both operands a lane (which
+// of the k they are does not matter as long as both sides agree).
 template <class Act>
 GDN_DEV f32x4 mfma_pieces(const uint4& a, const uint4& b, f32x4 c) {
     if constexpr (Act::code == GDN_BF16) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+        return mfma_bf16(a, b, c);
     } else if constexpr (Act::code == GDN_F16) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     } else {
@@ -85,235 +98,241 @@ GDN_DEV uint4 piece_of(const S* p, int count) {
     return v;
 }
 
-// t for a tile of kRF x 16 rows and kNR x 16 of its adapter's ranks. Ranks are the
-// left operand, so a lane ends with four ranks of one row.
-template <class Act, int kRF, int kNR>
-__global__ __launch_bounds__(64 * kLowRankWaves) void low_rank_down_kernel(LowRankArgs p) {
+// The upper 8 bits of a float32 value as bfloat16 (cut off: rounded up, the largest
+// would overflow), and what they leave, rounded; what is not finite has no rest.
+GDN_DEV void two_pieces(float v, uint16_t& high, uint16_t& low) {
+    high = v != v ? 0x7FC0 : uint16_t(__float_as_uint(v) >> 16);
+    low = (high & 0x7F80) == 0x7F80 ? 0 : f32_to_bf16_bits(v - bf16_bits_to_f32(high));
+}
+
+// t for 16 rows of a tile and kNR x 16 of its adapter's ranks. Ranks are the left
+// operand, so a lane ends with four ranks of one row. The waves share out K and add
+// their sums in LDS; a step's loads are under way while the one before is
+// multiplied.
+template <class Act, int kNR>
+__global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_down_kernel(LowRankArgs p) {
     using S = typename Act::storage;
     constexpr int kStep = 128 / sizeof(S), kPiece = 16 / sizeof(S);
-    __shared__ f32x4 sums[kLowRankWaves][kRF * kNR][64];
+    __shared__ f32x4 sums[kLowRankDownWaves][kNR][64];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, lr = lane & 15;
-    const Tile tile = tile_of<16 * kRF>(p, blockIdx.x);
+    const Tile tile = part_of(p, blockIdx.x);
     if (tile.count <= 0) return;
     const AdapterBlock* ab = p.table + int64_t(tile.adapter) * p.blocks;
     const int total = ab[p.blocks - 1].t_col + pad16(ab[p.blocks - 1].rank), r0 = blockIdx.y * 16 * kNR;
     if (r0 >= total) return;
-    const S* xr[kRF];
-    const S* ar[kNR];
-#pragma unroll
-    for (int i = 0; i < kRF; ++i) {
-        const int row = p.order[tile.start + min(16 * i + lr, tile.count - 1)];
-        xr[i] = static_cast<const S*>(p.x) + int64_t(min(max(row, 0), p.M - 1)) * p.x_stride + g * 2 * kPiece;
-    }
+    const int row = p.order[tile.start + min(lr, tile.count - 1)];
+    const S* xr = static_cast<const S*>(p.x) + int64_t(min(max(row, 0), p.M - 1)) * p.x_stride + g * kPiece;
+    const uint8_t* ar[kNR];
 #pragma unroll
     for (int j = 0; j < kNR; ++j)
-        ar[j] = static_cast<const S*>(p.A) + int64_t(ab[0].a_row + min(r0 + 16 * j + lr, total - 1)) * p.Kp + g * 2 * kPiece;
-    f32x4 acc[kRF][kNR];
+        ar[j] = static_cast<const uint8_t*>(p.A) + int64_t(ab[0].a_row + min(r0 + 16 * j, total - 16)) * (p.steps * 128) + lane * 16;
+    f32x4 acc[kNR];
 #pragma unroll
-    for (int i = 0; i < kRF; ++i)
+    for (int j = 0; j < kNR; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const auto load = [&](int s, uint4 (&xv)[2], uint4 (&av)[kNR][2]) {
+        const int k = s * kStep;
 #pragma unroll
-        for (int j = 0; j < kNR; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int s0 = (blockIdx.z * kLowRankWaves + wave) * p.per_wave, s1 = min(p.steps, s0 + p.per_wave);
-    const auto multiply = [&](const uint4 (&xv)[kRF][2], const uint4 (&av)[kNR][2]) {
+        for (int j = 0; j < kNR; ++j) {
+            av[j][0] = *reinterpret_cast<const uint4*>(ar[j] + s * 2048);
+            av[j][1] = *reinterpret_cast<const uint4*>(ar[j] + s * 2048 + 1024);
+        }
+        if (k + kStep <= p.K) {
+            __builtin_memcpy(&xv[0], xr + k, 16);
+            __builtin_memcpy(&xv[1], xr + k + kStep / 2, 16);
+        } else {  // the last step of a K that is no multiple of it
+            const int left = p.K - k - g * kPiece;
+            xv[0] = piece_of(xr + k, left);
+            xv[1] = piece_of(xr + k + kStep / 2, left - kStep / 2);
+        }
+    };
+    const auto multiply = [&](const uint4 (&xv)[2], const uint4 (&av)[kNR][2]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < kRF; ++i)
-#pragma unroll
-                for (int j = 0; j < kNR; ++j) acc[i][j] = mfma_pieces<Act>(av[j][h], xv[i][h], acc[i][j]);
+            for (int j = 0; j < kNR; ++j) acc[j] = mfma_pieces<Act>(av[j][h], xv[h], acc[j]);
     };
-    const auto load_a = [&](int k, uint4 (&av)[kNR][2]) {
-#pragma unroll
-        for (int j = 0; j < kNR; ++j) {
-            av[j][0] = *reinterpret_cast<const uint4*>(ar[j] + k);
-            av[j][1] = *reinterpret_cast<const uint4*>(ar[j] + k + kPiece);
-        }
-    };
-    const int whole = min(s1, p.K / kStep);
-    for (int s = s0; s < whole; ++s) {
-        uint4 xv[kRF][2], av[kNR][2];
-        load_a(s * kStep, av);
-#pragma unroll
-        for (int i = 0; i < kRF; ++i) {
-            __builtin_memcpy(&xv[i][0], xr[i] + s * kStep, 16);
-            __builtin_memcpy(&xv[i][1], xr[i] + s * kStep + kPiece, 16);
-        }
-        multiply(xv, av);
-    }
-    if (s1 > whole && s1 > s0) {  // the last step of a K that is no multiple of it
-        uint4 xv[kRF][2], av[kNR][2];
-        const int k = (s1 - 1) * kStep, left = p.K - k - g * 2 * kPiece;
-        load_a(k, av);
-#pragma unroll
-        for (int i = 0; i < kRF; ++i) {
-            xv[i][0] = piece_of(xr[i] + k, left);
-            xv[i][1] = piece_of(xr[i] + k + kPiece, left - kPiece);
-        }
-        multiply(xv, av);
+    uint4 xv[2][2], av[2][kNR][2];
+    int s = wave;
+    if (s < p.steps) load(s, xv[0], av[0]);
+    for (; s < p.steps; s += 2 * kLowRankDownWaves) {
+        const int s1 = s + kLowRankDownWaves, s2 = s1 + kLowRankDownWaves;
+        if (s1 < p.steps) load(s1, xv[1], av[1]);
+        multiply(xv[0], av[0]);
+        if (s1 >= p.steps) break;
+        if (s2 < p.steps) load(s2, xv[0], av[0]);
+        multiply(xv[1], av[1]);
     }
 #pragma unroll
-    for (int i = 0; i < kRF; ++i)
-#pragma unroll
-        for (int j = 0; j < kNR; ++j) sums[wave][i * kNR + j][lane] = acc[i][j];
+    for (int j = 0; j < kNR; ++j) sums[wave][j][lane] = acc[j];
     __syncthreads();
-    for (int u = wave; u < kRF * kNR; u += kLowRankWaves) {
-        f32x4 v = sums[0][u][lane];
+    const int r = r0 + wave * 16;  // wave j adds the shares of ranks 16 j
+    if (wave >= kNR || r >= total) return;
+    f32x4 v = sums[0][wave][lane];
 #pragma unroll
-        for (int w = 1; w < kLowRankWaves; ++w) v += sums[w][u][lane];
-        const int row = u / kNR * 16 + lr, r = r0 + u % kNR * 16;
-        if (row < tile.count && r < total)
-            *reinterpret_cast<f32x4*>(p.t + (int64_t(blockIdx.z) * p.M + tile.start + row) * p.rank_total + r + 4 * g) = v;
-    }
-}
-
-// Eight ranks of t (summed over the shares of K, times the adapter's scale) as the
-// second product's operand: float32 as they are; 16 bits as two pieces, `low`
-// 32 bytes behind `high`. bfloat16: the upper 8 bits and what they leave (16
-// bits in all, and no overflow by rounding up); float16: t times `fit`, a power of
-// two that brings the row's largest to between 2^13 and 2^14, so that both pieces
-// are within the type. What is not finite has no rest.
-template <class Act>
-GDN_DEV void store_pieces(uint8_t* at, const float (&t)[8], float fit) {
+    for (int w = 1; w < kLowRankDownWaves; ++w) v += sums[w][wave][lane];
+    int block = 0;
+    while (r >= ab[block].t_col + pad16(ab[block].rank)) ++block;
+    const int rank = ab[block].t_col + ab[block].rank - r - 4 * g;  // (padding: 0 times what is not finite)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < rank ? v[e] * ab[block].scale : 0.f;
+    uint8_t* to = p.t + (tile.block * (p.rank_total / 16) + r / 16) * 1024 + lr * 16;
     if constexpr (Act::code == GDN_F32) {
-        *reinterpret_cast<float4*>(at) = make_float4(t[0], t[1], t[2], t[3]);
-        *reinterpret_cast<float4*>(at + 16) = make_float4(t[4], t[5], t[6], t[7]);
-    } else {
-        uint16_t high[8], low[8];
+        *reinterpret_cast<f32x4*>(to + 256 * g) = v;
+    } else {  // quarters of 1 KB: ranks 0 to 7 and 8 to 15 high, then low
+        uint16_t high[4], low[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if constexpr (Act::code == GDN_BF16) {
-                high[e] = uint16_t(__float_as_uint(t[e]) >> 16);
-                const float rest = t[e] - bf16_bits_to_f32(high[e]);
-                low[e] = (high[e] & 0x7F80) == 0x7F80 ? 0 : f32_to_bf16_bits(rest);
-                if (t[e] != t[e]) high[e] = 0x7FC0;
-            } else {
-                const float v = t[e] * fit;
-                high[e] = f32_to_f16_bits(v);
-                low[e] = (high[e] & 0x7C00) == 0x7C00 ? 0 : f32_to_f16_bits(v - f16_bits_to_f32(high[e]));
-            }
-        }
-        __builtin_memcpy(__builtin_assume_aligned(at, 16), high, 16);
-        __builtin_memcpy(__builtin_assume_aligned(at + 32, 16), low, 16);
+        for (int e = 0; e < 4; ++e) two_pieces(v[e], high[e], low[e]);
+        to += g / 2 * 256 + g % 2 * 8;
+        __builtin_memcpy(__builtin_assume_aligned(to, 8), high, 8);
+        __builtin_memcpy(__builtin_assume_aligned(to + 512, 8), low, 8);
     }
 }
 
-// out += c t B^T for a tile of kRF x 16 rows and 256 columns of one block, 64 a
-// wave. B is the left operand and its rows are dealt out so that a lane ends with
-// 16 consecutive columns of one row. The 32 values of k of a 16-bit product are 16
-// ranks of t's high piece and the same of its low one, B the same for both.
-template <class Act, int kRF>
-__global__ __launch_bounds__(64 * kLowRankWaves) void low_rank_up_kernel(LowRankArgs p) {
+// One piece of B as the second product's operand.
+template <class Act>
+struct Operand {
+    uint4 v;
+    GDN_DEV void of(const uint4& raw) { v = raw; }
+    GDN_DEV f32x4 times(const uint4& t, f32x4 c) const { return mfma_pieces<Act>(v, t, c); }
+};
+
+template <>
+struct Operand<ActF16> {
+    uint4 high, low;
+    GDN_DEV void of(const uint4& raw) {
+        uint16_t e[8], h[8], l[8];
+        __builtin_memcpy(e, &raw, 16);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) two_pieces(f16_bits_to_f32(e[i]), h[i], l[i]);
+        __builtin_memcpy(&high, h, 16);
+        __builtin_memcpy(&low, l, 16);
+    }
+    GDN_DEV f32x4 times(const uint4& t, f32x4 c) const { return mfma_bf16(low, t, mfma_bf16(high, t, c)); }
+};
+
+// out += t B^T for a part of a tile and 256 columns of one block, 64 a wave, 16
+// rows at a time. B is the left operand and its rows are dealt out so that a lane
+// ends with 16-byte pieces of one row's output, the four lanes of a row beside each
+// other in each piece. The 32 values of k of a 16-bit
+// product are 16 ranks of t's high piece and the same of its low one, B the same for
+// both. A wave keeps its part of B (kHeld pieces of 16 ranks; 0: more ranks than
+// that, read again for each 16 rows) and streams the rows: the next ones' output and
+// t are under way while these are multiplied and stored.
+template <class Act, int kHeld>
+__global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRankArgs p) {
     using S = typename Act::storage;
-    constexpr int kRows = 16 * kRF, kChunk = 64, kLine = kChunk / 16 * 64 + 16;  // (rows 16 bytes apart in the banks)
-    constexpr int kPer = 64 * kLowRankWaves / kRows;                              // threads a row
-    __shared__ __attribute__((aligned(16))) uint8_t pieces[kRows * kLine];
-    __shared__ float fits[kRows];
+    constexpr int kY = sizeof(S), kCount = 16 / kY, kT = kHeld ? kHeld : 1;  // 16-byte pieces of 16 columns
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, lr = lane & 15;
-    const int group = blockIdx.x / p.tile_count;
-    const Tile tile = tile_of<kRows>(p, blockIdx.x % p.tile_count);
+    // neighbours take neighbouring columns: workgroups that run at once cover whole
+    // rows, not one window of columns at strides that fall on few memory channels
+    const int groups = p.group_end[p.blocks - 1], group = blockIdx.x % groups;
+    const Tile tile = part_of(p, blockIdx.x / groups);
     if (tile.count <= 0) return;
     int block = 0;
     while (group >= p.group_end[block]) ++block;
     const AdapterBlock ab = p.table[int64_t(tile.adapter) * p.blocks + block];
     if (ab.rank <= 0) return;
-    const int R = pad16(ab.rank), width = p.width[block];
+    const int pieces = (ab.rank + 15) / 16, R = 16 * pieces, width = p.width[block];
     const int n0 = (group - (block ? p.group_end[block - 1] : 0)) * kLowRankColumns + wave * 64;
+    // the rows' numbers, all at first: a number fetched among the rows' output would
+    // be there only after the output before it
+    __shared__ int rows[kLowRankTile];
+    if (tid < p.rows) rows[tid] = tid < tile.count ? p.order[tile.start + tid] : -1;
+    __syncthreads();
+    if (n0 >= width) return;
+    // four columns from quad_at(q, j) are one lane's acc[j], q its g
+    const auto quad_at = [](int q, int j) { return j / (4 / kY) * 4 * kCount + q * kCount + j % (4 / kY) * 4; };
+    const int n = n0 + kCount * g;
+    const bool whole = n0 + 64 <= width;  // (of the wave: one branch)
 
-    const int own = tid / kPer;  // the row whose ranks this thread brings in
-    const float* t = p.t + (int64_t(tile.start) + min(own, tile.count - 1)) * p.rank_total + ab.t_col;
-    const int64_t share = int64_t(p.M) * p.rank_total;
-    const bool there = own < tile.count;
-    const auto ranks8 = [&](int r, float (&v)[8]) {
+    // B: for each 64 columns and 16 ranks four operands, of 512 bytes where both of
+    // t's pieces meet the same
+    constexpr int kB = Act::code == GDN_F32 ? 1024 : 512;
+    const uint8_t* br = static_cast<const uint8_t*>(p.B) + ab.b * kY + int64_t(n0) * R * kY + lane * 16 % kB;
+    Operand<Act> b[kT][4];
+    const auto load_b = [&](int i, Operand<Act> (&v)[4]) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.f;
-        if (!there || r >= R) return;
-        for (int s = 0; s < p.splits; ++s) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(t + s * share + r);
-            const f32x4 b = *reinterpret_cast<const f32x4*>(t + s * share + r + 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += a[e], v[4 + e] += b[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = r + e < ab.rank ? v[e] * ab.scale : 0.f;  // (padding: 0 times what is not finite)
+        for (int j = 0; j < 4; ++j) v[j].of(*reinterpret_cast<const uint4*>(br + (4 * i + j) * kB));
     };
-    float fit = 1.f;
-    if constexpr (Act::code == GDN_F16) {
-        float most = 0.f;
-        for (int r = tid % kPer * 8; r < R; r += kPer * 8) {
-            float v[8];
-            ranks8(r, v);
+    if constexpr (kHeld != 0) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
-        }
-#pragma unroll
-        for (int o = 1; o < kPer; o *= 2) most = fmaxf(most, __shfl_xor(most, o));
-        const int up = int(__float_as_uint(most) >> 23) - 127;  // 2^up <= most < 2^(up + 1)
-        const bool usable = most > 0x1p-100f && most < 0x1p100f;
-        fit = usable ? __uint_as_float(uint32_t(127 + 13 - up) << 23) : 1.f;
-        if (tid % kPer == 0) fits[own] = usable ? __uint_as_float(uint32_t(127 - 13 + up) << 23) : 1.f;
+        for (int i = 0; i < kHeld; ++i)
+            if (i < pieces) load_b(i, b[i]);
     }
+    S* out = static_cast<S*>(p.out[block]) + n;
+    const int64_t stride = p.out_stride[block];
+    const int64_t t_stride = int64_t(p.rank_total / 16) * 1024;
+    const uint8_t* t = p.t + tile.block * t_stride + ab.t_col / 16 * 1024 + lane * 16;
+    const int steps = (tile.count + 15) / 16;
 
-    const S* br[4];
+    struct Rows {
+        S* y;  // null: no row
+        uint4 yv[kY], tv[kT];
+    };
+    const auto fetch = [&](Rows& r, int s) {
+        const int row = rows[16 * s + lr];
+        r.y = uint32_t(row) < uint32_t(p.M) ? out + row * stride : nullptr;
+        if (r.y && whole) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int n = n0 + lr / 4 * 16 + 4 * i + lr % 4;
-        br[i] = static_cast<const S*>(p.B) + ab.b + int64_t(min(n, width - 1)) * R + (Act::code == GDN_F32 ? 4 * g : 8 * (g & 1));
-    }
-    f32x4 acc[kRF][4];
-#pragma unroll
-    for (int i = 0; i < kRF; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int r0 = 0; r0 < R; r0 += kChunk) {
-        if (r0) __syncthreads();
-        for (int r = tid % kPer * 8; r < min(kChunk, R - r0); r += kPer * 8) {
-            float v[8];
-            ranks8(r0 + r, v);
-            store_pieces<Act>(pieces + own * kLine + r / 16 * 64 + r % 16 * (Act::code == GDN_F32 ? 4 : 2), v, fit);
+            for (int k = 0; k < kY; ++k) __builtin_memcpy(&r.yv[k], r.y + k * 4 * kCount, 16);
         }
-        __syncthreads();
-        for (int c = 0; c < min(kChunk, R - r0); c += 16) {
-            uint4 b[4];
+        if constexpr (kHeld != 0) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const uint4*>(br[j] + r0 + c);
+            for (int i = 0; i < kHeld; ++i)
+                if (i < pieces) r.tv[i] = *reinterpret_cast<const uint4*>(t + s * t_stride + 1024 * i);
+        }
+    };
+    const auto finish = [&](Rows& r, int s) {
+        f32x4 acc[4];
 #pragma unroll
-            for (int i = 0; i < kRF; ++i) {
-                const uint4 v = *reinterpret_cast<const uint4*>(pieces + (16 * i + lr) * kLine + c * 4 + g * 16);
+        for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (kHeld != 0) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = mfma_pieces<Act>(b[j], v, acc[i][j]);
+            for (int i = 0; i < kHeld; ++i)
+                if (i < pieces) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[j] = b[i][j].times(r.tv[i], acc[j]);
+                }
+        } else {
+            for (int i = 0; i < pieces; ++i) {
+                load_b(i, b[0]);
+                const uint4 v = *reinterpret_cast<const uint4*>(t + s * t_stride + 1024 * i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = b[0][j].times(v, acc[j]);
             }
         }
-    }
-    const int n = n0 + 16 * g;
-    if (n >= width) return;
-#pragma unroll
-    for (int i = 0; i < kRF; ++i) {
-        if (16 * i + lr >= tile.count) continue;
-        const int row = p.order[tile.start + 16 * i + lr];
-        if (uint32_t(row) >= uint32_t(p.M)) continue;
-        S* y = static_cast<S*>(p.out[block]) + int64_t(row) * p.out_stride[block] + n;
-        const float back = Act::code == GDN_F16 ? fits[16 * i + lr] : 1.f;
-        if (n + 16 <= width) {
+        if (!r.y) return;
+        if (whole) {
             S e[16];
-            __builtin_memcpy(e, y, sizeof(e));
+            __builtin_memcpy(e, r.yv, sizeof(e));
 #pragma unroll
-            for (int j = 0; j < 16; ++j) Act::store(e, j, __builtin_fmaf(acc[i][j / 4][j % 4], back, Act::load(e, j)));
-            __builtin_memcpy(y, e, sizeof(e));
+            for (int j = 0; j < 16; ++j) Act::store(e, j, acc[j / 4][j % 4] + Act::load(e, j));
+#pragma unroll
+            for (int k = 0; k < kY; ++k) __builtin_memcpy(r.y + k * 4 * kCount, e + k * kCount, 16);
         } else {
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (n + j < width) Act::store(y, j, __builtin_fmaf(acc[i][j / 4][j % 4], back, Act::load(y, j)));
+            for (int j = 0; j < 16; ++j) {
+                const int at = quad_at(0, j / 4) + j % 4;
+                if (n + at < width) Act::store(r.y, at, acc[j / 4][j % 4] + Act::load(r.y, at));
+            }
         }
+    };
+    Rows even, odd;
+    fetch(even, 0);
+    for (int s = 0; s < steps; s += 2) {
+        if (s + 1 < steps) fetch(odd, s + 1);
+        finish(even, s);
+        if (s + 1 >= steps) break;
+        if (s + 2 < steps) fetch(even, s + 2);
+        finish(odd, s + 1);
     }
 }
 
-int ranks_per_group(int rank_total) { return rank_total <= 16 ? 16 : rank_total <= 32 ? 32 : 64; }
-
 bool low_rank_sizes_ok(int tiles, int tile_rows, int rank_total, int M, int K) {
-    return tiles >= 0 && (tile_rows == 16 || tile_rows == 64) && rank_total > 0 && rank_total % 16 == 0 &&
-           rank_total <= (1 << 16) && M >= 0 && M <= INT32_MAX - 256 && K > 0 && K <= (1 << 28);
+    return tiles >= 0 && (tile_rows == 16 || tile_rows == kLowRankTile) && rank_total > 0 && rank_total % 16 == 0 &&
+           rank_total <= (1 << 16) && M >= 0 && M <= INT32_MAX - 512 && K > 0 && K <= (1 << 24);
 }
 
 }  // namespace
@@ -321,34 +340,33 @@ bool low_rank_sizes_ok(int tiles, int tile_rows, int rank_total, int M, int K) {
 
 using namespace gdn;
 
-extern "C" int64_t gdn_add_low_rank_workspace_size(int dtype, int tiles, int tile_rows, int rank_total, int M, int K) {
-    if (!valid_dtype(dtype) || !low_rank_sizes_ok(tiles, tile_rows, rank_total, M, K)) return 0;
-    const LowRankPlan plan = low_rank_plan(tiles, rank_total, K, dtype_size(dtype), ranks_per_group(rank_total));
-    return int64_t(plan.splits) * M * rank_total * 4;
+extern "C" int64_t gdn_add_low_rank_workspace_size(int rank_total, int tile_count, int tile_rows) {
+    if (!low_rank_sizes_ok(tile_count, tile_rows, rank_total, 0, 1)) return 0;
+    return int64_t(tile_count) * tile_rows * rank_total * 4;
 }
 
 extern "C" int gdn_add_low_rank(const void* x, int64_t x_stride, int dtype, const void* A, const void* B, const void* table,
-                                int adapters, int blocks, int rank_total, void* const* outs, const int64_t* out_strides,
-                                const int* widths, const int32_t* order, const int32_t* tiles, int tile_count, int tile_rows,
-                                int M, int K, void* workspace, int64_t workspace_bytes, void* stream) {
-    GDN_REQUIRE(low_rank_sizes_ok(tile_count, tile_rows, rank_total, M, K) && adapters > 0,
-                "gdn_add_low_rank: bad sizes M=%d K=%d rank_total=%d tiles=%d of %d, %d adapters", M, K, rank_total, tile_count,
-                tile_rows, adapters);
+                                int adapters, int blocks, int rank_total, int rank_block, void* const* outs,
+                                const int64_t* out_strides, const int* widths, const int32_t* order, const int32_t* tiles,
+                                int tile_count, int tile_rows, int M, int K, void* workspace, int64_t workspace_bytes,
+                                void* stream) {
+    GDN_REQUIRE(low_rank_sizes_ok(tile_count, tile_rows, rank_total, M, K) && adapters > 0 && rank_block > 0 &&
+                    rank_block <= rank_total,
+                "gdn_add_low_rank: bad sizes M=%d K=%d ranks %d of %d, tiles %d of %d, %d adapters", M, K, rank_block,
+                rank_total, tile_count, tile_rows, adapters);
     GDN_REQUIRE(blocks >= 1 && blocks <= kLowRankBlocks, "gdn_add_low_rank: %d blocks of columns, 1 to %d", blocks,
                 kLowRankBlocks);
     GDN_REQUIRE(valid_dtype(dtype), "gdn_add_low_rank: bad dtype");
     if (M == 0 || tile_count == 0) return 0;
     GDN_REQUIRE(x && A && B && table && outs && out_strides && widths && order && tiles, "gdn_add_low_rank: null pointer");
     GDN_REQUIRE(x_stride >= K || M == 1, "gdn_add_low_rank: rows of x closer than their width");
-    const int es = dtype_size(dtype), per = ranks_per_group(rank_total);
-    const LowRankPlan plan = low_rank_plan(tile_count, rank_total, K, es, per);
-    const int64_t need = int64_t(plan.splits) * M * rank_total * 4;
+    const int64_t need = int64_t(tile_count) * tile_rows * rank_total * 4;
     GDN_REQUIRE(workspace && workspace_bytes >= need, "gdn_add_low_rank: workspace of %lld bytes, %lld needed",
                 (long long)workspace_bytes, (long long)need);
     GDN_REQUIRE((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(table) |
                  reinterpret_cast<uintptr_t>(workspace)) % 16 == 0,
                 "gdn_add_low_rank: A, B, table and workspace must be 16-byte aligned");
-    LowRankArgs p{x, A, B, static_cast<const AdapterBlock*>(table), order, tiles, static_cast<float*>(workspace)};
+    LowRankArgs p{x, A, B, static_cast<const AdapterBlock*>(table), order, tiles, static_cast<uint8_t*>(workspace)};
     int64_t groups = 0;
     for (int j = 0; j < blocks; ++j) {
         GDN_REQUIRE(widths[j] >= 0 && (widths[j] == 0 || (outs[j] && (out_strides[j] >= widths[j] || M == 1))),
@@ -357,36 +375,44 @@ extern "C" int gdn_add_low_rank(const void* x, int64_t x_stride, int dtype, cons
         p.out_stride[j] = out_strides[j];
         p.width[j] = widths[j];
         groups += (int64_t(widths[j]) + kLowRankColumns - 1) / kLowRankColumns;
-        GDN_REQUIRE(groups * tile_count <= INT32_MAX, "gdn_add_low_rank: too many rows and columns");
         p.group_end[j] = int(groups);
     }
     if (groups == 0) return 0;
-    GDN_REQUIRE(one_grid_row(groups * tile_count, 256), "gdn_add_low_rank: too many rows and columns");
+    const int es = dtype_size(dtype);
+    const LowRankPlan plan = low_rank_plan(tile_count, tile_rows, rank_total, rank_block, K, es, groups);
+    const int64_t down_parts = tile_rows / 16, up_parts = tile_rows / plan.up_rows;
+    GDN_REQUIRE(one_grid_row(tile_count * down_parts, 64 * kLowRankDownWaves) &&
+                    one_grid_row(groups * tile_count * up_parts, 64 * kLowRankUpWaves),
+                "gdn_add_low_rank: too many rows and columns");
     p.x_stride = x_stride;
     p.S = adapters;
     p.blocks = blocks;
     p.rank_total = rank_total;
     p.M = M;
     p.K = K;
-    p.Kp = plan.steps * (128 / es);
-    p.tile_count = tile_count;
-    p.splits = plan.splits;
-    p.per_wave = plan.per_wave;
     p.steps = plan.steps;
+    p.tile_count = tile_count;
     hipStream_t s = as_stream(stream);
-    const auto go = [&](auto act, auto rf) {
-        using Act = decltype(act);
-        constexpr int RF = decltype(rf)::value;
-        const dim3 down(unsigned(tile_count), unsigned((rank_total + per - 1) / per), unsigned(plan.splits));
-        const dim3 threads(64 * kLowRankWaves);
-        if (per == 16) hipLaunchKernelGGL((low_rank_down_kernel<Act, RF, 1>), down, threads, 0, s, p);
-        else if (per == 32) hipLaunchKernelGGL((low_rank_down_kernel<Act, RF, 2>), down, threads, 0, s, p);
-        else hipLaunchKernelGGL((low_rank_down_kernel<Act, RF, 4>), down, threads, 0, s, p);
-        hipLaunchKernelGGL((low_rank_up_kernel<Act, RF>), dim3(unsigned(groups * tile_count)), threads, 0, s, p);
-    };
     const auto typed = [&](auto act) {
-        if (tile_rows == 64) go(act, std::integral_constant<int, 4>{});
-        else go(act, std::integral_constant<int, 1>{});
+        using Act = decltype(act);
+        const auto down = [&](auto kernel) {
+            p.parts = int(down_parts);
+            p.rows = 16;
+            hipLaunchKernelGGL(kernel, dim3(unsigned(tile_count * down_parts), unsigned((rank_total + plan.ranks - 1) / plan.ranks)),
+                               dim3(64 * kLowRankDownWaves), 0, s, p);
+        };
+        const auto up = [&](auto kernel) {
+            p.parts = int(up_parts);
+            p.rows = plan.up_rows;
+            hipLaunchKernelGGL(kernel, dim3(unsigned(groups * tile_count * up_parts)), dim3(64 * kLowRankUpWaves), 0, s, p);
+        };
+        if (plan.ranks == 16) down(low_rank_down_kernel<Act, 1>);
+        else if (plan.ranks == 32) down(low_rank_down_kernel<Act, 2>);
+        else down(low_rank_down_kernel<Act, 4>);
+        if (plan.held == 1) up(low_rank_up_kernel<Act, 1>);
+        else if (plan.held == 2) up(low_rank_up_kernel<Act, 2>);
+        else if (plan.held == 4) up(low_rank_up_kernel<Act, 4>);
+        else up(low_rank_up_kernel<Act, 0>);
     };
     if (dtype == GDN_F32) typed(ActF32{});
     else if (dtype == GDN_BF16) typed(ActBF16{});

@@ -18,7 +18,6 @@ there. No gradient: tensors that need one raise ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes
-import functools
 
 import numpy as np
 import torch
@@ -29,9 +28,10 @@ from .quant import QuantizedRows, _followed, _kept_rows
 
 _MAX_BLOCKS = 8
 _MAX_RANKS = 1 << 16
-# Rows a tile: 64 where an adapter has that many on average. (A tile's rows share one
-# reading of the adapter; small ones have shorter products.)
-_TILE_ROWS, _LARGE_TILE_ROWS = 16, 64
+_MAX_HIDDEN = 1 << 24
+# Rows a tile: the large ones where adapters have at least _LARGE_FROM rows on average
+# (the kernels cut them as they need; small ones leave fewer places empty).
+_TILE_ROWS, _LARGE_TILE_ROWS = 16, 256
 _LARGE_FROM = 32
 _TABLE = np.dtype([("b", "<i8"), ("a_row", "<i4"), ("rank", "<i4"), ("scale", "<f4"), ("t_col", "<i4")])
 
@@ -83,8 +83,8 @@ class LowRankAdapters:
                     raise ValueError(f"projection {j} has {width} outputs, an adapter {B.shape[0]}")
                 width = B.shape[0]
             widths.append(width)
-        if self.hidden == 0:
-            raise ValueError("adapters need rows of at least one value")
+        if not 0 < self.hidden <= _MAX_HIDDEN:
+            raise ValueError(f"adapters take rows of 1 to {_MAX_HIDDEN} values, got {self.hidden}")
         self.widths = tuple(widths)
         step = 128 // self.dtype.itemsize
         table = np.zeros((self.count, len(projections)), dtype=_TABLE)
@@ -97,21 +97,34 @@ class LowRankAdapters:
                 table[a, j] = (b_size, a_rows, rank, 0.0 if pair is None else float(pair[2]), t_col)
                 t_col += _pad16(rank)
                 a_rows += _pad16(rank)
-                b_size += widths[j] * _pad16(rank)
+                b_size += -(-widths[j] // 64) * 64 * _pad16(rank)
         self.rank_total = max(int(table[a, -1]["t_col"]) + _pad16(int(table[a, -1]["rank"])) for a in range(self.count))
+        self.rank_block = max(_pad16(int(r)) for r in table["rank"].reshape(-1))
         if self.rank_total > _MAX_RANKS:
             raise ValueError(f"an adapter's ranks add up to at most {_MAX_RANKS}, got {self.rank_total}")
-        self._A = torch.zeros((a_rows, -(-self.hidden // step) * step), dtype=self.dtype, device=self.device)
+        per, steps = 16 // self.dtype.itemsize, -(-self.hidden // step)
+        # both in the order in which a wave's lanes take them (include/gdn.h)
+        self._A = torch.zeros((a_rows // 16, steps, 2, 4, 16, per), dtype=self.dtype, device=self.device)
         self._B = torch.zeros(b_size, dtype=self.dtype, device=self.device)
         for j, block in enumerate(projections):
             for a, pair in enumerate(block or ()):
                 if pair is None:
                     continue
-                at, padded = table[a, j], _pad16(int(table[a, j]["rank"]))
-                rank = pair[0].shape[0]
-                self._A[int(at["a_row"]):int(at["a_row"]) + rank, :self.hidden] = pair[0]
-                rows = self._B[int(at["b"]):int(at["b"]) + widths[j] * padded].view(widths[j], padded)
-                rows[:, :rank] = pair[1]
+                at, rank = table[a, j], pair[0].shape[0]
+                padded, columns = _pad16(rank), -(-widths[j] // 64) * 64
+                wide = torch.zeros((padded, steps * step), dtype=self.dtype, device=self.device)
+                wide[:rank, :self.hidden] = pair[0]
+                first = int(at["a_row"]) // 16
+                self._A[first:first + padded // 16] = wide.view(padded // 16, 16, steps, 2, 4, per).permute(0, 2, 3, 4, 1, 5)
+                wide = torch.zeros((columns, padded), dtype=self.dtype, device=self.device)
+                wide[:widths[j], :rank] = pair[1]
+                laid = self._B[int(at["b"]):int(at["b"]) + columns * padded]
+                if per == 8:
+                    laid.view(columns // 64, padded // 16, 2, 2, 2, 4, 4, 8).copy_(
+                        wide.view(columns // 64, 2, 4, 2, 4, padded // 16, 2, 8).permute(0, 5, 1, 3, 6, 2, 4, 7))
+                else:
+                    laid.view(columns // 64, padded // 16, 4, 4, 4, 4, 4).copy_(
+                        wide.view(columns // 64, 4, 4, 4, padded // 16, 4, 4).permute(0, 4, 1, 5, 2, 3, 6))
         self._table = torch.from_numpy(table.reshape(-1).view(np.uint8)).to(self.device)
 
 
@@ -119,19 +132,21 @@ class AdapterRows:
     """Which of ``count`` adapters each row of a batch has, -1 for none: checked,
     sorted and copied to ``device`` once, for every projection of every layer.
     ``index`` is a host sequence or a tensor of whole numbers (read back to the host
-    if it is on the GPU)."""
+    if it is on the GPU). ``distinct``: room for batches of that many different
+    adapters, for :meth:`assign`; without it there is room for as many tiles as
+    ``index`` takes."""
 
-    def __init__(self, index, count: int, device: torch.device | str = "cuda") -> None:
+    def __init__(self, index, count: int, device: torch.device | str = "cuda", *, distinct: int | None = None) -> None:
         if count < 1:
             raise ValueError(f"AdapterRows needs at least one adapter, got {count}")
         self.count = int(count)
         index = self._checked(index)
         self.rows = len(index)
-        used = len(np.unique(index[index >= 0]))
-        with_one = int((index >= 0).sum())
+        used, with_one = len(np.unique(index[index >= 0])), int((index >= 0).sum())
         self.tile_rows = _LARGE_TILE_ROWS if used and with_one >= _LARGE_FROM * used else _TILE_ROWS
-        # as many tiles as any such batch takes: one that is not full an adapter
-        self.tiles = min(self.rows, -(-self.rows // self.tile_rows) + min(self.count, self.rows))
+        self.tiles = int((-(-np.unique(index[index >= 0], return_counts=True)[1] // self.tile_rows)).sum())
+        if distinct is not None:  # one tile that is not full an adapter
+            self.tiles = max(self.tiles, min(self.rows, -(-self.rows // self.tile_rows) + distinct))
         self._plan = torch.from_numpy(self._planned(index)).to(device)
         self.device = self._plan.device
 
@@ -147,7 +162,8 @@ class AdapterRows:
 
     def assign(self, index) -> None:
         """Other adapters for the same number of rows, in the same device memory: what
-        a captured graph's next replay uses. The copy goes to the current stream."""
+        a captured graph's next replay uses. The copy goes to the current stream.
+        ``ValueError`` if there is no room for them (``distinct``)."""
 
         index = self._checked(index)
         if len(index) != self.rows:
@@ -181,6 +197,9 @@ class AdapterRows:
         plan[:len(order)] = order
         adapters, first, rows = np.unique(index[order], return_index=True, return_counts=True)
         pieces = -(-rows // self.tile_rows)
+        if pieces.sum() > self.tiles:
+            raise ValueError(f"{len(adapters)} adapters over these rows take {pieces.sum()} tiles, there is room for "
+                             f"{self.tiles}; reserve it (distinct=)")
         which = np.repeat(np.arange(len(adapters)), pieces)
         piece = np.arange(len(which)) - np.repeat(np.cumsum(pieces) - pieces, pieces)
         tiles = plan[self.rows:].reshape(-1, 3)
@@ -188,11 +207,6 @@ class AdapterRows:
         tiles[:len(which), 1] = first[which] + piece * self.tile_rows
         tiles[:len(which), 2] = np.minimum(rows[which] - piece * self.tile_rows, self.tile_rows)
         return plan
-
-
-@functools.lru_cache(maxsize=1024)
-def _workspace(*sizes: int) -> int:
-    return int(_lib.load().gdn_add_low_rank_workspace_size(*sizes))
 
 
 def add_low_rank(outs, x: torch.Tensor, adapters: LowRankAdapters, rows: AdapterRows):
@@ -204,7 +218,7 @@ def add_low_rank(outs, x: torch.Tensor, adapters: LowRankAdapters, rows: Adapter
     a tensor ``(M, N)``, else a list with one for each projection of ``adapters``
     (None where it has no adapters), in x's dtype at any row stride, e.g. column
     slices of a stacked output. Sums are float32; a result is rounded once more to
-    its dtype. ``x A^T`` is kept to 16 bits at least for 16-bit dtypes, in full for
+    its dtype. ``scale x A^T`` is kept to 16 bits for 16-bit dtypes, in full for
     float32. Rows without an adapter are left as they are."""
 
     single = isinstance(outs, torch.Tensor)
@@ -246,11 +260,11 @@ def add_low_rank(outs, x: torch.Tensor, adapters: LowRankAdapters, rows: Adapter
         raise RuntimeError("adapters have no gradient and no forward mode; call add_low_rank under torch.no_grad()")
     n = len(pointers)
     code = _lib.dtype_code(dtype)
-    nbytes = _workspace(code, rows.tiles, rows.tile_rows, adapters.rank_total, M, adapters.hidden)
+    nbytes = rows.tiles * rows.tile_rows * adapters.rank_total * 4  # (gdn_add_low_rank_workspace_size)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     plan = rows._plan.data_ptr()
     _lib.call_on(device, "gdn_add_low_rank", x.data_ptr(), x_stride, code, adapters._A.data_ptr(), adapters._B.data_ptr(),
-                 adapters._table.data_ptr(), adapters.count, n, adapters.rank_total, (ctypes.c_void_p * n)(*pointers),
+                 adapters._table.data_ptr(), adapters.count, n, adapters.rank_total, adapters.rank_block, (ctypes.c_void_p * n)(*pointers),
                  (ctypes.c_int64 * n)(*strides), (ctypes.c_int * n)(*adapters.widths), plan, plan + 4 * M, rows.tiles,
                  rows.tile_rows, M, adapters.hidden, ws.data_ptr(), nbytes, _stream(device))
     return outs

@@ -24,7 +24,7 @@ def _tiles(rows):
 def test_every_row_with_an_adapter_is_in_one_tile(M, S, without):
     rng = np.random.default_rng(M + S)
     index = np.where(rng.random(M) < without, -1, rng.integers(0, S, M))
-    rows = gdn.AdapterRows(index, S, device="cpu")
+    assert gdn.AdapterRows(index, S, device="cpu").tiles <= (rows := gdn.AdapterRows(index, S, device="cpu", distinct=S)).tiles
     for _ in range(2):
         order, tiles = _tiles(rows)
         seen = []
@@ -42,7 +42,7 @@ def test_every_row_with_an_adapter_is_in_one_tile(M, S, without):
 
 def test_large_tiles_where_adapters_have_many_rows():
     assert gdn.AdapterRows([0] * 31, 1, device="cpu").tile_rows == 16
-    assert gdn.AdapterRows([0] * 32, 1, device="cpu").tile_rows == 64
+    assert gdn.AdapterRows([0] * 32, 1, device="cpu").tile_rows == 256
     assert gdn.AdapterRows([0, 1] * 31, 2, device="cpu").tile_rows == 16
 
 
@@ -50,6 +50,9 @@ def test_numbers_that_are_none_are_refused():
     for index, count in (([0, 2], 2), ([-2], 2), ([0.0], 2), ([[0]], 2), ([True], 2), ([0], 0)):
         with pytest.raises(ValueError):
             gdn.AdapterRows(index, count, device="cpu")
+    with pytest.raises(ValueError, match="room"):
+        gdn.AdapterRows([0, 0], 2, device="cpu").assign([0, 1])
+    gdn.AdapterRows([0, 0], 2, device="cpu", distinct=2).assign([0, 1])
     rows = gdn.AdapterRows([0, 1], 2, device="cpu")
     for index in ([0], [0, 2], [0, 1, 1]):
         with pytest.raises(ValueError):
@@ -65,12 +68,11 @@ def test_argument_checks():
     lib = _lib.load()
     err = lambda: lib.gdn_last_error().decode()
     size = lib.gdn_add_low_rank_workspace_size
-    need = size(1, 4, 16, 32, 40, 2048)
-    assert need > 0 and need % (40 * 32 * 4) == 0
-    assert size(1, 4, 17, 32, 40, 2048) == 0 and size(1, 4, 16, 33, 40, 2048) == 0
+    need = size(32, 4, 16)
+    assert need == 4 * 16 * 32 * 4 and size(33, 4, 16) == 0 and size(32, -1, 16) == 0 and size(32, 4, 64) == 0
 
     def call(widths=(100, 64), outs=(P(0), P(1)), strides=(164, 164), **over):
-        a = dict(x=P(2), xs=2048, dt=1, A=P(3), B=P(4), table=P(5), S=3, blocks=len(widths), rt=32)
+        a = dict(x=P(2), xs=2048, dt=1, A=P(3), B=P(4), table=P(5), S=3, blocks=len(widths), rt=32, rb=16)
         b = dict(order=P(6), tiles=P(7), nt=4, tr=16, M=40, K=2048, ws=P(8), wsb=need)
         a.update({k: v for k, v in over.items() if k in a})
         b.update({k: v for k, v in over.items() if k in b})
@@ -80,7 +82,7 @@ def test_argument_checks():
 
     assert call(M=0) == 0 and call(nt=0) == 0
     assert call(widths=(0, 0), outs=(None, None)) == 0
-    for over, what in [(dict(K=0), "sizes"), (dict(tr=32), "sizes"), (dict(rt=20), "sizes"), (dict(S=0), "sizes"),
+    for over, what in [(dict(K=0), "sizes"), (dict(tr=32), "sizes"), (dict(rt=20), "sizes"), (dict(rb=48), "sizes"), (dict(rb=0), "sizes"), (dict(S=0), "sizes"),
                        (dict(dt=5), "dtype"), (dict(x=None), "null"), (dict(tiles=None), "null"), (dict(xs=2047), "width"),
                        (dict(wsb=need - 1), "workspace"), (dict(ws=None), "workspace"), (dict(A=ctypes.c_void_p(8)), "aligned"),
                        (dict(widths=(100, -1)), "block 1"), (dict(strides=(99, 164)), "block 0"),
