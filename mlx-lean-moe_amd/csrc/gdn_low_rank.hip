@@ -105,15 +105,15 @@ GDN_DEV void two_pieces(float v, uint16_t& high, uint16_t& low) {
     low = (high & 0x7F80) == 0x7F80 ? 0 : f32_to_bf16_bits(v - bf16_bits_to_f32(high));
 }
 
-// t for 16 rows of a tile and kNR x 16 of its adapter's ranks. Ranks are the left
-// operand, so a lane ends with four ranks of one row. The waves share out K and add
-// their sums in LDS; a step's loads are under way while the one before is
+// t for kRF x 16 rows of a tile and kNR x 16 of its adapter's ranks. Ranks are the
+// left operand, so a lane ends with four ranks of one row. The waves share out K and
+// add their sums in LDS; a step's loads are under way while the one before is
 // multiplied.
-template <class Act, int kNR>
+template <class Act, int kRF, int kNR>
 __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_down_kernel(LowRankArgs p) {
     using S = typename Act::storage;
     constexpr int kStep = 128 / sizeof(S), kPiece = 16 / sizeof(S);
-    __shared__ f32x4 sums[kLowRankDownWaves][kNR][64];
+    __shared__ f32x4 sums[kLowRankDownWaves][kRF * kNR][64];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, lr = lane & 15;
     const Tile tile = part_of(p, blockIdx.x);
@@ -121,16 +121,22 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_down_kernel(L
     const AdapterBlock* ab = p.table + int64_t(tile.adapter) * p.blocks;
     const int total = ab[p.blocks - 1].t_col + pad16(ab[p.blocks - 1].rank), r0 = blockIdx.y * 16 * kNR;
     if (r0 >= total) return;
-    const int row = p.order[tile.start + min(lr, tile.count - 1)];
-    const S* xr = static_cast<const S*>(p.x) + int64_t(min(max(row, 0), p.M - 1)) * p.x_stride + g * kPiece;
+    const S* xr[kRF];
+#pragma unroll
+    for (int i = 0; i < kRF; ++i) {
+        const int row = p.order[tile.start + min(16 * i + lr, tile.count - 1)];
+        xr[i] = static_cast<const S*>(p.x) + int64_t(min(max(row, 0), p.M - 1)) * p.x_stride + g * kPiece;
+    }
     const uint8_t* ar[kNR];
 #pragma unroll
     for (int j = 0; j < kNR; ++j)
         ar[j] = static_cast<const uint8_t*>(p.A) + int64_t(ab[0].a_row + min(r0 + 16 * j, total - 16)) * (p.steps * 128) + lane * 16;
-    f32x4 acc[kNR];
+    f32x4 acc[kRF][kNR];
 #pragma unroll
-    for (int j = 0; j < kNR; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const auto load = [&](int s, uint4 (&xv)[2], uint4 (&av)[kNR][2]) {
+    for (int i = 0; i < kRF; ++i)
+#pragma unroll
+        for (int j = 0; j < kNR; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const auto load = [&](int s, uint4 (&xv)[kRF][2], uint4 (&av)[kNR][2]) {
         const int k = s * kStep;
 #pragma unroll
         for (int j = 0; j < kNR; ++j) {
@@ -138,21 +144,29 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_down_kernel(L
             av[j][1] = *reinterpret_cast<const uint4*>(ar[j] + s * 2048 + 1024);
         }
         if (k + kStep <= p.K) {
-            __builtin_memcpy(&xv[0], xr + k, 16);
-            __builtin_memcpy(&xv[1], xr + k + kStep / 2, 16);
+#pragma unroll
+            for (int i = 0; i < kRF; ++i) {
+                __builtin_memcpy(&xv[i][0], xr[i] + k, 16);
+                __builtin_memcpy(&xv[i][1], xr[i] + k + kStep / 2, 16);
+            }
         } else {  // the last step of a K that is no multiple of it
             const int left = p.K - k - g * kPiece;
-            xv[0] = piece_of(xr + k, left);
-            xv[1] = piece_of(xr + k + kStep / 2, left - kStep / 2);
+#pragma unroll
+            for (int i = 0; i < kRF; ++i) {
+                xv[i][0] = piece_of(xr[i] + k, left);
+                xv[i][1] = piece_of(xr[i] + k + kStep / 2, left - kStep / 2);
+            }
         }
     };
-    const auto multiply = [&](const uint4 (&xv)[2], const uint4 (&av)[kNR][2]) {
+    const auto multiply = [&](const uint4 (&xv)[kRF][2], const uint4 (&av)[kNR][2]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int j = 0; j < kNR; ++j) acc[j] = mfma_pieces<Act>(av[j][h], xv[h], acc[j]);
+            for (int i = 0; i < kRF; ++i)
+#pragma unroll
+                for (int j = 0; j < kNR; ++j) acc[i][j] = mfma_pieces<Act>(av[j][h], xv[i][h], acc[i][j]);
     };
-    uint4 xv[2][2], av[2][kNR][2];
+    uint4 xv[2][kRF][2], av[2][kNR][2];
     int s = wave;
     if (s < p.steps) load(s, xv[0], av[0]);
     for (; s < p.steps; s += 2 * kLowRankDownWaves) {
@@ -164,10 +178,13 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_down_kernel(L
         multiply(xv[1], av[1]);
     }
 #pragma unroll
-    for (int j = 0; j < kNR; ++j) sums[wave][j][lane] = acc[j];
+    for (int i = 0; i < kRF; ++i)
+#pragma unroll
+        for (int j = 0; j < kNR; ++j) sums[wave][i * kNR + j][lane] = acc[i][j];
     __syncthreads();
-    const int r = r0 + wave * 16;  // wave j adds the shares of ranks 16 j
-    if (wave >= kNR || r >= total) return;
+    static_assert(kRF * kNR <= kLowRankDownWaves, "a wave for each 16 x 16 of t");
+    const int r = r0 + wave % kNR * 16, rows = wave / kNR * 16;  // of the 16 x 16 that this wave finishes
+    if (wave >= kRF * kNR || r >= total || rows >= tile.count) return;
     f32x4 v = sums[0][wave][lane];
 #pragma unroll
     for (int w = 1; w < kLowRankDownWaves; ++w) v += sums[w][wave][lane];
@@ -176,7 +193,7 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_down_kernel(L
     const int rank = ab[block].t_col + ab[block].rank - r - 4 * g;  // (padding: 0 times what is not finite)
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = e < rank ? v[e] * ab[block].scale : 0.f;
-    uint8_t* to = p.t + (tile.block * (p.rank_total / 16) + r / 16) * 1024 + lr * 16;
+    uint8_t* to = p.t + ((tile.block + rows / 16) * (p.rank_total / 16) + r / 16) * 1024 + lr * 16;
     if constexpr (Act::code == GDN_F32) {
         *reinterpret_cast<f32x4*>(to + 256 * g) = v;
     } else {  // quarters of 1 KB: ranks 0 to 7 and 8 to 15 high, then low
@@ -380,7 +397,7 @@ extern "C" int gdn_add_low_rank(const void* x, int64_t x_stride, int dtype, cons
     if (groups == 0) return 0;
     const int es = dtype_size(dtype);
     const LowRankPlan plan = low_rank_plan(tile_count, tile_rows, rank_total, rank_block, K, es, groups);
-    const int64_t down_parts = tile_rows / 16, up_parts = tile_rows / plan.up_rows;
+    const int64_t down_parts = tile_rows / plan.down_rows, up_parts = tile_rows / plan.up_rows;
     GDN_REQUIRE(one_grid_row(tile_count * down_parts, 64 * kLowRankDownWaves) &&
                     one_grid_row(groups * tile_count * up_parts, 64 * kLowRankUpWaves),
                 "gdn_add_low_rank: too many rows and columns");
@@ -397,7 +414,7 @@ extern "C" int gdn_add_low_rank(const void* x, int64_t x_stride, int dtype, cons
         using Act = decltype(act);
         const auto down = [&](auto kernel) {
             p.parts = int(down_parts);
-            p.rows = 16;
+            p.rows = plan.down_rows;
             hipLaunchKernelGGL(kernel, dim3(unsigned(tile_count * down_parts), unsigned((rank_total + plan.ranks - 1) / plan.ranks)),
                                dim3(64 * kLowRankDownWaves), 0, s, p);
         };
@@ -406,9 +423,15 @@ extern "C" int gdn_add_low_rank(const void* x, int64_t x_stride, int dtype, cons
             p.rows = plan.up_rows;
             hipLaunchKernelGGL(kernel, dim3(unsigned(groups * tile_count * up_parts)), dim3(64 * kLowRankUpWaves), 0, s, p);
         };
-        if (plan.ranks == 16) down(low_rank_down_kernel<Act, 1>);
-        else if (plan.ranks == 32) down(low_rank_down_kernel<Act, 2>);
-        else down(low_rank_down_kernel<Act, 4>);
+        if (plan.down_rows == 32) {
+            if (plan.ranks == 16) down(low_rank_down_kernel<Act, 2, 1>);
+            else if (plan.ranks == 32) down(low_rank_down_kernel<Act, 2, 2>);
+            else down(low_rank_down_kernel<Act, 2, 4>);
+        } else {
+            if (plan.ranks == 16) down(low_rank_down_kernel<Act, 1, 1>);
+            else if (plan.ranks == 32) down(low_rank_down_kernel<Act, 1, 2>);
+            else down(low_rank_down_kernel<Act, 1, 4>);
+        }
         if (plan.held == 1) up(low_rank_up_kernel<Act, 1>);
         else if (plan.held == 2) up(low_rank_up_kernel<Act, 2>);
         else if (plan.held == 4) up(low_rank_up_kernel<Act, 4>);
