@@ -625,12 +625,14 @@ int gdn_fp8_dequantize(const void *w, const float *scales, void *out, int out_dt
  *      tile_rows (16 or 256) rows each; no row in two. A tile of no rows, or with an
  *      adapter or places that do not exist, is skipped. Rows in no tile are left as
  *      they are.
- *   workspace: gdn_add_low_rank_workspace_size(...) bytes, 4 for each rank of each
- *      place for a row in the tiles; calls sharing one must not overlap
+ *   workspace: gdn_add_low_rank_workspace_size(...) bytes of the same sizes: 4 for each
+ *      rank of each place for a row in the tiles, or none for few rows; calls sharing
+ *      one must not overlap
  * A, B, table and workspace 16-byte aligned; x and outs at any element. No
  * reference counterpart.
  */
-int64_t gdn_add_low_rank_workspace_size(int rank_total, int tile_count, int tile_rows);
+int64_t gdn_add_low_rank_workspace_size(int dtype, int blocks, int rank_total, int rank_block, const int *widths,
+                                        int tile_count, int tile_rows, int K);
 int gdn_add_low_rank(const void *x, int64_t x_stride, int dtype, const void *A, const void *B, const void *table,
                      int adapters, int blocks, int rank_total, int rank_block, void *const *outs,
                      const int64_t *out_strides, const int *widths, const int32_t *order, const int32_t *tiles,

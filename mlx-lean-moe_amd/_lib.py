@@ -112,7 +112,7 @@ _SIGNATURES = {
                               _c_void_p, _c_void_p, _c_void_p, _c_int, _c_i64, _c_int, _c_void_p]),
     "gdn_add_low_rank": (_c_int, [_c_void_p, _c_i64, _c_int] + [_c_void_p] * 3 + [_c_int] * 4 + [_c_void_p] * 5
                          + [_c_int] * 4 + [_c_void_p, _c_i64, _c_void_p]),
-    "gdn_add_low_rank_workspace_size": (_c_i64, [_c_int] * 3),
+    "gdn_add_low_rank_workspace_size": (_c_i64, [_c_int] * 4 + [_c_void_p] + [_c_int] * 3),
     "gdn_fp8_dequantize": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p]),
 }
 

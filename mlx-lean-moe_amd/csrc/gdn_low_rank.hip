@@ -20,6 +20,8 @@
 namespace gdn {
 namespace {
 
+constexpr int kDepth = 2;  // steps of K under way at once (3, 4 and 6: the same within 2 %)
+
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 struct AdapterBlock {
@@ -105,10 +107,30 @@ GDN_DEV void two_pieces(float v, uint16_t& high, uint16_t& low) {
     low = (high & 0x7F80) == 0x7F80 ? 0 : f32_to_bf16_bits(v - bf16_bits_to_f32(high));
 }
 
+// 16 rows' sums over 16 ranks, four ranks of a row a lane, as the second product's
+// operand: 1 KB, of which that product's lanes take 16 bytes each. Of the ranks the
+// first `rank` exist (what is padding is 0, also 0 times what is not finite).
+template <class Act>
+GDN_DEV void store_t(uint8_t* to, f32x4 v, int rank, float scale) {
+    const int g = (threadIdx.x & 63) >> 4, lr = threadIdx.x & 15;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = 4 * g + e < rank ? v[e] * scale : 0.f;
+    to += lr * 16;
+    if constexpr (Act::code == GDN_F32) {
+        *reinterpret_cast<f32x4*>(to + 256 * g) = v;
+    } else {  // quarters of 1 KB: ranks 0 to 7 and 8 to 15 high, then low
+        uint16_t high[4], low[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) two_pieces(v[e], high[e], low[e]);
+        to += g / 2 * 256 + g % 2 * 8;
+        __builtin_memcpy(__builtin_assume_aligned(to, 8), high, 8);
+        __builtin_memcpy(__builtin_assume_aligned(to + 512, 8), low, 8);
+    }
+}
+
 // t for kRF x 16 rows of a tile and kNR x 16 of its adapter's ranks. Ranks are the
 // left operand, so a lane ends with four ranks of one row. The waves share out K and
-// add their sums in LDS; a step's loads are under way while the one before is
-// multiplied.
+// add their sums in LDS; kDepth steps' loads are under way at once.
 template <class Act, int kRF, int kNR>
 __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_down_kernel(LowRankArgs p) {
     using S = typename Act::storage;
@@ -166,17 +188,18 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_down_kernel(L
 #pragma unroll
                 for (int j = 0; j < kNR; ++j) acc[i][j] = mfma_pieces<Act>(av[j][h], xv[i][h], acc[i][j]);
     };
-    uint4 xv[2][kRF][2], av[2][kNR][2];
-    int s = wave;
-    if (s < p.steps) load(s, xv[0], av[0]);
-    for (; s < p.steps; s += 2 * kLowRankDownWaves) {
-        const int s1 = s + kLowRankDownWaves, s2 = s1 + kLowRankDownWaves;
-        if (s1 < p.steps) load(s1, xv[1], av[1]);
-        multiply(xv[0], av[0]);
-        if (s1 >= p.steps) break;
-        if (s2 < p.steps) load(s2, xv[0], av[0]);
-        multiply(xv[1], av[1]);
-    }
+    uint4 xv[kDepth][kRF][2], av[kDepth][kNR][2];
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d)
+        if (wave + d * kLowRankDownWaves < p.steps) load(wave + d * kLowRankDownWaves, xv[d], av[d]);
+    for (int s0 = wave; s0 < p.steps; s0 += kDepth * kLowRankDownWaves)
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) {
+            const int s = s0 + d * kLowRankDownWaves;
+            if (s >= p.steps) break;
+            multiply(xv[d], av[d]);
+            if (s + kDepth * kLowRankDownWaves < p.steps) load(s + kDepth * kLowRankDownWaves, xv[d], av[d]);
+        }
 #pragma unroll
     for (int i = 0; i < kRF; ++i)
 #pragma unroll
@@ -190,20 +213,8 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_down_kernel(L
     for (int w = 1; w < kLowRankDownWaves; ++w) v += sums[w][wave][lane];
     int block = 0;
     while (r >= ab[block].t_col + pad16(ab[block].rank)) ++block;
-    const int rank = ab[block].t_col + ab[block].rank - r - 4 * g;  // (padding: 0 times what is not finite)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = e < rank ? v[e] * ab[block].scale : 0.f;
-    uint8_t* to = p.t + ((tile.block + rows / 16) * (p.rank_total / 16) + r / 16) * 1024 + lr * 16;
-    if constexpr (Act::code == GDN_F32) {
-        *reinterpret_cast<f32x4*>(to + 256 * g) = v;
-    } else {  // quarters of 1 KB: ranks 0 to 7 and 8 to 15 high, then low
-        uint16_t high[4], low[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) two_pieces(v[e], high[e], low[e]);
-        to += g / 2 * 256 + g % 2 * 8;
-        __builtin_memcpy(__builtin_assume_aligned(to, 8), high, 8);
-        __builtin_memcpy(__builtin_assume_aligned(to + 512, 8), low, 8);
-    }
+    store_t<Act>(p.t + ((tile.block + rows / 16) * (p.rank_total / 16) + r / 16) * 1024, v,
+                 ab[block].t_col + ab[block].rank - r, ab[block].scale);
 }
 
 // One piece of B as the second product's operand.
@@ -228,6 +239,44 @@ struct Operand<ActF16> {
     GDN_DEV f32x4 times(const uint4& t, f32x4 c) const { return mfma_bf16(low, t, mfma_bf16(high, t, c)); }
 };
 
+// A wave's 64 columns: the lane's 16 values of a row in 16-byte pieces, the four lanes
+// of a row beside each other in each. acc[j] holds four columns from quad_at(g, j).
+template <class Act>
+struct Columns {
+    using S = typename Act::storage;
+    static constexpr int kY = sizeof(S), kCount = 16 / kY;
+    static GDN_DEV int quad_at(int q, int j) { return j / (4 / kY) * 4 * kCount + q * kCount + j % (4 / kY) * 4; }
+    static GDN_DEV void load(const S* y, uint4 (&v)[kY]) {
+#pragma unroll
+        for (int k = 0; k < kY; ++k) __builtin_memcpy(&v[k], y + k * 4 * kCount, 16);
+    }
+    // y (read into v if the wave's columns are `whole`) + acc; else the `left` columns
+    // that there are from y on
+    static GDN_DEV void add(S* y, const uint4 (&v)[kY], const f32x4 (&acc)[4], bool whole, int left) {
+        if (whole) {
+            S e[16];
+            __builtin_memcpy(e, v, sizeof(e));
+#pragma unroll
+            for (int j = 0; j < 16; ++j) Act::store(e, j, acc[j / 4][j % 4] + Act::load(e, j));
+#pragma unroll
+            for (int k = 0; k < kY; ++k) __builtin_memcpy(y + k * 4 * kCount, e + k * kCount, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int at = quad_at(0, j / 4) + j % 4;
+                if (at < left) Act::store(y, at, acc[j / 4][j % 4] + Act::load(y, at));
+            }
+        }
+    }
+    // B: for each 64 columns and 16 ranks four operands, of 512 bytes where both of
+    // t's pieces meet the same
+    static constexpr int kB = Act::code == GDN_F32 ? 1024 : 512;
+    static GDN_DEV const uint8_t* operands(const LowRankArgs& p, const AdapterBlock& ab, int n0) {
+        return static_cast<const uint8_t*>(p.B) + ab.b * kY + int64_t(n0) * pad16(ab.rank) * kY +
+               (threadIdx.x & 63) * 16 % kB;
+    }
+};
+
 // out += t B^T for a part of a tile and 256 columns of one block, 64 a wave, 16
 // rows at a time. B is the left operand and its rows are dealt out so that a lane
 // ends with 16-byte pieces of one row's output, the four lanes of a row beside each
@@ -239,7 +288,8 @@ struct Operand<ActF16> {
 template <class Act, int kHeld>
 __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRankArgs p) {
     using S = typename Act::storage;
-    constexpr int kY = sizeof(S), kCount = 16 / kY, kT = kHeld ? kHeld : 1;  // 16-byte pieces of 16 columns
+    using Own = Columns<Act>;
+    constexpr int kT = kHeld ? kHeld : 1;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, lr = lane & 15;
     // neighbours take neighbouring columns: workgroups that run at once cover whole
@@ -251,7 +301,7 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
     while (group >= p.group_end[block]) ++block;
     const AdapterBlock ab = p.table[int64_t(tile.adapter) * p.blocks + block];
     if (ab.rank <= 0) return;
-    const int pieces = (ab.rank + 15) / 16, R = 16 * pieces, width = p.width[block];
+    const int pieces = (ab.rank + 15) / 16, width = p.width[block];
     const int n0 = (group - (block ? p.group_end[block - 1] : 0)) * kLowRankColumns + wave * 64;
     // the rows' numbers, all at first: a number fetched among the rows' output would
     // be there only after the output before it
@@ -259,19 +309,13 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
     if (tid < p.rows) rows[tid] = tid < tile.count ? p.order[tile.start + tid] : -1;
     __syncthreads();
     if (n0 >= width) return;
-    // four columns from quad_at(q, j) are one lane's acc[j], q its g
-    const auto quad_at = [](int q, int j) { return j / (4 / kY) * 4 * kCount + q * kCount + j % (4 / kY) * 4; };
-    const int n = n0 + kCount * g;
+    const int n = n0 + Own::kCount * g;
     const bool whole = n0 + 64 <= width;  // (of the wave: one branch)
-
-    // B: for each 64 columns and 16 ranks four operands, of 512 bytes where both of
-    // t's pieces meet the same
-    constexpr int kB = Act::code == GDN_F32 ? 1024 : 512;
-    const uint8_t* br = static_cast<const uint8_t*>(p.B) + ab.b * kY + int64_t(n0) * R * kY + lane * 16 % kB;
+    const uint8_t* br = Own::operands(p, ab, n0);
     Operand<Act> b[kT][4];
     const auto load_b = [&](int i, Operand<Act> (&v)[4]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j].of(*reinterpret_cast<const uint4*>(br + (4 * i + j) * kB));
+        for (int j = 0; j < 4; ++j) v[j].of(*reinterpret_cast<const uint4*>(br + (4 * i + j) * Own::kB));
     };
     if constexpr (kHeld != 0) {
 #pragma unroll
@@ -286,15 +330,12 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
 
     struct Rows {
         S* y;  // null: no row
-        uint4 yv[kY], tv[kT];
+        uint4 yv[Own::kY], tv[kT];
     };
     const auto fetch = [&](Rows& r, int s) {
         const int row = rows[16 * s + lr];
         r.y = uint32_t(row) < uint32_t(p.M) ? out + row * stride : nullptr;
-        if (r.y && whole) {
-#pragma unroll
-            for (int k = 0; k < kY; ++k) __builtin_memcpy(&r.yv[k], r.y + k * 4 * kCount, 16);
-        }
+        if (r.y && whole) Own::load(r.y, r.yv);
         if constexpr (kHeld != 0) {
 #pragma unroll
             for (int i = 0; i < kHeld; ++i)
@@ -320,21 +361,7 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
                 for (int j = 0; j < 4; ++j) acc[j] = b[0][j].times(v, acc[j]);
             }
         }
-        if (!r.y) return;
-        if (whole) {
-            S e[16];
-            __builtin_memcpy(e, r.yv, sizeof(e));
-#pragma unroll
-            for (int j = 0; j < 16; ++j) Act::store(e, j, acc[j / 4][j % 4] + Act::load(e, j));
-#pragma unroll
-            for (int k = 0; k < kY; ++k) __builtin_memcpy(r.y + k * 4 * kCount, e + k * kCount, 16);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int at = quad_at(0, j / 4) + j % 4;
-                if (n + at < width) Act::store(r.y, at, acc[j / 4][j % 4] + Act::load(r.y, at));
-            }
-        }
+        if (r.y) Own::add(r.y, r.yv, acc, whole, width - n);
     };
     Rows even, odd;
     fetch(even, 0);
@@ -347,6 +374,116 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
     }
 }
 
+// Both products in one launch, for few rows: 16 rows of a tile and 512 columns of one
+// block a workgroup, which forms their t itself (its waves share out K) while the
+// output and B are on their way. Every workgroup of a block reads the same rows of A,
+// so there is an end to it: low_rank_plan.
+template <class Act, int kNR>
+__global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_small_kernel(LowRankArgs p) {
+    using S = typename Act::storage;
+    using Own = Columns<Act>;
+    constexpr int kStep = 128 / sizeof(S), kPiece = 16 / sizeof(S);
+    __shared__ f32x4 sums[kLowRankDownWaves][kNR][64];
+    __shared__ __attribute__((aligned(16))) uint8_t t[kNR * 1024];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int g = lane >> 4, lr = lane & 15;
+    const int groups = p.group_end[p.blocks - 1], group = blockIdx.x % groups;
+    const Tile tile = part_of(p, blockIdx.x / groups);
+    if (tile.count <= 0) return;
+    int block = 0;
+    while (group >= p.group_end[block]) ++block;
+    const AdapterBlock ab = p.table[int64_t(tile.adapter) * p.blocks + block];
+    if (ab.rank <= 0) return;
+    const int row = p.order[tile.start + min(lr, tile.count - 1)], pieces = (ab.rank + 15) / 16;
+    const S* xr = static_cast<const S*>(p.x) + int64_t(min(max(row, 0), p.M - 1)) * p.x_stride + g * kPiece;
+    const uint8_t* ar = static_cast<const uint8_t*>(p.A) + int64_t(ab.a_row) * (p.steps * 128) + lane * 16;
+    const int64_t a_stride = int64_t(p.steps) * 2048;
+    const auto load = [&](int s, uint4 (&xv)[2], uint4 (&av)[kNR][2]) {
+        const int k = s * kStep;
+#pragma unroll
+        for (int j = 0; j < kNR; ++j) {
+            const uint8_t* a = ar + min(j, pieces - 1) * a_stride + s * 2048;
+            av[j][0] = *reinterpret_cast<const uint4*>(a);
+            av[j][1] = *reinterpret_cast<const uint4*>(a + 1024);
+        }
+        if (k + kStep <= p.K) {
+            __builtin_memcpy(&xv[0], xr + k, 16);
+            __builtin_memcpy(&xv[1], xr + k + kStep / 2, 16);
+        } else {  // the last step of a K that is no multiple of it
+            const int left = p.K - k - g * kPiece;
+            xv[0] = piece_of(xr + k, left);
+            xv[1] = piece_of(xr + k + kStep / 2, left - kStep / 2);
+        }
+    };
+    f32x4 acc[kNR];
+#pragma unroll
+    for (int j = 0; j < kNR; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const auto multiply = [&](const uint4 (&xv)[2], const uint4 (&av)[kNR][2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < kNR; ++j) acc[j] = mfma_pieces<Act>(av[j][h], xv[h], acc[j]);
+    };
+    uint4 xv[kDepth][2], av[kDepth][kNR][2];
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d)
+        if (wave + d * kLowRankDownWaves < p.steps) load(wave + d * kLowRankDownWaves, xv[d], av[d]);
+
+    const int width = p.width[block];
+    const int n0 = (group - (block ? p.group_end[block - 1] : 0)) * kLowRankSmallColumns + wave * 64;
+    const int n = n0 + Own::kCount * g;
+    const bool whole = n0 + 64 <= width;  // (of the wave: one branch)
+    uint4 raw[kNR][4], yv[Own::kY];
+    S* y = nullptr;
+    if (n0 < width) {
+        const uint8_t* br = Own::operands(p, ab, n0);
+#pragma unroll
+        for (int i = 0; i < kNR; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                raw[i][j] = *reinterpret_cast<const uint4*>(br + (4 * min(i, pieces - 1) + j) * Own::kB);
+        if (lr < tile.count && uint32_t(row) < uint32_t(p.M)) {
+            y = static_cast<S*>(p.out[block]) + int64_t(row) * p.out_stride[block] + n;
+            if (whole) Own::load(y, yv);
+        }
+    }
+
+    for (int s0 = wave; s0 < p.steps; s0 += kDepth * kLowRankDownWaves)
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) {
+            const int s = s0 + d * kLowRankDownWaves;
+            if (s >= p.steps) break;
+            multiply(xv[d], av[d]);
+            if (s + kDepth * kLowRankDownWaves < p.steps) load(s + kDepth * kLowRankDownWaves, xv[d], av[d]);
+        }
+#pragma unroll
+    for (int j = 0; j < kNR; ++j) sums[wave][j][lane] = acc[j];
+    __syncthreads();
+    if (wave < kNR) {
+        f32x4 v = sums[0][wave][lane];
+#pragma unroll
+        for (int w = 1; w < kLowRankDownWaves; ++w) v += sums[w][wave][lane];
+        store_t<Act>(t + wave * 1024, v, ab.rank - wave * 16, ab.scale);
+    }
+    __syncthreads();
+    if (n0 >= width) return;
+    f32x4 sum[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kNR; ++i)
+        if (i < pieces) {
+            const uint4 v = *reinterpret_cast<const uint4*>(t + i * 1024 + lane * 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                Operand<Act> b;
+                b.of(raw[i][j]);
+                sum[j] = b.times(v, sum[j]);
+            }
+        }
+    if (y) Own::add(y, yv, sum, whole, width - n);
+}
+
 bool low_rank_sizes_ok(int tiles, int tile_rows, int rank_total, int M, int K) {
     return tiles >= 0 && (tile_rows == 16 || tile_rows == kLowRankTile) && rank_total > 0 && rank_total % 16 == 0 &&
            rank_total <= (1 << 16) && M >= 0 && M <= INT32_MAX - 512 && K > 0 && K <= (1 << 24);
@@ -357,9 +494,33 @@ bool low_rank_sizes_ok(int tiles, int tile_rows, int rank_total, int M, int K) {
 
 using namespace gdn;
 
-extern "C" int64_t gdn_add_low_rank_workspace_size(int rank_total, int tile_count, int tile_rows) {
-    if (!low_rank_sizes_ok(tile_count, tile_rows, rank_total, 0, 1)) return 0;
-    return int64_t(tile_count) * tile_rows * rank_total * 4;
+namespace {
+
+// Columns of each block in groups of `columns`: how many, and where each block's end.
+int64_t column_groups(const int* widths, int blocks, int columns, int* ends) {
+    int64_t groups = 0;
+    for (int j = 0; j < blocks; ++j) {
+        groups += (int64_t(widths[j]) + columns - 1) / columns;
+        if (ends) ends[j] = int(groups < INT32_MAX ? groups : INT32_MAX);
+    }
+    return groups;
+}
+
+LowRankPlan plan_of(int dtype, int rank_total, int rank_block, const int* widths, int blocks, int tiles, int tile_rows, int K) {
+    return low_rank_plan(tiles, tile_rows, rank_total, rank_block, K, dtype_size(dtype),
+                         column_groups(widths, blocks, kLowRankColumns, nullptr),
+                         column_groups(widths, blocks, kLowRankSmallColumns, nullptr));
+}
+
+}  // namespace
+
+extern "C" int64_t gdn_add_low_rank_workspace_size(int dtype, int blocks, int rank_total, int rank_block, const int* widths,
+                                                   int tile_count, int tile_rows, int K) {
+    if (!valid_dtype(dtype) || !low_rank_sizes_ok(tile_count, tile_rows, rank_total, 0, K) || blocks < 1 ||
+        blocks > kLowRankBlocks || !widths)
+        return 0;
+    const LowRankPlan plan = plan_of(dtype, rank_total, rank_block, widths, blocks, tile_count, tile_rows, K);
+    return plan.small ? 0 : int64_t(tile_count) * tile_rows * rank_total * 4;
 }
 
 extern "C" int gdn_add_low_rank(const void* x, int64_t x_stride, int dtype, const void* A, const void* B, const void* table,
@@ -377,26 +538,23 @@ extern "C" int gdn_add_low_rank(const void* x, int64_t x_stride, int dtype, cons
     if (M == 0 || tile_count == 0) return 0;
     GDN_REQUIRE(x && A && B && table && outs && out_strides && widths && order && tiles, "gdn_add_low_rank: null pointer");
     GDN_REQUIRE(x_stride >= K || M == 1, "gdn_add_low_rank: rows of x closer than their width");
-    const int64_t need = int64_t(tile_count) * tile_rows * rank_total * 4;
-    GDN_REQUIRE(workspace && workspace_bytes >= need, "gdn_add_low_rank: workspace of %lld bytes, %lld needed",
-                (long long)workspace_bytes, (long long)need);
     GDN_REQUIRE((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(table) |
                  reinterpret_cast<uintptr_t>(workspace)) % 16 == 0,
                 "gdn_add_low_rank: A, B, table and workspace must be 16-byte aligned");
     LowRankArgs p{x, A, B, static_cast<const AdapterBlock*>(table), order, tiles, static_cast<uint8_t*>(workspace)};
-    int64_t groups = 0;
     for (int j = 0; j < blocks; ++j) {
         GDN_REQUIRE(widths[j] >= 0 && (widths[j] == 0 || (outs[j] && (out_strides[j] >= widths[j] || M == 1))),
                     "gdn_add_low_rank: block %d of %d columns, rows %lld apart", j, widths[j], (long long)out_strides[j]);
         p.out[j] = outs[j];
         p.out_stride[j] = out_strides[j];
         p.width[j] = widths[j];
-        groups += (int64_t(widths[j]) + kLowRankColumns - 1) / kLowRankColumns;
-        p.group_end[j] = int(groups);
     }
+    const int64_t groups = column_groups(widths, blocks, kLowRankColumns, p.group_end);
     if (groups == 0) return 0;
-    const int es = dtype_size(dtype);
-    const LowRankPlan plan = low_rank_plan(tile_count, tile_rows, rank_total, rank_block, K, es, groups);
+    const LowRankPlan plan = plan_of(dtype, rank_total, rank_block, widths, blocks, tile_count, tile_rows, K);
+    const int64_t need = plan.small ? 0 : int64_t(tile_count) * tile_rows * rank_total * 4;
+    GDN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "gdn_add_low_rank: workspace of %lld bytes, %lld needed",
+                (long long)workspace_bytes, (long long)need);
     const int64_t down_parts = tile_rows / plan.down_rows, up_parts = tile_rows / plan.up_rows;
     GDN_REQUIRE(one_grid_row(tile_count * down_parts, 64 * kLowRankDownWaves) &&
                     one_grid_row(groups * tile_count * up_parts, 64 * kLowRankUpWaves),
@@ -412,6 +570,19 @@ extern "C" int gdn_add_low_rank(const void* x, int64_t x_stride, int dtype, cons
     hipStream_t s = as_stream(stream);
     const auto typed = [&](auto act) {
         using Act = decltype(act);
+        if (plan.small) {
+            p.parts = tile_rows / 16;
+            p.rows = 16;
+            const int64_t small_groups = column_groups(widths, blocks, kLowRankSmallColumns, p.group_end);
+            const auto small = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, dim3(unsigned(small_groups * tile_count * p.parts)), dim3(64 * kLowRankDownWaves), 0,
+                                   s, p);
+            };
+            if (plan.held == 1) small(low_rank_small_kernel<Act, 1>);
+            else if (plan.held == 2) small(low_rank_small_kernel<Act, 2>);
+            else small(low_rank_small_kernel<Act, 4>);
+            return;
+        }
         const auto down = [&](auto kernel) {
             p.parts = int(down_parts);
             p.rows = plan.down_rows;

@@ -125,7 +125,21 @@ class LowRankAdapters:
                 else:
                     laid.view(columns // 64, padded // 16, 4, 4, 4, 4, 4).copy_(
                         wide.view(columns // 64, 4, 4, 4, padded // 16, 4, 4).permute(0, 4, 1, 5, 2, 3, 6))
+        self._index = self._A.get_device()
+        self._c_widths = (ctypes.c_int * len(widths))(*widths)
+        self._workspaces: dict[tuple[int, int], int] = {}
         self._table = torch.from_numpy(table.reshape(-1).view(np.uint8)).to(self.device)
+
+
+    def _workspace(self, tiles: int, tile_rows: int) -> int:
+        nbytes = self._workspaces.get((tiles, tile_rows))
+        if nbytes is None:
+            if len(self._workspaces) >= 1024:
+                self._workspaces.clear()
+            nbytes = self._workspaces[tiles, tile_rows] = int(_lib.load().gdn_add_low_rank_workspace_size(
+                _lib.dtype_code(self.dtype), len(self.widths), self.rank_total, self.rank_block, self._c_widths, tiles,
+                tile_rows, self.hidden))
+        return nbytes
 
 
 class AdapterRows:
@@ -148,7 +162,7 @@ class AdapterRows:
         if distinct is not None:  # one tile that is not full an adapter
             self.tiles = max(self.tiles, min(self.rows, -(-self.rows // self.tile_rows) + distinct))
         self._plan = torch.from_numpy(self._planned(index)).to(device)
-        self.device = self._plan.device
+        self.device, self._index = self._plan.device, self._plan.get_device()
 
     @classmethod
     def of_runs(cls, runs, index, count: int) -> "AdapterRows":
@@ -221,52 +235,58 @@ def add_low_rank(outs, x: torch.Tensor, adapters: LowRankAdapters, rows: Adapter
     its dtype. ``scale x A^T`` is kept to 16 bits for 16-bit dtypes, in full for
     float32. Rows without an adapter are left as they are."""
 
-    single = isinstance(outs, torch.Tensor)
-    blocks = [outs] if single else outs
-    x = _kept_rows(x)
-    if x.ndim != 2 or x.shape[1] != adapters.hidden:
-        raise ValueError(f"x must be (rows, {adapters.hidden}), got {tuple(x.shape)}")
-    M, dtype = x.shape[0], x.dtype
-    if dtype is not adapters.dtype:
-        raise ValueError(f"the adapters are {adapters.dtype}, x {dtype}")
+    # decode steps are host-bound, hence the integer comparisons and the quick look
+    # at the arrays' ends in front of _overlap
+    blocks = [outs] if isinstance(outs, torch.Tensor) else outs
+    if isinstance(x, QuantizedRows):
+        x = _kept_rows(x)
+    K, dtype, index = adapters.hidden, adapters.dtype, adapters._index
+    if x.ndim != 2 or x.shape[1] != K:
+        raise ValueError(f"x must be (rows, {K}), got {tuple(x.shape)}")
+    M = x.shape[0]
+    if x.dtype is not dtype:
+        raise ValueError(f"the adapters are {dtype}, x {x.dtype}")
     if rows.rows != M or rows.count != adapters.count:
         raise ValueError(f"rows of {rows.rows} with {rows.count} adapters, x has {M} and there are {adapters.count}")
     if len(blocks) != len(adapters.widths):
         raise ValueError(f"{len(adapters.widths)} projections, {len(blocks)} outputs")
-    device = adapters.device
-    if x.device != device or rows.device != device:
-        raise ValueError(f"the adapters are on {device}, x on {x.device}, its adapters' numbers on {rows.device}")
-    if x.stride(1) != 1 or (M > 1 and x.stride(0) < adapters.hidden):
+    if x.get_device() != index or rows._index != index:
+        raise ValueError(f"the adapters are on {adapters.device}, x on {x.device}, its adapters' numbers on {rows.device}")
+    x_stride, step = x.stride()
+    if step != 1 or (M > 1 and x_stride < K):
         x = x.contiguous()
-    x_stride = x.stride(0)
-    pointers, strides = [], []
-    written = [x]
+        x_stride = K
+    n, size = len(blocks), dtype.itemsize
+    pointers, strides = [None] * n, [0] * n
+    begin = x.data_ptr()
+    ends = [(begin, begin + ((M - 1) * x_stride + K) * size, x)]
     for j, (out, width) in enumerate(zip(blocks, adapters.widths)):
         if not width:
-            pointers.append(None)
-            strides.append(0)
             continue
-        if out is None or out.shape != (M, width) or out.dtype is not dtype or out.device != device:
-            raise ValueError(f"output {j} must be {(M, width)} {dtype} on {device}")
-        if (out.stride(1) != 1 and width > 1) or (M > 1 and out.stride(0) < width):
+        if out is None or out.ndim != 2 or out.shape[0] != M or out.shape[1] != width or out.dtype is not dtype \
+                or out.get_device() != index:
+            raise ValueError(f"output {j} must be {(M, width)} {dtype} on {adapters.device}")
+        stride, step = out.stride()
+        if (step != 1 and width > 1) or (M > 1 and stride < width):
             raise ValueError(f"output {j} must consist of packed rows")
-        for other in written:
-            if _overlap(out, other):
+        begin = out.data_ptr()
+        end = begin + ((M - 1) * stride + width) * size
+        for b, e, other in ends:
+            if begin < e and b < end and M and _overlap(out, other):
                 raise ValueError(f"output {j} overlaps {'x' if other is x else 'another output'}")
-        written.append(out)
-        pointers.append(out.data_ptr())
-        strides.append(out.stride(0))
-    if _followed(*written):
+        ends.append((begin, end, out))
+        pointers[j], strides[j] = begin, stride
+    if _followed(*(t for _, _, t in ends)):
         raise RuntimeError("adapters have no gradient and no forward mode; call add_low_rank under torch.no_grad()")
-    n = len(pointers)
-    code = _lib.dtype_code(dtype)
-    nbytes = rows.tiles * rows.tile_rows * adapters.rank_total * 4  # (gdn_add_low_rank_workspace_size)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    device = x.device
+    nbytes = adapters._workspace(rows.tiles, rows.tile_rows)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     plan = rows._plan.data_ptr()
-    _lib.call_on(device, "gdn_add_low_rank", x.data_ptr(), x_stride, code, adapters._A.data_ptr(), adapters._B.data_ptr(),
-                 adapters._table.data_ptr(), adapters.count, n, adapters.rank_total, adapters.rank_block, (ctypes.c_void_p * n)(*pointers),
-                 (ctypes.c_int64 * n)(*strides), (ctypes.c_int * n)(*adapters.widths), plan, plan + 4 * M, rows.tiles,
-                 rows.tile_rows, M, adapters.hidden, ws.data_ptr(), nbytes, _stream(device))
+    _lib.call_on(device, "gdn_add_low_rank", ends[0][0], x_stride, _lib.dtype_code(dtype), adapters._A.data_ptr(),
+                 adapters._B.data_ptr(), adapters._table.data_ptr(), adapters.count, n, adapters.rank_total,
+                 adapters.rank_block, (ctypes.c_void_p * n)(*pointers), (ctypes.c_int64 * n)(*strides),
+                 adapters._c_widths, plan, plan + 4 * M, rows.tiles, rows.tile_rows, M, K, _lib.ptr(ws), nbytes,
+                 _stream(device))
     return outs
 
 

@@ -29,6 +29,10 @@ def _row_layout(t: torch.Tensor, K: int) -> int:
     return 0
 
 
+def _new_rows(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *, residual: torch.Tensor | None = None,
              quantize: bool = False, keep_rows: bool = False, sum_out: torch.Tensor | None = None):
     """``s * weight / sqrt(mean(s * s) + eps)`` over the last axis, ``s = x``, or
@@ -76,10 +80,15 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *, residu
         raise RuntimeError("rms_norm has no gradient and no forward mode; call it under torch.no_grad()")
     device = x.device
     M = x.numel() // K
-    x_stride = r_stride = s_stride = K
+    x_stride = _row_layout(x, K)
+    if not x_stride:
+        x, x_stride = x.contiguous(), K
+    # (a third of torch.empty's time, and a norm of few rows is host-bound)
+    new = torch.empty_like if x.is_contiguous() else _new_rows
+    r_stride = s_stride = K
     if residual is not None:
         if sum_out is None:
-            sum_out = torch.empty(x.shape, dtype=dtype, device=device)
+            sum_out = new(x)
         else:
             if sum_out.shape != x.shape or sum_out.dtype is not dtype or sum_out.get_device() != index:
                 raise ValueError(f"sum_out must be {tuple(x.shape)} {dtype} on {device}")
@@ -91,21 +100,19 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *, residu
         r_stride = _row_layout(residual, K)
         if not r_stride:
             residual, r_stride = residual.contiguous(), K
-    x_stride = _row_layout(x, K)
-    if not x_stride:
-        x, x_stride = x.contiguous(), K
-    out = codes = scales = None
-    if not quantize or keep_rows:
-        out = torch.empty(x.shape, dtype=dtype, device=device)
+    out = data = codes = scales = None
     apart = 0
+    if not quantize or keep_rows:
+        out = new(x)
     if quantize:
-        blocks, apart = (K + 127) // 128, (M + 255) // 256 * 256
-        codes = torch.empty((M, blocks * 128), dtype=torch.uint8, device=device)
-        scales = torch.empty((blocks, apart), dtype=_F32, device=device)
+        apart = (M + 255) // 256 * 256
+        data = torch.empty(QuantizedRows.nbytes(M, K), dtype=torch.uint8, device=device)
+        codes = data.data_ptr()
+        scales = codes + (K + 127) // 128 * 128 * M
     _lib.call_on(device, "gdn_rms_norm", x.data_ptr(), x_stride, _lib.ptr(residual), r_stride, _lib.ptr(sum_out), s_stride,
-                 _lib.ptr(weight), float(eps), _lib.dtype_code(dtype), _lib.ptr(out), _lib.ptr(codes), _lib.ptr(scales),
-                 apart, M, K, _stream(device))
-    normed = out if not quantize else QuantizedRows(x.shape, dtype, codes, scales, out)
+                 _lib.ptr(weight), float(eps), _lib.dtype_code(dtype), _lib.ptr(out), codes, scales, apart, M, K,
+                 _stream(device))
+    normed = out if not quantize else QuantizedRows(x.shape, dtype, data, out)
     return normed if residual is None else (normed, sum_out)
 
 

@@ -192,34 +192,46 @@ class QuantizedRows:
     values in that dtype where they were kept (``keep_rows=True``), which every
     other kind of weights, and low-rank adapters, take instead of the codes."""
 
-    __slots__ = ("shape", "dtype", "rows", "_codes", "_scales")
+    __slots__ = ("shape", "dtype", "rows", "_data")
 
-    def __init__(self, shape, dtype: torch.dtype, codes: torch.Tensor, scales: torch.Tensor,
-                 rows: torch.Tensor | None = None) -> None:
-        """``codes (M, ceil(K / 128) * 128)`` uint8, ``scales (ceil(K / 128), S)``
-        float32 with row m's in column m (S a multiple of 256): the layout that the
-        products read."""
+    def __init__(self, shape, dtype: torch.dtype, data: torch.Tensor, rows: torch.Tensor | None = None) -> None:
+        """``data``: uint8, the codes ``(M, ceil(K / 128) * 128)`` and behind them the
+        scales ``(ceil(K / 128), S)`` float32, row m's in column m, S = M rounded up to
+        256 (:meth:`nbytes` in all): the layout that the products read."""
 
-        self.shape, self.dtype, self.rows = torch.Size(shape), dtype, rows
-        self._codes, self._scales = codes, scales
+        self.shape, self.dtype, self.rows, self._data = torch.Size(shape), dtype, rows, data
+
+    @staticmethod
+    def nbytes(M: int, K: int) -> int:
+        return -(-K // 128) * (128 * M + 4 * (-(-M // 256) * 256))
 
     @property
     def device(self) -> torch.device:
-        return self._codes.device
+        return self._data.device
 
     @property
     def ndim(self) -> int:
         return len(self.shape)
 
+    def _sizes(self) -> tuple[int, int, int]:
+        """Rows, values a row, bytes of the codes."""
+        K = self.shape[-1]
+        M = self.shape.numel() // K
+        return M, K, M * (-(-K // 128) * 128)
+
     @property
     def codes(self) -> torch.Tensor:
         """The codes ``(..., K)`` as float8_e4m3fn values."""
-        return self._codes[:, :self.shape[-1]].view(torch.float8_e4m3fn).view(self.shape)
+        M, K, size = self._sizes()
+        return self._data[:size].view(torch.float8_e4m3fn).view(M, size // M if M else 0)[:, :K].view(self.shape)
 
     @property
     def scales(self) -> torch.Tensor:
         """The scales ``(..., ceil(K / 128))``."""
-        return self._scales[:, :self._codes.shape[0]].T.reshape(*self.shape[:-1], -1)
+        M, K, size = self._sizes()
+        if not M:
+            return torch.empty((*self.shape[:-1], -(-K // 128)), device=self.device)
+        return self._data[size:].view(torch.float32).view(-(-K // 128), -1)[:, :M].T.reshape(*self.shape[:-1], -1)
 
     def dequantize(self) -> torch.Tensor:
         """The float32 values ``(..., K)`` that codes and scales stand for."""
@@ -231,8 +243,7 @@ class QuantizedRows:
         shape = torch.empty(self.shape, device="meta").reshape(*lead_and_width).shape
         if shape[-1:] != self.shape[-1:]:
             raise ValueError(f"the width {self.shape[-1]} of quantized rows stays")
-        return QuantizedRows(shape, self.dtype, self._codes, self._scales,
-                             None if self.rows is None else self.rows.reshape(shape))
+        return QuantizedRows(shape, self.dtype, self._data, None if self.rows is None else self.rows.reshape(shape))
 
 
 @dataclass(frozen=True)
@@ -551,21 +562,21 @@ def _fp8_matmul_codes(x: QuantizedRows, tensors, quant: QuantScheme, residual):
     w, scales, _, N, K = _check_quantized(tensors, quant, x.shape[-1])
     if _followed(residual, w, scales):
         raise RuntimeError("fp8_block products have no gradient and no forward mode; call them under torch.no_grad()")
-    codes, lead = x._codes, x.shape[:-1]
-    if w.get_device() != codes.get_device() or codes.get_device() < 0:
+    data, lead = x._data, x.shape[:-1]
+    if w.get_device() != data.get_device() or data.get_device() < 0:
         raise ValueError(f"x is on {x.device}, the weights on {w.device}")
-    M = codes.shape[0]
-    y = torch.empty((*lead, N), dtype=x.dtype, device=codes.device)
+    M, _, size = x._sizes()
+    y = torch.empty((*lead, N), dtype=x.dtype, device=data.device)
     r = None if residual is None else _residual_rows(residual, y, lead, M, N)
     w, scales = _c(w), _c(scales)
     if w.data_ptr() % 16:
         w = w.clone()
     code = _lib.dtype_code(x.dtype)
     ws_bytes = fp8_codes_workspace_bytes(code, M, N, K)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=codes.device) if ws_bytes else None
-    _lib.call_on(codes.device, "gdn_fp8_matmul_codes", codes.data_ptr(), x._scales.data_ptr(), x._scales.shape[1],
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=data.device) if ws_bytes else None
+    _lib.call_on(data.device, "gdn_fp8_matmul_codes", data.data_ptr(), data.data_ptr() + size, (M + 255) // 256 * 256,
                  w.data_ptr(), scales.data_ptr(), y.data_ptr(), code, _lib.ptr(r), M, N, K, _lib.ptr(ws), ws_bytes,
-                 _lib.stream_ptr(codes.device))
+                 _lib.stream_ptr(data.device))
     return y
 
 

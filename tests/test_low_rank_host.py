@@ -68,12 +68,16 @@ def test_argument_checks():
     lib = _lib.load()
     err = lambda: lib.gdn_last_error().decode()
     size = lib.gdn_add_low_rank_workspace_size
-    need = size(32, 4, 16)
-    assert need == 4 * 16 * 32 * 4 and size(33, 4, 16) == 0 and size(32, -1, 16) == 0 and size(32, 4, 64) == 0
+    wide = (ctypes.c_int * 2)(100, 64)
+    need = size(1, 2, 32, 16, wide, 200, 16, 2048)  # more than one round of workgroups: two launches
+    assert need == 200 * 16 * 32 * 4 and size(1, 2, 32, 16, wide, 4, 16, 2048) == 0
+    for bad in ((9, 2, 32, 16, wide, 200, 16, 2048), (1, 2, 33, 16, wide, 200, 16, 2048), (1, 9, 32, 16, wide, 200, 16, 2048),
+                (1, 2, 32, 16, wide, 200, 64, 2048), (1, 2, 32, 16, None, 200, 16, 2048), (1, 2, 32, 16, wide, -1, 16, 2048)):
+        assert size(*bad) == 0
 
     def call(widths=(100, 64), outs=(P(0), P(1)), strides=(164, 164), **over):
         a = dict(x=P(2), xs=2048, dt=1, A=P(3), B=P(4), table=P(5), S=3, blocks=len(widths), rt=32, rb=16)
-        b = dict(order=P(6), tiles=P(7), nt=4, tr=16, M=40, K=2048, ws=P(8), wsb=need)
+        b = dict(order=P(6), tiles=P(7), nt=200, tr=16, M=40, K=2048, ws=P(8), wsb=need)
         a.update({k: v for k, v in over.items() if k in a})
         b.update({k: v for k, v in over.items() if k in b})
         n = len(widths)
