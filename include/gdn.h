@@ -622,7 +622,7 @@ int gdn_fp8_dequantize(const void *w, const float *scales, void *out, int out_dt
  *      ranks that an adapter has in all, rank_block: in one block
  *   order: (M) int32, the rows that have an adapter, sorted by it; tiles:
  *      (tile_count, 3) int32 {adapter, first place in order, rows}, at most
- *      tile_rows (16 or 256) rows each; no row in two. A tile of no rows, or with an
+ *      tile_rows rows each (16, 32, 64, 128 or 256); no row in two. A tile of no rows, or with an
  *      adapter or places that do not exist, is skipped. Rows in no tile are left as
  *      they are.
  *   workspace: gdn_add_low_rank_workspace_size(...) bytes of the same sizes: 4 for each

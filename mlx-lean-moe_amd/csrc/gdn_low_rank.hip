@@ -43,6 +43,7 @@ struct LowRankArgs {
     int64_t x_stride;
     int S, blocks, rank_total, M, K, steps;
     int tile_count, parts, rows;   // parts of `rows` rows a tile
+    int columns;                   // of a block a workgroup takes (both products in one launch)
 };
 
 GDN_DEV int pad16(int r) { return (r + 15) & ~15; }
@@ -374,12 +375,14 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
     }
 }
 
-// Both products in one launch, for few rows: 16 rows of a tile and 512 columns of one
-// block a workgroup, which forms their t itself (its waves share out K) while the
-// output and B are on their way. Every workgroup of a block reads the same rows of A,
-// so there is an end to it: low_rank_plan.
+// Both products in one launch, for few rows: 16 rows of a tile and p.columns columns of
+// one block a workgroup, which forms their t itself, its waves sharing out K, while the
+// first of its output and B are on their way. Then each wave takes every eighth 64
+// columns, t from LDS; the next ones' output is under way while these are multiplied,
+// their B while these are stored. Every workgroup of a block reads the same rows of
+// A: low_rank_plan says where that is too much.
 template <class Act, int kNR>
-__global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_small_kernel(LowRankArgs p) {
+__global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_whole_kernel(LowRankArgs p) {
     using S = typename Act::storage;
     using Own = Columns<Act>;
     constexpr int kStep = 128 / sizeof(S), kPiece = 16 / sizeof(S);
@@ -394,7 +397,8 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_small_kernel(
     while (group >= p.group_end[block]) ++block;
     const AdapterBlock ab = p.table[int64_t(tile.adapter) * p.blocks + block];
     if (ab.rank <= 0) return;
-    const int row = p.order[tile.start + min(lr, tile.count - 1)], pieces = (ab.rank + 15) / 16;
+    const int pieces = (ab.rank + 15) / 16, width = p.width[block];
+    const int row = p.order[tile.start + min(lr, tile.count - 1)];
     const S* xr = static_cast<const S*>(p.x) + int64_t(min(max(row, 0), p.M - 1)) * p.x_stride + g * kPiece;
     const uint8_t* ar = static_cast<const uint8_t*>(p.A) + int64_t(ab.a_row) * (p.steps * 128) + lane * 16;
     const int64_t a_stride = int64_t(p.steps) * 2048;
@@ -415,49 +419,52 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_small_kernel(
             xv[1] = piece_of(xr + k + kStep / 2, left - kStep / 2);
         }
     };
-    f32x4 acc[kNR];
-#pragma unroll
-    for (int j = 0; j < kNR; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const auto multiply = [&](const uint4 (&xv)[2], const uint4 (&av)[kNR][2]) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < kNR; ++j) acc[j] = mfma_pieces<Act>(av[j][h], xv[h], acc[j]);
-    };
-    uint4 xv[kDepth][2], av[kDepth][kNR][2];
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d)
-        if (wave + d * kLowRankDownWaves < p.steps) load(wave + d * kLowRankDownWaves, xv[d], av[d]);
 
-    const int width = p.width[block];
-    const int n0 = (group - (block ? p.group_end[block - 1] : 0)) * kLowRankSmallColumns + wave * 64;
-    const int n = n0 + Own::kCount * g;
-    const bool whole = n0 + 64 <= width;  // (of the wave: one branch)
-    uint4 raw[kNR][4], yv[Own::kY];
-    S* y = nullptr;
-    if (n0 < width) {
-        const uint8_t* br = Own::operands(p, ab, n0);
+    int n0 = (group - (block ? p.group_end[block - 1] : 0)) * p.columns;
+    const int n_end = min(width, n0 + p.columns);
+    n0 += wave * 64;
+    S* yr = lr < tile.count && uint32_t(row) < uint32_t(p.M)  // (null: no row)
+                ? static_cast<S*>(p.out[block]) + int64_t(row) * p.out_stride[block] + Own::kCount * g : nullptr;
+    const uint8_t* br = Own::operands(p, ab, 0);
+    const int64_t b_stride = int64_t(pieces) * 4 * Own::kB / 64;  // bytes a column
+    uint4 raw[kNR][4];
+    const auto load_b = [&](int n) {
 #pragma unroll
         for (int i = 0; i < kNR; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                raw[i][j] = *reinterpret_cast<const uint4*>(br + (4 * min(i, pieces - 1) + j) * Own::kB);
-        if (lr < tile.count && uint32_t(row) < uint32_t(p.M)) {
-            y = static_cast<S*>(p.out[block]) + int64_t(row) * p.out_stride[block] + n;
-            if (whole) Own::load(y, yv);
+                raw[i][j] = *reinterpret_cast<const uint4*>(br + n * b_stride + (4 * min(i, pieces - 1) + j) * Own::kB);
+    };
+    const auto load_y = [&](int n, uint4 (&v)[Own::kY]) {
+        if (yr && n + 64 <= width) Own::load(yr + n, v);  // (else read where it is written)
+    };
+    uint4 even[Own::kY], odd[Own::kY];
+    {
+        f32x4 acc[kNR];
+#pragma unroll
+        for (int j = 0; j < kNR; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        uint4 xv[kDepth][2], av[kDepth][kNR][2];
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d)
+            if (wave + d * kLowRankDownWaves < p.steps) load(wave + d * kLowRankDownWaves, xv[d], av[d]);
+        if (n0 < n_end) {
+            load_y(n0, even);
+            load_b(n0);
         }
+        for (int s0 = wave; s0 < p.steps; s0 += kDepth * kLowRankDownWaves)
+#pragma unroll
+            for (int d = 0; d < kDepth; ++d) {
+                const int s = s0 + d * kLowRankDownWaves;
+                if (s >= p.steps) break;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < kNR; ++j) acc[j] = mfma_pieces<Act>(av[d][j][h], xv[d][h], acc[j]);
+                if (s + kDepth * kLowRankDownWaves < p.steps) load(s + kDepth * kLowRankDownWaves, xv[d], av[d]);
+            }
+#pragma unroll
+        for (int j = 0; j < kNR; ++j) sums[wave][j][lane] = acc[j];
     }
-
-    for (int s0 = wave; s0 < p.steps; s0 += kDepth * kLowRankDownWaves)
-#pragma unroll
-        for (int d = 0; d < kDepth; ++d) {
-            const int s = s0 + d * kLowRankDownWaves;
-            if (s >= p.steps) break;
-            multiply(xv[d], av[d]);
-            if (s + kDepth * kLowRankDownWaves < p.steps) load(s + kDepth * kLowRankDownWaves, xv[d], av[d]);
-        }
-#pragma unroll
-    for (int j = 0; j < kNR; ++j) sums[wave][j][lane] = acc[j];
     __syncthreads();
     if (wave < kNR) {
         f32x4 v = sums[0][wave][lane];
@@ -466,26 +473,36 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_small_kernel(
         store_t<Act>(t + wave * 1024, v, ab.rank - wave * 16, ab.scale);
     }
     __syncthreads();
-    if (n0 >= width) return;
-    f32x4 sum[4];
+
+    const auto step = [&](int n, uint4 (&now)[Own::kY], uint4 (&next)[Own::kY]) {
+        const int n2 = n + 64 * kLowRankDownWaves;
+        if (n2 < n_end) load_y(n2, next);
+        f32x4 sum[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < 4; ++j) sum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < kNR; ++i)
-        if (i < pieces) {
-            const uint4 v = *reinterpret_cast<const uint4*>(t + i * 1024 + lane * 16);
+        for (int c = 0; c < kNR; ++c)
+            if (c < pieces) {
+                const uint4 v = *reinterpret_cast<const uint4*>(t + c * 1024 + lane * 16);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                Operand<Act> b;
-                b.of(raw[i][j]);
-                sum[j] = b.times(v, sum[j]);
+                for (int j = 0; j < 4; ++j) {
+                    Operand<Act> b;
+                    b.of(raw[c][j]);
+                    sum[j] = b.times(v, sum[j]);
+                }
             }
-        }
-    if (y) Own::add(y, yv, sum, whole, width - n);
+        if (n2 < n_end) load_b(n2);
+        if (yr) Own::add(yr + n, now, sum, n + 64 <= width, width - n - Own::kCount * g);
+    };
+    for (; n0 < n_end; n0 += 2 * 64 * kLowRankDownWaves) {
+        step(n0, even, odd);
+        if (n0 + 64 * kLowRankDownWaves >= n_end) break;
+        step(n0 + 64 * kLowRankDownWaves, odd, even);
+    }
 }
 
 bool low_rank_sizes_ok(int tiles, int tile_rows, int rank_total, int M, int K) {
-    return tiles >= 0 && (tile_rows == 16 || tile_rows == kLowRankTile) && rank_total > 0 && rank_total % 16 == 0 &&
+    return tiles >= 0 && tile_rows >= 16 && tile_rows <= kLowRankTile && (tile_rows & (tile_rows - 1)) == 0 && rank_total > 0 && rank_total % 16 == 0 &&
            rank_total <= (1 << 16) && M >= 0 && M <= INT32_MAX - 512 && K > 0 && K <= (1 << 24);
 }
 
@@ -496,20 +513,8 @@ using namespace gdn;
 
 namespace {
 
-// Columns of each block in groups of `columns`: how many, and where each block's end.
-int64_t column_groups(const int* widths, int blocks, int columns, int* ends) {
-    int64_t groups = 0;
-    for (int j = 0; j < blocks; ++j) {
-        groups += (int64_t(widths[j]) + columns - 1) / columns;
-        if (ends) ends[j] = int(groups < INT32_MAX ? groups : INT32_MAX);
-    }
-    return groups;
-}
-
 LowRankPlan plan_of(int dtype, int rank_total, int rank_block, const int* widths, int blocks, int tiles, int tile_rows, int K) {
-    return low_rank_plan(tiles, tile_rows, rank_total, rank_block, K, dtype_size(dtype),
-                         column_groups(widths, blocks, kLowRankColumns, nullptr),
-                         column_groups(widths, blocks, kLowRankSmallColumns, nullptr));
+    return low_rank_plan(tiles, tile_rows, rank_total, rank_block, K, dtype_size(dtype), widths, blocks);
 }
 
 }  // namespace
@@ -520,7 +525,7 @@ extern "C" int64_t gdn_add_low_rank_workspace_size(int dtype, int blocks, int ra
         blocks > kLowRankBlocks || !widths)
         return 0;
     const LowRankPlan plan = plan_of(dtype, rank_total, rank_block, widths, blocks, tile_count, tile_rows, K);
-    return plan.small ? 0 : int64_t(tile_count) * tile_rows * rank_total * 4;
+    return plan.columns ? 0 : int64_t(tile_count) * tile_rows * rank_total * 4;
 }
 
 extern "C" int gdn_add_low_rank(const void* x, int64_t x_stride, int dtype, const void* A, const void* B, const void* table,
@@ -552,7 +557,7 @@ extern "C" int gdn_add_low_rank(const void* x, int64_t x_stride, int dtype, cons
     const int64_t groups = column_groups(widths, blocks, kLowRankColumns, p.group_end);
     if (groups == 0) return 0;
     const LowRankPlan plan = plan_of(dtype, rank_total, rank_block, widths, blocks, tile_count, tile_rows, K);
-    const int64_t need = plan.small ? 0 : int64_t(tile_count) * tile_rows * rank_total * 4;
+    const int64_t need = plan.columns ? 0 : int64_t(tile_count) * tile_rows * rank_total * 4;
     GDN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "gdn_add_low_rank: workspace of %lld bytes, %lld needed",
                 (long long)workspace_bytes, (long long)need);
     const int64_t down_parts = tile_rows / plan.down_rows, up_parts = tile_rows / plan.up_rows;
@@ -570,17 +575,16 @@ extern "C" int gdn_add_low_rank(const void* x, int64_t x_stride, int dtype, cons
     hipStream_t s = as_stream(stream);
     const auto typed = [&](auto act) {
         using Act = decltype(act);
-        if (plan.small) {
-            p.parts = tile_rows / 16;
-            p.rows = 16;
-            const int64_t small_groups = column_groups(widths, blocks, kLowRankSmallColumns, p.group_end);
-            const auto small = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3(unsigned(small_groups * tile_count * p.parts)), dim3(64 * kLowRankDownWaves), 0,
-                                   s, p);
+        if (plan.columns) {
+            const auto whole = [&](auto kernel) {
+                p.parts = tile_rows / 16;
+                p.rows = 16;
+                p.columns = plan.columns;
+                const int64_t all = column_groups(widths, blocks, plan.columns, p.group_end);
+                hipLaunchKernelGGL(kernel, dim3(unsigned(all * tile_count * p.parts)), dim3(64 * kLowRankDownWaves), 0, s, p);
             };
-            if (plan.held == 1) small(low_rank_small_kernel<Act, 1>);
-            else if (plan.held == 2) small(low_rank_small_kernel<Act, 2>);
-            else small(low_rank_small_kernel<Act, 4>);
+            if (plan.held == 1) whole(low_rank_whole_kernel<Act, 1>);
+            else whole(low_rank_whole_kernel<Act, 2>);
             return;
         }
         const auto down = [&](auto kernel) {

@@ -29,10 +29,9 @@ from .quant import QuantizedRows, _followed, _kept_rows
 _MAX_BLOCKS = 8
 _MAX_RANKS = 1 << 16
 _MAX_HIDDEN = 1 << 24
-# Rows a tile: the large ones where adapters have at least _LARGE_FROM rows on average
-# (the kernels cut them as they need; small ones leave fewer places empty).
-_TILE_ROWS, _LARGE_TILE_ROWS = 16, 256
-_LARGE_FROM = 32
+# Rows a tile: about as many as adapters have on average, a power of two between these
+# (the kernels cut tiles as they need; places that stay empty cost workgroups).
+_LEAST_ROWS, _MOST_ROWS = 16, 256
 _TABLE = np.dtype([("b", "<i8"), ("a_row", "<i4"), ("rank", "<i4"), ("scale", "<f4"), ("t_col", "<i4")])
 
 
@@ -157,7 +156,8 @@ class AdapterRows:
         index = self._checked(index)
         self.rows = len(index)
         used, with_one = len(np.unique(index[index >= 0])), int((index >= 0).sum())
-        self.tile_rows = _LARGE_TILE_ROWS if used and with_one >= _LARGE_FROM * used else _TILE_ROWS
+        mean = -(-with_one // max(used, 1))
+        self.tile_rows = min(_MOST_ROWS, max(_LEAST_ROWS, 1 << max(mean - 1, 0).bit_length()))
         self.tiles = int((-(-np.unique(index[index >= 0], return_counts=True)[1] // self.tile_rows)).sum())
         if distinct is not None:  # one tile that is not full an adapter
             self.tiles = max(self.tiles, min(self.rows, -(-self.rows // self.tile_rows) + distinct))

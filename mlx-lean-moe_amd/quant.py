@@ -219,19 +219,26 @@ class QuantizedRows:
         M = self.shape.numel() // K
         return M, K, M * (-(-K // 128) * 128)
 
+    def _strides(self, row: int) -> list[int]:
+        """Of the leading axes, rows ``row`` elements apart."""
+        strides = []
+        for n in reversed(self.shape[:-1]):
+            strides.insert(0, row)
+            row *= n
+        return strides
+
     @property
     def codes(self) -> torch.Tensor:
         """The codes ``(..., K)`` as float8_e4m3fn values."""
         M, K, size = self._sizes()
-        return self._data[:size].view(torch.float8_e4m3fn).view(M, size // M if M else 0)[:, :K].view(self.shape)
+        return self._data.view(torch.float8_e4m3fn).as_strided(self.shape, (*self._strides(-(-K // 128) * 128), 1))
 
     @property
     def scales(self) -> torch.Tensor:
         """The scales ``(..., ceil(K / 128))``."""
         M, K, size = self._sizes()
-        if not M:
-            return torch.empty((*self.shape[:-1], -(-K // 128)), device=self.device)
-        return self._data[size:].view(torch.float32).view(-(-K // 128), -1)[:, :M].T.reshape(*self.shape[:-1], -1)
+        return self._data.view(torch.float32).as_strided(
+            (*self.shape[:-1], -(-K // 128)), (*self._strides(1), -(-M // 256) * 256), size // 4)
 
     def dequantize(self) -> torch.Tensor:
         """The float32 values ``(..., K)`` that codes and scales stand for."""

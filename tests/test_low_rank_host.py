@@ -40,10 +40,10 @@ def test_every_row_with_an_adapter_is_in_one_tile(M, S, without):
         rows.assign(index)
 
 
-def test_large_tiles_where_adapters_have_many_rows():
-    assert gdn.AdapterRows([0] * 31, 1, device="cpu").tile_rows == 16
-    assert gdn.AdapterRows([0] * 32, 1, device="cpu").tile_rows == 256
-    assert gdn.AdapterRows([0, 1] * 31, 2, device="cpu").tile_rows == 16
+def test_tiles_have_about_as_many_rows_as_adapters():
+    for rows, adapters, want in ((1, 1, 16), (16, 1, 16), (17, 1, 32), (31, 2, 16), (64, 1, 64), (65, 1, 128), (5000, 1, 256),
+                                 (5000, 100, 64), (0, 1, 16)):
+        assert gdn.AdapterRows([i % adapters for i in range(rows)], adapters, device="cpu").tile_rows == want
 
 
 def test_numbers_that_are_none_are_refused():
@@ -72,7 +72,7 @@ def test_argument_checks():
     need = size(1, 2, 32, 16, wide, 200, 16, 2048)  # more than one round of workgroups: two launches
     assert need == 200 * 16 * 32 * 4 and size(1, 2, 32, 16, wide, 4, 16, 2048) == 0
     for bad in ((9, 2, 32, 16, wide, 200, 16, 2048), (1, 2, 33, 16, wide, 200, 16, 2048), (1, 9, 32, 16, wide, 200, 16, 2048),
-                (1, 2, 32, 16, wide, 200, 64, 2048), (1, 2, 32, 16, None, 200, 16, 2048), (1, 2, 32, 16, wide, -1, 16, 2048)):
+                (1, 2, 32, 16, wide, 200, 48, 2048), (1, 2, 32, 16, wide, 200, 512, 2048), (1, 2, 32, 16, None, 200, 16, 2048), (1, 2, 32, 16, wide, -1, 16, 2048)):
         assert size(*bad) == 0
 
     def call(widths=(100, 64), outs=(P(0), P(1)), strides=(164, 164), **over):
@@ -86,7 +86,7 @@ def test_argument_checks():
 
     assert call(M=0) == 0 and call(nt=0) == 0
     assert call(widths=(0, 0), outs=(None, None)) == 0
-    for over, what in [(dict(K=0), "sizes"), (dict(tr=32), "sizes"), (dict(rt=20), "sizes"), (dict(rb=48), "sizes"), (dict(rb=0), "sizes"), (dict(S=0), "sizes"),
+    for over, what in [(dict(K=0), "sizes"), (dict(tr=48), "sizes"), (dict(rt=20), "sizes"), (dict(rb=48), "sizes"), (dict(rb=0), "sizes"), (dict(S=0), "sizes"),
                        (dict(dt=5), "dtype"), (dict(x=None), "null"), (dict(tiles=None), "null"), (dict(xs=2047), "width"),
                        (dict(wsb=need - 1), "workspace"), (dict(ws=None), "workspace"), (dict(A=ctypes.c_void_p(8)), "aligned"),
                        (dict(widths=(100, -1)), "block 1"), (dict(strides=(99, 164)), "block 0"),
