@@ -27,34 +27,53 @@ struct NormArgs {
     float eps;
 };
 
-// Eight consecutive values at any alignment of their own type (global memory
-// takes 16-byte accesses at any address); beyond `count` of them zeros.
-template <class Act>
-GDN_DEV void load_up_to8(const typename Act::storage* p, int count, float (&v)[8]) {
-    if (count >= 8) {
-        typename Act::storage raw[8];
+// kN consecutive values at any alignment of their own type (global memory takes
+// 16-byte accesses at any address); beyond `count` of them zeros, or left alone.
+template <class A, int kN>
+GDN_DEV void load_some(const typename A::storage* p, int count, float* v) {
+    if (count >= kN) {
+        typename A::storage raw[kN];
         __builtin_memcpy(raw, p, sizeof(raw));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = Act::load(raw, e);
+        for (int e = 0; e < kN; ++e) v[e] = A::load(raw, e);
         return;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < count ? Act::load(p, e) : 0.f;
+    for (int e = 0; e < kN; ++e) v[e] = e < count ? A::load(p, e) : 0.f;
 }
 
-template <class Act>
-GDN_DEV void store_up_to8(typename Act::storage* p, int count, const float (&v)[8]) {
-    if (count >= 8) {
-        typename Act::storage raw[8];
+template <class A, int kN>
+GDN_DEV void store_some(typename A::storage* p, int count, const float* v) {
+    if (count >= kN) {
+        typename A::storage raw[kN];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) Act::store(raw, e, v[e]);
+        for (int e = 0; e < kN; ++e) A::store(raw, e, v[e]);
         __builtin_memcpy(p, raw, sizeof(raw));
         return;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (e < count) Act::store(p, e, v[e]);
+    for (int e = 0; e < kN; ++e)
+        if (e < count) A::store(p, e, v[e]);
 }
+
+// A thread's eight columns, number c of a row's: rows of 16 bits eight beside each
+// other, 16 bytes; float32 rows four and the four 64 further on, so that a load of 16
+// bytes a lane leaves no holes between lanes (1531 rows of 2501: 10.0 us with 32 bytes a
+// lane, 9.6 so). Sixteen threads have 128 columns either way.
+template <class Act>
+struct Eight {
+    static constexpr int kN = Act::code == GDN_F32 ? 4 : 8;
+    static GDN_DEV int first(int c) { return kN == 8 ? c * 8 : c / 16 * 128 + c % 16 * 4; }
+    template <class A>  // (the weights are float32 whatever the rows are)
+    static GDN_DEV void load(const typename A::storage* row, int c, int K, float (&v)[8]) {
+#pragma unroll
+        for (int h = 0; h < 8 / kN; ++h) load_some<A, kN>(row + first(c) + 64 * h, K - first(c) - 64 * h, v + kN * h);
+    }
+    static GDN_DEV void store(typename Act::storage* row, int c, int K, const float (&v)[8]) {
+#pragma unroll
+        for (int h = 0; h < 8 / kN; ++h) store_some<Act, kN>(row + first(c) + 64 * h, K - first(c) - 64 * h, v + kN * h);
+    }
+};
 
 // y of eight values, rounded to the rows' type. In 16 bits the float32 product
 // of three factors, each rounding at most half a last place, lies within 3 last
@@ -87,17 +106,17 @@ GDN_DEV void scaled8(const float (&v)[8], double r, float r32, bool wild, const 
     }
 }
 
-// The eight columns from k of a row: the stream's values (kept or read again).
+// Eight columns of a row: the stream's values (kept or read again).
 template <class Act>
-GDN_DEV void stream8(const NormArgs& a, int64_t row, int k, bool live, float (&v)[8]) {
+GDN_DEV void stream8(const NormArgs& a, int64_t row, int c, bool live, float (&v)[8]) {
     using S = typename Act::storage;
-    load_up_to8<Act>(static_cast<const S*>(a.x) + row * a.x_stride + k, a.K - k, v);
+    Eight<Act>::template load<Act>(static_cast<const S*>(a.x) + row * a.x_stride, c, a.K, v);
     if (!a.residual) return;
     float r[8];
-    load_up_to8<Act>(static_cast<const S*>(a.residual) + row * a.r_stride + k, a.K - k, r);
+    Eight<Act>::template load<Act>(static_cast<const S*>(a.residual) + row * a.r_stride, c, a.K, r);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = Act::round(v[e] + r[e]);
-    if (live) store_up_to8<Act>(static_cast<S*>(a.sum) + row * a.s_stride + k, a.K - k, v);
+    if (live) Eight<Act>::store(static_cast<S*>(a.sum) + row * a.s_stride, c, a.K, v);
 }
 
 GDN_DEV double squares8(const float (&v)[8], double acc) {
@@ -120,74 +139,84 @@ GDN_DEV Factor factor_of(double sum, int K, float eps) {
     return f;
 }
 
-// y of the eight columns from k, stored as they are asked for. With codes,
-// sixteen consecutive lanes hold the columns of one scale.
+// y of eight columns, stored as it is asked for. With codes, sixteen consecutive
+// lanes hold the columns of one scale.
 template <class Act, bool kCodes>
-GDN_DEV void finish8(const NormArgs& a, int64_t row, int k, bool live, const float (&v)[8], const Factor& f) {
+GDN_DEV void finish8(const NormArgs& a, int64_t row, int c, bool live, const float (&v)[8], const Factor& f) {
+    using E = Eight<Act>;
     float w[8], y[8];
     if (a.w) {
-        load_up_to8<ActF32>(a.w + k, a.K - k, w);
+        E::template load<ActF32>(a.w, c, a.K, w);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = 1.f;
     }
     scaled8<Act>(v, f.r, f.r32, f.wild, w, y);
-    if (a.out && live) store_up_to8<Act>(static_cast<typename Act::storage*>(a.out) + row * a.K + k, a.K - k, y);
+    if (a.out && live) E::store(static_cast<typename Act::storage*>(a.out) + row * a.K, c, a.K, y);
     if constexpr (kCodes) {
-        if (k >= a.K)  // (w of one where there is none: a row of NaN has them here too)
+        const int k = E::first(c);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = 0.f;
+        for (int e = 0; e < 8; ++e)  // (behind the last column: zeros, also in a row of NaN)
+            if (k + e / E::kN * 64 >= a.K) y[e] = 0.f;
         uint32_t top = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(y[e]) & 0x7FFFFFFFu);
         const float s = scale_of(row16_max(top));
         divide_all(y, s);
         if (live && k < a.kb * kB) {
-            *reinterpret_cast<uint2*>(a.codes + row * (int64_t(a.kb) * kB) + k) =
-                make_uint2(codes4(y[0], y[1], y[2], y[3]), codes4(y[4], y[5], y[6], y[7]));
-            if ((threadIdx.x & 15) == 0) a.scales[int64_t(k / kB) * a.ldx + row] = s;
+            uint8_t* to = a.codes + row * (int64_t(a.kb) * kB) + k;
+            const uint32_t low = codes4(y[0], y[1], y[2], y[3]), high = codes4(y[4], y[5], y[6], y[7]);
+            if constexpr (E::kN == 8) {
+                *reinterpret_cast<uint2*>(to) = make_uint2(low, high);
+            } else {
+                *reinterpret_cast<uint32_t*>(to) = low;
+                *reinterpret_cast<uint32_t*>(to + 64) = high;
+            }
+            if (c % 16 == 0) a.scales[int64_t(c / 16) * a.ldx + row] = s;
         }
     }
 }
 
-// The sum over a row's kLanes threads, in all of them.
+// The sum over a row's threads, in all of them: kLanes of a wave, or (0) the whole
+// workgroup.
 template <int kLanes>
 GDN_DEV double row_sum(double v) {
-    if constexpr (kLanes <= kWave) {
+    if constexpr (kLanes != 0) {
         return group_sum<kLanes>(v);
     } else {
-        __shared__ double part[kLanes / kWave];
+        __shared__ double part[1024 / kWave];
+        const int waves = blockDim.x / kWave;
         v = group_sum<kWave>(v);
         if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = v;
         __syncthreads();
         v = part[0];
-#pragma unroll
-        for (int i = 1; i < kLanes / kWave; ++i) v += part[i];
+        for (int i = 1; i < waves; ++i) v += part[i];
         return v;
     }
 }
 
-// A row's columns stay in the registers of its kLanes threads, kVec times eight
-// in each: memory is read once and written once, and that is what bounds it.
+// A row's columns stay in the registers of its threads, kVec times eight in each:
+// memory is read once and written once, and that is what bounds it. kLanes threads
+// of a wave a row, or (0) a workgroup of as many waves as the row's columns take.
 template <class Act, int kLanes, int kVec, bool kCodes>
-__global__ __launch_bounds__(kLanes <= kWave ? 256 : kLanes) void rms_norm_kernel(NormArgs a) {
-    constexpr int kRows = kLanes <= kWave ? 256 / kLanes : 1;
+__global__ __launch_bounds__(kLanes ? 256 : 1024) void rms_norm_kernel(NormArgs a) {
+    const int lanes = kLanes ? kLanes : blockDim.x, per = kLanes ? 256 / kLanes : 1;
     const int64_t id = int64_t(blockIdx.y) * gridDim.x + blockIdx.x;
-    const int64_t mine = id * kRows + (kRows > 1 ? int(threadIdx.x) / kLanes : 0);
-    if (id * kRows >= a.rows) return;  // (the last row of the grid may be short)
+    const int64_t mine = id * per + (kLanes ? int(threadIdx.x) / lanes : 0);
+    if (id * per >= a.rows) return;  // (the last row of the grid may be short)
     const bool live = mine < a.rows;
     const int64_t row = live ? mine : a.rows - 1;
-    const int lane = threadIdx.x % kLanes;
+    const int lane = kLanes ? threadIdx.x % lanes : threadIdx.x;
     float v[kVec][8];
     double sum = 0.0;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-        stream8<Act>(a, row, (j * kLanes + lane) * 8, live, v[j]);
+        stream8<Act>(a, row, j * lanes + lane, live, v[j]);
         sum = squares8(v[j], sum);
     }
     const Factor f = factor_of(row_sum<kLanes>(sum), a.K, a.eps);
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) finish8<Act, kCodes>(a, row, (j * kLanes + lane) * 8, live, v[j], f);
+    for (int j = 0; j < kVec; ++j) finish8<Act, kCodes>(a, row, j * lanes + lane, live, v[j], f);
 }
 
 // Rows longer than registers hold: the stream is read again for the second pass
@@ -196,35 +225,33 @@ template <class Act, bool kCodes>
 __global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs a) {
     const int64_t row = int64_t(blockIdx.y) * gridDim.x + blockIdx.x;
     if (row >= a.rows) return;
-    const int end = (a.K + 8191) / 8192 * 8192;
+    const int end = (a.K + 8191) / 8192 * 1024;
     float v[8];
     double sum = 0.0;
-    for (int k = threadIdx.x * 8; k < end; k += 8192) {
-        stream8<Act>(a, row, k, true, v);
+    for (int c = threadIdx.x; c < end; c += 1024) {
+        stream8<Act>(a, row, c, true, v);
         sum = squares8(v, sum);
     }
-    const Factor f = factor_of(row_sum<1024>(sum), a.K, a.eps);
+    const Factor f = factor_of(row_sum<0>(sum), a.K, a.eps);
     NormArgs again = a;
     if (a.residual) again.x = a.sum, again.x_stride = a.s_stride, again.residual = nullptr;
-    for (int k = threadIdx.x * 8; k < end; k += 8192) {
-        stream8<Act>(again, row, k, true, v);
-        finish8<Act, kCodes>(a, row, k, true, v, f);
+    for (int c = threadIdx.x; c < end; c += 1024) {
+        stream8<Act>(again, row, c, true, v);
+        finish8<Act, kCodes>(a, row, c, true, v, f);
     }
 }
 
 template <class Act, bool kCodes>
 void launch_norm(const NormArgs& a, hipStream_t s) {
-    const auto rows = [&](auto kernel, int lanes) {
-        const int per = lanes <= kWave ? 256 / lanes : 1;
-        hipLaunchKernelGGL(kernel, rows_of_blocks((a.rows + per - 1) / per), dim3(lanes <= kWave ? 256 : lanes), 0, s, a);
+    const auto rows = [&](auto kernel, int per, int threads) {
+        hipLaunchKernelGGL(kernel, rows_of_blocks((a.rows + per - 1) / per), dim3(threads), 0, s, a);
     };
-    if (a.K <= 128) rows(rms_norm_kernel<Act, 16, 1, kCodes>, 16);
-    else if (a.K <= 512) rows(rms_norm_kernel<Act, 64, 1, kCodes>, 64);
-    else if (a.K <= 2048) rows(rms_norm_kernel<Act, 256, 1, kCodes>, 256);
-    else if (a.K <= 4096) rows(rms_norm_kernel<Act, 256, 2, kCodes>, 256);
-    else if (a.K <= 8192) rows(rms_norm_kernel<Act, 256, 4, kCodes>, 256);
-    else if (a.K <= 16384) rows(rms_norm_kernel<Act, 1024, 2, kCodes>, 1024);
-    else rows(rms_norm_long_kernel<Act, kCodes>, 1024);
+    const int waves = (a.K + 511) / 512;  // of eight columns a thread
+    if (a.K <= 128) rows(rms_norm_kernel<Act, 16, 1, kCodes>, 16, 256);
+    else if (a.K <= 512) rows(rms_norm_kernel<Act, 64, 1, kCodes>, 4, 256);
+    else if (waves <= 8) rows(rms_norm_kernel<Act, 0, 1, kCodes>, 1, waves * kWave);
+    else if (waves <= 32) rows(rms_norm_kernel<Act, 0, 2, kCodes>, 1, (waves + 1) / 2 * kWave);
+    else rows(rms_norm_long_kernel<Act, kCodes>, 1, 1024);
 }
 
 }  // namespace
