@@ -314,7 +314,7 @@ int gdn_gated_rmsnorm(const void *x, int x_dtype, const void *z, int z_dtype, in
  * decoder layer's norm (transformer.py:110-112).
  */
 int gdn_rms_norm(const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, void *sum,
-                 int64_t sum_stride, const float *w, float eps, int dtype, void *out, void *codes,
+                 int64_t sum_stride, const float *w, double eps, int dtype, void *out, void *codes,
                  float *scales, int scale_stride, int64_t rows, int K, void *stream);
 
 /*
@@ -614,8 +614,8 @@ int gdn_fp8_dequantize(const void *w, const float *scales, void *out, int out_dt
  *      element (16 c + l, 8 P s + 4 P h + P g + e) at [c][s][h][g][l][e]
  *   B: block j of adapter a, its columns rounded up to 64 and its ranks to 16, zeros in
  *      both, from element table[a][j].b: in 16 bits element (64 n + 32 p + 8 q + 4 u +
- *      v, 16 c + 8 g + e) at [n][c][p][u][g][q][v][e], in float32 (64 n + 16 p + 4 q +
- *      v, 16 c + 4 g + e) at [n][c][p][g][q][v][e]
+ *      v, 16 c + 8 g + e) at [c][n][p][u][g][q][v][e], in float32 (64 n + 16 p + 4 q +
+ *      v, 16 c + 4 g + e) at [c][n][p][g][q][v][e]
  *   table: (adapters, blocks) of {int64 b; int32 a_row; int32 rank; float c; int32
  *      t_col}: B's first element, A's first rank, the ranks (0: none), the scale, and
  *      the ranks rounded up of the blocks before it; rank_total: the most padded

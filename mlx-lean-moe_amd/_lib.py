@@ -27,6 +27,7 @@ _c_void_p = ctypes.c_void_p
 _c_int = ctypes.c_int
 _c_i64 = ctypes.c_int64
 _c_float = ctypes.c_float
+_c_double = ctypes.c_double
 _c_i64_p = ctypes.POINTER(ctypes.c_int64)
 
 # name -> (restype, argtypes); must match include/gdn.h
@@ -108,7 +109,7 @@ _SIGNATURES = {
     "gdn_fp8_matmul_codes": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p,
                                       _c_int, _c_int, _c_int, _c_void_p, _c_i64, _c_void_p]),
     "gdn_fp8_matmul_codes_workspace_size": (_c_i64, [_c_int, _c_int, _c_int, _c_int]),
-    "gdn_rms_norm": (_c_int, [_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_float, _c_int,
+    "gdn_rms_norm": (_c_int, [_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_double, _c_int,
                               _c_void_p, _c_void_p, _c_void_p, _c_int, _c_i64, _c_int, _c_void_p]),
     "gdn_add_low_rank": (_c_int, [_c_void_p, _c_i64, _c_int] + [_c_void_p] * 3 + [_c_int] * 4 + [_c_void_p] * 5
                          + [_c_int] * 4 + [_c_void_p, _c_i64, _c_void_p]),

@@ -25,7 +25,7 @@ constexpr int kDepth = 2;  // steps of K under way at once (3, 4 and 6: the same
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 struct AdapterBlock {
-    int64_t b;      // first element of B (width rounded up to 64, padded rank)
+    int64_t b;      // first element of B: 16 ranks after each other, all columns of each
     int32_t a_row;  // first rank in A
     int32_t rank;   // without padding to 16; 0: no adapter here
     float scale;
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_down_kernel(L
     const Tile tile = part_of(p, blockIdx.x);
     if (tile.count <= 0) return;
     const AdapterBlock* ab = p.table + int64_t(tile.adapter) * p.blocks;
-    const int total = ab[p.blocks - 1].t_col + pad16(ab[p.blocks - 1].rank), r0 = blockIdx.y * 16 * kNR;
+    const int total = min(ab[p.blocks - 1].t_col + pad16(ab[p.blocks - 1].rank), p.rank_total), r0 = blockIdx.y * 16 * kNR;
     if (r0 >= total) return;
     const S* xr[kRF];
 #pragma unroll
@@ -269,13 +269,13 @@ struct Columns {
             }
         }
     }
-    // B: for each 64 columns and 16 ranks four operands, of 512 bytes where both of
+    // B: for each 16 ranks and 64 columns four operands, of 512 bytes where both of
     // t's pieces meet the same
     static constexpr int kB = Act::code == GDN_F32 ? 1024 : 512;
     static GDN_DEV const uint8_t* operands(const LowRankArgs& p, const AdapterBlock& ab, int n0) {
-        return static_cast<const uint8_t*>(p.B) + ab.b * kY + int64_t(n0) * pad16(ab.rank) * kY +
-               (threadIdx.x & 63) * 16 % kB;
+        return static_cast<const uint8_t*>(p.B) + ab.b * kY + int64_t(n0 / 64) * (4 * kB) + (threadIdx.x & 63) * 16 % kB;
     }
+    static GDN_DEV int64_t next_ranks(int width) { return int64_t((width + 63) / 64) * (4 * kB); }
 };
 
 // out += t B^T for a part of a tile and 256 columns of one block, 64 a wave, 16
@@ -303,6 +303,7 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
     const AdapterBlock ab = p.table[int64_t(tile.adapter) * p.blocks + block];
     if (ab.rank <= 0) return;
     const int pieces = (ab.rank + 15) / 16, width = p.width[block];
+    if (ab.t_col < 0 || ab.t_col + 16 * pieces > p.rank_total) return;  // (not what a table of these sizes holds)
     const int n0 = (group - (block ? p.group_end[block - 1] : 0)) * kLowRankColumns + wave * 64;
     // the rows' numbers, all at first: a number fetched among the rows' output would
     // be there only after the output before it
@@ -313,10 +314,11 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
     const int n = n0 + Own::kCount * g;
     const bool whole = n0 + 64 <= width;  // (of the wave: one branch)
     const uint8_t* br = Own::operands(p, ab, n0);
+    const int64_t b_stride = Own::next_ranks(width);
     Operand<Act> b[kT][4];
     const auto load_b = [&](int i, Operand<Act> (&v)[4]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j].of(*reinterpret_cast<const uint4*>(br + (4 * i + j) * Own::kB));
+        for (int j = 0; j < 4; ++j) v[j].of(*reinterpret_cast<const uint4*>(br + i * b_stride + j * Own::kB));
     };
     if constexpr (kHeld != 0) {
 #pragma unroll
@@ -426,14 +428,14 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_whole_kernel(
     S* yr = lr < tile.count && uint32_t(row) < uint32_t(p.M)  // (null: no row)
                 ? static_cast<S*>(p.out[block]) + int64_t(row) * p.out_stride[block] + Own::kCount * g : nullptr;
     const uint8_t* br = Own::operands(p, ab, 0);
-    const int64_t b_stride = int64_t(pieces) * 4 * Own::kB / 64;  // bytes a column
+    const int64_t b_stride = Own::next_ranks(width);
     uint4 raw[kNR][4];
     const auto load_b = [&](int n) {
 #pragma unroll
         for (int i = 0; i < kNR; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                raw[i][j] = *reinterpret_cast<const uint4*>(br + n * b_stride + (4 * min(i, pieces - 1) + j) * Own::kB);
+                raw[i][j] = *reinterpret_cast<const uint4*>(br + min(i, pieces - 1) * b_stride + (n / 64 * 4 + j) * Own::kB);
     };
     const auto load_y = [&](int n, uint4 (&v)[Own::kY]) {
         if (yr && n + 64 <= width) Own::load(yr + n, v);  // (else read where it is written)

@@ -24,7 +24,7 @@ struct NormArgs {
     float* scales;
     int64_t x_stride, r_stride, s_stride, rows;
     int K, kb, ldx;
-    float eps;
+    double eps;
 };
 
 // kN consecutive values at any alignment of their own type (global memory takes
@@ -131,9 +131,9 @@ struct Factor {
     bool wild;
 };
 
-GDN_DEV Factor factor_of(double sum, int K, float eps) {
+GDN_DEV Factor factor_of(double sum, int K, double eps) {
     Factor f;
-    f.r = 1.0 / sqrt(sum / double(K) + double(eps));
+    f.r = 1.0 / sqrt(sum / double(K) + eps);
     f.r32 = float(f.r);
     f.wild = !(f.r32 > 0x1p-60f && f.r32 < 0x1p60f);
     return f;
@@ -260,7 +260,7 @@ void launch_norm(const NormArgs& a, hipStream_t s) {
 using namespace gdn;
 
 extern "C" int gdn_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, void* sum,
-                            int64_t sum_stride, const float* w, float eps, int dtype, void* out, void* codes,
+                            int64_t sum_stride, const float* w, double eps, int dtype, void* out, void* codes,
                             float* scales, int scale_stride, int64_t rows, int K, void* stream) {
     GDN_REQUIRE(rows >= 0 && K > 0 && K <= INT32_MAX - 8192, "gdn_rms_norm: bad sizes rows=%lld K=%d", (long long)rows, K);
     GDN_REQUIRE(valid_dtype(dtype), "gdn_rms_norm: bad dtype");

@@ -35,10 +35,6 @@ _LEAST_ROWS, _MOST_ROWS = 16, 256
 _TABLE = np.dtype([("b", "<i8"), ("a_row", "<i4"), ("rank", "<i4"), ("scale", "<f4"), ("t_col", "<i4")])
 
 
-def _pad16(n: int) -> int:
-    return -(-n // 16) * 16
-
-
 class LowRankAdapters:
     """The adapters of the projections that share one input, in the layout that
     :func:`add_low_rank` reads.
@@ -47,8 +43,9 @@ class LowRankAdapters:
     S adapters in order: ``(A (r, K), B (N, r), scale)``, or None where that adapter
     leaves the projection alone. Ranks may differ. A whole projection without
     adapters is None. All tensors are of one float dtype, which is that of the rows,
-    on one device. The adapters' values are copied: changing the tensors later
-    changes nothing here."""
+    on one device. The adapters' values are copied, on the current stream: changing
+    the tensors later changes nothing here, and a call on another stream has to wait
+    for that copy."""
 
     def __init__(self, projections) -> None:
         projections = list(projections)
@@ -85,50 +82,63 @@ class LowRankAdapters:
         if not 0 < self.hidden <= _MAX_HIDDEN:
             raise ValueError(f"adapters take rows of 1 to {_MAX_HIDDEN} values, got {self.hidden}")
         self.widths = tuple(widths)
-        step = 128 // self.dtype.itemsize
         table = np.zeros((self.count, len(projections)), dtype=_TABLE)
-        a_rows = b_size = 0
-        for a in range(self.count):
-            t_col = 0
-            for j, block in enumerate(projections):
-                pair = None if block is None else block[a]
-                rank = 0 if pair is None else pair[0].shape[0]
-                table[a, j] = (b_size, a_rows, rank, 0.0 if pair is None else float(pair[2]), t_col)
-                t_col += _pad16(rank)
-                a_rows += _pad16(rank)
-                b_size += -(-widths[j] // 64) * 64 * _pad16(rank)
-        self.rank_total = max(int(table[a, -1]["t_col"]) + _pad16(int(table[a, -1]["rank"])) for a in range(self.count))
-        self.rank_block = max(_pad16(int(r)) for r in table["rank"].reshape(-1))
-        if self.rank_total > _MAX_RANKS:
-            raise ValueError(f"an adapter's ranks add up to at most {_MAX_RANKS}, got {self.rank_total}")
-        per, steps = 16 // self.dtype.itemsize, -(-self.hidden // step)
-        # both in the order in which a wave's lanes take them (include/gdn.h)
-        self._A = torch.zeros((a_rows // 16, steps, 2, 4, 16, per), dtype=self.dtype, device=self.device)
-        self._B = torch.zeros(b_size, dtype=self.dtype, device=self.device)
+        a_rows, b_size = 0, 0
         for j, block in enumerate(projections):
             for a, pair in enumerate(block or ()):
-                if pair is None:
-                    continue
-                at, rank = table[a, j], pair[0].shape[0]
-                padded, columns = _pad16(rank), -(-widths[j] // 64) * 64
-                wide = torch.zeros((padded, steps * step), dtype=self.dtype, device=self.device)
-                wide[:rank, :self.hidden] = pair[0]
-                first = int(at["a_row"]) // 16
-                self._A[first:first + padded // 16] = wide.view(padded // 16, 16, steps, 2, 4, per).permute(0, 2, 3, 4, 1, 5)
-                wide = torch.zeros((columns, padded), dtype=self.dtype, device=self.device)
-                wide[:widths[j], :rank] = pair[1]
-                laid = self._B[int(at["b"]):int(at["b"]) + columns * padded]
-                if per == 8:
-                    laid.view(columns // 64, padded // 16, 2, 2, 2, 4, 4, 8).copy_(
-                        wide.view(columns // 64, 2, 4, 2, 4, padded // 16, 2, 8).permute(0, 5, 1, 3, 6, 2, 4, 7))
-                else:
-                    laid.view(columns // 64, padded // 16, 4, 4, 4, 4, 4).copy_(
-                        wide.view(columns // 64, 4, 4, 4, padded // 16, 4, 4).permute(0, 4, 1, 5, 2, 3, 6))
+                if pair is not None:
+                    table[a, j]["rank"], table[a, j]["scale"] = pair[0].shape[0], float(pair[2])
+        padded = -(-table["rank"] // 16) * 16
+        table["t_col"] = np.cumsum(padded, axis=1) - padded
+        table["a_row"] = (np.cumsum(padded) - padded.reshape(-1)).reshape(padded.shape)
+        columns = [-(-n // 64) * 64 for n in widths]
+        for j, n in enumerate(columns):  # B block by block
+            table["b"][:, j] = b_size + (np.cumsum(padded[:, j], dtype=np.int64) - padded[:, j]) * n
+            b_size += int(padded[:, j].sum()) * n
+        self.rank_total, self.rank_block = int(padded.sum(axis=1).max()), int(padded.max())
+        if self.rank_total > _MAX_RANKS or int(padded.sum()) >= 2 ** 31:
+            raise ValueError(f"an adapter's ranks add up to at most {_MAX_RANKS}, got {self.rank_total}")
+        self._A, self._B = self._laid_out(projections, padded, columns)
         self._index = self._A.get_device()
         self._c_widths = (ctypes.c_int * len(widths))(*widths)
         self._workspaces: dict[tuple[int, int], int] = {}
         self._table = torch.from_numpy(table.reshape(-1).view(np.uint8)).to(self.device)
 
+    def _laid_out(self, projections, padded, columns) -> tuple[torch.Tensor, torch.Tensor]:
+        """A of all adapters and B of all, in the order in which a wave's lanes take them
+        (include/gdn.h), from a few operations whatever the number of adapters."""
+
+        per = 16 // self.dtype.itemsize
+        steps = -(-self.hidden // (8 * per))
+        no_ranks = torch.zeros((15, self.hidden), dtype=self.dtype, device=self.device)
+        no_columns = torch.zeros((max(self.widths), 15), dtype=self.dtype, device=self.device)
+        parts = []
+        for a in range(self.count):
+            for j, block in enumerate(projections):
+                if block is not None and block[a] is not None:
+                    A = block[a][0]
+                    parts.append(A)
+                    if padded[a, j] > A.shape[0]:
+                        parts.append(no_ranks[:padded[a, j] - A.shape[0]])
+        wide = torch.nn.functional.pad(torch.cat(parts), (0, steps * 8 * per - self.hidden))
+        laid_a = wide.view(-1, 16, steps, 2, 4, per).permute(0, 2, 3, 4, 1, 5).contiguous()
+        laid_b = []
+        for j, block in enumerate(projections):
+            if not self.widths[j]:
+                continue
+            parts = []
+            for a, pair in enumerate(block):
+                if pair is not None:
+                    parts.append(pair[1])
+                    if padded[a, j] > pair[1].shape[1]:
+                        parts.append(no_columns[:self.widths[j], :padded[a, j] - pair[1].shape[1]])
+            wide = torch.nn.functional.pad(torch.cat(parts, dim=1), (0, 0, 0, columns[j] - self.widths[j]))
+            if per == 8:
+                wide = wide.view(columns[j] // 64, 2, 4, 2, 4, -1, 2, 8).permute(5, 0, 1, 3, 6, 2, 4, 7)
+            else:
+                wide = wide.view(columns[j] // 64, 4, 4, 4, -1, 4, 4).permute(4, 0, 1, 5, 2, 3, 6)
+            laid_b.append(wide.reshape(-1))
+        return laid_a, laid_b[0] if len(laid_b) == 1 else torch.cat(laid_b)
 
     def _workspace(self, tiles: int, tile_rows: int) -> int:
         nbytes = self._workspaces.get((tiles, tile_rows))
@@ -147,7 +157,8 @@ class AdapterRows:
     ``index`` is a host sequence or a tensor of whole numbers (read back to the host
     if it is on the GPU). ``distinct``: room for batches of that many different
     adapters, for :meth:`assign`; without it there is room for as many tiles as
-    ``index`` takes."""
+    ``index`` takes. Made outside of a graph's capture; its copy on the device
+    belongs to the stream it was made on until that is done."""
 
     def __init__(self, index, count: int, device: torch.device | str = "cuda", *, distinct: int | None = None) -> None:
         if count < 1:
@@ -233,7 +244,8 @@ def add_low_rank(outs, x: torch.Tensor, adapters: LowRankAdapters, rows: Adapter
     (None where it has no adapters), in x's dtype at any row stride, e.g. column
     slices of a stacked output. Sums are float32; a result is rounded once more to
     its dtype. ``scale x A^T`` is kept to 16 bits for 16-bit dtypes, in full for
-    float32. Rows without an adapter are left as they are."""
+    float32. Rows without an adapter are left as they are, and a row's result does not
+    depend on the rows beside it."""
 
     # decode steps are host-bound, hence the integer comparisons and the quick look
     # at the arrays' ends in front of _overlap

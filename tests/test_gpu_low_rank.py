@@ -201,20 +201,33 @@ def test_values_that_are_not_finite_stay_in_their_row(gpu, act):
     assert ((got.double() - ref).abs() <= tol).all()
 
 
-def test_results_do_not_depend_on_the_batch(gpu):
-    """A row's bits are the same whichever rows it comes with, as long as the sums
-    are split alike; and from call to call."""
-    m = _Maker(gpu, "bf16")
-    adapters = gdn.LowRankAdapters([_pairs(m, [16] * 4, 2048, 600)])
-    x, y = m(512, 2048), m(512, 600)
-    index = _index(512, 4)
+@pytest.mark.parametrize("act", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("r", [16, 64])
+def test_results_do_not_depend_on_the_batch(gpu, act, r):
+    """A row's bits are the same from call to call and whichever rows and projections it
+    comes with: one launch, two, and every cut of both add in the same order."""
+    m = _Maker(gpu, act)
+    blocks = [_pairs(m, [r, 7, r, r], 1100, N) for N in (600, 70)]
+    adapters, alone = gdn.LowRankAdapters(blocks), gdn.LowRankAdapters(blocks[1:])
+    M = 9000
+    x, ys, index = m(M, 1100), [m(M, 600), m(M, 70)], _index(M, 4, without=0.1)
     rows = gdn.AdapterRows(index, 4, device=gpu)
-    first = gdn.add_low_rank(y.clone(), x, adapters, rows)
-    for _ in range(3):
-        assert torch.equal(gdn.add_low_rank(y.clone(), x, adapters, rows), first)
-    order = torch.randperm(512, generator=torch.Generator().manual_seed(1))
-    shuffled = gdn.AdapterRows(torch.tensor(index)[order], 4, device=gpu)
-    assert torch.equal(gdn.add_low_rank(y[order], x[order], adapters, shuffled), first[order])
+    first = gdn.add_low_rank([y.clone() for y in ys], x, adapters, rows)
+    again = gdn.add_low_rank([y.clone() for y in ys], x, adapters, rows)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    order = torch.randperm(M, generator=torch.Generator().manual_seed(1)).to(gpu)
+    for at in (order[:1], order[:2], order[:17], order[:300], order[:2000], order):
+        part = gdn.AdapterRows([index[i] for i in at.tolist()], 4, device=gpu)
+        got = gdn.add_low_rank([y[at] for y in ys], x[at], adapters, part)
+        assert all(torch.equal(g, f[at]) for g, f in zip(got, first))
+        assert torch.equal(gdn.add_low_rank(ys[1][at], x[at], alone, part), first[1][at])
+
+
+@pytest.mark.parametrize("act", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("ranks", [[16], [30], [64, 1], [100]])
+def test_prompts_of_many_rows(gpu, act, ranks):
+    """Two launches, with the first product's larger workgroups."""
+    _run(gpu, act, [0] * 8300 + [-1] * 5 + [len(ranks) - 1] * 70, [ranks], 104, [70])
 
 
 def test_numbers_from_tensors_and_runs(gpu):

@@ -12,6 +12,7 @@ import pytest
 import torch
 
 import mlx_lean_moe_amd as gdn
+from mlx_lean_moe_amd import quant
 
 pytestmark = pytest.mark.gpu
 
@@ -115,6 +116,20 @@ def test_products_of_codes_are_those_of_the_rows(gpu, act, M, N, K):
                        gdn.quantized_linear(y, W, FP8, residual=res))
 
 
+@pytest.mark.parametrize("M", [1, 40, 2100])
+def test_codes_times_stacked_projections(gpu, M):
+    """The blocks that quantized_linear_split gives of rows and of their codes."""
+    sizes, K = [384, 128, 70], 272
+    g = torch.Generator(device=gpu)
+    g.manual_seed(3)
+    W = gdn.LinearWeights({"weight": (torch.randn(582, K, generator=g, device=gpu) * 60).clamp(-440, 440).to(torch.float8_e4m3fn),
+                           "scales": torch.rand(5, 3, generator=g, device=gpu)}, FP8)
+    x = _x(gpu, M, K)
+    q = gdn.rms_norm(x, None, 1e-6, quantize=True)
+    for got, want in zip(quant.quantized_linear_split(q, W, sizes), quant.quantized_linear_split(gdn.rms_norm(x, None, 1e-6), W, sizes)):
+        assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("act", ["bf16", "f16", "f32"])
 def test_values_that_are_not_ordinary(gpu, act):
     K = 272
@@ -187,7 +202,7 @@ def test_strides_alignment_and_ranks(gpu, act, K):
         one = gdn.rms_norm(x[2], w, 1e-6, quantize=True)
         assert one.codes.shape == (K,) and torch.equal(one.codes.float(), flat.codes.float()[2])
         none = gdn.rms_norm(x[:0], w, 1e-6, quantize=True)
-        assert none.codes.shape == (0, K)
+        assert none.codes.shape == (0, K) and none.scales.shape == (0, -(-K // 128)) and none.dequantize().shape == (0, K)
         W = {"weight": torch.ones(4, K, device=gpu).to(torch.float8_e4m3fn), "scales": torch.ones(1, -(-K // 128), device=gpu)}
         assert gdn.quantized_linear(none, W, FP8).shape == (0, 4)
         assert gdn.quantized_linear(one, W, FP8).shape == (4,)
