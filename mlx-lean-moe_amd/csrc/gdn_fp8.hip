@@ -5,7 +5,9 @@
 //   y[m, n] = sum_b s[m, b] sw[n / 128, b] sum_{k in b} q[m, k] w[n, k],
 // the inner sums on the 8-bit matrix cores (one 16x16x128 product per block, so
 // scales meet float32 sums only), the outer one in float32. float32 results take
-// the codes widened to bfloat16 instead (at mfma_widened).
+// the codes widened to bfloat16 instead (at mfma_widened). Rows may come in such codes
+// already, from the norm in front of the product (gdn_fp8_matmul_codes), which saves
+// the launch that makes them: 2048 -> 12352, 64 rows 11.6 us and 8.1, 4096 118 and 110.
 #include <type_traits>
 
 #include "gdn_common.h"
@@ -322,7 +324,8 @@ __global__ __launch_bounds__(64 * kWN * kWM) void fp8_tile_kernel(Fp8Args a) {
     }
 }
 
-// Up to 16 rows of x, in one launch: each workgroup quantizes them itself into
+// Up to 16 rows of x, in one launch: each workgroup quantizes them itself (or copies
+// their codes) into
 // LDS (codes and scales, K whole), while its first blocks of W are on their
 // way, then its 16 waves take kNs x 16 rows of W and every (16 / kNs)-th block
 // of K each, straight from memory into the left operand, and add their sums in

@@ -9,8 +9,12 @@
 // in two such pieces as well (8 + 3 bits: all of it), since t need not fit float16.
 //
 // A, B and t lie in memory in the order in which a wave's lanes take them: a load of
-// 16 bytes a lane is 1 KB in one piece (rows of them instead, 32 to 128 bytes a row
-// and load, cost the second product a third of its time at 64 ranks).
+// 16 bytes a lane is 1 KB in one piece (8192 rows, 2048 -> 4096, rank 64: rows of them
+// instead, 32 to 128 bytes a row and load, 25.0 + 50.3 us, so 18.9 + 39.4).
+//
+// Every kernel adds in the same order: K's steps w, w + 8, ... in wave w, the waves
+// in turn, then 16 ranks after each other. So a row's result has the same bits
+// whichever rows and projections it comes with.
 #include <type_traits>
 
 #include "gdn_common.h"
@@ -132,6 +136,11 @@ GDN_DEV void store_t(uint8_t* to, f32x4 v, int rank, float scale) {
 // t for kRF x 16 rows of a tile and kNR x 16 of its adapter's ranks. Ranks are the
 // left operand, so a lane ends with four ranks of one row. The waves share out K and
 // add their sums in LDS; kDepth steps' loads are under way at once.
+//
+// One round of workgroups, bound by its chain of waits (tile, row numbers, x, LDS) and
+// by x's way from memory: 8192 rows of 2048, rank 64, 14.4 us (33.5 MB), rank 16 10.9;
+// 9.0 at 2112 values a row, which do not lie a power of two apart (a part of K in one
+// piece a wave, to read at eight places far apart, took as long in all).
 template <class Act, int kRF, int kNR>
 __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_down_kernel(LowRankArgs p) {
     using S = typename Act::storage;
@@ -281,11 +290,16 @@ struct Columns {
 // out += t B^T for a part of a tile and 256 columns of one block, 64 a wave, 16
 // rows at a time. B is the left operand and its rows are dealt out so that a lane
 // ends with 16-byte pieces of one row's output, the four lanes of a row beside each
-// other in each piece. The 32 values of k of a 16-bit
-// product are 16 ranks of t's high piece and the same of its low one, B the same for
-// both. A wave keeps its part of B (kHeld pieces of 16 ranks; 0: more ranks than
-// that, read again for each 16 rows) and streams the rows: the next ones' output and
-// t are under way while these are multiplied and stored.
+// other in each piece (32 bytes a lane instead: 45 us for 34 at rank 16). The 32 values
+// of k of a 16-bit product are 16 ranks of t's high piece and the same of its low one, B
+// the same for both. A wave keeps its part of B (kHeld pieces of 16 ranks; 0: more ranks
+// than that, read again for each 16 rows) and streams the rows: the next ones' output
+// and t are under way while these are multiplied and stored.
+//
+// Bound by the output's way through memory and back: 8192 x 4096, rank 16 about 30 us
+// (134 MB, 4.5 TB/s), rank 64 40; 4096 x 12288, rank up to 32, 43 (201 MB, 4.7 TB/s).
+// At rank 64 without t and the products 28 of 36 us (from a graph): t is twice the
+// output's bytes at the vector caches, and 160 registers leave three waves a SIMD.
 template <class Act, int kHeld>
 __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRankArgs p) {
     using S = typename Act::storage;
@@ -382,7 +396,8 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
 // first of its output and B are on their way. Then each wave takes every eighth 64
 // columns, t from LDS; the next ones' output is under way while these are multiplied,
 // their B while these are stored. Every workgroup of a block reads the same rows of
-// A: low_rank_plan says where that is too much.
+// A: low_rank_plan says where that is too much. Bound by its chain of waits: 1 row,
+// 2048 -> 8192 | 4096, rank 16, 5.3 us; 64 rows of 27 adapters 9.5 (17.6 MB).
 template <class Act, int kNR>
 __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_whole_kernel(LowRankArgs p) {
     using S = typename Act::storage;

@@ -198,6 +198,8 @@ GDN_DEV double row_sum(double v) {
 // A row's columns stay in the registers of its threads, kVec times eight in each:
 // memory is read once and written once, and that is what bounds it. kLanes threads
 // of a wave a row, or (0) a workgroup of as many waves as the row's columns take.
+// Measured, with the residual, bf16: 4096 rows of 2048 14.8 us (67 MB, 4.5 TB/s; a
+// large copy 5.1), 8192 to codes 25.4 (118 MB); 1 row 2.9, a launch and its waits.
 template <class Act, int kLanes, int kVec, bool kCodes>
 __global__ __launch_bounds__(kLanes ? 256 : 1024) void rms_norm_kernel(NormArgs a) {
     const int lanes = kLanes ? kLanes : blockDim.x, per = kLanes ? 256 / kLanes : 1;
@@ -246,6 +248,10 @@ void launch_norm(const NormArgs& a, hipStream_t s) {
     const auto rows = [&](auto kernel, int per, int threads) {
         hipLaunchKernelGGL(kernel, rows_of_blocks((a.rows + per - 1) / per), dim3(threads), 0, s, a);
     };
+    // One eight a thread up to 4096 columns, two beyond (us, one and two: 1 x 4096 to
+    // codes 4.0 and 4.9, 4096 x 4096 25.7 and 26.2, to codes without a residual 21.0 and
+    // 19.9; 8 x 8192 4.8 and 5.4, 1000 x 5120 to codes 10.4 and 9.3, 2048 x 8192 28.6 and
+    // 27.4). Rows of up to 512 columns share a workgroup.
     const int waves = (a.K + 511) / 512;  // of eight columns a thread
     if (a.K <= 128) rows(rms_norm_kernel<Act, 16, 1, kCodes>, 16, 256);
     else if (a.K <= 512) rows(rms_norm_kernel<Act, 64, 1, kCodes>, 4, 256);

@@ -407,8 +407,8 @@ class Qwen3_5LinearAttention:
         scheme (linear_attention.py:95-101).
 
         With ``input_norm_weight (hidden,)`` the layer takes the decoder layer's
-        stream and norms it itself (:func:`rms_norm` with ``rms_norm_eps``, in
-        e4m3 codes where fp8_block projections follow): ``layer(x, cache,
+        stream and norms it itself (:func:`rms_norm` with ``rms_norm_eps``, several
+        rows in e4m3 codes where fp8_block projections follow): ``layer(x, cache,
         residual=x)`` is then ``x + attention(rms_norm(x))``
         (transformer.py:110-112). Without, x is normed already, and may be
         :class:`QuantizedRows`."""
@@ -524,8 +524,11 @@ class Qwen3_5LinearAttention:
         if self.input_norm_weight is not None:
             if isinstance(rows, QuantizedRows):
                 raise ValueError("the layer norms its input itself (input_norm_weight) and takes plain rows")
-            rows = rms_norm(rows, self.input_norm_weight, self.rms_norm_eps, quantize=self._any_codes,
-                            keep_rows=self._any_codes and (adapt or not self._all_codes))
+            # (the product quantizes a single row itself: 2048 -> 12352, norm and product, 9.2 us
+            # so and 9.5 by codes; 16 rows 13.8 and 12.8, 64 15.0 and 13.3, 4096 129 and 124)
+            codes = self._any_codes and rows.shape[0] > 1
+            rows = rms_norm(rows, self.input_norm_weight, self.rms_norm_eps, quantize=codes,
+                            keep_rows=codes and (adapt or not self._all_codes))
         qkv, z, a, b = self._projected(rows)
         if adapt:
             add_low_rank([qkv, z.view(z.shape[0], self.linear.value_dim), a, b], rows, self._in_adapters, adapter_rows)
