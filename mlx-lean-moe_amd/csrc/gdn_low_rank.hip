@@ -4,9 +4,10 @@
 // The rows come sorted by adapter and cut into tiles of one adapter (a plan that
 // the caller keeps for all projections of a step), so each product is a plain
 // one on the matrix cores, with float32 sums. The first leaves t as the second's
-// operand: float32, or (16-bit adapters) two bfloat16 pieces, the upper 8 bits of
-// the float32 value and what they leave, which is 16 bits of it. float16 B is taken
-// in two such pieces as well (8 + 3 bits: all of it), since t need not fit float16.
+// operand: float32, or (16-bit adapters) two pieces of their type, the second what the
+// first leaves: 16 bits of t in bfloat16, 22 in float16, which t need not fit: there
+// 16 ranks of a row come times a power of two of their own, and their product goes
+// back by it.
 //
 // A, B and t lie in memory in the order in which a wave's lanes take them: a load of
 // 16 bytes a lane is 1 KB in one piece (8192 rows, 2048 -> 4096, rank 64: rows of them
@@ -40,7 +41,7 @@ struct LowRankArgs {
     const void *x, *A, *B;
     const AdapterBlock* table;     // (S, blocks)
     const int32_t *order, *tiles;  // rows by adapter; {adapter, first place in order, rows} a tile
-    uint8_t* t;                    // (16 rows of a tile, 16 ranks) after each other: 1 KB each
+    uint8_t* t;                    // (16 rows of a tile, 16 ranks) after each other, kBlockOfT bytes each
     void* out[kLowRankBlocks];
     int64_t out_stride[kLowRankBlocks];
     int width[kLowRankBlocks], group_end[kLowRankBlocks];
@@ -107,31 +108,72 @@ GDN_DEV uint4 piece_of(const S* p, int count) {
 
 // The upper 8 bits of a float32 value as bfloat16 (cut off: rounded up, the largest
 // would overflow), and what they leave, rounded; what is not finite has no rest.
-GDN_DEV void two_pieces(float v, uint16_t& high, uint16_t& low) {
+GDN_DEV void two_bf16(float v, uint16_t& high, uint16_t& low) {
     high = v != v ? 0x7FC0 : uint16_t(__float_as_uint(v) >> 16);
     low = (high & 0x7F80) == 0x7F80 ? 0 : f32_to_bf16_bits(v - bf16_bits_to_f32(high));
 }
 
+GDN_DEV void two_f16(float v, uint16_t& high, uint16_t& low) {
+    high = f32_to_f16_bits(v);
+    low = (high & 0x7C00) == 0x7C00 ? 0 : f32_to_f16_bits(v - f16_bits_to_f32(high));
+}
+
+// Bytes of t for 16 rows and 16 ranks: 16 a lane of the second product, and in float16
+// a float a row.
+template <class Act>
+constexpr int kBlockOfT = Act::code == GDN_F16 ? 1024 + 64 : 1024;
+
 // 16 rows' sums over 16 ranks, four ranks of a row a lane, as the second product's
-// operand: 1 KB, of which that product's lanes take 16 bytes each. Of the ranks the
-// first `rank` exist (what is padding is 0, also 0 times what is not finite).
+// operand. Of the ranks the first `rank` exist (what is padding is 0, also 0 times what
+// is not finite). float16: a row's largest is brought to between 2^13 and 2^14, so that
+// both pieces are normal numbers of the type.
 template <class Act>
 GDN_DEV void store_t(uint8_t* to, f32x4 v, int rank, float scale) {
     const int g = (threadIdx.x & 63) >> 4, lr = threadIdx.x & 15;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = 4 * g + e < rank ? v[e] * scale : 0.f;
-    to += lr * 16;
     if constexpr (Act::code == GDN_F32) {
-        *reinterpret_cast<f32x4*>(to + 256 * g) = v;
+        *reinterpret_cast<f32x4*>(to + lr * 16 + 256 * g) = v;
     } else {  // quarters of 1 KB: ranks 0 to 7 and 8 to 15 high, then low
         uint16_t high[4], low[4];
+        if constexpr (Act::code == GDN_F16) {
+            float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            const int up = int(__float_as_uint(most) >> 23) - 127;  // 2^up <= most < 2^(up + 1)
+            const bool usable = most > 0x1p-100f && most < 0x1p100f;
+            const float fit = usable ? __uint_as_float(uint32_t(127 + 13 - up) << 23) : 1.f;
+            if (g == 0) *reinterpret_cast<float*>(to + 1024 + lr * 4) = usable ? __uint_as_float(uint32_t(127 - 13 + up) << 23) : 1.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) two_pieces(v[e], high[e], low[e]);
-        to += g / 2 * 256 + g % 2 * 8;
+            for (int e = 0; e < 4; ++e) two_f16(v[e] * fit, high[e], low[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) two_bf16(v[e], high[e], low[e]);
+        }
+        to += lr * 16 + g / 2 * 256 + g % 2 * 8;
         __builtin_memcpy(__builtin_assume_aligned(to, 8), high, 8);
         __builtin_memcpy(__builtin_assume_aligned(to + 512, 8), low, 8);
     }
 }
+
+// t of 16 rows and 16 ranks, as a lane of the second product has it.
+template <class Act>
+struct Ranks {
+    uint4 v;
+    float back;
+    GDN_DEV void load(const uint8_t* block) {
+        v = *reinterpret_cast<const uint4*>(block + (threadIdx.x & 63) * 16);
+        if constexpr (Act::code == GDN_F16) back = *reinterpret_cast<const float*>(block + 1024 + (threadIdx.x & 15) * 4);
+    }
+    // sum + B t for one operand of B
+    GDN_DEV f32x4 add(const uint4& b, f32x4 sum) const {
+        if constexpr (Act::code != GDN_F16) return mfma_pieces<Act>(b, v, sum);
+        const f32x4 p = mfma_pieces<Act>(b, v, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(p[e], back, sum[e]);
+        return sum;
+    }
+};
 
 // t for kRF x 16 rows of a tile and kNR x 16 of its adapter's ranks. Ranks are the
 // left operand, so a lane ends with four ranks of one row. The waves share out K and
@@ -223,31 +265,9 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_down_kernel(L
     for (int w = 1; w < kLowRankDownWaves; ++w) v += sums[w][wave][lane];
     int block = 0;
     while (r >= ab[block].t_col + pad16(ab[block].rank)) ++block;
-    store_t<Act>(p.t + ((tile.block + rows / 16) * (p.rank_total / 16) + r / 16) * 1024, v,
+    store_t<Act>(p.t + ((tile.block + rows / 16) * (p.rank_total / 16) + r / 16) * kBlockOfT<Act>, v,
                  ab[block].t_col + ab[block].rank - r, ab[block].scale);
 }
-
-// One piece of B as the second product's operand.
-template <class Act>
-struct Operand {
-    uint4 v;
-    GDN_DEV void of(const uint4& raw) { v = raw; }
-    GDN_DEV f32x4 times(const uint4& t, f32x4 c) const { return mfma_pieces<Act>(v, t, c); }
-};
-
-template <>
-struct Operand<ActF16> {
-    uint4 high, low;
-    GDN_DEV void of(const uint4& raw) {
-        uint16_t e[8], h[8], l[8];
-        __builtin_memcpy(e, &raw, 16);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) two_pieces(f16_bits_to_f32(e[i]), h[i], l[i]);
-        __builtin_memcpy(&high, h, 16);
-        __builtin_memcpy(&low, l, 16);
-    }
-    GDN_DEV f32x4 times(const uint4& t, f32x4 c) const { return mfma_bf16(low, t, mfma_bf16(high, t, c)); }
-};
 
 // A wave's 64 columns: the lane's 16 values of a row in 16-byte pieces, the four lanes
 // of a row beside each other in each. acc[j] holds four columns from quad_at(g, j).
@@ -329,10 +349,10 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
     const bool whole = n0 + 64 <= width;  // (of the wave: one branch)
     const uint8_t* br = Own::operands(p, ab, n0);
     const int64_t b_stride = Own::next_ranks(width);
-    Operand<Act> b[kT][4];
-    const auto load_b = [&](int i, Operand<Act> (&v)[4]) {
+    uint4 b[kT][4];
+    const auto load_b = [&](int i, uint4 (&v)[4]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j].of(*reinterpret_cast<const uint4*>(br + i * b_stride + j * Own::kB));
+        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(br + i * b_stride + j * Own::kB);
     };
     if constexpr (kHeld != 0) {
 #pragma unroll
@@ -341,13 +361,15 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
     }
     S* out = static_cast<S*>(p.out[block]) + n;
     const int64_t stride = p.out_stride[block];
-    const int64_t t_stride = int64_t(p.rank_total / 16) * 1024;
-    const uint8_t* t = p.t + tile.block * t_stride + ab.t_col / 16 * 1024 + lane * 16;
+    constexpr int kBlock = kBlockOfT<Act>;
+    const int64_t t_stride = int64_t(p.rank_total / 16) * kBlock;
+    const uint8_t* t = p.t + tile.block * t_stride + int64_t(ab.t_col / 16) * kBlock;
     const int steps = (tile.count + 15) / 16;
 
     struct Rows {
         S* y;  // null: no row
-        uint4 yv[Own::kY], tv[kT];
+        uint4 yv[Own::kY];
+        Ranks<Act> tv[kT];
     };
     const auto fetch = [&](Rows& r, int s) {
         const int row = rows[16 * s + lr];
@@ -356,7 +378,7 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
         if constexpr (kHeld != 0) {
 #pragma unroll
             for (int i = 0; i < kHeld; ++i)
-                if (i < pieces) r.tv[i] = *reinterpret_cast<const uint4*>(t + s * t_stride + 1024 * i);
+                if (i < pieces) r.tv[i].load(t + s * t_stride + kBlock * i);
         }
     };
     const auto finish = [&](Rows& r, int s) {
@@ -368,14 +390,15 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
             for (int i = 0; i < kHeld; ++i)
                 if (i < pieces) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[j] = b[i][j].times(r.tv[i], acc[j]);
+                    for (int j = 0; j < 4; ++j) acc[j] = r.tv[i].add(b[i][j], acc[j]);
                 }
         } else {
             for (int i = 0; i < pieces; ++i) {
                 load_b(i, b[0]);
-                const uint4 v = *reinterpret_cast<const uint4*>(t + s * t_stride + 1024 * i);
+                Ranks<Act> v;
+                v.load(t + s * t_stride + int64_t(kBlock) * i);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[j] = b[0][j].times(v, acc[j]);
+                for (int j = 0; j < 4; ++j) acc[j] = v.add(b[0][j], acc[j]);
             }
         }
         if (r.y) Own::add(r.y, r.yv, acc, whole, width - n);
@@ -404,7 +427,7 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_whole_kernel(
     using Own = Columns<Act>;
     constexpr int kStep = 128 / sizeof(S), kPiece = 16 / sizeof(S);
     __shared__ f32x4 sums[kLowRankDownWaves][kNR][64];
-    __shared__ __attribute__((aligned(16))) uint8_t t[kNR * 1024];
+    __shared__ __attribute__((aligned(16))) uint8_t t[kNR * kBlockOfT<Act>];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, lr = lane & 15;
     const int groups = p.group_end[p.blocks - 1], group = blockIdx.x % groups;
@@ -487,7 +510,7 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_whole_kernel(
         f32x4 v = sums[0][wave][lane];
 #pragma unroll
         for (int w = 1; w < kLowRankDownWaves; ++w) v += sums[w][wave][lane];
-        store_t<Act>(t + wave * 1024, v, ab.rank - wave * 16, ab.scale);
+        store_t<Act>(t + wave * kBlockOfT<Act>, v, ab.rank - wave * 16, ab.scale);
     }
     __syncthreads();
 
@@ -500,13 +523,10 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_whole_kernel(
 #pragma unroll
         for (int c = 0; c < kNR; ++c)
             if (c < pieces) {
-                const uint4 v = *reinterpret_cast<const uint4*>(t + c * 1024 + lane * 16);
+                Ranks<Act> v;
+                v.load(t + c * kBlockOfT<Act>);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    Operand<Act> b;
-                    b.of(raw[c][j]);
-                    sum[j] = b.times(v, sum[j]);
-                }
+                for (int j = 0; j < 4; ++j) sum[j] = v.add(raw[c][j], sum[j]);
             }
         if (n2 < n_end) load_b(n2);
         if (yr) Own::add(yr + n, now, sum, n + 64 <= width, width - n - Own::kCount * g);
@@ -530,6 +550,10 @@ using namespace gdn;
 
 namespace {
 
+int64_t t_bytes(int dtype, int tiles, int tile_rows, int rank_total) {
+    return int64_t(tiles) * (tile_rows / 16) * (rank_total / 16) * (dtype == GDN_F16 ? kBlockOfT<ActF16> : 1024);
+}
+
 LowRankPlan plan_of(int dtype, int rank_total, int rank_block, const int* widths, int blocks, int tiles, int tile_rows, int K) {
     return low_rank_plan(tiles, tile_rows, rank_total, rank_block, K, dtype_size(dtype), widths, blocks);
 }
@@ -542,7 +566,7 @@ extern "C" int64_t gdn_add_low_rank_workspace_size(int dtype, int blocks, int ra
         blocks > kLowRankBlocks || !widths)
         return 0;
     const LowRankPlan plan = plan_of(dtype, rank_total, rank_block, widths, blocks, tile_count, tile_rows, K);
-    return plan.columns ? 0 : int64_t(tile_count) * tile_rows * rank_total * 4;
+    return plan.columns ? 0 : t_bytes(dtype, tile_count, tile_rows, rank_total);
 }
 
 extern "C" int gdn_add_low_rank(const void* x, int64_t x_stride, int dtype, const void* A, const void* B, const void* table,
@@ -574,7 +598,7 @@ extern "C" int gdn_add_low_rank(const void* x, int64_t x_stride, int dtype, cons
     const int64_t groups = column_groups(widths, blocks, kLowRankColumns, p.group_end);
     if (groups == 0) return 0;
     const LowRankPlan plan = plan_of(dtype, rank_total, rank_block, widths, blocks, tile_count, tile_rows, K);
-    const int64_t need = plan.columns ? 0 : int64_t(tile_count) * tile_rows * rank_total * 4;
+    const int64_t need = plan.columns ? 0 : t_bytes(dtype, tile_count, tile_rows, rank_total);
     GDN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "gdn_add_low_rank: workspace of %lld bytes, %lld needed",
                 (long long)workspace_bytes, (long long)need);
     const int64_t down_parts = tile_rows / plan.down_rows, up_parts = tile_rows / plan.up_rows;

@@ -2,10 +2,12 @@
 
 The inner sum t = x A^T is float32: K products, each sum off by at most half a last
 place, twice over for the matrix cores' own order. 16-bit adapters then take c t in two
-bfloat16 pieces: the upper 8 bits leave less than 2^-7 of the power of two below c t,
-and rounding that to 8 bits is off by at most 2^-16 of it. The outer sum is float32
-over the ranks (twice as many terms for the pieces, twice again for float16 B's), and
-the result is rounded once."""
+pieces of their type. bfloat16: the upper 8 bits leave less than 2^-7 of the power of
+two below c t, and rounding that to 8 bits is off by at most 2^-16 of it. float16: 11
+bits and 11 of what they leave, 2^-22, where the row's largest of 16 lies above 2^13 and
+the pieces' smallest step is 2^-24 (2^-25 off): 2^-38 of that largest. The outer sum is
+float32 over the ranks (twice as many terms for the pieces), and the result is rounded
+once."""
 
 from __future__ import annotations
 
@@ -19,7 +21,7 @@ pytestmark = pytest.mark.gpu
 
 DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 U = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11, "f32": 2.0 ** -24}
-PIECES = {"bf16": 2.0 ** -16, "f16": 2.0 ** -16, "f32": 0.0}
+PIECES = {"bf16": 2.0 ** -16, "f16": 2.0 ** -21, "f32": 0.0}
 
 
 class _Maker:
@@ -51,6 +53,8 @@ def _reference(y, x, block, index):
         K, r = A.shape[1], A.shape[0]
         ref[rows] += c * (t @ B.T.contiguous())
         tol[rows] += c * mag * (2 * (K + 4 * r + 24) * 2.0 ** -24 + PIECES[act])
+        if act == "f16":
+            tol[rows] += c * 2.0 ** -38 * t.abs().amax(1, keepdim=True) * B.abs().sum(1)
     touched = torch.tensor([v >= 0 and block[v] is not None for v in index], device=y.device)
     # one rounding: half a last place, U of the value, and among the type's smallest numbers, which lie
     # 2 U times its smallest normal number apart, half of that step (float16: 2^-24 apart, off by 2^-25)
@@ -194,6 +198,17 @@ def test_values_that_are_not_finite_stay_in_their_row(gpu, act):
     ref, tol = _reference(torch.zeros_like(y), x3, block, index)
     fine = ref.abs() + tol < torch.finfo(DT[act]).max * (1 - 2 * U[act])
     assert fine.any() and ((got.double() - ref).abs() <= tol)[fine].all()
+    # factors among the type's smallest numbers, which the matrix cores take as they are
+    tiny = [(A, (B.double() * torch.finfo(DT[act]).tiny * 0.3).to(B.dtype), c) for A, B, c in block]
+    tiny += [((A.double() * torch.finfo(DT[act]).tiny * 0.3).to(A.dtype), B, c) for A, B, c in block]
+    assert all((t != 0).any() and (t.abs() < torch.finfo(DT[act]).tiny).sum() > t.numel() / 2
+               for t in (tiny[0][1], tiny[1][1], tiny[2][0], tiny[3][0]))
+    if act == "f16":
+        index2 = [i + 2 * (r % 2) for r, i in enumerate(index)]
+        x5 = x * 500
+        got = gdn.add_low_rank(torch.zeros_like(y), x5, gdn.LowRankAdapters([tiny]), gdn.AdapterRows(index2, 4, device=gpu))
+        ref, tol = _reference(torch.zeros_like(y), x5, tiny, index2)
+        assert ((got.double() - ref).abs() <= tol).all() and (ref.abs() > 2.0 ** -16).any()
     # and small ones
     x4 = x * (1e-6 if act == "f16" else 1e-30)
     got = gdn.add_low_rank(torch.zeros_like(y), x4, adapters, rows)
