@@ -278,11 +278,16 @@ extern "C" int gdn_rms_norm(const void* x, int64_t x_stride, const void* residua
     if (residual) {  // in place in either input, or apart from both
         const int es = dtype_size(dtype);
         const auto span = [&](int64_t stride) { return ((rows - 1) * stride + K) * es; };
-        GDN_REQUIRE((sum == x && sum_stride == x_stride) || !overlaps(sum, span(sum_stride), x, span(x_stride)),
-                    "gdn_rms_norm: sum overlaps x");
-        GDN_REQUIRE((sum == residual && sum_stride == residual_stride) ||
-                        !overlaps(sum, span(sum_stride), residual, span(residual_stride)),
-                    "gdn_rms_norm: sum overlaps residual");
+        const auto apart = [&](const void* in, int64_t stride) {
+            if ((sum == in && sum_stride == stride) || !overlaps(sum, span(sum_stride), in, span(stride))) return true;
+            if (sum_stride != stride || rows == 1) return false;
+            // columns of one buffer beside each other
+            const int64_t row = stride * es, off = (reinterpret_cast<intptr_t>(in) - reinterpret_cast<intptr_t>(sum)) % row;
+            const int64_t at = off < 0 ? off + row : off, width = int64_t(K) * es;
+            return at >= width && at <= row - width;
+        };
+        GDN_REQUIRE(apart(x, x_stride), "gdn_rms_norm: sum overlaps x");
+        GDN_REQUIRE(apart(residual, residual_stride), "gdn_rms_norm: sum overlaps residual");
     }
     const int kb = (K + kB - 1) / kB;
     if (codes) {

@@ -24,7 +24,7 @@ import torch
 
 from . import _lib
 from .gated_delta import _FLOATS, _require_device, _stream
-from .quant import QuantizedRows, _followed, _kept_rows
+from .quant import QuantizedRows, _followed, _kept_rows, rows_overlap
 
 _MAX_BLOCKS = 8
 _MAX_RANKS = 1 << 16
@@ -304,18 +304,9 @@ def add_low_rank(outs, x: torch.Tensor, adapters: LowRankAdapters, rows: Adapter
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two arrays of packed rows share an element: column slices of one
-    buffer lie between each other without doing so."""
+    """Whether two arrays of packed rows, whose ends lie in each other, share an
+    element."""
 
-    size, rows = a.element_size(), a.shape[0]
-    if not rows:
-        return False
-    pa, pb = a.data_ptr(), b.data_ptr()
-    wa, wb = a.shape[1] * size, b.shape[1] * size
-    sa, sb = a.stride(0) * size, b.stride(0) * size
-    if pa + (rows - 1) * sa + wa <= pb or pb + (rows - 1) * sb + wb <= pa:
-        return False
-    if sa != sb or rows == 1:
-        return True
-    off = (pb - pa) % sa
-    return off < wa or off > sa - wb
+    stride = a.stride(0)
+    return stride != b.stride(0) or rows_overlap(a.data_ptr(), b.data_ptr(), stride, a.shape[1], b.shape[1], a.shape[0],
+                                                 a.element_size())

@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 from .gated_delta import _FLOATS, _require_device, _stream
-from .quant import QuantizedRows, _followed
+from .quant import QuantizedRows, _followed, rows_overlap
 
 _F32 = torch.float32
 
@@ -95,8 +95,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *, residu
             s_stride = _row_layout(sum_out, K)
             if not s_stride:
                 raise ValueError("sum_out must consist of packed rows evenly apart")
-            _check_sum(sum_out, x, "x")
-            _check_sum(sum_out, residual, "residual")
+            _check_sum(sum_out, s_stride, x, K, "x")
+            _check_sum(sum_out, s_stride, residual, K, "residual")
         r_stride = _row_layout(residual, K)
         if not r_stride:
             residual, r_stride = residual.contiguous(), K
@@ -116,10 +116,13 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *, residu
     return normed if residual is None else (normed, sum_out)
 
 
-def _check_sum(out: torch.Tensor, src: torch.Tensor, name: str) -> None:
-    """``out`` is ``src`` itself or does not overlap it."""
+def _check_sum(out: torch.Tensor, stride: int, src: torch.Tensor, K: int, name: str) -> None:
+    """``out``, rows of K ``stride`` apart, is ``src`` itself or does not overlap it."""
 
     if out.data_ptr() == src.data_ptr() and out.stride() == src.stride():
+        return
+    if _row_layout(src, K) == stride and not rows_overlap(out.data_ptr(), src.data_ptr(), stride, K, K, out.numel() // K,
+                                                          out.element_size()):
         return
     ends = [(t.data_ptr(), t.data_ptr() + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size())
             for t in (out, src) if t.numel()]

@@ -587,6 +587,18 @@ def _fp8_matmul_codes(x: QuantizedRows, tensors, quant: QuantScheme, residual):
     return y
 
 
+def rows_overlap(a: int, b: int, stride: int, a_width: int, b_width: int, rows: int, size: int) -> bool:
+    """Whether two arrays of ``rows`` packed rows, ``stride`` elements of ``size`` bytes
+    apart in both, share a byte: column slices of one buffer lie between each other
+    without doing so."""
+
+    stride, a_width, b_width = stride * size, a_width * size, b_width * size
+    if not rows or a + (rows - 1) * stride + a_width <= b or b + (rows - 1) * stride + b_width <= a:
+        return False
+    off = (b - a) % stride
+    return rows == 1 or off < a_width or off > stride - b_width
+
+
 def _followed(*operands: torch.Tensor | None) -> bool:
     """Whether autograd or forward mode follows these operands, for calls that
     may cost little: tangents are looked for only inside a level of forward mode,

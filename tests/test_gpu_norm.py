@@ -233,6 +233,26 @@ def test_the_stream_in_place(gpu, act, K):
     assert torch.equal(s2, (x.float() * 2).to(DT[act]))
 
 
+@pytest.mark.parametrize("act", ["bf16", "f32"])
+def test_the_stream_beside_its_inputs(gpu, act):
+    """Columns of one buffer: the sum's lie between x's and the residual's and share none."""
+    K, w = 96, _w(gpu, 96)
+    buf = torch.full((19, 3 * K + 4), 7.0, dtype=DT[act], device=gpu)
+    x, s, r = buf[:, :K], buf[:, K:2 * K], buf[:, 2 * K:3 * K]
+    x.copy_(_x(gpu, 19, K, act=act))
+    r.copy_(_x(gpu, 19, K, act=act, seed=5))
+    want, stream = gdn.rms_norm(x.clone(), w, 1e-6, residual=r.clone())
+    before = buf.clone()
+    got, out = gdn.rms_norm(x, w, 1e-6, residual=r, sum_out=s)
+    assert out is s and torch.equal(got, want) and torch.equal(s, stream)
+    assert torch.equal(x, before[:, :K]) and torch.equal(buf[:, 2 * K:], before[:, 2 * K:])
+    for out in (buf[:, K - 1:2 * K - 1], buf[:, K + 1:2 * K + 1]):  # the last column of x, the first of the residual
+        with pytest.raises(ValueError, match="overlap"):
+            gdn.rms_norm(x, w, 1e-6, residual=r, sum_out=out)
+    with pytest.raises(ValueError, match="overlap"):  # in x's columns, another distance apart
+        gdn.rms_norm(x[:9], w, 1e-6, residual=r[:9], sum_out=buf.view(-1).as_strided((9, K), (2 * K, 1), 11))
+
+
 def test_rows_beyond_one_row_of_the_grid(gpu):
     M, K = (1 << 21) * 16 + 21, 16
     x, w = torch.ones(M, K, dtype=torch.bfloat16, device=gpu), _w(gpu, K)
