@@ -454,8 +454,12 @@ class Qwen3_5LinearAttention:
                 continue
             if any(n not in (0, w) for n, w in zip(made.widths, widths)):
                 raise ValueError(f"in_proj adapters have {made.widths} outputs, the projections {widths}")
-        if with_out is not None and with_out.hidden != d.value_dim:
-            raise ValueError(f"out_proj adapters take {with_out.hidden} values, the projection {d.value_dim}")
+        if with_out is not None:
+            tensors, _ = self._scheme_of(self.out_proj)
+            width = (tensors if isinstance(tensors, torch.Tensor) else tensors["weight"]).shape[0]
+            if (with_out.hidden, with_out.widths[0]) != (d.value_dim, width):
+                raise ValueError(f"out_proj adapters are {with_out.hidden} -> {with_out.widths[0]}, the projection "
+                                 f"{d.value_dim} -> {width}")
         self._in_adapters, self._out_adapters = with_in, with_out
 
     def new_cache(self, dtype: torch.dtype = torch.float32) -> RecurrentCache:
@@ -521,6 +525,12 @@ class Qwen3_5LinearAttention:
         if adapter_rows is not None and self._in_adapters is None and self._out_adapters is None:
             raise ValueError("adapter_rows given, but the layer has no adapters (set_adapters)")
         adapt = adapter_rows is not None and self._in_adapters is not None
+        after = None if adapter_rows is None else self._out_adapters
+        # what out_proj's adapters would refuse, before a state changes
+        if after is not None and (adapter_rows.rows != rows.shape[0] or adapter_rows.count != after.count or
+                                  adapter_rows._index != after._index):
+            raise ValueError(f"rows of {adapter_rows.rows} with {adapter_rows.count} adapters on {adapter_rows.device}, x has "
+                             f"{rows.shape[0]} and there are {after.count} on {after.device}")
         if self.input_norm_weight is not None:
             if isinstance(rows, QuantizedRows):
                 raise ValueError("the layer norms its input itself (input_norm_weight) and takes plain rows")
@@ -530,6 +540,8 @@ class Qwen3_5LinearAttention:
             rows = rms_norm(rows, self.input_norm_weight, self.rms_norm_eps, quantize=codes,
                             keep_rows=codes and (adapt or not self._all_codes))
         qkv, z, a, b = self._projected(rows)
+        if after is not None and (after.dtype is not qkv.dtype or after._index != qkv.get_device()):
+            raise ValueError(f"out_proj's adapters are {after.dtype} on {after.device}, its rows {qkv.dtype} on {qkv.device}")
         if adapt:
             add_low_rank([qkv, z.view(z.shape[0], self.linear.value_dim), a, b], rows, self._in_adapters, adapter_rows)
         return qkv, z, a, b

@@ -246,6 +246,28 @@ def test_refusals(gpu):
         layer(x, layer.new_cache(torch.bfloat16), adapter_rows=rows)
 
 
+def test_a_refused_step_leaves_the_pool_as_it_was(gpu):
+    """What only out_proj's adapters would notice, at the step's end."""
+    layer, _, _, _ = _layer(gpu, "dense")
+    x = torch.randn(3, HIDDEN, device=gpu).bfloat16()
+    rows = lambda index, count, device=gpu: gdn.AdapterRows(index, count, device=device)
+    only_out = _adapters(gpu, torch.bfloat16, names=("out_proj",))
+    with pytest.raises(ValueError, match="projection"):
+        layer.set_adapters(out_proj=[(A, B[:-1].contiguous(), c) for A, B, c in only_out["out_proj"]])
+    pool = gdn.RecurrentStatePool(4, 4, D.conv_dim, HV, 128, 128, dtype=torch.bfloat16, device=gpu)
+    layer.decode_batch(x, pool, slots=[3, 0, 1])
+    kept = [t.clone() for t in (pool.ssm_state, pool.conv_buf, pool.conv_half_dev)]
+    sizes = pool.size.clone()
+    for adapters, bad in ((only_out, rows([0, 1], 3)), (only_out, rows([0, 1, 1], 2)), (only_out, rows([0, 1, 2], 3, "cpu")),
+                          (_adapters(gpu, torch.float32, names=("out_proj",)), rows([0, 1, 2], 3))):
+        layer.set_adapters(**adapters)
+        with pytest.raises(ValueError):
+            layer.decode_batch(x, pool, slots=[3, 0, 1], adapter_rows=bad)
+        assert torch.equal(pool.size, sizes)
+        for was, now in zip(kept, (pool.ssm_state, pool.conv_buf, pool.conv_half_dev)):
+            assert torch.equal(was, now)
+
+
 def test_norm_from_a_checkpoint(gpu, tmp_path):
     g = torch.Generator().manual_seed(0)
     prefix = "language_model.model.layers.0"
