@@ -141,7 +141,7 @@ GDN_DEV void store_t(uint8_t* to, f32x4 v, int rank, float scale) {
             most = fmaxf(most, __shfl_xor(most, 16));
             most = fmaxf(most, __shfl_xor(most, 32));
             const int up = int(__float_as_uint(most) >> 23) - 127;  // 2^up <= most < 2^(up + 1)
-            const bool usable = most > 0x1p-100f && most < 0x1p100f;
+            const bool usable = most > 0x1p-100f && most <= 0x1.fffffep127f;
             const float fit = usable ? __uint_as_float(uint32_t(127 + 13 - up) << 23) : 1.f;
             if (g == 0) *reinterpret_cast<float*>(to + 1024 + lr * 4) = usable ? __uint_as_float(uint32_t(127 - 13 + up) << 23) : 1.f;
 #pragma unroll
@@ -589,7 +589,7 @@ extern "C" int gdn_add_low_rank(const void* x, int64_t x_stride, int dtype, cons
                 "gdn_add_low_rank: A, B, table and workspace must be 16-byte aligned");
     LowRankArgs p{x, A, B, static_cast<const AdapterBlock*>(table), order, tiles, static_cast<uint8_t*>(workspace)};
     for (int j = 0; j < blocks; ++j) {
-        GDN_REQUIRE(widths[j] >= 0 && (widths[j] == 0 || (outs[j] && (out_strides[j] >= widths[j] || M == 1))),
+        GDN_REQUIRE(widths[j] >= 0 && widths[j] <= kLowRankMostColumns && (widths[j] == 0 || (outs[j] && (out_strides[j] >= widths[j] || M == 1))),
                     "gdn_add_low_rank: block %d of %d columns, rows %lld apart", j, widths[j], (long long)out_strides[j]);
         p.out[j] = outs[j];
         p.out_stride[j] = out_strides[j];

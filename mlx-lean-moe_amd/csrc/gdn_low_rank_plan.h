@@ -7,6 +7,7 @@
 namespace gdn {
 
 constexpr int kLowRankBlocks = 8;      // blocks of columns a call takes
+constexpr int kLowRankMostColumns = 1 << 30;  // of a block
 constexpr int kLowRankTile = 256;      // rows of a plan's large tiles
 constexpr int kLowRankDownWaves = 8;   // waves a workgroup of the first product, which share out K
 constexpr int kLowRankUpWaves = 4;     // of the second, 64 columns each

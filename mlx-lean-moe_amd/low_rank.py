@@ -21,6 +21,7 @@ import ctypes
 
 import numpy as np
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .gated_delta import _FLOATS, _require_device, _stream
@@ -29,6 +30,7 @@ from .quant import QuantizedRows, _followed, _kept_rows, rows_overlap
 _MAX_BLOCKS = 8
 _MAX_RANKS = 1 << 16
 _MAX_HIDDEN = 1 << 24
+_MAX_WIDTH = 1 << 30
 # Rows a tile: about as many as adapters have on average, a power of two between these
 # (the kernels cut tiles as they need; places that stay empty cost workgroups).
 _LEAST_ROWS, _MOST_ROWS = 16, 256
@@ -81,6 +83,8 @@ class LowRankAdapters:
             widths.append(width)
         if not 0 < self.hidden <= _MAX_HIDDEN:
             raise ValueError(f"adapters take rows of 1 to {_MAX_HIDDEN} values, got {self.hidden}")
+        if max(widths) > _MAX_WIDTH:
+            raise ValueError(f"adapters take projections of at most {_MAX_WIDTH} outputs, got {max(widths)}")
         self.widths = tuple(widths)
         table = np.zeros((self.count, len(projections)), dtype=_TABLE)
         a_rows, b_size = 0, 0
@@ -291,6 +295,7 @@ def add_low_rank(outs, x: torch.Tensor, adapters: LowRankAdapters, rows: Adapter
         pointers[j], strides[j] = begin, stride
     if _followed(*(t for _, _, t in ends)):
         raise RuntimeError("adapters have no gradient and no forward mode; call add_low_rank under torch.no_grad()")
+    increment_version([t for _, _, t in ends[1:]])  # (a graph that saved an output has to see this)
     device = x.device
     nbytes = adapters._workspace(rows.tiles, rows.tile_rows)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None

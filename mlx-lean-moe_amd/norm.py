@@ -10,6 +10,7 @@ pass of memory, the addition of the layer before it included.
 from __future__ import annotations
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .gated_delta import _FLOATS, _require_device, _stream
@@ -78,7 +79,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *, residu
         raise ValueError(f"quantized rows have a multiple of 16 values, got {K}")
     if _followed(x, weight, residual, sum_out):
         raise RuntimeError("rms_norm has no gradient and no forward mode; call it under torch.no_grad()")
-    device = x.device
+    device, given = x.device, sum_out is not None
     M = x.numel() // K
     x_stride = _row_layout(x, K)
     if not x_stride:
@@ -109,6 +110,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *, residu
         data = torch.empty(QuantizedRows.nbytes(M, K), dtype=torch.uint8, device=device)
         codes = data.data_ptr()
         scales = codes + (K + 127) // 128 * 128 * M
+    if given:  # (a graph that saved it has to see this)
+        increment_version(sum_out)
     _lib.call_on(device, "gdn_rms_norm", x.data_ptr(), x_stride, _lib.ptr(residual), r_stride, _lib.ptr(sum_out), s_stride,
                  _lib.ptr(weight), float(eps), _lib.dtype_code(dtype), _lib.ptr(out), codes, scales, apart, M, K,
                  _stream(device))

@@ -209,6 +209,10 @@ def test_values_that_are_not_finite_stay_in_their_row(gpu, act):
         got = gdn.add_low_rank(torch.zeros_like(y), x5, gdn.LowRankAdapters([tiny]), gdn.AdapterRows(index2, 4, device=gpu))
         ref, tol = _reference(torch.zeros_like(y), x5, tiny, index2)
         assert ((got.double() - ref).abs() <= tol).all() and (ref.abs() > 2.0 ** -16).any()
+        # inner products far beyond the type: infinite results, and none where B is zero
+        far = [(A, B * (torch.arange(N, device=gpu)[:, None] % 2), 2.0 ** 110) for A, B, _ in block]
+        got = gdn.add_low_rank(y.clone(), x, gdn.LowRankAdapters([far]), rows)
+        assert torch.equal(got[:, ::2], y[:, ::2]) and not torch.isfinite(got[:, 1::2]).any()
     # and small ones
     x4 = x * (1e-6 if act == "f16" else 1e-30)
     got = gdn.add_low_rank(torch.zeros_like(y), x4, adapters, rows)
@@ -299,6 +303,20 @@ def test_two_streams_at_once(gpu):
             got.append(gdn.add_low_rank(y.clone(), x, adapters, rows))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
+
+
+def test_a_saved_output_is_noticed(gpu):
+    m = _Maker(gpu, "f32")
+    adapters = gdn.LowRankAdapters([_pairs(m, [4], 64, 48)])
+    rows = gdn.AdapterRows([0, -1, 0], 1, device=gpu)
+    x, y, w = m(3, 64), m(3, 48), m(48, 5).requires_grad_()
+    loss = (y @ w).sum()
+    with torch.no_grad():
+        gdn.add_low_rank(y, x, adapters, rows)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        gdn.add_low_rank(m(3, 48), x, adapters, rows)
 
 
 def test_refusals(gpu):

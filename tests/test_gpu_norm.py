@@ -253,6 +253,20 @@ def test_the_stream_beside_its_inputs(gpu, act):
         gdn.rms_norm(x[:9], w, 1e-6, residual=r[:9], sum_out=buf.view(-1).as_strided((9, K), (2 * K, 1), 11))
 
 
+def test_a_saved_stream_written_in_place_is_noticed(gpu):
+    x, w = _x(gpu, 3, 96, act="f32"), torch.ones(96, device=gpu, requires_grad=True)
+    saved = x.clone()
+    loss = (saved * w).sum()
+    with torch.no_grad():
+        gdn.rms_norm(saved, None, 1e-6, residual=x, sum_out=saved)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        kept = x.clone()
+        gdn.rms_norm(kept, None, 1e-6, residual=x, sum_out=kept)
+    gdn.rms_norm(kept, None, 1e-6, residual=x, sum_out=x.clone())
+
+
 def test_rows_beyond_one_row_of_the_grid(gpu):
     M, K = (1 << 21) * 16 + 21, 16
     x, w = torch.ones(M, K, dtype=torch.bfloat16, device=gpu), _w(gpu, K)
