@@ -104,7 +104,9 @@ class LowRankAdapters:
             raise ValueError(f"an adapter's ranks add up to at most {_MAX_RANKS}, got {self.rank_total}")
         self._A, self._B = self._laid_out(projections, padded, columns)
         self._index = self._A.get_device()
-        self._c_widths = (ctypes.c_int * len(widths))(*widths)
+        n = len(widths)
+        self._c_widths, self._c_pointers, self._c_strides = (ctypes.c_int * n)(*widths), ctypes.c_void_p * n, ctypes.c_int64 * n
+        self._code = _lib.dtype_code(self.dtype)
         self._workspaces: dict[tuple[int, int], int] = {}
         self._table = torch.from_numpy(table.reshape(-1).view(np.uint8)).to(self.device)
 
@@ -150,7 +152,7 @@ class LowRankAdapters:
             if len(self._workspaces) >= 1024:
                 self._workspaces.clear()
             nbytes = self._workspaces[tiles, tile_rows] = int(_lib.load().gdn_add_low_rank_workspace_size(
-                _lib.dtype_code(self.dtype), len(self.widths), self.rank_total, self.rank_block, self._c_widths, tiles,
+                self._code, len(self.widths), self.rank_total, self.rank_block, self._c_widths, tiles,
                 tile_rows, self.hidden))
         return nbytes
 
@@ -274,9 +276,9 @@ def add_low_rank(outs, x: torch.Tensor, adapters: LowRankAdapters, rows: Adapter
         x = x.contiguous()
         x_stride = K
     n, size = len(blocks), dtype.itemsize
-    pointers, strides = [None] * n, [0] * n
-    begin = x.data_ptr()
-    ends = [(begin, begin + ((M - 1) * x_stride + K) * size, x)]
+    pointers, strides, written = [None] * n, [0] * n, []
+    at = x.data_ptr()
+    ends = [(at, at + ((M - 1) * x_stride + K) * size, x)]
     for j, (out, width) in enumerate(zip(blocks, adapters.widths)):
         if not width:
             continue
@@ -292,19 +294,19 @@ def add_low_rank(outs, x: torch.Tensor, adapters: LowRankAdapters, rows: Adapter
             if begin < e and b < end and M and _overlap(out, other):
                 raise ValueError(f"output {j} overlaps {'x' if other is x else 'another output'}")
         ends.append((begin, end, out))
+        written.append(out)
         pointers[j], strides[j] = begin, stride
-    if _followed(*(t for _, _, t in ends)):
+    if _followed(x, *written):
         raise RuntimeError("adapters have no gradient and no forward mode; call add_low_rank under torch.no_grad()")
-    increment_version([t for _, _, t in ends[1:]])  # (a graph that saved an output has to see this)
+    increment_version(written)  # (a graph that saved an output has to see this)
     device = x.device
     nbytes = adapters._workspace(rows.tiles, rows.tile_rows)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     plan = rows._plan.data_ptr()
-    _lib.call_on(device, "gdn_add_low_rank", ends[0][0], x_stride, _lib.dtype_code(dtype), adapters._A.data_ptr(),
+    _lib.call_on(device, "gdn_add_low_rank", at, x_stride, adapters._code, adapters._A.data_ptr(),
                  adapters._B.data_ptr(), adapters._table.data_ptr(), adapters.count, n, adapters.rank_total,
-                 adapters.rank_block, (ctypes.c_void_p * n)(*pointers), (ctypes.c_int64 * n)(*strides),
-                 adapters._c_widths, plan, plan + 4 * M, rows.tiles, rows.tile_rows, M, K, _lib.ptr(ws), nbytes,
-                 _stream(device))
+                 adapters.rank_block, adapters._c_pointers(*pointers), adapters._c_strides(*strides), adapters._c_widths,
+                 plan, plan + 4 * M, rows.tiles, rows.tile_rows, M, K, _lib.ptr(ws), nbytes, _stream(device))
     return outs
 
 
