@@ -32,11 +32,15 @@ struct LowRankPlan {
 };
 
 // Two launches. Few tiles: the first product's ranks apart, 16 a workgroup, so that the
-// reading of an adapter is spread; many: together, so that x is read once, and 32 rows
-// share a reading of the adapter where that leaves a workgroup for each CU (8192 rows of
-// rank 64 50.1 us in all, 52.6 with 16 rows). The second product takes as many rows of a
-// tile as leave 4096 workgroups, since those share a reading of B (8192 x 4096, rank 64,
-// and 4096 x 12288, rank 32: 54.5 and 53.2 us in all, with 512 workgroups 57 and 58).
+// reading of an adapter is spread; many: together, so that x is read once; between, 32
+// (both launches, 64 columns, us, 16, 32 and 64 ranks a workgroup: 1024 rows of 2048, rank
+// 64 8.0, 8.4, 9.8, float32 12.1, 14.3, 21.1; 2048 rows 11.1, 9.5, 10.6, float32 17.2,
+// 15.7, 22.6; 4096 rows 15.7, 12.7, 12.2, float32 26.3, 22.7, 23.4; 2048 rows of 8
+// adapters, rank 96 17.3, 14.5, 16.3, float32 27.4, 24.8, 37.2). 32 rows share a reading of
+// the adapter where that leaves a workgroup for each CU (8192 rows of rank 64 50.1 us in
+// all, 52.6 with 16 rows). The second product takes as many rows of a tile as leave 4096
+// workgroups, since those share a reading of B (8192 x 4096, rank 64, and 4096 x 12288,
+// rank 32: 54.5 and 53.2 us in all, with 512 workgroups 57 and 58).
 //
 // One, where that is one round of workgroups of not many columns, and what each reads of
 // A (its own adapter's rows, as every other workgroup of its block) is little. us, one
@@ -49,7 +53,9 @@ inline LowRankPlan low_rank_plan(int tiles, int tile_rows, int rank_total, int r
                                  const int* widths, int blocks) {
     LowRankPlan p;
     const int64_t parts = int64_t(tiles) * (tile_rows / 16);
-    p.ranks = parts * (rank_total / 16) <= 256 || rank_total <= 16 ? 16 : rank_total <= 32 ? 32 : 64;
+    p.ranks = 64;
+    if (rank_total <= 32 || parts * ((rank_total + 31) / 32) <= 384) p.ranks = 32;
+    if (rank_total <= 16 || parts * (rank_total / 16) <= 256) p.ranks = 16;
     p.down_rows = tile_rows > 16 && parts / 2 * ((rank_total + p.ranks - 1) / p.ranks) >= 256 ? 32 : 16;
     const int64_t groups = column_groups(widths, blocks, kLowRankColumns, nullptr);
     p.up_rows = tile_rows;

@@ -50,6 +50,12 @@ def test_one_launch_for_few_rows(plan):
         assert plan(*call)["columns"] == 0, call
 
 
+def test_ranks_apart_for_few_rows(plan):
+    for parts, total, ranks in ((64, 64, 16), (65, 64, 32), (128, 64, 32), (192, 64, 32), (193, 64, 64), (128, 96, 32), (129, 96, 64),
+                                (128, 32, 16), (129, 32, 32), (5000, 32, 32), (5000, 16, 16), (1, 65536, 64)):
+        assert plan(parts, 16, total, min(total, 64), 2048, 2, (4096,))["ranks"] == ranks, (parts, total)
+
+
 def test_every_kernel_is_reached(plan):
     """By the calls of the GPU tests: (M as tiles, ranks, K, outputs)."""
     one, two = set(), set()
