@@ -39,8 +39,11 @@ struct LowRankPlan {
 // adapters, rank 96 17.3, 14.5, 16.3, float32 27.4, 24.8, 37.2). 32 rows share a reading of
 // the adapter where that leaves a workgroup for each CU (8192 rows of rank 64 50.1 us in
 // all, 52.6 with 16 rows). The second product takes as many rows of a tile as leave 4096
-// workgroups, since those share a reading of B (8192 x 4096, rank 64, and 4096 x 12288,
-// rank 32: 54.5 and 53.2 us in all, with 512 workgroups 57 and 58).
+// workgroups, since those share a reading of B (4096 x 12288, rank 32: 53.0 us in all, with
+// 2048 54.5, with 512 58; 8192 x 4096, rank 16 40.0, 42.3, 41.4); with four pieces of B to
+// read as many as leave 512, up to 64 (rank 64, us, 16 rows, 32 and 64: 2048 x 4096 20.1,
+// 18.3, 17.8, float16 23.4, 20.4, 19.1, float32 35.2, 32.6, 32.5; 1024 x 4096 14.2, 13.0,
+// 13.7; 8192 x 4096, 32 rows, 64 and 128 50.7, 50.3, 53.0).
 //
 // One, where that is one round of workgroups of not many columns, and what each reads of
 // A (its own adapter's rows, as every other workgroup of its block) is little. us, one
@@ -57,11 +60,11 @@ inline LowRankPlan low_rank_plan(int tiles, int tile_rows, int rank_total, int r
     if (rank_total <= 32 || parts * ((rank_total + 31) / 32) <= 384) p.ranks = 32;
     if (rank_total <= 16 || parts * (rank_total / 16) <= 256) p.ranks = 16;
     p.down_rows = tile_rows > 16 && parts / 2 * ((rank_total + p.ranks - 1) / p.ranks) >= 256 ? 32 : 16;
-    const int64_t groups = column_groups(widths, blocks, kLowRankColumns, nullptr);
-    p.up_rows = tile_rows;
-    while (p.up_rows > 16 && tiles * (tile_rows / p.up_rows) * groups < 4096) p.up_rows /= 2;
     p.steps = int((int64_t(K) * elem + 127) / 128);
     p.held = rank_block <= 16 ? 1 : rank_block <= 32 ? 2 : rank_block <= 64 ? 4 : 0;
+    const int64_t groups = column_groups(widths, blocks, kLowRankColumns, nullptr);
+    p.up_rows = p.held == 4 && tile_rows > 64 ? 64 : tile_rows;
+    while (p.up_rows > 16 && tiles * (tile_rows / p.up_rows) * groups < (p.held == 4 ? 512 : 4096)) p.up_rows /= 2;
 
     p.columns = 0;
     if ((p.held == 1 || p.held == 2) && p.held * 16 * int64_t(K) * elem <= 1 << 17)
