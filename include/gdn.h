@@ -605,7 +605,7 @@ int gdn_fp8_dequantize(const void *w, const float *scales, void *out, int out_dt
  * gdn_add_low_rank - low-rank adapters of many requests, added to a projection's
  * output in place: for row i with adapter a and each block j of its columns,
  *   outs[j][i] = dtype(outs[j][i] + c sum_r (sum_k x[i,k] A[r,k]) B[n,r]),
- * sums in float32; c times the inner one is kept to 16 bits at least where dtype has 16.
+ * sums in float32; c times the inner one is kept to float32's 24 bits, 22 in float16.
  *   x: (M, K) dtype at its row stride; outs[j]: (M, widths[j]) dtype at
  *      out_strides[j] (host arrays of `blocks` entries, 1 to 8), not overlapping x
  *      or each other; a block of width 0 is left out

@@ -3,11 +3,11 @@
 //   t = c x_i A_a^T (all blocks' ranks side by side),   out_j[i] += t_j B_aj^T.
 // The rows come sorted by adapter and cut into tiles of one adapter (a plan that
 // the caller keeps for all projections of a step), so each product is a plain
-// one on the matrix cores, with float32 sums. The first leaves t as the second's
-// operand: float32, or (16-bit adapters) two pieces of their type, the second what the
-// first leaves: 16 bits of t in bfloat16, 22 in float16, which t need not fit: there
-// 16 ranks of a row come times a power of two of their own, and their product goes
-// back by it.
+// one on the matrix cores, with float32 sums. The first leaves t for the second: in
+// float32, which the second cuts into three bfloat16 pieces where B is bfloat16 (exact, at
+// Ranks), or in float16 as two pieces of that type, the second what the first leaves, 22
+// bits: t need not fit the type, so there 16 ranks of a row come times a power of two of
+// their own, and their product goes back by it.
 //
 // A, B and t lie in memory in the order in which a wave's lanes take them: a load of
 // 16 bytes a lane is 1 KB in one piece (8192 rows, 2048 -> 4096, rank 64: rows of them
@@ -28,6 +28,7 @@ namespace {
 constexpr int kDepth = 2;  // steps of K under way at once (3, 4 and 6: the same within 2 %)
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 struct AdapterBlock {
     int64_t b;      // first element of B: 16 ranks after each other, all columns of each
@@ -106,13 +107,6 @@ GDN_DEV uint4 piece_of(const S* p, int count) {
     return v;
 }
 
-// The upper 8 bits of a float32 value as bfloat16 (cut off: rounded up, the largest
-// would overflow), and what they leave, rounded; what is not finite has no rest.
-GDN_DEV void two_bf16(float v, uint16_t& high, uint16_t& low) {
-    high = v != v ? 0x7FC0 : uint16_t(__float_as_uint(v) >> 16);
-    low = (high & 0x7F80) == 0x7F80 ? 0 : f32_to_bf16_bits(v - bf16_bits_to_f32(high));
-}
-
 GDN_DEV void two_f16(float v, uint16_t& high, uint16_t& low) {
     high = f32_to_f16_bits(v);
     low = (high & 0x7C00) == 0x7C00 ? 0 : f32_to_f16_bits(v - f16_bits_to_f32(high));
@@ -132,46 +126,100 @@ GDN_DEV void store_t(uint8_t* to, f32x4 v, int rank, float scale) {
     const int g = (threadIdx.x & 63) >> 4, lr = threadIdx.x & 15;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = 4 * g + e < rank ? v[e] * scale : 0.f;
-    if constexpr (Act::code == GDN_F32) {
+    if constexpr (Act::code != GDN_F16) {
         *reinterpret_cast<f32x4*>(to + lr * 16 + 256 * g) = v;
     } else {  // quarters of 1 KB: ranks 0 to 7 and 8 to 15 high, then low
         uint16_t high[4], low[4];
-        if constexpr (Act::code == GDN_F16) {
-            float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-            most = fmaxf(most, __shfl_xor(most, 16));
-            most = fmaxf(most, __shfl_xor(most, 32));
-            const int up = int(__float_as_uint(most) >> 23) - 127;  // 2^up <= most < 2^(up + 1)
-            const bool usable = most > 0x1p-100f && most <= 0x1.fffffep127f;
-            const float fit = usable ? __uint_as_float(uint32_t(127 + 13 - up) << 23) : 1.f;
-            if (g == 0) *reinterpret_cast<float*>(to + 1024 + lr * 4) = usable ? __uint_as_float(uint32_t(127 - 13 + up) << 23) : 1.f;
+        float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        const int up = int(__float_as_uint(most) >> 23) - 127;  // 2^up <= most < 2^(up + 1)
+        const bool usable = most > 0x1p-100f && most <= 0x1.fffffep127f;
+        const float fit = usable ? __uint_as_float(uint32_t(127 + 13 - up) << 23) : 1.f;
+        if (g == 0) *reinterpret_cast<float*>(to + 1024 + lr * 4) = usable ? __uint_as_float(uint32_t(127 - 13 + up) << 23) : 1.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) two_f16(v[e] * fit, high[e], low[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) two_bf16(v[e], high[e], low[e]);
-        }
+        for (int e = 0; e < 4; ++e) two_f16(v[e] * fit, high[e], low[e]);
         to += lr * 16 + g / 2 * 256 + g % 2 * 8;
         __builtin_memcpy(__builtin_assume_aligned(to, 8), high, 8);
         __builtin_memcpy(__builtin_assume_aligned(to + 512, 8), low, 8);
     }
 }
 
-// t of 16 rows and 16 ranks, as a lane of the second product has it.
+// 16 ranks of one operand of B (16 columns), as a lane of the second product has them.
 template <class Act>
-struct Ranks {
+using PartOfB = std::conditional_t<Act::code == GDN_BF16, uint2, uint4>;
+
+// t of 16 rows and 16 ranks, as a lane of the second product has it. add: sum + B t for
+// the four operands of a wave's 64 columns.
+template <class Act>
+struct Ranks {  // float32
+    f32x4 v;
+    GDN_DEV void load(const uint8_t* block) { v = *reinterpret_cast<const f32x4*>(block + (threadIdx.x & 63) * 16); }
+    GDN_DEV void cut() {}
+    GDN_DEV void add(const uint4 (&b)[4], f32x4 (&sum)[4]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] = mfma_pieces<Act>(b[j], __builtin_bit_cast(uint4, v), sum[j]);
+    }
+};
+
+// bfloat16: t's float32 value as three pieces, each the upper 8 bits of what those before
+// it leave (cut off, so exact; rounded up, the largest would overflow), in three products
+// of 16 ranks. Two pieces in one product of 32 would lose 2^-16 of t: both launches, us,
+// 8192 rows of rank 64 53.5 and with two 50.5, 4096 packed ones 54.4 and 53.3. The pieces
+// made by the first product instead: half as many bytes of t again, 59.4 and 57.3; two of
+// the three in one product, B's ranks held twice: 54.0 and 55.6.
+template <>
+struct Ranks<ActBF16> {
+    f32x4 v;
+    uint2 p[3];
+    GDN_DEV void load(const uint8_t* block) { v = *reinterpret_cast<const f32x4*>(block + (threadIdx.x & 63) * 16); }
+    static GDN_DEV float upper(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
+    static GDN_DEV uint2 upper_halves(const f32x4& x) {
+        const uint4 u = __builtin_bit_cast(uint4, x);
+        return make_uint2(__builtin_amdgcn_perm(u.y, u.x, 0x07060302u), __builtin_amdgcn_perm(u.w, u.z, 0x07060302u));
+    }
+    GDN_DEV void cut() {
+        f32x4 rest, last;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rest[e] = v[e] - upper(v[e]);
+        const float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+        if (__builtin_expect(most > 0x1.fffffep127f, 0)) {  // what is infinite has no rest
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (fabsf(v[e]) > 0x1.fffffep127f) rest[e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) last[e] = rest[e] - upper(rest[e]);
+        p[0] = upper_halves(v);
+        p[1] = upper_halves(rest);
+        p[2] = upper_halves(last);
+    }
+    GDN_DEV void add(const uint2 (&b)[4], f32x4 (&sum)[4]) const {
+#pragma unroll
+        for (int i = 2; i >= 0; --i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                sum[j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(i16x4, b[j]), __builtin_bit_cast(i16x4, p[i]),
+                                                                   sum[j], 0, 0, 0);
+    }
+};
+
+template <>
+struct Ranks<ActF16> {
     uint4 v;
     float back;
     GDN_DEV void load(const uint8_t* block) {
         v = *reinterpret_cast<const uint4*>(block + (threadIdx.x & 63) * 16);
-        if constexpr (Act::code == GDN_F16) back = *reinterpret_cast<const float*>(block + 1024 + (threadIdx.x & 15) * 4);
+        back = *reinterpret_cast<const float*>(block + 1024 + (threadIdx.x & 15) * 4);
     }
-    // sum + B t for one operand of B
-    GDN_DEV f32x4 add(const uint4& b, f32x4 sum) const {
-        if constexpr (Act::code != GDN_F16) return mfma_pieces<Act>(b, v, sum);
-        const f32x4 p = mfma_pieces<Act>(b, v, f32x4{0.f, 0.f, 0.f, 0.f});
+    GDN_DEV void cut() {}
+    GDN_DEV void add(const uint4 (&b)[4], f32x4 (&sum)[4]) const {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(p[e], back, sum[e]);
-        return sum;
+        for (int j = 0; j < 4; ++j) {
+            const f32x4 p = mfma_pieces<ActF16>(b[j], v, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[j][e] = __builtin_fmaf(p[e], back, sum[j][e]);
+        }
     }
 };
 
@@ -298,11 +346,13 @@ struct Columns {
             }
         }
     }
-    // B: for each 16 ranks and 64 columns four operands, of 512 bytes where both of
-    // t's pieces meet the same
+    // B: for each 16 ranks and 64 columns four operands, of 512 bytes in 16 bits: float16's
+    // two pieces of t meet the same, in bfloat16 a lane has four ranks, half of 16 bytes
     static constexpr int kB = Act::code == GDN_F32 ? 1024 : 512;
     static GDN_DEV const uint8_t* operands(const LowRankArgs& p, const AdapterBlock& ab, int n0) {
-        return static_cast<const uint8_t*>(p.B) + ab.b * kY + int64_t(n0 / 64) * (4 * kB) + (threadIdx.x & 63) * 16 % kB;
+        const int lane = threadIdx.x & 63;
+        return static_cast<const uint8_t*>(p.B) + ab.b * kY + int64_t(n0 / 64) * (4 * kB) +
+               (Act::code == GDN_BF16 ? lane / 32 * 256 + lane % 16 * 16 + lane / 16 % 2 * 8 : lane * 16 % kB);
     }
     static GDN_DEV int64_t next_ranks(int width) { return int64_t((width + 63) / 64) * (4 * kB); }
 };
@@ -311,17 +361,18 @@ struct Columns {
 // rows at a time. B is the left operand and its rows are dealt out so that a lane
 // ends with 16-byte pieces of one row's output, the four lanes of a row beside each
 // other in each piece (32 bytes a lane instead: 45 us for 34 at rank 16). The 32 values
-// of k of a 16-bit product are 16 ranks of t's high piece and the same of its low one, B
+// of k of a float16 product are 16 ranks of t's high piece and the same of its low one, B
 // the same for both. A wave keeps its part of B (kHeld pieces of 16 ranks; 0: more ranks
 // than that, read again for each 16 rows) and streams the rows: the next ones' output
 // and t are under way while these are multiplied and stored.
 //
 // Bound by the output's way through memory and back: 8192 x 4096, rank 16 about 30 us
 // (134 MB, 4.5 TB/s), rank 64 40; 4096 x 12288, rank up to 32, 43 (201 MB, 4.7 TB/s).
-// At rank 64 without t and the products 28 of 36 us (from a graph): t is twice the
-// output's bytes at the vector caches, and 160 registers leave three waves a SIMD.
+// At rank 64 t is twice the output's bytes at the vector caches, and cutting it is more of
+// the arithmetic than the output's sums. Four waves a SIMD there in bfloat16 (120
+// registers; left alone 132 and three: 8192 rows 53.5 us and 54.1, 2048 20.2 and 20.6).
 template <class Act, int kHeld>
-__global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRankArgs p) {
+__global__ __launch_bounds__(64 * kLowRankUpWaves, Act::code == GDN_BF16 && kHeld == 4 ? 4 : 1) void low_rank_up_kernel(LowRankArgs p) {
     using S = typename Act::storage;
     using Own = Columns<Act>;
     constexpr int kT = kHeld ? kHeld : 1;
@@ -349,10 +400,11 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
     const bool whole = n0 + 64 <= width;  // (of the wave: one branch)
     const uint8_t* br = Own::operands(p, ab, n0);
     const int64_t b_stride = Own::next_ranks(width);
-    uint4 b[kT][4];
-    const auto load_b = [&](int i, uint4 (&v)[4]) {
+    using Part = PartOfB<Act>;
+    Part b[kT][4];
+    const auto load_b = [&](int i, Part (&v)[4]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(br + i * b_stride + j * Own::kB);
+        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const Part*>(br + i * b_stride + j * Own::kB);
     };
     if constexpr (kHeld != 0) {
 #pragma unroll
@@ -389,16 +441,16 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves) void low_rank_up_kernel(LowRa
 #pragma unroll
             for (int i = 0; i < kHeld; ++i)
                 if (i < pieces) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[j] = r.tv[i].add(b[i][j], acc[j]);
+                    r.tv[i].cut();
+                    r.tv[i].add(b[i], acc);
                 }
         } else {
             for (int i = 0; i < pieces; ++i) {
                 load_b(i, b[0]);
                 Ranks<Act> v;
                 v.load(t + s * t_stride + int64_t(kBlock) * i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[j] = v.add(b[0][j], acc[j]);
+                v.cut();
+                v.add(b[0], acc);
             }
         }
         if (r.y) Own::add(r.y, r.yv, acc, whole, width - n);
@@ -467,13 +519,14 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_whole_kernel(
                 ? static_cast<S*>(p.out[block]) + int64_t(row) * p.out_stride[block] + Own::kCount * g : nullptr;
     const uint8_t* br = Own::operands(p, ab, 0);
     const int64_t b_stride = Own::next_ranks(width);
-    uint4 raw[kNR][4];
+    using Part = PartOfB<Act>;
+    Part raw[kNR][4];
     const auto load_b = [&](int n) {
 #pragma unroll
         for (int i = 0; i < kNR; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                raw[i][j] = *reinterpret_cast<const uint4*>(br + min(i, pieces - 1) * b_stride + (n / 64 * 4 + j) * Own::kB);
+                raw[i][j] = *reinterpret_cast<const Part*>(br + min(i, pieces - 1) * b_stride + (n / 64 * 4 + j) * Own::kB);
     };
     const auto load_y = [&](int n, uint4 (&v)[Own::kY]) {
         if (yr && n + 64 <= width) Own::load(yr + n, v);  // (else read where it is written)
@@ -525,8 +578,8 @@ __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_whole_kernel(
             if (c < pieces) {
                 Ranks<Act> v;
                 v.load(t + c * kBlockOfT<Act>);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sum[j] = v.add(raw[c][j], sum[j]);
+                v.cut();
+                v.add(raw[c], sum);
             }
         if (n2 < n_end) load_b(n2);
         if (yr) Own::add(yr + n, now, sum, n + 64 <= width, width - n - Own::kCount * g);

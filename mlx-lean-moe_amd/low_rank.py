@@ -249,10 +249,10 @@ def add_low_rank(outs, x: torch.Tensor, adapters: LowRankAdapters, rows: Adapter
     a tensor ``(M, N)``, else a list with one for each projection of ``adapters``
     (None where it has no adapters), in x's dtype at any row stride, e.g. column
     slices of a stacked output. Sums are float32; a result is rounded once more to
-    its dtype. ``scale x A^T`` is kept to 16 bits at least for 16-bit dtypes, in
-    full for float32. Rows without an adapter are left as they are, and a row's result does not
-    depend on the rows beside it. Values that are not finite stay in their row, which
-    may then be NaN where float32 sums would be infinite."""
+    its dtype. ``scale x A^T`` is kept to float32's 24 bits, 22 for float16. Rows
+    without an adapter are left as they are, and a row's result does not depend on the
+    rows beside it. Values that are not finite stay in their row, which may then be NaN
+    where float32 sums would be infinite."""
 
     # decode steps are host-bound, hence the integer comparisons and the quick look
     # at the arrays' ends in front of _overlap
