@@ -33,7 +33,7 @@ from .gated_delta import (PREFILL_MIN_TOKENS, _as, _c, _check_cu_seqlens, _check
                           _require_device, _stream, _with_longest, gated_delta_update)
 from .low_rank import AdapterRows, LowRankAdapters, add_low_rank
 from .norm import rms_norm
-from .quant import (LinearWeights, QuantizedRows, QuantScheme, concat_quantized, quantized_linear,
+from .quant import (LinearWeights, QuantizedRows, QuantScheme, _followed, concat_quantized, quantized_linear,
                     quantized_linear_split, stackable)
 from .recurrent_cache import RecurrentCache, RecurrentStatePool
 
@@ -440,7 +440,8 @@ class Qwen3_5LinearAttention:
         before: for each projection the list of its S adapters as
         :class:`LowRankAdapters` takes one, or None. A call uses them where it is
         given ``adapter_rows``; graphs captured before keep the adapters that they
-        were captured with."""
+        were captured with. Adapters have no gradient: a call whose out_proj (dense) or
+        residual needs one raises ``RuntimeError`` before a state changes."""
 
         ins = [in_proj_qkv, in_proj_z, in_proj_a, in_proj_b]
         counts = {len(p) for p in (*ins, out_proj) if p is not None}
@@ -518,9 +519,11 @@ class Qwen3_5LinearAttention:
             add_low_rank(y, rows, self._out_adapters, adapter_rows)
         return y
 
-    def _project(self, rows: torch.Tensor, adapter_rows: AdapterRows | None = None):
+    def _project(self, rows: torch.Tensor, adapter_rows: AdapterRows | None = None,
+                 residual: torch.Tensor | None = None):
         """The input projections of ``rows``, normed first if the layer does that,
-        with what the rows' adapters add."""
+        with what the rows' adapters add. ``residual``: what out_proj's product will
+        add."""
 
         if adapter_rows is not None and self._in_adapters is None and self._out_adapters is None:
             raise ValueError("adapter_rows given, but the layer has no adapters (set_adapters)")
@@ -531,6 +534,11 @@ class Qwen3_5LinearAttention:
                                   adapter_rows._index != after._index):
             raise ValueError(f"rows of {adapter_rows.rows} with {adapter_rows.count} adapters on {adapter_rows.device}, x has "
                              f"{rows.shape[0]} and there are {after.count} on {after.device}")
+        if after is not None:
+            tensors, _ = self._scheme_of(self.out_proj)
+            if _followed(residual, tensors if isinstance(tensors, torch.Tensor) else None):
+                raise RuntimeError("out_proj's adapters have no gradient and no forward mode; call the layer under "
+                                   "torch.no_grad()")
         if self.input_norm_weight is not None:
             if isinstance(rows, QuantizedRows):
                 raise ValueError("the layer norms its input itself (input_norm_weight) and takes plain rows")
@@ -629,7 +637,7 @@ class Qwen3_5LinearAttention:
         tensors, or in ``conv_out`` and ``ssm_out`` when given."""
 
         d = self.linear
-        qkv, z, a, b = self._project(rows, adapter_rows)
+        qkv, z, a, b = self._project(rows, adapter_rows, residual)
         act = qkv.dtype
         outs = conv_out is not None or ssm_out is not None
         if rows.shape[0] == 1 and _fused_decode_ok(d, act) and not outs:
@@ -666,7 +674,7 @@ class Qwen3_5LinearAttention:
         if x.ndim != 2 or x.shape[0] != rows:
             raise ValueError("decode_batch expects x of shape (pool.batch, hidden), or "
                              "(len(slots), hidden) with slots")
-        qkv, z, a, b = self._project(x, adapter_rows)
+        qkv, z, a, b = self._project(x, adapter_rows, residual)
         if not _fused_decode_ok(d, qkv.dtype) or pool.conv_buf.dtype != qkv.dtype:
             raise ValueError("decode_batch needs Dk = Dv = 128, K = 4 and a pool in the "
                              "activation dtype (float32 or bfloat16)")
