@@ -115,7 +115,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *, residu
     _lib.call_on(device, "gdn_rms_norm", x.data_ptr(), x_stride, _lib.ptr(residual), r_stride, _lib.ptr(sum_out), s_stride,
                  _lib.ptr(weight), float(eps), _lib.dtype_code(dtype), _lib.ptr(out), codes, scales, apart, M, K,
                  _stream(device))
-    normed = out if not quantize else QuantizedRows(x.shape, dtype, data, out)
+    normed = out if not quantize else QuantizedRows._made(x.shape, dtype, data, out)
     return normed if residual is None else (normed, sum_out)
 
 

@@ -29,6 +29,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib
+from .gated_delta import _FLOATS
 
 _SUPPORTED = {
     "affine": ({2, 3, 4, 5, 6, 8}, {32, 64, 128}),
@@ -195,11 +196,30 @@ class QuantizedRows:
     __slots__ = ("shape", "dtype", "rows", "_data")
 
     def __init__(self, shape, dtype: torch.dtype, data: torch.Tensor, rows: torch.Tensor | None = None) -> None:
-        """``data``: uint8, the codes ``(M, ceil(K / 128) * 128)`` and behind them the
-        scales ``(ceil(K / 128), S)`` float32, row m's in column m, S = M rounded up to
-        256 (:meth:`nbytes` in all): the layout that the products read."""
+        """``data``: uint8, the codes ``(M, ceil(K / 128) * 128)``, zeros past K, and
+        behind them the scales ``(ceil(K / 128), S)`` float32, row m's in column m, S = M
+        rounded up to 256 (:meth:`nbytes` in all, from a multiple of 16 bytes on): the
+        layout that the products read. ``ValueError`` for data of another size or kind."""
 
-        self.shape, self.dtype, self.rows, self._data = torch.Size(shape), dtype, rows, data
+        shape = torch.Size(shape)
+        if not shape or min(shape) < 0 or shape[-1] == 0 or shape[-1] % 16 or dtype not in _FLOATS:
+            raise ValueError(f"quantized rows are (..., K) of a float dtype, K a multiple of 16, got {tuple(shape)} {dtype}")
+        nbytes = self.nbytes(shape.numel() // shape[-1], shape[-1])
+        if data.dtype != torch.uint8 or data.shape != (nbytes,) or not data.is_contiguous() or data.data_ptr() % 16:
+            raise ValueError(f"quantized rows {tuple(shape)} lie in {nbytes} bytes one after the other (uint8) from a multiple "
+                             f"of 16 on, got {tuple(data.shape)} {data.dtype}")
+        if rows is not None and (rows.shape != shape or rows.dtype != dtype or rows.device != data.device):
+            raise ValueError(f"the rows kept beside the codes are {tuple(shape)} {dtype} on {data.device}, got "
+                             f"{tuple(rows.shape)} {rows.dtype} on {rows.device}")
+        self.shape, self.dtype, self.rows, self._data = shape, dtype, rows, data
+
+    @classmethod
+    def _made(cls, shape: torch.Size, dtype: torch.dtype, data: torch.Tensor, rows: torch.Tensor | None) -> "QuantizedRows":
+        """Of parts that fit each other by their making (a decode step is host-bound)."""
+
+        self = cls.__new__(cls)
+        self.shape, self.dtype, self.rows, self._data = shape, dtype, rows, data
+        return self
 
     @staticmethod
     def nbytes(M: int, K: int) -> int:
@@ -250,7 +270,7 @@ class QuantizedRows:
         shape = torch.empty(self.shape, device="meta").reshape(*lead_and_width).shape
         if shape[-1:] != self.shape[-1:]:
             raise ValueError(f"the width {self.shape[-1]} of quantized rows stays")
-        return QuantizedRows(shape, self.dtype, self._data, None if self.rows is None else self.rows.reshape(shape))
+        return QuantizedRows._made(shape, self.dtype, self._data, None if self.rows is None else self.rows.reshape(shape))
 
 
 @dataclass(frozen=True)
