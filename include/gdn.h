@@ -302,8 +302,8 @@ int gdn_gated_rmsnorm(const void *x, int x_dtype, const void *z, int z_dtype, in
  * residual rounded to dtype, which is written to sum. y is the exact value rounded
  * to float32, then to dtype; sums are held in 64 bits.
  *   x, residual (or NULL), sum (NULL without a residual): (rows, K) dtype at their
- *      own row strides in elements; sum may be x or residual (the same pointer and
- *      stride) and must not overlap them otherwise
+ *      own row strides in elements; sum may be x or residual (the same pointer and,
+ *      of several rows, stride) and must not overlap them otherwise
  *   w: (K) float32 or NULL (ones)
  *   out: (rows, K) dtype packed, or NULL
  *   codes, scales: NULL, or y in e4m3 as gdn_fp8_matmul_codes takes it (K a

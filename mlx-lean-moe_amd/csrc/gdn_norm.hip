@@ -279,7 +279,7 @@ extern "C" int gdn_rms_norm(const void* x, int64_t x_stride, const void* residua
         const int es = dtype_size(dtype);
         const auto span = [&](int64_t stride) { return ((rows - 1) * stride + K) * es; };
         const auto apart = [&](const void* in, int64_t stride) {
-            if ((sum == in && sum_stride == stride) || !overlaps(sum, span(sum_stride), in, span(stride))) return true;
+            if ((sum == in && (sum_stride == stride || rows == 1)) || !overlaps(sum, span(sum_stride), in, span(stride))) return true;
             if (sum_stride != stride || rows == 1) return false;
             // columns of one buffer beside each other
             const int64_t row = stride * es, off = (reinterpret_cast<intptr_t>(in) - reinterpret_cast<intptr_t>(sum)) % row;

@@ -120,11 +120,13 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *, residu
 
 
 def _check_sum(out: torch.Tensor, stride: int, src: torch.Tensor, K: int, name: str) -> None:
-    """``out``, rows of K ``stride`` apart, is ``src`` itself or does not overlap it."""
+    """``out``, rows of K ``stride`` apart, is ``src`` itself (of one row the stride says
+    nothing) or does not overlap it."""
 
-    if out.data_ptr() == src.data_ptr() and out.stride() == src.stride():
+    apart = _row_layout(src, K)
+    if out.data_ptr() == src.data_ptr() and apart == stride:
         return
-    if _row_layout(src, K) == stride and not rows_overlap(out.data_ptr(), src.data_ptr(), stride, K, K, out.numel() // K,
+    if apart == stride and not rows_overlap(out.data_ptr(), src.data_ptr(), stride, K, K, out.numel() // K,
                                                           out.element_size()):
         return
     ends = [(t.data_ptr(), t.data_ptr() + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size())
