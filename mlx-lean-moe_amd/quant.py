@@ -434,13 +434,18 @@ def quantized_linear(x: torch.Tensor, tensors, quant: QuantScheme | None = None,
     ``adapters`` (:class:`LowRankAdapters` of this projection) with
     ``adapter_rows`` (:class:`AdapterRows` of x's rows): what each row's adapter
     makes of it is added to the result (:func:`add_low_rank`), which is rounded once
-    more."""
+    more. The result then has x's dtype whatever the weights: dense ones of another
+    are cast to it first, as the layer casts its own (keep them in x's dtype to spare
+    the copy)."""
 
     if (adapters is None) != (adapter_rows is None):
         raise ValueError("adapters and adapter_rows go together")
     if adapters is not None:
         from .low_rank import add_low_rank
 
+        plain = tensors.tensors if isinstance(tensors, LinearWeights) else tensors
+        if isinstance(plain, torch.Tensor):
+            tensors = plain.to(x.dtype)
         y = quantized_linear(x, tensors, quant, residual=residual)
         add_low_rank(y.view(-1, y.shape[-1]), _kept_rows(x).reshape(-1, x.shape[-1]), adapters, adapter_rows)
         return y
