@@ -299,8 +299,8 @@ int gdn_gated_rmsnorm(const void *x, int x_dtype, const void *z, int z_dtype, in
 
 /*
  * gdn_rms_norm - y = s w / sqrt(mean(s^2) + eps) over rows of K, s = x, or x +
- * residual rounded to dtype, which is written to sum. y is the exact value rounded
- * to float32, then to dtype; sums are held in 64 bits.
+ * residual rounded to dtype, which is written to sum. y is formed in 64 bits and
+ * rounded to float32, then to dtype.
  *   x, residual (or NULL), sum (NULL without a residual): (rows, K) dtype at their
  *      own row strides in elements; sum may be x or residual (the same pointer and,
  *      of several rows, stride) and must not overlap them otherwise

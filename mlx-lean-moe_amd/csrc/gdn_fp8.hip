@@ -7,7 +7,9 @@
 // scales meet float32 sums only), the outer one in float32. float32 results take
 // the codes widened to bfloat16 instead (at mfma_widened). Rows may come in such codes
 // already, from the norm in front of the product (gdn_fp8_matmul_codes), which saves
-// the launch that makes them: 2048 -> 12352, 64 rows 11.6 us and 8.1, 4096 118 and 110.
+// the launch that makes them: 2048 -> 12352, 64 rows 11.6 us and 8.1 by codes, 4096 118 and
+// 110, the weights in the caches; 16 weights in turn, so from memory, 16 rows 12.0 and
+// 10.3, 64 19.3 and 16.6, 200 23.5 and 20.8, 4096 137 and 127.
 #include <type_traits>
 
 #include "gdn_common.h"

@@ -228,9 +228,10 @@ struct Ranks<ActF16> {
 // add their sums in LDS; kDepth steps' loads are under way at once.
 //
 // One round of workgroups, bound by its chain of waits (tile, row numbers, x, LDS) and
-// by x's way from memory: 8192 rows of 2048, rank 64, 14.4 us (33.5 MB), rank 16 10.9;
+// by x's way from memory: 8192 rows of 2048, rank 64, 14.0 us (33.5 MB), rank 16 10.8;
 // 9.0 at 2112 values a row, which do not lie a power of two apart (a part of K in one
-// piece a wave, to read at eight places far apart, took as long in all).
+// piece a wave, to read at eight places far apart, took as long in all). A is read by each
+// workgroup: of 4096 packed rows 59 MB pass the vector caches for 17 MB of x.
 template <class Act, int kRF, int kNR>
 __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_down_kernel(LowRankArgs p) {
     using S = typename Act::storage;
@@ -367,7 +368,9 @@ struct Columns {
 // and t are under way while these are multiplied and stored.
 //
 // Bound by the output's way through memory and back: 8192 x 4096, rank 16 about 30 us
-// (134 MB, 4.5 TB/s), rank 64 40; 4096 x 12288, rank up to 32, 43 (201 MB, 4.7 TB/s).
+// (134 MB, 4.5 TB/s), rank 64 42; 4096 x 12288, rank up to 32, 45 (201 MB, 4.4 TB/s).
+// Past rank 64 by B, which is read for each 16 rows with nothing under way behind it: 4096 x
+// 4096, rank 100, 32 us (225 MB of reads at the vector caches, 67 MB of output).
 // At rank 64 t is twice the output's bytes at the vector caches, and cutting it is more of
 // the arithmetic than the output's sums. Four waves a SIMD there in bfloat16 (120
 // registers; left alone 132 and three: 8192 rows 53.5 us and 54.1, 2048 20.2 and 20.6).
@@ -472,7 +475,7 @@ __global__ __launch_bounds__(64 * kLowRankUpWaves, Act::code == GDN_BF16 && kHel
 // columns, t from LDS; the next ones' output is under way while these are multiplied,
 // their B while these are stored. Every workgroup of a block reads the same rows of
 // A: low_rank_plan says where that is too much. Bound by its chain of waits: 1 row,
-// 2048 -> 8192 | 4096, rank 16, 5.3 us; 64 rows of 27 adapters 9.5 (17.6 MB).
+// 2048 -> 8192 | 4096, rank 16, 5.3 us; 64 rows of 27 adapters 9.2 (17.6 MB).
 template <class Act, int kNR>
 __global__ __launch_bounds__(64 * kLowRankDownWaves) void low_rank_whole_kernel(LowRankArgs p) {
     using S = typename Act::storage;

@@ -34,24 +34,26 @@ struct LowRankPlan {
 // Two launches. Few tiles: the first product's ranks apart, 16 a workgroup, so that the
 // reading of an adapter is spread; many: together, so that x is read once; between, 32
 // (both launches, 64 columns, us, 16, 32 and 64 ranks a workgroup: 1024 rows of 2048, rank
-// 64 8.0, 8.4, 9.8, float32 12.1, 14.3, 21.1; 2048 rows 11.1, 9.5, 10.6, float32 17.2,
-// 15.7, 22.6; 4096 rows 15.7, 12.7, 12.2, float32 26.3, 22.7, 23.4; 2048 rows of 8
-// adapters, rank 96 17.3, 14.5, 16.3, float32 27.4, 24.8, 37.2). 32 rows share a reading of
-// the adapter where that leaves a workgroup for each CU (8192 rows of rank 64 50.1 us in
-// all, 52.6 with 16 rows). The second product takes as many rows of a tile as leave 4096
-// workgroups, since those share a reading of B (4096 x 12288, rank 32: 53.0 us in all, with
-// 2048 54.5, with 512 58; 8192 x 4096, rank 16 40.0, 42.3, 41.4); with four pieces of B to
-// read as many as leave 512, up to 64 (rank 64, us, 16 rows, 32 and 64: 2048 x 4096 20.1,
-// 18.3, 17.8, float16 23.4, 20.4, 19.1, float32 35.2, 32.6, 32.5; 1024 x 4096 14.2, 13.0,
-// 13.7; 8192 x 4096, 32 rows, 64 and 128 50.7, 50.3, 53.0).
+// 64 8.9, 9.5, 11.0, float32 12.2, 14.5, 21.7; 2048 rows 11.5, 10.3, 11.3, float32 17.0,
+// 15.5, 22.5; 4096 rows 15.9, 13.0, 12.5, float32 27.2, 23.5, 24.5; 2048 rows of 8
+// adapters, rank 96 17.8, 14.7, 16.9, float32 27.4, 24.8, 37.1). 32 rows share a reading of
+// the adapter where that leaves a workgroup for each CU (8192 rows of rank 64 53.8 us in
+// all, 56.2 with 16 rows). The second product takes as many rows of a tile as leave 4096
+// workgroups, since those share a reading of B (4096 packed rows of 6 adapters x 12288, rank
+// 32: 68.4 us in all, with 2048 69.6, with 512 79.2; 8192 x 4096, rank 16 41.7, 44.1, 44.0);
+// with four pieces of B to read as many as leave 512, up to 64 (rank 64, us, 16 rows, 32 and
+// 64: 2048 x 4096 20.0, 18.8, 19.5, float16 23.1, 20.4, 19.3, float32 36.7, 35.0, 34.5; 1024
+// x 4096 14.0, 13.7, 15.1, which 512 leaves at 32; 4096 x 8192 49.9, 44.5, 41.3, float16
+// 65.0, 53.9, 48.7; 8192 x 4096, 32 rows, 64 and 128 51.8, 53.5, 54.2, float16 61.1 and 59.3
+// with 32 and 64).
 //
 // One, where that is one round of workgroups of not many columns, and what each reads of
 // A (its own adapter's rows, as every other workgroup of its block) is little. us, one
-// launch and two, 2048 -> 8192 | 4096: rank 16, 1 row 4.6 and 6.5, 64 rows of 27 adapters
-// 9.0 and 11.2 (4096 values a row: 10.9 and 12.4), 512 rows of one 11.9 and 14.7, 1024
-// 16.7 and 19.4, 2048 (16 steps of columns) 29.5 and 27.9, 4096 63 and 55; rank 32, 1 row
-// 5.4 and 6.4, 64 rows of 8 adapters 9.7 and 8.5, of 27 11.6 and 12.2, 512 rows of one
-// 13.8 and 15.1; rank 64, 1 row 7.0 and 6.7, 8 rows 8.0 and 7.4, 512 16.9 and 16.6.
+// launch and two, 2048 -> 8192 | 4096: rank 16, 1 row 4.5 and 6.4, 64 rows of 27 adapters
+// 9.3 and 10.3 (4096 values a row: 11.2 and 11.5), 512 rows of one 11.9 and 13.9, 1024
+// 17.1 and 18.4, 2048 (16 steps of columns) 31.7 and 27.0, 4096 54 and 54; rank 32, 1 row
+// 5.5 and 6.6, 64 rows of 8 adapters 10.1 and 9.3, of 27 12.3 and 12.3, 512 rows of one
+// 13.8 and 15.2; rank 64, 1 row 7.5 and 7.1, 8 rows 8.4 and 7.8, 512 19.0 and 16.2.
 inline LowRankPlan low_rank_plan(int tiles, int tile_rows, int rank_total, int rank_block, int K, int elem,
                                  const int* widths, int blocks) {
     LowRankPlan p;

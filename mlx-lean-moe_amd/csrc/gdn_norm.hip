@@ -2,11 +2,13 @@
 // the result in e4m3 codes:
 //   s = T(x + r),   y = T(s w / sqrt(mean(s^2) + eps)),
 //   per 128 columns: scale = max(amax |y| / 448, 2^-126), code = e4m3(y / scale),
-// T the rounding to the rows' type. y is the exact value rounded to float32 and
-// then to T: sums are held in 64 bits (a square of two float32 values is exact
-// there), and so is each product that falls near a border of T. So neither y nor
-// the codes depend on the order of a sum, and the codes are those that
-// gdn_fp8_matmul makes of y.
+// T the rounding to the rows' type. y is formed in 64 bits and rounded to float32 and
+// then to T: sums are held in 64 bits (a square of a float32 value is exact there), and so
+// is each product that falls near a border of T. That is within 2^-48 of the exact value
+// for rows of up to 16384 (at most 38 roundings a sum, of which the root leaves half,
+// and six more), so y is the exact value's rounding but where that lies so near a border.
+// A row's sum is added in an order of K alone: its y and codes do not depend on
+// the rows beside it, and the codes are those that gdn_fp8_matmul makes of y.
 #include <type_traits>
 
 #include "gdn_common.h"
@@ -198,8 +200,9 @@ GDN_DEV double row_sum(double v) {
 // A row's columns stay in the registers of its threads, kVec times eight in each:
 // memory is read once and written once, and that is what bounds it. kLanes threads
 // of a wave a row, or (0) a workgroup of as many waves as the row's columns take.
-// Measured, with the residual, bf16: 4096 rows of 2048 14.8 us (67 MB, 4.5 TB/s; a
-// large copy 5.1), 8192 to codes 25.4 (118 MB); 1 row 2.9, a launch and its waits.
+// Measured, with the residual, bf16, calls one after the other: 4096 rows of 2048 13.8 us
+// (67 MB, 4.9 TB/s; a large copy 5.1), 8192 to codes 26.3 (118 MB); 1 row 3.0 by
+// itself, a launch and its waits.
 template <class Act, int kLanes, int kVec, bool kCodes>
 __global__ __launch_bounds__(kLanes ? 256 : 1024) void rms_norm_kernel(NormArgs a) {
     const int lanes = kLanes ? kLanes : blockDim.x, per = kLanes ? 256 / kLanes : 1;

@@ -164,7 +164,8 @@ class AdapterRows:
     if it is on the GPU). ``distinct``: room for batches of that many different
     adapters, for :meth:`assign`; without it there is room for as many tiles as
     ``index`` takes. Made outside of a graph's capture; its copy on the device
-    belongs to the stream it was made on until that is done."""
+    belongs to the stream it was made on until that is done. Host work of 42 us for one
+    row, 45 for 64, 73 for 4096 (of an array; a list of 4096 takes 200 more)."""
 
     def __init__(self, index, count: int, device: torch.device | str = "cuda", *, distinct: int | None = None) -> None:
         if count < 1:
@@ -193,8 +194,10 @@ class AdapterRows:
 
     def assign(self, index) -> None:
         """Other adapters for the same number of rows, in the same device memory: what
-        a captured graph's next replay uses. The copy goes to the current stream.
-        ``ValueError`` if there is no room for them (``distinct``)."""
+        a captured graph's next replay uses. The copy goes to the current stream, and
+        the host waits for it and for what that stream still has to do (31 us for one row,
+        44 for 4096, of an idle one). ``ValueError`` if there is no room for them
+        (``distinct``)."""
 
         index = self._checked(index)
         if len(index) != self.rows:

@@ -40,8 +40,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *, residu
     ``x + residual`` rounded to their dtype.
 
     ``x`` and ``residual (..., K)`` of one float dtype (rows at any stride, e.g.
-    column slices); ``weight (K,)`` or None (ones). The result is the exact value
-    rounded to float32 and then to x's dtype, whatever the order of the sums.
+    column slices); ``weight (K,)`` or None (ones). The result is formed in 64 bits
+    and rounded to float32 and then to x's dtype; it does not depend on the other rows.
 
     Without a residual the normed rows are returned, with one ``(normed, s)``:
     ``s`` is the stream that the next layer's result is added to, written to
